@@ -214,6 +214,90 @@ int myl_sample_dev(myl_ctx* ctx, const int32_t* logits, size_t M, size_t n, size
 int myl_logsoftmax_dev(myl_ctx* ctx, const int32_t* logits, size_t M, size_t n, size_t ldz, const int16_t* exp_lut,
                        size_t lut_len, const int64_t* targets, int64_t* out);
 
+/* ---- a serving step: adapters, a shared prefix, drafted tokens ---------------
+ * No counterparts in the reference; each step is a reference primitive.  These
+ * forms keep nothing between calls: their scratch is the caller's `workspace`
+ * (device memory, 16-byte aligned, of at least the bytes that the matching
+ * *_workspace function names; it returns 0 for sizes the call refuses), whose
+ * contents before and after a call mean nothing.  So they can be captured into
+ * HIP graphs, and calls on different contexts and streams run at once as long
+ * as each has its own workspace.  Operands and outputs do not overlap unless
+ * stated. */
+
+/* linear_w8a16_dev with the low-rank adapter of each row's request added:
+ *   u[m]   = linear_w8a16(x[m], A[id], a_shifts[id], act_frac, mid_frac)
+ *   d[m]   = linear_w8a16(u[m], B[id], b_shifts[id], mid_frac, out_frac)
+ *   out[m] = clamp_i16(linear_w8a16(x[m], W, w_shifts, act_frac, out_frac) + d[m])
+ * (linear.rs:43-70; out_frac_pc as in myl_linear_w8a16_dev, for both terms),
+ * id = ids[m].  A row whose id is outside [0, n_adapters) has no adapter (d = 0).
+ * A [n_adapters x rank x K], a_shifts [n_adapters x rank], B [n_adapters x N x
+ * rank], b_shifts [n_adapters x N]; rank is at most 256 (an adapter of lower
+ * rank is padded with zero rows of A and zero columns of B). */
+size_t myl_linear_w8a16_adapters_workspace(const myl_ctx* ctx, size_t M, size_t N, size_t K, size_t rank);
+int myl_linear_w8a16_adapters_dev(myl_ctx* ctx, const int16_t* x, size_t M, size_t ldx, const int8_t* W, size_t N,
+                                  size_t K, const uint8_t* w_shifts, uint8_t act_frac, uint8_t out_frac,
+                                  const uint8_t* out_frac_pc, const int32_t* ids, const int8_t* A,
+                                  const uint8_t* a_shifts, uint8_t mid_frac, const int8_t* B, const uint8_t* b_shifts,
+                                  size_t n_adapters, size_t rank, int16_t* out, size_t ldo, void* workspace,
+                                  size_t workspace_bytes);
+
+/* Attention (attention.rs:42-90) of a batch that shares a prefix: row
+ * r = s * rows_per_seq + i of sequence s attends all prefix_len prefix
+ * positions, then the first lens[r] (at most max_tail) positions of its
+ * sequence's tail; drafted rows of one sequence take rising lens.
+ *   q, out    [n_seqs * rows_per_seq] rows of heads x head_dim, row strides ldq, ldo
+ *   k_prefix, v_prefix  [kv_heads][prefix_len][head_dim], heads prefix_head_stride apart
+ *   k_tail, v_tail      [n_slots][kv_heads][max_tail][head_dim], strides
+ *             tail_slot_stride and tail_head_stride; sequence s's tail is slot
+ *             slots[s] (slots NULL: slot s)
+ *   lens      [rows] int32.  A negative one leaves the row out: its output is
+ *             zero.  A row with no key at all gives zero too; one whose slot is
+ *             outside [0, n_slots) attends the prefix alone.
+ * The keys' order for softmax_int's uniform split is prefix, then tail.  Query
+ * head h reads KV head h / (heads / kv_heads).  head_dim is 64 or 128
+ * (MYL_E_UNSUPPORTED otherwise), prob_frac at most 14, prefix_len + max_tail at
+ * most 65536, heads and rows at most 65535 each; negative exp table entries
+ * count as 0.  Pointers are 16-byte aligned, strides (in elements) multiples of 8. */
+size_t myl_attention_prefix_workspace(const myl_ctx* ctx, size_t n_seqs, size_t rows_per_seq, size_t heads,
+                                      size_t kv_heads, size_t head_dim, size_t prefix_len, size_t max_tail);
+int myl_attention_prefix_dev(myl_ctx* ctx, const int16_t* q, size_t n_seqs, size_t rows_per_seq, size_t ldq,
+                             size_t heads, size_t kv_heads, size_t head_dim, const int16_t* k_prefix,
+                             const int16_t* v_prefix, size_t prefix_len, size_t prefix_head_stride,
+                             const int16_t* k_tail, const int16_t* v_tail, size_t n_slots, size_t tail_slot_stride,
+                             size_t tail_head_stride, size_t max_tail, const int32_t* slots, const int32_t* lens,
+                             int64_t score_mult, uint8_t score_shift, const int16_t* exp_lut, size_t lut_len,
+                             uint8_t lut_shift, uint8_t prob_frac, int16_t* out, size_t ldo, void* workspace,
+                             size_t workspace_bytes);
+
+/* Drafted tokens checked against the target's probabilities (speculative
+ * sampling) with given random numbers.  A row of Q6 logits has the weights of
+ * myl_logsoftmax_dev, p_j = exp_lut[(max z - z_j) << 2] (0 past the table and
+ * for negative entries), P = sum p_j.  Draft i of a sequence, token t, is
+ * accepted when all before it were and
+ *   floor(r_i q_t P / 2^64) < p_t Q         (r_i / 2^64 < (p_t / P) / (q_t / Q))
+ * with q, Q of the draft's row i; draft = NULL stands for drafts without
+ * probabilities (q_t = Q = 1).  The next token is the first j with
+ *   floor(r_k W / 2^64) < w_0 + ... + w_j,  W = sum w_j,
+ * where w_j = p_j of row i behind the last draft, and max(0, p_j Q - q_j P) of
+ * row i where draft i was rejected (p_j if that leaves nothing; the row's first
+ * maximum if P = 0).  So the tokens follow the target's probabilities whatever
+ * was drafted.  exp_lut = NULL checks greedily: draft i is accepted when it is
+ * the first maximum of row i (sampling.rs:8-18), the next token is the row's
+ * first maximum; draft and randoms are not read.
+ *   target   [n_seqs * (k + 1)] rows (stride ldt): row b (k + 1) + i follows draft i - 1
+ *   draft    [n_seqs * k] rows (stride ldd)       tokens   [n_seqs x k]
+ *   n_draft  [n_seqs], clamped to 0 .. k (NULL: k) randoms  [n_seqs x (k + 1)]
+ *   accepted [n_seqs]: drafts accepted            out      [n_seqs x (k + 1)]: the
+ *            accepted drafts, the next token, then -1
+ * A drafted token outside the vocabulary is rejected.  vocab is at most 2^20,
+ * k at most 1024 (0 samples a token per row), the table at most 32768 entries
+ * (trailing zeros left off make it faster). */
+size_t myl_verify_drafts_workspace(const myl_ctx* ctx, size_t n_seqs, size_t k, size_t vocab, size_t lut_len);
+int myl_verify_drafts_dev(myl_ctx* ctx, const int32_t* target, size_t ldt, const int32_t* draft, size_t ldd,
+                          size_t n_seqs, size_t k, size_t vocab, const int64_t* tokens, const int32_t* n_draft,
+                          const uint64_t* randoms, const int16_t* exp_lut, size_t lut_len, int32_t* accepted,
+                          int64_t* out, void* workspace, size_t workspace_bytes);
+
 /* ======================================================================
  * 3. Device-resident model (runtime/src/model.rs, kv_cache.rs)
  * ==================================================================== */

@@ -33,6 +33,26 @@ def _p(a):
     return None if a is None else a.ctypes.data
 
 
+def _need(ok, what: str) -> None:
+    if not ok:
+        raise ValueError(what)
+
+
+def _need_dev(what: str, device, **tensors) -> None:
+    """name=(tensor, dtype name, shape): on the device, of that type and shape (-1:
+    any size), its elements in order (strides are the caller's to check where shape is None)."""
+    for name, (t, dtype, shape) in tensors.items():
+        if t.device != device or str(t.dtype) != "torch." + dtype:
+            raise ValueError(f"{what}: {name} must be {dtype} on {device}")
+        if shape is not None and not (tuple(t.shape) == shape and t.is_contiguous()):
+            raise ValueError(f"{what}: {name} must be contiguous {list(shape)}, not {list(t.shape)}")
+
+
+def _strides(t):
+    """The strides that an element's place depends on (0 for dimensions of one element or none)."""
+    return tuple(st if n > 1 else 0 for st, n in zip(t.stride(), t.shape)) if t.numel() else (0,) * t.ndim
+
+
 class RocmBackend:
     """One HIP context on one device (rocm.rs:41-60)."""
 
@@ -342,3 +362,170 @@ class RocmBackend:
         self.check(lib().myl_logsoftmax_dev(self._h, z.data_ptr(), M, n, z.stride(0), lut.data_ptr(), lut.numel(),
                                             t.data_ptr(), out.data_ptr()), "logsoftmax_dev")
         return out
+
+    # ---- a serving step: adapters, a shared prefix, drafted tokens ---------------
+    def _workspace(self, nbytes: int, device, workspace):
+        """The caller's workspace, or one for this call alone (the allocator keeps
+        it until the context's stream has passed it)."""
+        if workspace is not None:
+            _need(workspace.device == device and workspace.is_contiguous(), "workspace: contiguous, on the operands' device")
+            return workspace
+        import torch
+        ws = torch.empty(max(nbytes, 1), dtype=torch.uint8, device=device)
+        stream = lib().myl_stream(self._h) or 0
+        if stream != torch.cuda.current_stream(device).cuda_stream:
+            ws.record_stream(torch.cuda.ExternalStream(stream, device=device))
+        return ws
+
+    @staticmethod
+    def _new_workspace(nbytes: int, device, what: str):
+        import torch
+        _need(nbytes > 0, f"{what}: these sizes are not supported")
+        return torch.empty(nbytes, dtype=torch.uint8, device=device)
+
+    def linear_w8a16_adapters_workspace(self, x, W, A):
+        """A workspace for linear_w8a16_adapters_dev on operands of these shapes."""
+        n = lib().myl_linear_w8a16_adapters_workspace(self._h, x.shape[0], W.shape[0], x.shape[1], A.shape[1])
+        return self._new_workspace(n, x.device, "linear_w8a16_adapters_dev")
+
+    def linear_w8a16_adapters_dev(self, x, W, w_shifts, act_frac: int, ids, A, a_shifts, mid_frac: int, B, b_shifts,
+                                  out_frac: int = 0, out_frac_pc=None, out=None, workspace=None):
+        """linear_w8a16_dev plus each row's low-rank adapter: x int16 [M x K],
+        W int8 [N x K], ids int32 [M] (an id outside [0, n): none), A int8
+        [n x rank x K] with a_shifts uint8 [n x rank], B int8 [n x N x rank]
+        with b_shifts uint8 [n x N] (include/myl_hip.h states the arithmetic)."""
+        what = "linear_w8a16_adapters_dev"
+        M, K = x.shape
+        N = W.shape[0]
+        n, rank = A.shape[:2]
+        _need_dev(what, x.device, x=(x, "int16", None), W=(W, "int8", (N, K)), w_shifts=(w_shifts, "uint8", (N,)),
+                  ids=(ids, "int32", (M,)), A=(A, "int8", (n, rank, K)), a_shifts=(a_shifts, "uint8", (n, rank)),
+                  B=(B, "int8", (n, N, rank)), b_shifts=(b_shifts, "uint8", (n, N)))
+        _need(_strides(x)[1] in (0, 1), f"{what}: the elements of a row of x follow one another")
+        if out_frac_pc is not None:
+            _need_dev(what, x.device, out_frac_pc=(out_frac_pc, "uint8", (N,)))
+        if out is None:
+            import torch
+            out = torch.empty((M, N), dtype=torch.int16, device=x.device)
+        _need_dev(what, x.device, out=(out, "int16", None))
+        _need(tuple(out.shape) == (M, N) and _strides(out)[1] in (0, 1), f"{what}: out must be [M x N]")
+        ws = self._workspace(lib().myl_linear_w8a16_adapters_workspace(self._h, M, N, K, rank), x.device, workspace)
+        rc = lib().myl_linear_w8a16_adapters_dev(
+            self._h, x.data_ptr(), M, _strides(x)[0] or K, W.data_ptr(), N, K, w_shifts.data_ptr(), act_frac, out_frac,
+            None if out_frac_pc is None else out_frac_pc.data_ptr(), ids.data_ptr(), A.data_ptr(), a_shifts.data_ptr(),
+            mid_frac, B.data_ptr(), b_shifts.data_ptr(), n, rank, out.data_ptr(), _strides(out)[0] or N,
+            ws.data_ptr(), ws.numel() * ws.element_size())
+        if rc:
+            self.check(rc, what)
+        return out
+
+    def attention_prefix_workspace(self, q, k_prefix, k_tail, rows_per_seq: int = 1):
+        """A workspace for attention_prefix_dev on operands of these shapes."""
+        n = lib().myl_attention_prefix_workspace(self._h, q.shape[0] // max(1, rows_per_seq), rows_per_seq, q.shape[1],
+                                                 k_prefix.shape[0], q.shape[2], k_prefix.shape[1], k_tail.shape[2])
+        return self._new_workspace(n, q.device, "attention_prefix_dev")
+
+    def attention_prefix_dev(self, q, k_prefix, v_prefix, k_tail, v_tail, lens, score_mult: int, score_shift: int,
+                             exp_lut, lut_shift: int, prob_frac: int, rows_per_seq: int = 1, slots=None, max_tail=None,
+                             out=None, workspace=None):
+        """Attention of a batch behind a shared prefix, int16 throughout: q and out
+        [rows x heads x hd], rows_per_seq rows of each sequence in turn; k_prefix
+        and v_prefix [kv_heads x P x hd]; k_tail and v_tail [slots x kv_heads x
+        capacity x hd], sequence s's in slot slots[s] (None: slot s).  Row r
+        attends the prefix and the first lens[r] positions of its tail (at most
+        max_tail, by default the capacity; negative: the row is left out and
+        its output is zero).  include/myl_hip.h states the arithmetic."""
+        what = "attention_prefix_dev"
+        R, H, hd = q.shape
+        KH, P = k_prefix.shape[:2]
+        S, _, T = k_tail.shape[:3]
+        dev = q.device
+        _need(rows_per_seq > 0 and R % rows_per_seq == 0, f"{what}: rows must be a multiple of rows_per_seq")
+        _need(k_prefix.shape == v_prefix.shape == (KH, P, hd) and k_tail.shape == v_tail.shape == (S, KH, T, hd),
+              f"{what}: prefix [kv_heads x P x hd], tails [slots x kv_heads x capacity x hd]")
+        _need(max_tail is None or 0 <= max_tail <= T, f"{what}: max_tail is at most the tails' capacity")
+        _need_dev(what, dev, q=(q, "int16", None), k_prefix=(k_prefix, "int16", None), v_prefix=(v_prefix, "int16", None),
+                  k_tail=(k_tail, "int16", None), v_tail=(v_tail, "int16", None), lens=(lens, "int32", (R,)),
+                  exp_lut=(exp_lut, "int16", (exp_lut.numel(),)))
+        n_seqs = R // rows_per_seq
+        if slots is not None:
+            _need_dev(what, dev, slots=(slots, "int32", (n_seqs,)))
+        else:
+            _need(S >= n_seqs, f"{what}: fewer tails than sequences")
+        if out is None:
+            import torch
+            out = torch.empty((R, H, hd), dtype=torch.int16, device=dev)
+        _need_dev(what, dev, out=(out, "int16", None))
+        _need(out.shape == q.shape, f"{what}: out must have q's shape")
+
+        def rows_of(t, name):
+            _need(_strides(t)[1] in (0, hd) and _strides(t)[2] in (0, 1), f"{what}: the heads of a row of {name} follow one another")
+            return _strides(t)[0] or H * hd
+
+        ps, ts = _strides(k_prefix), _strides(k_tail)
+        _need(ps[1] in (0, hd) and ps[2] in (0, 1) and ts[2] in (0, hd) and ts[3] in (0, 1),
+              f"{what}: the positions of a KV head follow one another")
+        _need(ps == _strides(v_prefix) and ts == _strides(v_tail), f"{what}: keys and values have the same strides")
+        max_tail = T if max_tail is None else max_tail
+        ws = self._workspace(lib().myl_attention_prefix_workspace(self._h, n_seqs, rows_per_seq, H, KH, hd, P, max_tail),
+                             dev, workspace)
+        rc = lib().myl_attention_prefix_dev(
+            self._h, q.data_ptr(), n_seqs, rows_per_seq, rows_of(q, "q"), H, KH, hd, k_prefix.data_ptr(), v_prefix.data_ptr(),
+            P, ps[0] or P * hd, k_tail.data_ptr(), v_tail.data_ptr(), S, ts[0] or KH * T * hd, ts[1] or T * hd, max_tail,
+            None if slots is None else slots.data_ptr(), lens.data_ptr(), score_mult, score_shift, exp_lut.data_ptr(),
+            exp_lut.numel(), lut_shift, prob_frac, out.data_ptr(), rows_of(out, "out"), ws.data_ptr(),
+            ws.numel() * ws.element_size())
+        if rc:
+            self.check(rc, what)
+        return out
+
+    def verify_drafts_workspace(self, target, exp_lut=None, draft=None):
+        """A workspace for verify_drafts_dev on operands of these shapes."""
+        n = lib().myl_verify_drafts_workspace(self._h, target.shape[0], target.shape[1] - 1, target.shape[2],
+                                              0 if exp_lut is None else exp_lut.numel())
+        return self._new_workspace(n, target.device, "verify_drafts_dev")
+
+    def verify_drafts_dev(self, target, tokens, randoms, exp_lut=None, draft=None, n_draft=None, accepted=None, out=None,
+                          workspace=None):
+        """Drafted tokens against the target's probabilities: target int32
+        [B x k+1 x V] logits, tokens int64 [B x k], randoms uint64 [B x k+1]
+        (torch int64 tensors hold the bits), draft int32 [B x k x V] logits or
+        None (drafts without probabilities), n_draft int32 [B] or None (k each);
+        exp_lut None checks greedily (randoms may be None).  Returns (accepted
+        int32 [B], out int64 [B x k+1]: accepted drafts, the next token, -1).
+        include/myl_hip.h states the arithmetic."""
+        what = "verify_drafts_dev"
+        B, k1, V = target.shape
+        dev, k = target.device, k1 - 1
+        _need(k >= 0, f"{what}: target must be [B x k+1 x V]")
+        _need_dev(what, dev, target=(target, "int32", None), tokens=(tokens, "int64", (B, k)))
+
+        def rows_of(t, name, n):
+            seq, row, one = _strides(t)
+            _need(one in (0, 1) and (not seq or not row or seq == n * row), f"{what}: the rows of {name} are evenly spaced")
+            return row or seq or V
+
+        if exp_lut is not None:
+            _need(randoms is not None, f"{what}: random numbers are needed unless the check is greedy")
+            _need_dev(what, dev, exp_lut=(exp_lut, "int16", (exp_lut.numel(),)), randoms=(randoms, "int64", (B, k1)))
+        if draft is not None:
+            _need(tuple(draft.shape) == (B, k, V), f"{what}: draft must be [B x k x V]")
+            _need_dev(what, dev, draft=(draft, "int32", None))
+        if n_draft is not None:
+            _need_dev(what, dev, n_draft=(n_draft, "int32", (B,)))
+        if accepted is None or out is None:
+            import torch
+            accepted = torch.empty(B, dtype=torch.int32, device=dev) if accepted is None else accepted
+            out = torch.empty((B, k1), dtype=torch.int64, device=dev) if out is None else out
+        _need_dev(what, dev, accepted=(accepted, "int32", (B,)), out=(out, "int64", (B, k1)))
+        lut_len = 0 if exp_lut is None else exp_lut.numel()
+        ws = self._workspace(lib().myl_verify_drafts_workspace(self._h, B, k, V, lut_len), dev, workspace)
+        rc = lib().myl_verify_drafts_dev(
+            self._h, target.data_ptr(), rows_of(target, "target", k1), None if draft is None or k == 0 else draft.data_ptr(),
+            V if draft is None or k == 0 else rows_of(draft, "draft", k), B, k, V, tokens.data_ptr(),
+            None if n_draft is None else n_draft.data_ptr(), None if randoms is None else randoms.data_ptr(),
+            None if exp_lut is None else exp_lut.data_ptr(), lut_len, accepted.data_ptr(), out.data_ptr(), ws.data_ptr(),
+            ws.numel() * ws.element_size())
+        if rc:
+            self.check(rc, what)
+        return accepted, out

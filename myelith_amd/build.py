@@ -31,6 +31,9 @@ SOURCES = {  # source -> is HIP device code
     "moe.hip": True,
     "model_io.hip": True,
     "noalloc.hip": True,
+    "adapters.hip": True,
+    "prefix_attn.hip": True,
+    "verify.hip": True,
     "abi.cpp": False,
     "artifact.cpp": False,
 }

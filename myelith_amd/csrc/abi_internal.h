@@ -30,6 +30,32 @@ struct myl_ctx {
 
 namespace myl {
 
+// Makes the context's device current for a call and puts the caller's back.
+struct DeviceGuard {
+    int prev = -1;
+    explicit DeviceGuard(int device) {
+        if (hipGetDevice(&prev) != hipSuccess || prev == device) prev = -1;
+        else if (hipSetDevice(device) != hipSuccess) prev = -1;
+    }
+    ~DeviceGuard() {
+        if (prev >= 0) (void)hipSetDevice(prev);
+    }
+    DeviceGuard(const DeviceGuard&) = delete;
+    DeviceGuard& operator=(const DeviceGuard&) = delete;
+};
+
+// Pieces of a workspace the caller gave (256-byte steps); with base null, only the sizes are added up.
+struct Carve {
+    char* base;
+    size_t used = 0;
+    template <class T>
+    T* take(size_t n) {
+        const size_t off = used;
+        used += (n * sizeof(T) + 255) & ~(size_t)255;
+        return base ? reinterpret_cast<T*>(base + off) : nullptr;
+    }
+};
+
 inline bool fits_int(size_t v) { return v <= (size_t)INT32_MAX; }
 
 // Looks up, with `device` current, the device address of the scratch array of
