@@ -1,14 +1,34 @@
 // prefix_attn.hip -- integer attention (attention.rs:42-90 with
 // softmax.rs:12-64) of a batch whose sequences share a prefix of K/V rows and
 // continue with their own tails: myl_attention_prefix_dev.
+//
+// A probability p_j = RNE(e_j 2^f / S) needs the exact maximum and exp sum of
+// its whole row before it is rounded, so a row cannot be finished in one pass
+// with a running maximum; four launches follow one another:
+//   prefix_qk_kernel<MAX>  the maximum score of each vector (query head of a
+//                          row) over each range of keys
+//   prefix_qk_kernel<EXP>  the scores once more, e_j = exp_lut[(max - z_j) >> lut_shift]
+//                          as 16 bits, and the ranges' sums of them
+//   prefix_pv_kernel       p_j from e_j and S, sum p_j v_j over each range
+//   prefix_out_kernel      the sums over the ranges, rounded and clamped
+// The prefix is read once for 64 vectors of any rows: their tiles and the
+// tails' tiles (vectors of one sequence) run side by side in every launch.
 #include "abi_internal.h"
+#include "attn_fixed.h"
+#include "bufload.h"
 #include "gemm_mfma.h"
 #include "ops.h"
+#include "qk_planes.h"
+#include "serve_plan.h"
+#include "wave.h"
 
 #include <string>
 
 namespace myl {
 namespace {
+
+constexpr int kTile = kPrefixTile;  // vectors of a block
+constexpr int kSub = kTile / 16;    // 16-vector tiles of the matrix instructions
 
 // The call, as every kernel sees it.  Row r = seq * rows_per_seq + i attends
 // keys 0 .. P-1 of the prefix, then the first lens[r] of its sequence's tail.
@@ -17,105 +37,580 @@ struct PrefixAttn {
     const int32_t *slots, *lens;
     const int16_t* lut;
     int16_t* out;
+    int32_t *pmax, *psum, *pout;  // [range][pair], [range][pair], [range][pair][hd]; pair = row * heads + head
+    uint16_t* pexp;               // [pair][e]: prefix keys, then tail keys from pe on
     size_t ldq, ldo, ph, ts, th;  // strides in elements: q/out rows, prefix heads, tail slots, tail heads
     int64_t mult;
-    Divider n, G;  // rows per sequence, query heads per KV head
-    int R, heads, P, max_tail, n_slots, lcap;
-    uint32_t lut_len;
+    ScoreScale scale;
+    Divider n, G, tp, np, tt, nt, kvh;
+    int R, heads, P, max_tail, n_slots, vp_count, vt_count, np_count, nt_count, rp, rt, pe, e, blocks_p;
+    uint32_t pairs, lut_len;
     uint8_t shift, lut_shift, prob_frac;
 };
 
-// Tail positions of row r: -1 leaves the row out; a slot outside the cache has none.
-__device__ inline int quotient(const Divider& d, int n) {
+__device__ inline int divmod(const Divider& d, int n, int& rem) {
     uint32_t q, r;
     d.divmod((uint32_t)n, q, r);
+    rem = (int)r;
     return (int)q;
 }
-__device__ inline int slot_of(const PrefixAttn& a, int r) {
-    const int s = quotient(a.n, r);
-    return a.slots ? a.slots[s] : s;
+
+// The slot of sequence s, or -1; tail positions of row r (-1: left out).
+__device__ inline int slot_of(const PrefixAttn& a, int s) {
+    const int slot = a.slots ? a.slots[s] : s;
+    return slot < 0 || slot >= a.n_slots ? -1 : slot;
 }
-__device__ inline int tail_len(const PrefixAttn& a, int r) {
-    const int len = a.lens[r], slot = slot_of(a, r);
-    if (len < 0) return -1;
-    return slot < 0 || slot >= a.n_slots ? 0 : min(len, a.max_tail);
-}
-__device__ inline size_t tail_off(const PrefixAttn& a, int r, int g) {
-    return (size_t)slot_of(a, r) * a.ts + (size_t)g * a.th;
+__device__ inline int tail_of(const PrefixAttn& a, int r, int slot) {
+    const int len = a.lens[r];
+    return len < 0 ? -1 : (slot < 0 ? 0 : min(len, a.max_tail));
 }
 
-template <int HD>
-__global__ __launch_bounds__(256) void scores_kernel(PrefixAttn a, int32_t* __restrict__ z) {
-    const int j = blockIdx.x * 256 + threadIdx.x, h = blockIdx.y, r = blockIdx.z, g = quotient(a.G, h);
-    const int t = tail_len(a, r);
-    if (t < 0 || j >= a.P + t) return;
-    const int16_t* k = j < a.P ? a.kp + g * a.ph + (size_t)j * HD : a.kt + tail_off(a, r, g) + (size_t)(j - a.P) * HD;
-    const int16_t* q = a.q + (size_t)r * a.ldq + (size_t)h * HD;
-    int64_t dot = 0;
-    for (int d = 0; d < HD; ++d) dot += (int32_t)q[d] * (int32_t)k[d];
-    z[((size_t)r * a.heads + h) * a.lcap + j] = (int32_t)rshift_round64(wmul64(dot, a.mult), a.shift);
-}
-
-__device__ inline int32_t table(const PrefixAttn& a, int32_t below) {
-    return max(0, exp_lookup(below, a.lut, a.lut_len, a.lut_shift, (int32_t)a.lut[0]));
-}
-
-__global__ __launch_bounds__(256) void probs_kernel(PrefixAttn a, const int32_t* __restrict__ zs, int16_t* __restrict__ ps) {
-    __shared__ int32_t redm[4];
-    __shared__ uint32_t reds[4];
-    const int r = blockIdx.x, h = blockIdx.y, t = tail_len(a, r), L = a.P + t;
-    if (t < 0 || L == 0) return;
-    const int32_t* z = zs + ((size_t)r * a.heads + h) * a.lcap;
-    int16_t* p = ps + ((size_t)r * a.heads + h) * a.lcap;
-    int32_t mx = INT32_MIN;
-    for (int j = threadIdx.x; j < L; j += 256) mx = max(mx, z[j]);
-    mx = block_max_i32_dpp(mx, redm);
-    uint32_t s = 0;
-    for (int j = threadIdx.x; j < L; j += 256) s += (uint32_t)table(a, sat_sub32(mx, z[j]));
-    const int32_t S = (int32_t)block_sum_u32_dpp(s, reds);
-    const int32_t one = 1 << a.prob_frac;
-    if (S == 0) {  // the uniform split (softmax.rs:42-48)
-        uint32_t q, rem;
-        udivmod32((uint32_t)one, (uint32_t)L, recip32((uint32_t)L), &q, &rem);
-        for (int j = threadIdx.x; j < L; j += 256) p[j] = (int16_t)(q + ((uint32_t)j < rem ? 1 : 0));
-        return;
+// A block's part of the work.
+struct Part {
+    bool tail;
+    int g, v0, nv;         // KV head; first vector, vectors
+    int row0;              // row of vector 0 (of the batch or the sequence)
+    int range, j0, j1;     // range index among all, keys [j0, j1) of the prefix or the tail
+    int slot;
+    int subs;              // 16-vector tiles with a vector
+};
+// False: nothing to do.  Prefix blocks of one range follow one another on one XCD
+// (block b runs on XCD b % 8), so its L2 serves the range's K and V to all tiles.
+__device__ inline bool part_of(const PrefixAttn& a, Part& p) {
+    const int b = blockIdx.x;
+    p.tail = b >= a.blocks_p;
+    if (!p.tail) {
+        const int t = (b & 7) * (a.blocks_p >> 3) + (b >> 3);
+        int tile, rng;
+        const int q = divmod(a.tp, t, tile);
+        p.g = divmod(a.np, q, rng);
+        if (p.g >= (int)a.kvh.d) return false;
+        p.range = rng;
+        p.j0 = rng * a.rp;
+        p.j1 = min(a.P, p.j0 + a.rp);
+        p.v0 = tile * kTile;
+        p.nv = min(kTile, a.vp_count - p.v0);
+        p.row0 = 0;
+        p.slot = 0;
+    } else {
+        int tile, rng;
+        int q = divmod(a.tt, b - a.blocks_p, tile);
+        q = divmod(a.nt, q, rng);
+        const int s = divmod(a.kvh, q, p.g);
+        p.range = a.np_count + rng;
+        p.j0 = rng * a.rt;
+        p.j1 = min(a.max_tail, p.j0 + a.rt);
+        p.v0 = tile * kTile;
+        p.nv = min(kTile, a.vt_count - p.v0);
+        p.row0 = s * (int)a.n.d;
+        p.slot = __builtin_amdgcn_readfirstlane(slot_of(a, s));
+        if (p.slot < 0) return false;
     }
-    const uint32_t m = recip32_u32((uint32_t)S);
-    for (int j = threadIdx.x; j < L; j += 256) p[j] = (int16_t)softmax_div_round_pos(table(a, sat_sub32(mx, z[j])) << a.prob_frac, S, m);
+    p.subs = (p.nv + 15) >> 4;
+    return true;
 }
 
-template <int HD>
-__global__ __launch_bounds__(HD) void pv_kernel(PrefixAttn a, const int16_t* __restrict__ ps) {
-    const int r = blockIdx.x, h = blockIdx.y, g = quotient(a.G, h), d = threadIdx.x, t = tail_len(a, r);
-    int64_t s = 0;
-    if (t >= 0) {
-        const int16_t* p = ps + ((size_t)r * a.heads + h) * a.lcap;
-        for (int j = 0; j < a.P; ++j) s += (int32_t)p[j] * (int32_t)a.vp[g * a.ph + (size_t)j * HD + d];
-        if (t > 0) {
-            const int16_t* v = a.vt + tail_off(a, r, g);
-            for (int j = 0; j < t; ++j) s += (int32_t)p[a.P + j] * (int32_t)v[(size_t)j * HD + d];
+// Vector v of the tile: its row and query head.
+__device__ inline void vector_of(const PrefixAttn& a, const Part& p, int v, int& row, int& head) {
+    int h;
+    row = p.row0 + divmod(a.G, p.v0 + v, h);
+    head = p.g * (int)a.G.d + h;
+}
+
+__device__ inline const int16_t* keys_of(const PrefixAttn& a, const Part& p, const int16_t* prefix, const int16_t* tail) {
+    return uniform_ptr(p.tail ? tail + (size_t)p.slot * a.ts + (size_t)p.g * a.th : prefix + (size_t)p.g * a.ph);
+}
+
+__device__ inline int32_t sum_pairs(uint32_t w, int32_t acc) {
+    typedef short __attribute__((ext_vector_type(2))) s2;
+    return __builtin_amdgcn_sdot2(__builtin_bit_cast(s2, w), s2{1, 1}, acc, false);
+}
+// 8 int16 as their byte planes x = 256 hi + lo' + 128.
+__device__ inline void planes8(const uint4& x, uint32_t* h, uint32_t* l) {
+    h[0] = __builtin_amdgcn_perm(x.y, x.x, 0x07050301u);
+    h[1] = __builtin_amdgcn_perm(x.w, x.z, 0x07050301u);
+    l[0] = __builtin_amdgcn_perm(x.y, x.x, 0x06040200u) ^ 0x80808080u;
+    l[1] = __builtin_amdgcn_perm(x.w, x.z, 0x06040200u) ^ 0x80808080u;
+}
+// 16 dimensions (two 16-byte loads) as matrix operands.
+__device__ inline void planes16(const uint4 (&x)[2], v4i32_t& h, v4i32_t& l) {
+    uint32_t hw[4], lw[4];
+    planes8(x[0], hw, lw);
+    planes8(x[1], hw + 2, lw + 2);
+    h = v4i32_t{(int)hw[0], (int)hw[1], (int)hw[2], (int)hw[3]};
+    l = v4i32_t{(int)lw[0], (int)lw[1], (int)lw[2], (int)lw[3]};
+}
+
+__device__ inline void block_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
+
+// Over the four 16-lane rows of a wave.
+__device__ inline int32_t quarters_sum(int32_t v) {
+    v += __shfl_xor(v, 16, 64);
+    return v + __shfl_xor(v, 32, 64);
+}
+__device__ inline int32_t quarters_max(int32_t v) {
+    v = max(v, __shfl_xor(v, 16, 64));
+    return max(v, __shfl_xor(v, 32, 64));
+}
+
+enum Pass { kMaxPass, kExpPass };
+
+// Scores of a tile's vectors with a range's keys on v_mfma_i32_16x16x64_i8: K
+// positions are rows, vectors columns, so lane l holds vector l % 16 of each 16-vector
+// tile and positions 4 (l / 16) .. + 3 of its wave's 16-position group.  With byte
+// planes x = 256 hi + lo' + 128 of both operands
+//   q.k = 65536 hh + 256 (hl + lh + 128 sum k_hi) + ll + 128 sum k_lo' + 128 sum q
+// where the sums over k come from the matrix cores too (a B operand of 64s, doubled)
+// and start the accumulators, and sum q is one value per lane.  As 256 u + r the score
+// takes 32-bit steps (ScoreScale); other scales take the 64-bit form (FAST false).
+template <int HD, bool FAST, Pass PASS>
+__global__ __launch_bounds__(256, 2) void prefix_qk_kernel(PrefixAttn a) {
+    constexpr int NS = HD / 64;
+    extern __shared__ uint16_t tab[];  // kExpPass: the table and a 0
+    __shared__ int32_t red[4][kTile], s_max[kTile];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, c = lane & 15, kb = lane >> 4;
+    Part p;
+    if (!part_of(a, p)) return;
+    // the lane's vectors
+    uint32_t pair[kSub];
+    int lim[kSub];  // keys of this part that the vector attends
+    v4i32_t qh[kSub][NS], ql[kSub][NS];
+    int32_t qsum[kSub];
+    int lmax = 0, lmin = 0x7FFFFFFF;
+#pragma unroll
+    for (int t = 0; t < kSub; ++t) {
+        pair[t] = 0;
+        lim[t] = 0;
+        qsum[t] = 0;
+#pragma unroll
+        for (int s = 0; s < NS; ++s) qh[t][s] = ql[t][s] = v4i32_t{0, 0, 0, 0};
+        if (t < p.subs) {
+            const int v = 16 * t + c;
+            if (v < p.nv) {
+                int row, head;
+                vector_of(a, p, v, row, head);
+                pair[t] = (uint32_t)row * (uint32_t)a.heads + (uint32_t)head;
+                lim[t] = p.tail ? max(0, tail_of(a, row, p.slot)) : a.P;
+                lmax = max(lmax, lim[t]);
+                lmin = min(lmin, lim[t]);
+                const int16_t* qv = a.q + (size_t)row * a.ldq + (size_t)head * HD + 16 * kb;
+#pragma unroll
+                for (int s = 0; s < NS; ++s) {
+                    const uint4 x[2] = {*reinterpret_cast<const uint4*>(qv + 64 * s), *reinterpret_cast<const uint4*>(qv + 64 * s + 8)};
+                    planes16(x, qh[t][s], ql[t][s]);
+                    const uint32_t w[8] = {x[0].x, x[0].y, x[0].z, x[0].w, x[1].x, x[1].y, x[1].z, x[1].w};
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) qsum[t] = sum_pairs(w[i], qsum[t]);
+                }
+            }
+            qsum[t] = 128 * quarters_sum(qsum[t]);
         }
     }
-    a.out[(size_t)r * a.ldo + (size_t)h * HD + d] = clamp_i16_i64(rshift_round64(s, a.prob_frac));
+    lmax = wave_max_i32(lmax);
+    lmin = ~wave_max_i32(~lmin);
+    const int j1 = min(p.j1, lmax);  // uniform over the block: every wave holds every vector
+    if (p.j0 >= j1) return;
+    int32_t m[kSub];
+    if (PASS == kExpPass) {
+        for (uint32_t i = tid; i <= a.lut_len; i += 256) tab[i] = i < a.lut_len ? (uint16_t)max(0, (int32_t)a.lut[i]) : 0;
+        // the maxima of all ranges, four threads per vector
+        const int v = tid & (kTile - 1), share = tid / kTile;
+        int32_t mx = INT32_MIN;
+        if (v < p.nv) {
+            int row, head, rem;
+            vector_of(a, p, v, row, head);
+            const uint32_t pr = (uint32_t)row * (uint32_t)a.heads + (uint32_t)head;
+            const int seq = divmod(a.n, row, rem);
+            const int tail = a.nt_count ? tail_of(a, row, p.tail ? p.slot : slot_of(a, seq)) : 0;
+            for (int i = share; i < a.np_count; i += 4) mx = max(mx, a.pmax[(size_t)i * a.pairs + pr]);
+            for (int i = share; i < a.nt_count && i * a.rt < tail; i += 4)
+                mx = max(mx, a.pmax[(size_t)(a.np_count + i) * a.pairs + pr]);
+        }
+        red[share][v] = mx;
+        __syncthreads();
+        if (tid < kTile) s_max[tid] = max(max(red[0][tid], red[1][tid]), max(red[2][tid], red[3][tid]));
+        __syncthreads();
+#pragma unroll
+        for (int t = 0; t < kSub; ++t) m[t] = s_max[16 * t + c];
+    }
+    const int16_t* kg = keys_of(a, p, a.kp, a.kt);
+    const __amdgpu_buffer_rsrc_t rk = weight_rsrc(kg, (uint32_t)(p.tail ? a.max_tail : a.P) * HD * 2u);
+    // kMaxPass: the largest dot as (u, r), or the largest score; kExpPass: the sum
+    int32_t best[kSub], low[kSub];
+#pragma unroll
+    for (int t = 0; t < kSub; ++t) {
+        best[t] = PASS == kMaxPass ? INT32_MIN : 0;
+        low[t] = 0;
+    }
+    const v4i32_t sixty4 = {0x40404040, 0x40404040, 0x40404040, 0x40404040}, zero = {0, 0, 0, 0};
+    uint4 kx[NS][2];
+    auto load = [&](int j) {
+#pragma unroll
+        for (int s = 0; s < NS; ++s)
+#pragma unroll
+            for (int i = 0; i < 2; ++i) kx[s][i] = cload16(rk, ((uint32_t)(j + c) * HD + 64u * s + 16u * kb + 8u * i) * 2u);
+    };
+    load(p.j0 + 16 * wave);
+    for (int j = p.j0 + 16 * wave; j < j1; j += 64) {
+        v4i32_t kh[NS], kl[NS];
+#pragma unroll
+        for (int s = 0; s < NS; ++s) planes16(kx[s], kh[s], kl[s]);
+        load(j + 64);
+        v4i32_t mid0 = zero, ll0 = zero;
+#pragma unroll
+        for (int s = 0; s < NS; ++s) {
+            mid0 = __builtin_amdgcn_mfma_i32_16x16x64_i8(kh[s], sixty4, mid0, 0, 0, 0);
+            ll0 = __builtin_amdgcn_mfma_i32_16x16x64_i8(kl[s], sixty4, ll0, 0, 0, 0);
+        }
+        mid0 += mid0;
+        ll0 += ll0;
+        const bool whole = j + 16 <= lmin;
+#pragma unroll
+        for (int t = 0; t < kSub; ++t) {
+            if (t >= p.subs) break;
+            v4i32_t hh = zero, mid = mid0, ll = ll0;
+#pragma unroll
+            for (int s = 0; s < NS; ++s) {
+                hh = __builtin_amdgcn_mfma_i32_16x16x64_i8(kh[s], qh[t][s], hh, 0, 0, 0);
+                mid = __builtin_amdgcn_mfma_i32_16x16x64_i8(kh[s], ql[t][s], mid, 0, 0, 0);
+                mid = __builtin_amdgcn_mfma_i32_16x16x64_i8(kl[s], qh[t][s], mid, 0, 0, 0);
+                ll = __builtin_amdgcn_mfma_i32_16x16x64_i8(kl[s], ql[t][s], ll, 0, 0, 0);
+            }
+            uint32_t ev[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int32_t lo = ll[i] + qsum[t];
+                const int32_t u = 256 * hh[i] + mid[i] + (lo >> 8);
+                const uint32_t r = (uint32_t)lo & 255u;
+                const bool ok = whole || j + 4 * kb + i < lim[t];
+                if (PASS == kMaxPass) {
+                    if (FAST) {
+                        const bool up = ok && (u > best[t] || (u == best[t] && (int32_t)r > low[t]));
+                        best[t] = up ? u : best[t];
+                        low[t] = up ? (int32_t)r : low[t];
+                    } else {
+                        const int64_t dot = 256 * (int64_t)u + (int64_t)r;
+                        const int32_t z = (int32_t)rshift_round64(wmul64(dot, a.mult), a.shift);
+                        best[t] = ok ? max(best[t], z) : best[t];
+                    }
+                } else {
+                    const int32_t z = FAST ? a.scale(u, r)
+                                           : (int32_t)rshift_round64(wmul64(256 * (int64_t)u + (int64_t)r, a.mult), a.shift);
+                    // sat_sub and the lookup of softmax.rs:12-38; the table ends with a 0
+                    const uint32_t below = min((uint32_t)m[t] - (uint32_t)z, 0x7FFFFFFFu);
+                    uint32_t e = tab[min(below >> (a.lut_shift & 31u), a.lut_len)];
+                    ev[i] = ok ? e : 0u;
+                    best[t] += (int32_t)ev[i];
+                }
+            }
+            if (PASS == kExpPass && 16 * t + c < p.nv) {
+                uint16_t* o = a.pexp + (size_t)pair[t] * a.e + (p.tail ? a.pe : 0) + j + 4 * kb;
+                *reinterpret_cast<uint2*>(o) = make_uint2(ev[0] | (ev[1] << 16), ev[2] | (ev[3] << 16));
+            }
+        }
+    }
+    // the block's value per vector
+    __syncthreads();
+#pragma unroll
+    for (int t = 0; t < kSub; ++t) {
+        int32_t v = best[t];
+        if (PASS == kMaxPass) {
+            if (FAST) v = best[t] == INT32_MIN ? INT32_MIN : a.scale(best[t], (uint32_t)low[t]);
+            v = quarters_max(v);
+        } else {
+            v = quarters_sum(v);
+        }
+        if (kb == 0) red[wave][16 * t + c] = v;
+    }
+    __syncthreads();
+    if (tid < p.nv) {
+        int row, head;
+        vector_of(a, p, tid, row, head);
+        const size_t o = (size_t)p.range * a.pairs + (uint32_t)row * (uint32_t)a.heads + (uint32_t)head;
+        const int32_t r0 = red[0][tid], r1 = red[1][tid], r2 = red[2][tid], r3 = red[3][tid];
+        if (PASS == kMaxPass) a.pmax[o] = max(max(r0, r1), max(r2, r3));
+        else a.psum[o] = r0 + r1 + r2 + r3;
+    }
 }
 
-// At most 65536 keys per row: with non-negative table entries the exp sums stay
-// below 2^31.
-constexpr size_t kMaxKeys = 65536;
-
-struct Space {
-    int32_t* z;
-    int16_t* p;
-    size_t bytes;
-    static Space of(void* base, size_t R, size_t heads, size_t keys) {
-        Carve c{(char*)base};
-        Space s;
-        s.z = c.take<int32_t>(R * heads * keys);
-        s.p = c.take<int16_t>(R * heads * keys);
-        s.bytes = c.used ? c.used : 256;  // 0 stands for sizes that a call refuses
-        return s;
-    }
+// What a vector's probabilities need.
+struct ProbRow {
+    ProbDiv div;
+    uint32_t base, extra;  // S = 0: the uniform split (softmax.rs:42-48), 1 more for keys below `extra`
+    int32_t lim, uniform;
+    uint32_t pair;
+    int32_t pad;
 };
+
+// sum p_j v_j of a tile's vectors over a range, HD dimensions: the dimensions are the
+// rows of v_mfma_i32_16x16x64_i8, the vectors its columns.  A step covers 64 keys per
+// key wave.  p <= 2^14 splits into two signed bytes exactly (p = 256 ph + pl), v into
+// v = 256 vh + vl' + 128, so
+//   sum p v = 65536 hh + 256 (hl + lh) + ll + 128 sum p
+// modulo 2^32, and the whole sum fits 32 bits (serve_plan.h).  V is turned in registers:
+// lane l loads dimensions 2 (l % 16), + 1 of the 16 keys of its block l / 16 and
+// gathers each dimension's bytes of four keys with v_perm, which is the A operand.
+template <int HD>
+struct PvShape {
+    static constexpr int DW = HD / 32;  // waves side by side over the dimensions
+    static constexpr int KW = 4 / DW;   // over the keys
+};
+
+template <int HD, int SUB, int KU>
+struct PvLds {
+    static constexpr int kKeys = 64 * PvShape<HD>::KW * KU;  // keys of a step
+    static constexpr int kChunks = kKeys / 16;
+    static constexpr int kRow = 16 * SUB * 16 + 64;          // bytes of a 16-key chunk of all vectors; 64 spread the banks
+    static constexpr int kPlane = kChunks * kRow;
+    static constexpr int kBytes = 4 * kPlane;                // two planes, two steps
+};
+
+template <int HD, int SUB, int KU>
+__device__ inline void prefix_pv_part(const PrefixAttn& a, const Part& p, int8_t* lds, ProbRow* rows, int32_t* p_sum, int j1) {
+    using L = PvLds<HD, SUB, KU>;
+    constexpr int DW = PvShape<HD>::DW, KW = PvShape<HD>::KW, CH = L::kChunks;
+    constexpr int ITEMS = (16 * SUB * CH + 255) / 256;
+    const int tid = threadIdx.x, lane = tid & 63, c = lane & 15, kb = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), dw = wave % DW, kw = wave / DW;
+    const int16_t* vg = keys_of(a, p, a.vp, a.vt);
+    const __amdgpu_buffer_rsrc_t rv = weight_rsrc(vg, (uint32_t)(p.tail ? a.max_tail : a.P) * HD * 2u);
+    v4i32_t hh[SUB][2], mid[SUB][2], ll[SUB][2];
+#pragma unroll
+    for (int t = 0; t < SUB; ++t)
+#pragma unroll
+        for (int d = 0; d < 2; ++d) hh[t][d] = mid[t][d] = ll[t][d] = v4i32_t{0, 0, 0, 0};
+    int32_t psum[ITEMS];
+#pragma unroll
+    for (int i = 0; i < ITEMS; ++i) psum[i] = 0;
+    uint4 ex[ITEMS][2];
+    uint32_t vx[KU][16];
+    const int koff = p.tail ? a.pe : 0, kfirst = p.tail ? a.P : 0;
+    auto load = [&](int j) {
+#pragma unroll
+        for (int i = 0; i < ITEMS; ++i) {
+            const int it = tid + 256 * i, v = it / CH, jc = j + 16 * (it % CH);
+            ex[i][0] = ex[i][1] = make_uint4(0, 0, 0, 0);
+            if (v < p.nv && jc < min(rows[v].lim, j1)) {
+                const uint4* e = reinterpret_cast<const uint4*>(a.pexp + (size_t)rows[v].pair * a.e + koff + jc);
+                ex[i][0] = e[0];
+                ex[i][1] = e[1];
+            }
+        }
+#pragma unroll
+        for (int k = 0; k < KU; ++k)
+#pragma unroll
+            for (int i = 0; i < 16; ++i)
+                vx[k][i] = cload4(rv, ((uint32_t)(j + 64 * (k * KW + kw) + 16 * kb + i) * HD + 32u * dw + 2u * c) * 2u);
+    };
+    load(p.j0);
+    int buf = 0;
+    for (int j = p.j0; j < j1; j += L::kKeys, buf ^= 1) {
+        int8_t* ph = lds + buf * 2 * L::kPlane;
+        int8_t* pl = ph + L::kPlane;
+#pragma unroll
+        for (int i = 0; i < ITEMS; ++i) {
+            const int it = tid + 256 * i, v = it / CH, ch = it % CH;
+            if (it >= 16 * SUB * CH) break;
+            const uint32_t w[8] = {ex[i][0].x, ex[i][0].y, ex[i][0].z, ex[i][0].w, ex[i][1].x, ex[i][1].y, ex[i][1].z, ex[i][1].w};
+            uint32_t pw[8];
+            if (v >= p.nv || !rows[v].uniform) {
+                const ProbDiv div = rows[v].div;
+#pragma unroll
+                for (int k = 0; k < 8; ++k) pw[k] = div(w[k] & 0xFFFFu) | (div(w[k] >> 16) << 16);
+            } else {
+                const int jc = j + 16 * ch, lim = min(rows[v].lim, j1);
+#pragma unroll
+                for (int k = 0; k < 8; ++k) {
+                    uint32_t two = 0;
+#pragma unroll
+                    for (int b = 0; b < 2; ++b)
+                        if (jc + 2 * k + b < lim)
+                            two |= (rows[v].base + ((uint32_t)(kfirst + jc + 2 * k + b) < rows[v].extra ? 1u : 0u)) << (16 * b);
+                    pw[k] = two;
+                }
+            }
+            uint32_t hw[4], lw[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                psum[i] = sum_pairs(pw[2 * k], psum[i]);
+                psum[i] = sum_pairs(pw[2 * k + 1], psum[i]);
+                // pl = p as a signed byte, ph = (p - pl) / 256: 128 carries into the high byte
+                lw[k] = __builtin_amdgcn_perm(pw[2 * k + 1], pw[2 * k], 0x06040200u);
+                hw[k] = __builtin_amdgcn_perm(pw[2 * k + 1] + 0x00800080u, pw[2 * k] + 0x00800080u, 0x07050301u);
+            }
+            *reinterpret_cast<uint4*>(ph + ch * L::kRow + v * 16) = make_uint4(hw[0], hw[1], hw[2], hw[3]);
+            *reinterpret_cast<uint4*>(pl + ch * L::kRow + v * 16) = make_uint4(lw[0], lw[1], lw[2], lw[3]);
+        }
+        v4i32_t vh[KU][2], vl[KU][2];
+#pragma unroll
+        for (int k = 0; k < KU; ++k)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const uint32_t* x = vx[k] + 4 * i;
+                // bytes of two dimensions at four keys: low, high of the first, low, high of the second
+                const uint32_t a0 = __builtin_amdgcn_perm(x[1], x[0], 0x05010400u), a1 = __builtin_amdgcn_perm(x[3], x[2], 0x05010400u);
+                const uint32_t b0 = __builtin_amdgcn_perm(x[1], x[0], 0x07030602u), b1 = __builtin_amdgcn_perm(x[3], x[2], 0x07030602u);
+                vl[k][0][i] = (int)(__builtin_amdgcn_perm(a1, a0, 0x05040100u) ^ 0x80808080u);
+                vh[k][0][i] = (int)__builtin_amdgcn_perm(a1, a0, 0x07060302u);
+                vl[k][1][i] = (int)(__builtin_amdgcn_perm(b1, b0, 0x05040100u) ^ 0x80808080u);
+                vh[k][1][i] = (int)__builtin_amdgcn_perm(b1, b0, 0x07060302u);
+            }
+        load(j + L::kKeys);
+        block_barrier();
+#pragma unroll
+        for (int k = 0; k < KU; ++k)
+#pragma unroll
+            for (int t = 0; t < SUB; ++t) {
+                if (t >= p.subs) break;
+                const int off = (4 * (k * KW + kw) + kb) * L::kRow + (16 * t + c) * 16;
+                const v4i32_t bh = *reinterpret_cast<const v4i32_t*>(ph + off), bl = *reinterpret_cast<const v4i32_t*>(pl + off);
+#pragma unroll
+                for (int d = 0; d < 2; ++d) {
+                    hh[t][d] = __builtin_amdgcn_mfma_i32_16x16x64_i8(vh[k][d], bh, hh[t][d], 0, 0, 0);
+                    mid[t][d] = __builtin_amdgcn_mfma_i32_16x16x64_i8(vh[k][d], bl, mid[t][d], 0, 0, 0);
+                    mid[t][d] = __builtin_amdgcn_mfma_i32_16x16x64_i8(vl[k][d], bh, mid[t][d], 0, 0, 0);
+                    ll[t][d] = __builtin_amdgcn_mfma_i32_16x16x64_i8(vl[k][d], bl, ll[t][d], 0, 0, 0);
+                }
+            }
+    }
+#pragma unroll
+    for (int i = 0; i < ITEMS; ++i) {
+        const int it = tid + 256 * i;
+        if (it < 16 * SUB * CH) atomicAdd(&p_sum[it / CH], psum[i]);
+    }
+    __syncthreads();
+    // the key waves' sums meet in LDS (in place of the P planes)
+    int32_t* sums = reinterpret_cast<int32_t*>(lds);  // [vector][HD + 4]
+    constexpr int SROW = HD + 4;
+    static_assert(KW == 1 || 16 * SUB * SROW * 4 <= L::kBytes, "the sums fit the planes' place");
+    uint32_t o[SUB][8];
+#pragma unroll
+    for (int t = 0; t < SUB; ++t)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+#pragma unroll
+            for (int d = 0; d < 2; ++d)
+                o[t][2 * i + d] = ((uint32_t)hh[t][d][i] << 16) + ((uint32_t)mid[t][d][i] << 8) + (uint32_t)ll[t][d][i];
+    const int d0 = 32 * dw + 8 * kb;
+    if (KW == 2) {
+        if (kw == 1)
+#pragma unroll
+            for (int t = 0; t < SUB; ++t)
+#pragma unroll
+                for (int h = 0; h < 2; ++h)
+                    *reinterpret_cast<uint4*>(sums + (16 * t + c) * SROW + d0 + 4 * h) =
+                        make_uint4(o[t][4 * h], o[t][4 * h + 1], o[t][4 * h + 2], o[t][4 * h + 3]);
+        __syncthreads();
+        if (kw == 1) return;
+#pragma unroll
+        for (int t = 0; t < SUB; ++t)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) o[t][i] += (uint32_t)sums[(16 * t + c) * SROW + d0 + i];
+    }
+#pragma unroll
+    for (int t = 0; t < SUB; ++t) {
+        const int v = 16 * t + c;
+        if (v >= p.nv) continue;
+        const uint32_t add = 128u * (uint32_t)p_sum[v];
+        int32_t* dst = a.pout + ((size_t)p.range * a.pairs + rows[v].pair) * HD + d0;
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+            *reinterpret_cast<uint4*>(dst + 4 * h) = make_uint4(o[t][4 * h] + add, o[t][4 * h + 1] + add, o[t][4 * h + 2] + add, o[t][4 * h + 3] + add);
+    }
+}
+
+template <int HD>
+__global__ __launch_bounds__(256, 2) void prefix_pv_kernel(PrefixAttn a) {
+    constexpr int kLds = PvLds<HD, kSub, 1>::kBytes > PvLds<HD, 1, 4>::kBytes ? PvLds<HD, kSub, 1>::kBytes : PvLds<HD, 1, 4>::kBytes;
+    __shared__ __align__(16) int8_t lds[kLds];
+    __shared__ __align__(16) ProbRow rows[kTile];
+    __shared__ int32_t red[4][kTile], p_sum[kTile];
+    const int tid = threadIdx.x;
+    Part p;
+    if (!part_of(a, p)) return;
+    const int v = tid & (kTile - 1), share = tid / kTile;
+    uint32_t pair = 0, s = 0;
+    int tail = 0, lim = 0;
+    if (v < p.nv) {
+        int row, head, rem;
+        vector_of(a, p, v, row, head);
+        pair = (uint32_t)row * (uint32_t)a.heads + (uint32_t)head;
+        const int seq = divmod(a.n, row, rem);
+        tail = a.nt_count || p.tail ? tail_of(a, row, p.tail ? p.slot : slot_of(a, seq)) : 0;
+        lim = p.tail ? max(tail, 0) : a.P;
+    }
+    const int lmax = wave_max_i32(lim);
+    if (p.j0 >= lmax) return;  // uniform: every wave's lanes hold all vectors
+    if (v < p.nv) {
+        for (int i = share; i < a.np_count; i += 4) s += (uint32_t)a.psum[(size_t)i * a.pairs + pair];
+        for (int i = share; i < a.nt_count && i * a.rt < tail; i += 4)
+            s += (uint32_t)a.psum[(size_t)(a.np_count + i) * a.pairs + pair];
+    }
+    red[share][v] = (int32_t)s;
+    __syncthreads();
+    if (tid < kTile) {
+        const uint32_t S = (uint32_t)(red[0][tid] + red[1][tid] + red[2][tid] + red[3][tid]);
+        ProbRow r{};
+        r.div = ProbDiv::of(S ? S : 1u, a.prob_frac);
+        r.lim = lim;
+        r.pair = pair;
+        r.uniform = S == 0 ? 1 : 0;
+        const uint32_t keys = (uint32_t)(a.P + max(tail, 0)), one = 1u << a.prob_frac;
+        if (S == 0 && keys) udivmod32(one, keys, recip32(keys), &r.base, &r.extra);
+        rows[tid] = r;
+        p_sum[tid] = 0;
+    }
+    __syncthreads();
+    const int j1 = min(p.j1, lmax);
+    if (p.subs == 1) prefix_pv_part<HD, 1, 4>(a, p, lds, rows, p_sum, j1);
+    else prefix_pv_part<HD, kSub, 1>(a, p, lds, rows, p_sum, j1);
+}
+
+// The ranges' sums, one rounding (attention.rs:84-86); four dimensions per thread.
+template <int HD>
+__global__ __launch_bounds__(256) void prefix_out_kernel(PrefixAttn a) {
+    const int row = blockIdx.y, i = 4 * (blockIdx.x * 256 + (int)threadIdx.x);
+    if (i >= a.heads * HD) return;
+    int rem;
+    const int seq = divmod(a.n, row, rem), tail = tail_of(a, row, slot_of(a, seq));
+    uint32_t s[4] = {0, 0, 0, 0};
+    auto add = [&](int range) {
+        const uint4 x = *reinterpret_cast<const uint4*>(a.pout + ((size_t)range * a.pairs + (size_t)row * a.heads) * HD + i);
+        s[0] += x.x;
+        s[1] += x.y;
+        s[2] += x.z;
+        s[3] += x.w;
+    };
+    if (tail >= 0) {
+#pragma unroll 8
+        for (int r = 0; r < a.np_count; ++r) add(r);
+#pragma unroll 4
+        for (int r = 0; r < a.nt_count; ++r)
+            if (r * a.rt < tail) add(a.np_count + r);
+    }
+    uint32_t y[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) y[k] = (uint32_t)(uint16_t)clamp_i16(rshift_round32((int32_t)s[k], a.prob_frac));
+    *reinterpret_cast<uint2*>(a.out + (size_t)row * a.ldo + i) = make_uint2(y[0] | (y[1] << 16), y[2] | (y[3] << 16));
+}
+
+template <int HD>
+hipError_t prefix_launch(const PrefixAttn& a, const PrefixPlan& pl, hipStream_t st) {
+    const unsigned grid = (unsigned)(pl.blocks_p + pl.blocks_t);
+    if (grid) {
+        const size_t tab = ((size_t)a.lut_len + 1) * 2;
+        if (a.scale.fast) {
+            prefix_qk_kernel<HD, true, kMaxPass><<<grid, 256, 0, st>>>(a);
+            prefix_qk_kernel<HD, true, kExpPass><<<grid, 256, tab, st>>>(a);
+        } else {
+            prefix_qk_kernel<HD, false, kMaxPass><<<grid, 256, 0, st>>>(a);
+            prefix_qk_kernel<HD, false, kExpPass><<<grid, 256, tab, st>>>(a);
+        }
+        prefix_pv_kernel<HD><<<grid, 256, 0, st>>>(a);
+    }
+    prefix_out_kernel<HD><<<dim3((unsigned)((a.heads * HD + 1023) / 1024), (unsigned)a.R), 256, 0, st>>>(a);
+    return hipGetLastError();
+}
 
 }  // namespace
 }  // namespace myl
@@ -126,11 +621,9 @@ extern "C" {
 
 size_t myl_attention_prefix_workspace(const myl_ctx* ctx, size_t n_seqs, size_t rows_per_seq, size_t heads, size_t kv_heads,
                                       size_t head_dim, size_t prefix_len, size_t max_tail) {
-    if (!ctx || !fits_int(n_seqs) || !fits_int(rows_per_seq) || !fits_int(n_seqs * rows_per_seq) ||
-        (head_dim != 64 && head_dim != 128) || kv_heads == 0 || heads % kv_heads || heads > 65535 ||
-        prefix_len > kMaxKeys || max_tail > kMaxKeys - prefix_len)
-        return 0;
-    return Space::of(nullptr, n_seqs * rows_per_seq, heads, prefix_len + max_tail).bytes;
+    const PrefixShape s{n_seqs, rows_per_seq, heads, kv_heads, head_dim, prefix_len, max_tail};
+    if (!ctx || prefix_refuse(s) || (head_dim != 64 && head_dim != 128)) return 0;
+    return prefix_plan(s, ctx->prop.multiProcessorCount).bytes;
 }
 
 int myl_attention_prefix_dev(myl_ctx* ctx, const int16_t* q, size_t n_seqs, size_t rows_per_seq, size_t ldq, size_t heads,
@@ -144,46 +637,45 @@ int myl_attention_prefix_dev(myl_ctx* ctx, const int16_t* q, size_t n_seqs, size
     const char* what = "attention_prefix_dev";
     auto bad = [&](const char* why) { return ctx->fail(MYL_E_INVALID, std::string(what) + ": " + why); };
     if (head_dim != 64 && head_dim != 128) return ctx->fail(MYL_E_UNSUPPORTED, std::string(what) + ": head_dim 64 or 128");
-    if (kv_heads == 0 || heads == 0 || heads % kv_heads) return bad("heads must be a multiple of kv_heads");
-    if (heads > 65535 || !fits_int(n_seqs) || !fits_int(rows_per_seq) || n_seqs * rows_per_seq > 65535)
-        return bad("too many rows or heads (65535 each)");
-    if (prefix_len > kMaxKeys || max_tail > kMaxKeys - prefix_len) return bad("more than 65536 keys per row");
+    const PrefixShape s{n_seqs, rows_per_seq, heads, kv_heads, head_dim, prefix_len, max_tail};
+    if (const char* why = prefix_refuse(s)) return bad(why);
     if (ldq < heads * head_dim || ldo < heads * head_dim) return bad("leading dimension too small");
-    if (prefix_len && prefix_head_stride < prefix_len * head_dim && kv_heads > 1) return bad("prefix head stride too small");
-    if (max_tail && (tail_head_stride < max_tail * head_dim && kv_heads > 1)) return bad("tail head stride too small");
-    if (!fits_int(n_slots)) return bad("too many slots");
-    if (lut_len == 0 || !fits_int(lut_len)) return bad("the exp table must hold 1 to 2^31 - 1 entries");
+    if (kv_heads > 1 && (prefix_head_stride < prefix_len * head_dim || tail_head_stride < max_tail * head_dim))
+        return bad("head stride too small");
+    if (n_slots > kInt) return bad("too many slots");
+    if (lut_len == 0 || lut_len > kPrefixMaxLut) return bad("the exp table must hold 1 to 32768 entries");
     if (prob_frac > 14) return bad("prob_frac is at most 14");
     if (n_seqs == 0 || rows_per_seq == 0) return MYL_OK;
     if (!q || !out || !exp_lut || !lens) return bad("null operand");
     if (prefix_len && (!k_prefix || !v_prefix)) return bad("null prefix");
-    if (max_tail && (!k_tail || !v_tail)) return bad("null tail");
+    if (max_tail && n_slots && (!k_tail || !v_tail)) return bad("null tail");
     const uintptr_t ptrs = (uintptr_t)q | (uintptr_t)out | (uintptr_t)k_prefix | (uintptr_t)v_prefix | (uintptr_t)k_tail |
                            (uintptr_t)v_tail | (uintptr_t)workspace;
     if ((ptrs & 15) || ((ldq | ldo | prefix_head_stride | tail_slot_stride | tail_head_stride) & 7))
         return bad("operands must be 16-byte aligned, strides multiples of 8");
-    const size_t R = n_seqs * rows_per_seq;
-    const Space s = Space::of(workspace, R, heads, prefix_len + max_tail);
-    if (!workspace || workspace_bytes < s.bytes) return bad("workspace too small (myl_attention_prefix_workspace)");
+    const PrefixPlan pl = prefix_plan(s, ctx->prop.multiProcessorCount);
+    if (!workspace || workspace_bytes < pl.bytes) return bad("workspace too small (myl_attention_prefix_workspace)");
     const DeviceGuard guard(ctx->device);
-    const hipStream_t st = ctx->stream;
+    char* ws = static_cast<char*>(workspace);
     PrefixAttn a{};
     a.q = q; a.kp = k_prefix; a.vp = v_prefix; a.kt = k_tail; a.vt = v_tail;
     a.slots = slots; a.lens = lens; a.lut = exp_lut; a.out = out;
+    a.pmax = reinterpret_cast<int32_t*>(ws + pl.off_max);
+    a.psum = reinterpret_cast<int32_t*>(ws + pl.off_sum);
+    a.pexp = reinterpret_cast<uint16_t*>(ws + pl.off_exp);
+    a.pout = reinterpret_cast<int32_t*>(ws + pl.off_out);
     a.ldq = ldq; a.ldo = ldo; a.ph = prefix_head_stride; a.ts = tail_slot_stride; a.th = tail_head_stride;
-    a.mult = score_mult; a.R = (int)R; a.n = Divider::of((uint32_t)rows_per_seq); a.heads = (int)heads;
-    a.G = Divider::of((uint32_t)(heads / kv_heads));
-    a.P = (int)prefix_len; a.max_tail = (int)max_tail; a.n_slots = (int)n_slots; a.lcap = (int)(prefix_len + max_tail);
-    a.lut_len = (uint32_t)lut_len; a.shift = score_shift; a.lut_shift = lut_shift; a.prob_frac = prob_frac;
-    if (a.lcap > 0) {
-        const dim3 sg((unsigned)((a.lcap + 255) / 256), (unsigned)heads, (unsigned)R);
-        if (head_dim == 128) scores_kernel<128><<<sg, 256, 0, st>>>(a, s.z);
-        else scores_kernel<64><<<sg, 256, 0, st>>>(a, s.z);
-        probs_kernel<<<dim3((unsigned)R, (unsigned)heads), 256, 0, st>>>(a, s.z, s.p);
-    }
-    if (head_dim == 128) pv_kernel<128><<<dim3((unsigned)R, (unsigned)heads), 128, 0, st>>>(a, s.p);
-    else pv_kernel<64><<<dim3((unsigned)R, (unsigned)heads), 64, 0, st>>>(a, s.p);
-    return ctx->hip(hipGetLastError(), what);
+    a.mult = score_mult;
+    a.scale = ScoreScale::of(score_mult, score_shift, (int)head_dim);
+    auto div = [](size_t d) { return Divider::of((uint32_t)std::max<size_t>(d, 1)); };
+    a.n = div(rows_per_seq); a.G = div((size_t)pl.G); a.kvh = div(kv_heads);
+    a.tp = div((size_t)pl.tp); a.np = div((size_t)pl.np); a.tt = div((size_t)pl.tt); a.nt = div((size_t)pl.nt);
+    a.R = (int)(n_seqs * rows_per_seq); a.heads = (int)heads; a.P = (int)prefix_len; a.max_tail = (int)max_tail;
+    a.n_slots = (int)n_slots; a.vp_count = pl.vp; a.vt_count = pl.vt; a.np_count = pl.np; a.nt_count = pl.nt;
+    a.rp = pl.rp; a.rt = pl.rt; a.pe = pl.pe; a.e = pl.e; a.blocks_p = (int)pl.blocks_p;
+    a.pairs = (uint32_t)pl.pairs; a.lut_len = (uint32_t)lut_len;
+    a.shift = score_shift; a.lut_shift = lut_shift; a.prob_frac = prob_frac;
+    return ctx->hip(head_dim == 128 ? prefix_launch<128>(a, pl, ctx->stream) : prefix_launch<64>(a, pl, ctx->stream), what);
 }
 
 }  // extern "C"

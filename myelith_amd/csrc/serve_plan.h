@@ -1,0 +1,101 @@
+// serve_plan.h -- what the host decides for the operators of a serving step:
+// which calls are refused, how the work is cut, how the workspace is laid out.
+// Plain C++ with no HIP dependency: the entry points call these functions, and a
+// host build of them runs under AddressSanitizer and
+// UndefinedBehaviorSanitizer in the CPU tests.
+#pragma once
+
+#include <algorithm>
+#include <cstddef>
+#include <cstdint>
+
+namespace myl {
+
+constexpr size_t kInt = 0x7FFFFFFF;
+
+// Pieces of a workspace in 256-byte steps.
+struct Layout {
+    size_t used = 0;
+    size_t take(size_t n, size_t each) {
+        const size_t off = used;
+        used += (n * each + 255) & ~(size_t)255;
+        return off;
+    }
+};
+
+// ---- attention over a shared prefix ------------------------------------------
+
+// At most 65536 keys per row: with non-negative table entries below 2^15 the exp sums
+// stay below 2^31, and sum p |v| <= (2^14 + keys / 2) 2^15 < 2^31.
+constexpr size_t kPrefixMaxKeys = 65536;
+constexpr size_t kPrefixMaxRows = 65535;
+constexpr size_t kPrefixMaxPairs = (size_t)1 << 22;  // rows x heads
+constexpr size_t kPrefixMaxLut = 32768;
+
+struct PrefixShape {
+    size_t n_seqs, rows_per_seq, heads, kv_heads, head_dim, prefix_len, max_tail;
+};
+
+// The reason why a shape is refused, or null.
+inline const char* prefix_refuse(const PrefixShape& s) {
+    if (s.kv_heads == 0 || s.heads == 0 || s.heads % s.kv_heads) return "heads must be a multiple of kv_heads";
+    if (s.heads > kPrefixMaxRows || s.n_seqs > kPrefixMaxRows || s.rows_per_seq > kPrefixMaxRows ||
+        s.n_seqs * s.rows_per_seq > kPrefixMaxRows || s.n_seqs * s.rows_per_seq * s.heads > kPrefixMaxPairs)
+        return "too many rows or heads (65535 each, 2^22 together)";
+    if (s.prefix_len > kPrefixMaxKeys || s.max_tail > kPrefixMaxKeys - s.prefix_len) return "more than 65536 keys per row";
+    return nullptr;
+}
+
+// The work of a call.  The vectors (query heads of rows) that read one KV head are cut
+// into tiles of at most 64, the keys of the prefix and of the tails into ranges of a
+// multiple of 64; a block takes one tile and one range.  Prefix tiles hold vectors of every row,
+// tail tiles those of one sequence.
+struct PrefixPlan {
+    int G, vp, vt;          // query heads per KV head; vectors per KV head: of all rows, of one sequence
+    int tp, tt;             // tiles of each
+    int np, rp, nt, rt;     // ranges of prefix and tail keys, keys per range
+    int pe, e;              // keys of the prefix rounded up to 64, row stride of the exp values
+    int64_t blocks_p, blocks_t;
+    size_t pairs;           // rows x heads
+    size_t off_max, off_sum, off_exp, off_out, bytes;
+};
+
+constexpr int kPrefixTile = 64;
+
+inline PrefixPlan prefix_plan(const PrefixShape& s, int cus) {
+    PrefixPlan p{};
+    const int64_t R = (int64_t)(s.n_seqs * s.rows_per_seq), kvh = (int64_t)s.kv_heads;
+    p.G = (int)(s.heads / s.kv_heads);
+    p.vp = (int)(R * p.G);
+    p.vt = (int)(s.rows_per_seq * p.G);
+    p.tp = (p.vp + kPrefixTile - 1) / kPrefixTile;
+    p.tt = (p.vt + kPrefixTile - 1) / kPrefixTile;
+    const int P = (int)s.prefix_len, T = (int)s.max_tail;
+    // Blocks of about three per CU together, ranges of 64 keys at least.
+    auto cut = [&](int keys, int64_t per_range, int& n, int& len) {
+        n = len = 0;
+        if (keys == 0 || per_range == 0) return;
+        const int steps = (keys + 63) / 64;
+        const int64_t want = std::max<int64_t>(1, 3 * cus / per_range);
+        const int each = (int)((steps + std::min<int64_t>(want, steps) - 1) / std::min<int64_t>(want, steps));
+        len = 64 * each;
+        n = (steps + each - 1) / each;
+    };
+    cut(P, kvh * p.tp, p.np, p.rp);
+    cut(T, kvh * (int64_t)s.n_seqs * p.tt, p.nt, p.rt);
+    p.pe = (P + 63) / 64 * 64;
+    p.e = p.pe + (T + 63) / 64 * 64;
+    p.blocks_p = (kvh * p.tp * p.np + 7) / 8 * 8;
+    p.blocks_t = kvh * (int64_t)s.n_seqs * p.tt * p.nt;
+    p.pairs = (size_t)R * s.heads;
+    Layout l;
+    const size_t parts = p.pairs * (size_t)(p.np + p.nt);
+    p.off_max = l.take(parts, 4);
+    p.off_sum = l.take(parts, 4);
+    p.off_exp = l.take(p.pairs * (size_t)p.e, 2);
+    p.off_out = l.take(parts * s.head_dim, 4);
+    p.bytes = std::max<size_t>(l.used, 256);  // 0 stands for sizes that a call refuses
+    return p;
+}
+
+}  // namespace myl
