@@ -22,7 +22,9 @@
 #include "serve_plan.h"
 #include "wave.h"
 
+#include <algorithm>
 #include <string>
+#include <type_traits>
 
 namespace myl {
 namespace {
@@ -153,176 +155,256 @@ __device__ inline int32_t quarters_max(int32_t v) {
     return max(v, __shfl_xor(v, 32, 64));
 }
 
+// A thread's share of a vector's partials over its ranges (all of the prefix's, its
+// tail's up to `tail` positions, which follow them), kShares threads per vector: eight
+// loads in flight.
+constexpr int kShares = 256 / kTile;
+template <class Fold>
+__device__ inline void fold_ranges(const PrefixAttn& a, const int32_t* __restrict__ part, uint32_t pair, int tail, int share,
+                                   const Fold& fold) {
+    const int all = a.np_count + a.nt_count;
+    for (int i0 = share; i0 < all; i0 += 8 * kShares) {
+        int32_t x[8];
+        bool ok[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+            const int i = i0 + k * kShares;
+            ok[k] = i < all && (i < a.np_count || (i - a.np_count) * a.rt < tail);
+            x[k] = ok[k] ? part[(size_t)i * a.pairs + pair] : 0;
+        }
+#pragma unroll
+        for (int k = 0; k < 8; ++k)
+            if (ok[k]) fold(x[k]);
+    }
+}
+
+// Tail positions of the row of a vector, for its statistics.
+__device__ inline int vector_tail(const PrefixAttn& a, const Part& p, int row) {
+    if (a.nt_count == 0) return 0;
+    int rem;
+    return tail_of(a, row, p.tail ? p.slot : slot_of(a, divmod(a.n, row, rem)));
+}
+
 enum Pass { kMaxPass, kExpPass };
+
+// The exp table's copy in LDS, eight entries per load: entries past the table are 0 (one at
+// least follows it), negative ones count as 0.
+struct TablePiece {
+    uint4 x[4];
+    __device__ inline void load(const PrefixAttn& a, uint32_t i0) {
+        const __amdgpu_buffer_rsrc_t rl = weight_rsrc(a.lut, (a.lut_len * 2u + 3u) & ~3u);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) x[k] = cload16(rl, 2u * (i0 + 2048u * k));
+    }
+    __device__ inline void store(const PrefixAttn& a, uint32_t i0, uint16_t* tab) const {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const uint32_t i = i0 + 2048u * k;
+            if (i > a.lut_len) break;
+            uint32_t w[4] = {x[k].x, x[k].y, x[k].z, x[k].w};
+#pragma unroll
+            for (int b = 0; b < 4; ++b) {
+                const uint32_t lo = i + 2 * b < a.lut_len && !(w[b] & 0x8000u) ? w[b] & 0xFFFFu : 0u;
+                const uint32_t hi = i + 2 * b + 1 < a.lut_len && !(w[b] >> 31) ? w[b] & 0xFFFF0000u : 0u;
+                w[b] = lo | hi;
+            }
+            *reinterpret_cast<uint4*>(tab + i) = make_uint4(w[0], w[1], w[2], w[3]);
+        }
+    }
+};
 
 // Scores of a tile's vectors with a range's keys on v_mfma_i32_16x16x64_i8: K
 // positions are rows, vectors columns, so lane l holds vector l % 16 of each 16-vector
-// tile and positions 4 (l / 16) .. + 3 of its wave's 16-position group.  With byte
+// tile and positions 4 (l / 16) .. + 3 of a 16-position group.  With byte
 // planes x = 256 hi + lo' + 128 of both operands
 //   q.k = 65536 hh + 256 (hl + lh + 128 sum k_hi) + ll + 128 sum k_lo' + 128 sum q
 // where the sums over k come from the matrix cores too (a B operand of 64s, doubled)
 // and start the accumulators, and sum q is one value per lane.  As 256 u + r the score
 // takes 32-bit steps (ScoreScale); other scales take the 64-bit form (FAST false).
-template <int HD, bool FAST, Pass PASS>
-__global__ __launch_bounds__(256, 2) void prefix_qk_kernel(PrefixAttn a) {
-    constexpr int NS = HD / 64;
-    extern __shared__ uint16_t tab[];  // kExpPass: the table and a 0
-    __shared__ int32_t red[4][kTile], s_max[kTile];
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, c = lane & 15, kb = lane >> 4;
-    Part p;
-    if (!part_of(a, p)) return;
-    // the lane's vectors
-    uint32_t pair[kSub];
-    int lim[kSub];  // keys of this part that the vector attends
-    v4i32_t qh[kSub][NS], ql[kSub][NS];
-    int32_t qsum[kSub];
+// A wave holds the vectors' planes in registers and streams its groups of K rows
+// from memory to the operands, the next step's loads in flight: no LDS, no barrier.
+// SUBS 16-vector tiles, GU 16-position groups per wave and step.
+template <int HD, bool FAST, Pass PASS, int SUBS>
+__device__ inline void prefix_qk_part(const PrefixAttn& a, const Part& p, uint16_t* tab, int32_t (*red)[kTile],
+                                      int32_t* s_max) {
+    constexpr int NS = HD / 64, GU = SUBS == 1 ? 2 : 1;
+    const int tid = threadIdx.x, lane = tid & 63, c = lane & 15, kb = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    TablePiece piece;
+    if (PASS == kExpPass) piece.load(a, 8 * tid);
+    uint16_t* eo[SUBS];
+    int lim[SUBS];  // keys of this range that the vector attends end here
     int lmax = 0, lmin = 0x7FFFFFFF;
+    uint4 qx[SUBS][NS][2];
 #pragma unroll
-    for (int t = 0; t < kSub; ++t) {
-        pair[t] = 0;
-        lim[t] = 0;
-        qsum[t] = 0;
+    for (int t = 0; t < SUBS; ++t) {
+        // Places past the last vector repeat it: their lanes write the same values to
+        // the same addresses, and no store needs a branch.
+        int row, head;
+        vector_of(a, p, min(16 * t + c, p.nv - 1), row, head);
+        lim[t] = p.tail ? max(0, tail_of(a, row, p.slot)) : a.P;
+        const uint32_t pair = (uint32_t)row * (uint32_t)a.heads + (uint32_t)head;
+        eo[t] = a.pexp + (size_t)pair * a.e + (p.tail ? a.pe : 0) + 4 * kb;
+        const int16_t* qv = a.q + (size_t)row * a.ldq + (size_t)head * HD + 16 * kb;
 #pragma unroll
-        for (int s = 0; s < NS; ++s) qh[t][s] = ql[t][s] = v4i32_t{0, 0, 0, 0};
-        if (t < p.subs) {
-            const int v = 16 * t + c;
-            if (v < p.nv) {
-                int row, head;
-                vector_of(a, p, v, row, head);
-                pair[t] = (uint32_t)row * (uint32_t)a.heads + (uint32_t)head;
-                lim[t] = p.tail ? max(0, tail_of(a, row, p.slot)) : a.P;
-                lmax = max(lmax, lim[t]);
-                lmin = min(lmin, lim[t]);
-                const int16_t* qv = a.q + (size_t)row * a.ldq + (size_t)head * HD + 16 * kb;
-#pragma unroll
-                for (int s = 0; s < NS; ++s) {
-                    const uint4 x[2] = {*reinterpret_cast<const uint4*>(qv + 64 * s), *reinterpret_cast<const uint4*>(qv + 64 * s + 8)};
-                    planes16(x, qh[t][s], ql[t][s]);
-                    const uint32_t w[8] = {x[0].x, x[0].y, x[0].z, x[0].w, x[1].x, x[1].y, x[1].z, x[1].w};
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) qsum[t] = sum_pairs(w[i], qsum[t]);
-                }
-            }
-            qsum[t] = 128 * quarters_sum(qsum[t]);
+        for (int s = 0; s < NS; ++s) {
+            qx[t][s][0] = *reinterpret_cast<const uint4*>(qv + 64 * s);
+            qx[t][s][1] = *reinterpret_cast<const uint4*>(qv + 64 * s + 8);
         }
-    }
-    lmax = wave_max_i32(lmax);
-    lmin = ~wave_max_i32(~lmin);
-    const int j1 = min(p.j1, lmax);  // uniform over the block: every wave holds every vector
-    if (p.j0 >= j1) return;
-    int32_t m[kSub];
-    if (PASS == kExpPass) {
-        for (uint32_t i = tid; i <= a.lut_len; i += 256) tab[i] = i < a.lut_len ? (uint16_t)max(0, (int32_t)a.lut[i]) : 0;
-        // the maxima of all ranges, four threads per vector
-        const int v = tid & (kTile - 1), share = tid / kTile;
-        int32_t mx = INT32_MIN;
-        if (v < p.nv) {
-            int row, head, rem;
-            vector_of(a, p, v, row, head);
-            const uint32_t pr = (uint32_t)row * (uint32_t)a.heads + (uint32_t)head;
-            const int seq = divmod(a.n, row, rem);
-            const int tail = a.nt_count ? tail_of(a, row, p.tail ? p.slot : slot_of(a, seq)) : 0;
-            for (int i = share; i < a.np_count; i += 4) mx = max(mx, a.pmax[(size_t)i * a.pairs + pr]);
-            for (int i = share; i < a.nt_count && i * a.rt < tail; i += 4)
-                mx = max(mx, a.pmax[(size_t)(a.np_count + i) * a.pairs + pr]);
-        }
-        red[share][v] = mx;
-        __syncthreads();
-        if (tid < kTile) s_max[tid] = max(max(red[0][tid], red[1][tid]), max(red[2][tid], red[3][tid]));
-        __syncthreads();
-#pragma unroll
-        for (int t = 0; t < kSub; ++t) m[t] = s_max[16 * t + c];
     }
     const int16_t* kg = keys_of(a, p, a.kp, a.kt);
     const __amdgpu_buffer_rsrc_t rk = weight_rsrc(kg, (uint32_t)(p.tail ? a.max_tail : a.P) * HD * 2u);
-    // kMaxPass: the largest dot as (u, r), or the largest score; kExpPass: the sum
-    int32_t best[kSub], low[kSub];
-#pragma unroll
-    for (int t = 0; t < kSub; ++t) {
-        best[t] = PASS == kMaxPass ? INT32_MIN : 0;
-        low[t] = 0;
-    }
-    const v4i32_t sixty4 = {0x40404040, 0x40404040, 0x40404040, 0x40404040}, zero = {0, 0, 0, 0};
-    uint4 kx[NS][2];
+    const uint32_t klane = (uint32_t)c * HD + 16u * kb;
+    uint4 kx[GU][NS][2];
     auto load = [&](int j) {
 #pragma unroll
-        for (int s = 0; s < NS; ++s)
+        for (int g = 0; g < GU; ++g) {
+            const uint32_t at = ((uint32_t)(j + 64 * g) * HD + klane) * 2u;
 #pragma unroll
-            for (int i = 0; i < 2; ++i) kx[s][i] = cload16(rk, ((uint32_t)(j + c) * HD + 64u * s + 16u * kb + 8u * i) * 2u);
+            for (int s = 0; s < NS; ++s)
+#pragma unroll
+                for (int i = 0; i < 2; ++i) kx[g][s][i] = cload16(rk, at + 128u * s + 16u * i);
+        }
     };
     load(p.j0 + 16 * wave);
-    for (int j = p.j0 + 16 * wave; j < j1; j += 64) {
-        v4i32_t kh[NS], kl[NS];
 #pragma unroll
-        for (int s = 0; s < NS; ++s) planes16(kx[s], kh[s], kl[s]);
-        load(j + 64);
-        v4i32_t mid0 = zero, ll0 = zero;
-#pragma unroll
-        for (int s = 0; s < NS; ++s) {
-            mid0 = __builtin_amdgcn_mfma_i32_16x16x64_i8(kh[s], sixty4, mid0, 0, 0, 0);
-            ll0 = __builtin_amdgcn_mfma_i32_16x16x64_i8(kl[s], sixty4, ll0, 0, 0, 0);
+    for (int t = 0; t < SUBS; ++t) {
+        lmax = max(lmax, lim[t]);
+        lmin = min(lmin, lim[t]);
+    }
+    lmax = wave_max_i32(lmax);
+    lmin = min(p.j1, ~wave_max_i32(~lmin));
+    const int j1 = min(p.j1, lmax);  // uniform over the block: every wave holds every vector
+    if (p.j0 >= j1) return;
+    int32_t mx = INT32_MIN;
+    if (PASS == kExpPass) {
+        // the maxima over all ranges
+        const int v = tid & (kTile - 1), share = tid / kTile;
+        if (v < p.nv) {
+            int row, head;
+            vector_of(a, p, v, row, head);
+            fold_ranges(a, a.pmax, (uint32_t)row * (uint32_t)a.heads + (uint32_t)head, vector_tail(a, p, row), share,
+                        [&](int32_t x) { mx = max(mx, x); });
         }
-        mid0 += mid0;
-        ll0 += ll0;
-        const bool whole = j + 16 <= lmin;
-#pragma unroll
-        for (int t = 0; t < kSub; ++t) {
-            if (t >= p.subs) break;
-            v4i32_t hh = zero, mid = mid0, ll = ll0;
-#pragma unroll
-            for (int s = 0; s < NS; ++s) {
-                hh = __builtin_amdgcn_mfma_i32_16x16x64_i8(kh[s], qh[t][s], hh, 0, 0, 0);
-                mid = __builtin_amdgcn_mfma_i32_16x16x64_i8(kh[s], ql[t][s], mid, 0, 0, 0);
-                mid = __builtin_amdgcn_mfma_i32_16x16x64_i8(kl[s], qh[t][s], mid, 0, 0, 0);
-                ll = __builtin_amdgcn_mfma_i32_16x16x64_i8(kl[s], ql[t][s], ll, 0, 0, 0);
-            }
-            uint32_t ev[4];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const int32_t lo = ll[i] + qsum[t];
-                const int32_t u = 256 * hh[i] + mid[i] + (lo >> 8);
-                const uint32_t r = (uint32_t)lo & 255u;
-                const bool ok = whole || j + 4 * kb + i < lim[t];
-                if (PASS == kMaxPass) {
-                    if (FAST) {
-                        const bool up = ok && (u > best[t] || (u == best[t] && (int32_t)r > low[t]));
-                        best[t] = up ? u : best[t];
-                        low[t] = up ? (int32_t)r : low[t];
-                    } else {
-                        const int64_t dot = 256 * (int64_t)u + (int64_t)r;
-                        const int32_t z = (int32_t)rshift_round64(wmul64(dot, a.mult), a.shift);
-                        best[t] = ok ? max(best[t], z) : best[t];
-                    }
-                } else {
-                    const int32_t z = FAST ? a.scale(u, r)
-                                           : (int32_t)rshift_round64(wmul64(256 * (int64_t)u + (int64_t)r, a.mult), a.shift);
-                    // sat_sub and the lookup of softmax.rs:12-38; the table ends with a 0
-                    const uint32_t below = min((uint32_t)m[t] - (uint32_t)z, 0x7FFFFFFFu);
-                    uint32_t e = tab[min(below >> (a.lut_shift & 31u), a.lut_len)];
-                    ev[i] = ok ? e : 0u;
-                    best[t] += (int32_t)ev[i];
-                }
-            }
-            if (PASS == kExpPass && 16 * t + c < p.nv) {
-                uint16_t* o = a.pexp + (size_t)pair[t] * a.e + (p.tail ? a.pe : 0) + j + 4 * kb;
-                *reinterpret_cast<uint2*>(o) = make_uint2(ev[0] | (ev[1] << 16), ev[2] | (ev[3] << 16));
-            }
+        red[share][v] = mx;
+        piece.store(a, 8 * tid, tab);
+        for (uint32_t i0 = 8 * tid + 8192; i0 <= a.lut_len; i0 += 8192) {
+            piece.load(a, i0);
+            piece.store(a, i0, tab);
         }
     }
-    // the block's value per vector
-    __syncthreads();
+    v4i32_t qh[SUBS][NS], ql[SUBS][NS];
+    int32_t qsum[SUBS], m[SUBS];
 #pragma unroll
-    for (int t = 0; t < kSub; ++t) {
+    for (int t = 0; t < SUBS; ++t) {
+        qsum[t] = 0;
+#pragma unroll
+        for (int s = 0; s < NS; ++s) {
+            planes16(qx[t][s], qh[t][s], ql[t][s]);
+            const uint32_t w[8] = {qx[t][s][0].x, qx[t][s][0].y, qx[t][s][0].z, qx[t][s][0].w,
+                                   qx[t][s][1].x, qx[t][s][1].y, qx[t][s][1].z, qx[t][s][1].w};
+#pragma unroll
+            for (int i = 0; i < 8; ++i) qsum[t] = sum_pairs(w[i], qsum[t]);
+        }
+        qsum[t] = 128 * quarters_sum(qsum[t]);
+    }
+    if (PASS == kExpPass) {
+        block_barrier();
+        if (tid < kTile) s_max[tid] = max(max(red[0][tid], red[1][tid]), max(red[2][tid], red[3][tid]));
+        block_barrier();  // the table is complete as well
+#pragma unroll
+        for (int t = 0; t < SUBS; ++t) m[t] = s_max[min(16 * t + c, p.nv - 1)];
+    }
+    // kMaxPass: the largest dot as u * 2^32 + r (FAST), or the largest score; kExpPass: the sum
+    int64_t top[SUBS];
+    int32_t best[SUBS];
+#pragma unroll
+    for (int t = 0; t < SUBS; ++t) {
+        top[t] = INT64_MIN;
+        best[t] = PASS == kMaxPass ? INT32_MIN : 0;
+    }
+    const v4i32_t sixty4 = {0x40404040, 0x40404040, 0x40404040, 0x40404040}, zero = {0, 0, 0, 0};
+    // MASK: the step holds keys past some vector's (or the range's) end
+    auto step = [&](int j, auto mask) {
+        constexpr bool MASK = decltype(mask)::value;
+        v4i32_t kh[GU][NS], kl[GU][NS];
+#pragma unroll
+        for (int g = 0; g < GU; ++g)
+#pragma unroll
+            for (int s = 0; s < NS; ++s) planes16(kx[g][s], kh[g][s], kl[g][s]);
+        load(j + 64 * GU);
+#pragma unroll
+        for (int g = 0; g < GU; ++g) {
+            const int jg = j + 64 * g;
+            v4i32_t mid0 = zero, ll0 = zero;
+#pragma unroll
+            for (int s = 0; s < NS; ++s) {
+                mid0 = __builtin_amdgcn_mfma_i32_16x16x64_i8(kh[g][s], sixty4, mid0, 0, 0, 0);
+                ll0 = __builtin_amdgcn_mfma_i32_16x16x64_i8(kl[g][s], sixty4, ll0, 0, 0, 0);
+            }
+            mid0 += mid0;
+            ll0 += ll0;
+#pragma unroll
+            for (int t = 0; t < SUBS; ++t) {
+                v4i32_t hh = zero, mid = mid0, ll = ll0;
+#pragma unroll
+                for (int s = 0; s < NS; ++s) {
+                    hh = __builtin_amdgcn_mfma_i32_16x16x64_i8(kh[g][s], qh[t][s], hh, 0, 0, 0);
+                    mid = __builtin_amdgcn_mfma_i32_16x16x64_i8(kh[g][s], ql[t][s], mid, 0, 0, 0);
+                    mid = __builtin_amdgcn_mfma_i32_16x16x64_i8(kl[g][s], qh[t][s], mid, 0, 0, 0);
+                    ll = __builtin_amdgcn_mfma_i32_16x16x64_i8(kl[g][s], ql[t][s], ll, 0, 0, 0);
+                }
+                uint32_t ev[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int32_t lo = ll[i] + qsum[t];
+                    const int32_t u = 256 * hh[i] + mid[i] + (lo >> 8);
+                    const uint32_t r = (uint32_t)lo & 255u;
+                    const bool ok = !MASK || jg + 4 * kb + i < min(lim[t], j1);
+                    if (PASS == kMaxPass) {
+                        if (FAST) {
+                            const int64_t key = (int64_t)(((uint64_t)(uint32_t)u << 32) | r);
+                            const bool up = ok & (key > top[t]);
+                            top[t] = up ? key : top[t];
+                        } else {
+                            const int64_t dot = 256 * (int64_t)u + (int64_t)r;
+                            const int32_t z = (int32_t)rshift_round64(wmul64(dot, a.mult), a.shift);
+                            best[t] = ok ? max(best[t], z) : best[t];
+                        }
+                    } else {
+                        // sat_sub and the lookup of softmax.rs:12-38; the table ends with a 0.
+                        // FAST: a saturated difference is past the table as it is.
+                        const int32_t z = FAST ? a.scale(u, r)
+                                               : (int32_t)rshift_round64(wmul64(256 * (int64_t)u + (int64_t)r, a.mult), a.shift);
+                        const uint32_t diff = (uint32_t)m[t] - (uint32_t)z;
+                        const uint32_t below = FAST ? diff : min(diff, 0x7FFFFFFFu);
+                        const uint32_t e = tab[min(below >> (a.lut_shift & 31u), a.lut_len)];
+                        ev[i] = ok ? e : 0u;
+                        best[t] += (int32_t)ev[i];
+                    }
+                }
+                if (PASS == kExpPass && (!MASK || jg < j1))
+                    *reinterpret_cast<uint2*>(eo[t] + jg) = make_uint2(ev[0] | (ev[1] << 16), ev[2] | (ev[3] << 16));
+            }
+        }
+    };
+    int j = p.j0 + 16 * wave;
+    for (; j + 64 * (GU - 1) + 16 <= lmin; j += 64 * GU) step(j, std::false_type{});
+    for (; j < j1; j += 64 * GU) step(j, std::true_type{});
+    // the block's value per vector
+    block_barrier();
+#pragma unroll
+    for (int t = 0; t < SUBS; ++t) {
         int32_t v = best[t];
         if (PASS == kMaxPass) {
-            if (FAST) v = best[t] == INT32_MIN ? INT32_MIN : a.scale(best[t], (uint32_t)low[t]);
+            if (FAST) v = top[t] == INT64_MIN ? INT32_MIN : a.scale((int32_t)(top[t] >> 32), (uint32_t)top[t]);
             v = quarters_max(v);
         } else {
             v = quarters_sum(v);
         }
         if (kb == 0) red[wave][16 * t + c] = v;
     }
-    __syncthreads();
+    block_barrier();
     if (tid < p.nv) {
         int row, head;
         vector_of(a, p, tid, row, head);
@@ -333,23 +415,36 @@ __global__ __launch_bounds__(256, 2) void prefix_qk_kernel(PrefixAttn a) {
     }
 }
 
+template <int HD, bool FAST, Pass PASS>
+__global__ __launch_bounds__(256, 3) void prefix_qk_kernel(PrefixAttn a) {
+    extern __shared__ __align__(16) uint16_t tab[];  // kExpPass: the table and a 0
+    __shared__ int32_t red[4][kTile], s_max[kTile];
+    Part p;
+    if (!part_of(a, p)) return;
+    if (p.subs == 1) prefix_qk_part<HD, FAST, PASS, 1>(a, p, tab, red, s_max);
+    else if (p.subs == 2) prefix_qk_part<HD, FAST, PASS, 2>(a, p, tab, red, s_max);
+    else if (p.subs == 3) prefix_qk_part<HD, FAST, PASS, 3>(a, p, tab, red, s_max);
+    else prefix_qk_part<HD, FAST, PASS, kSub>(a, p, tab, red, s_max);
+}
+
 // What a vector's probabilities need.
 struct ProbRow {
     ProbDiv div;
     uint32_t base, extra;  // S = 0: the uniform split (softmax.rs:42-48), 1 more for keys below `extra`
-    int32_t lim, uniform;
+    int32_t uniform, lim;
     uint32_t pair;
-    int32_t pad;
+    int32_t pad[3];
 };
 
 // sum p_j v_j of a tile's vectors over a range, HD dimensions: the dimensions are the
-// rows of v_mfma_i32_16x16x64_i8, the vectors its columns.  A step covers 64 keys per
+// rows of v_mfma_i32_16x16x64_i8, the vectors its columns.  A step covers KU x 64 keys per
 // key wave.  p <= 2^14 splits into two signed bytes exactly (p = 256 ph + pl), v into
 // v = 256 vh + vl' + 128, so
 //   sum p v = 65536 hh + 256 (hl + lh) + ll + 128 sum p
 // modulo 2^32, and the whole sum fits 32 bits (serve_plan.h).  V is turned in registers:
 // lane l loads dimensions 2 (l % 16), + 1 of the 16 keys of its block l / 16 and
 // gathers each dimension's bytes of four keys with v_perm, which is the A operand.
+// The p planes pass through LDS, two steps' places in turn, one barrier a step.
 template <int HD>
 struct PvShape {
     static constexpr int DW = HD / 32;  // waves side by side over the dimensions
@@ -366,7 +461,8 @@ struct PvLds {
 };
 
 template <int HD, int SUB, int KU>
-__device__ inline void prefix_pv_part(const PrefixAttn& a, const Part& p, int8_t* lds, ProbRow* rows, int32_t* p_sum, int j1) {
+__device__ inline void prefix_pv_part(const PrefixAttn& a, const Part& p, int8_t* lds, ProbRow* rows, int32_t* p_sum,
+                                      int32_t (*red)[kTile]) {
     using L = PvLds<HD, SUB, KU>;
     constexpr int DW = PvShape<HD>::DW, KW = PvShape<HD>::KW, CH = L::kChunks;
     constexpr int ITEMS = (16 * SUB * CH + 255) / 256;
@@ -374,35 +470,80 @@ __device__ inline void prefix_pv_part(const PrefixAttn& a, const Part& p, int8_t
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), dw = wave % DW, kw = wave / DW;
     const int16_t* vg = keys_of(a, p, a.vp, a.vt);
     const __amdgpu_buffer_rsrc_t rv = weight_rsrc(vg, (uint32_t)(p.tail ? a.max_tail : a.P) * HD * 2u);
+    const uint32_t vlane = (uint32_t)(64 * kw + 16 * kb) * HD + 32u * dw + 2u * c;
+    uint32_t vx[KU][16];
+    auto load_v = [&](int j) {
+#pragma unroll
+        for (int k = 0; k < KU; ++k) {
+            const uint32_t at = ((uint32_t)(j + 64 * k * KW) * HD + vlane) * 2u;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) vx[k][i] = cload4(rv, at + 2u * HD * i);
+        }
+    };
+    load_v(p.j0);
+    // the vectors' exp sums over all ranges, and what follows from them
+    int j1;
+    {
+        const int v = tid & (kTile - 1), share = tid / kTile;
+        uint32_t pair = 0, s = 0;
+        int tail = 0, lim = 0;
+        if (v < p.nv) {
+            int row, head;
+            vector_of(a, p, v, row, head);
+            pair = (uint32_t)row * (uint32_t)a.heads + (uint32_t)head;
+            tail = vector_tail(a, p, row);
+            lim = p.tail ? max(tail, 0) : a.P;
+        }
+        j1 = min(p.j1, wave_max_i32(lim));
+        if (p.j0 >= j1) return;  // uniform: every wave's lanes hold all vectors
+        if (v < p.nv) fold_ranges(a, a.psum, pair, tail, share, [&](int32_t x) { s += (uint32_t)x; });
+        red[share][v] = (int32_t)s;
+        block_barrier();
+        if (tid < kTile) {
+            const uint32_t S = (uint32_t)(red[0][tid] + red[1][tid] + red[2][tid] + red[3][tid]);
+            ProbRow r{};
+            r.div = ProbDiv::of(S ? S : 1u, a.prob_frac);
+            r.lim = lim;
+            r.pair = pair;
+            r.uniform = S == 0 && v < p.nv ? 1 : 0;
+            const uint32_t keys = (uint32_t)(a.P + max(tail, 0)), one = 1u << a.prob_frac;
+            if (S == 0 && keys) udivmod32(one, keys, recip32(keys), &r.base, &r.extra);
+            rows[tid] = r;
+            p_sum[tid] = 0;
+        }
+        block_barrier();
+    }
     v4i32_t hh[SUB][2], mid[SUB][2], ll[SUB][2];
 #pragma unroll
     for (int t = 0; t < SUB; ++t)
 #pragma unroll
         for (int d = 0; d < 2; ++d) hh[t][d] = mid[t][d] = ll[t][d] = v4i32_t{0, 0, 0, 0};
-    int32_t psum[ITEMS];
-#pragma unroll
-    for (int i = 0; i < ITEMS; ++i) psum[i] = 0;
+    // the thread's vectors and its 16-key chunk of a step
+    int32_t psum[ITEMS], lim[ITEMS];
+    ProbDiv div[ITEMS];
+    const uint16_t* erow[ITEMS];
     uint4 ex[ITEMS][2];
-    uint32_t vx[KU][16];
     const int koff = p.tail ? a.pe : 0, kfirst = p.tail ? a.P : 0;
-    auto load = [&](int j) {
+#pragma unroll
+    for (int i = 0; i < ITEMS; ++i) {
+        const int it = tid + 256 * i, v = it / CH;
+        psum[i] = 0;
+        lim[i] = v < p.nv ? min(rows[v & (kTile - 1)].lim, j1) - 16 * (it % CH) : 0;
+        div[i] = rows[v & (kTile - 1)].div;
+        erow[i] = a.pexp + (size_t)rows[v & (kTile - 1)].pair * a.e + koff + 16 * (it % CH);
+    }
+    auto load_e = [&](int j) {
 #pragma unroll
         for (int i = 0; i < ITEMS; ++i) {
-            const int it = tid + 256 * i, v = it / CH, jc = j + 16 * (it % CH);
             ex[i][0] = ex[i][1] = make_uint4(0, 0, 0, 0);
-            if (v < p.nv && jc < min(rows[v].lim, j1)) {
-                const uint4* e = reinterpret_cast<const uint4*>(a.pexp + (size_t)rows[v].pair * a.e + koff + jc);
+            if (j < lim[i]) {
+                const uint4* e = reinterpret_cast<const uint4*>(erow[i] + j);
                 ex[i][0] = e[0];
                 ex[i][1] = e[1];
             }
         }
-#pragma unroll
-        for (int k = 0; k < KU; ++k)
-#pragma unroll
-            for (int i = 0; i < 16; ++i)
-                vx[k][i] = cload4(rv, ((uint32_t)(j + 64 * (k * KW + kw) + 16 * kb + i) * HD + 32u * dw + 2u * c) * 2u);
     };
-    load(p.j0);
+    load_e(p.j0);
     int buf = 0;
     for (int j = p.j0; j < j1; j += L::kKeys, buf ^= 1) {
         int8_t* ph = lds + buf * 2 * L::kPlane;
@@ -413,19 +554,16 @@ __device__ inline void prefix_pv_part(const PrefixAttn& a, const Part& p, int8_t
             if (it >= 16 * SUB * CH) break;
             const uint32_t w[8] = {ex[i][0].x, ex[i][0].y, ex[i][0].z, ex[i][0].w, ex[i][1].x, ex[i][1].y, ex[i][1].z, ex[i][1].w};
             uint32_t pw[8];
-            if (v >= p.nv || !rows[v].uniform) {
-                const ProbDiv div = rows[v].div;
 #pragma unroll
-                for (int k = 0; k < 8; ++k) pw[k] = div(w[k] & 0xFFFFu) | (div(w[k] >> 16) << 16);
-            } else {
-                const int jc = j + 16 * ch, lim = min(rows[v].lim, j1);
+            for (int k = 0; k < 8; ++k) pw[k] = div[i](w[k] & 0xFFFFu) | (div[i](w[k] >> 16) << 16);
+            if (rows[v].uniform) {
 #pragma unroll
                 for (int k = 0; k < 8; ++k) {
                     uint32_t two = 0;
 #pragma unroll
                     for (int b = 0; b < 2; ++b)
-                        if (jc + 2 * k + b < lim)
-                            two |= (rows[v].base + ((uint32_t)(kfirst + jc + 2 * k + b) < rows[v].extra ? 1u : 0u)) << (16 * b);
+                        if (j + 2 * k + b < lim[i])
+                            two |= (rows[v].base + ((uint32_t)(kfirst + j + 16 * ch + 2 * k + b) < rows[v].extra ? 1u : 0u)) << (16 * b);
                     pw[k] = two;
                 }
             }
@@ -455,13 +593,13 @@ __device__ inline void prefix_pv_part(const PrefixAttn& a, const Part& p, int8_t
                 vl[k][1][i] = (int)(__builtin_amdgcn_perm(b1, b0, 0x05040100u) ^ 0x80808080u);
                 vh[k][1][i] = (int)__builtin_amdgcn_perm(b1, b0, 0x07060302u);
             }
-        load(j + L::kKeys);
+        load_e(j + L::kKeys);
+        load_v(j + L::kKeys);
         block_barrier();
 #pragma unroll
         for (int k = 0; k < KU; ++k)
 #pragma unroll
             for (int t = 0; t < SUB; ++t) {
-                if (t >= p.subs) break;
                 const int off = (4 * (k * KW + kw) + kb) * L::kRow + (16 * t + c) * 16;
                 const v4i32_t bh = *reinterpret_cast<const v4i32_t*>(ph + off), bl = *reinterpret_cast<const v4i32_t*>(pl + off);
 #pragma unroll
@@ -478,7 +616,7 @@ __device__ inline void prefix_pv_part(const PrefixAttn& a, const Part& p, int8_t
         const int it = tid + 256 * i;
         if (it < 16 * SUB * CH) atomicAdd(&p_sum[it / CH], psum[i]);
     }
-    __syncthreads();
+    block_barrier();
     // the key waves' sums meet in LDS (in place of the P planes)
     int32_t* sums = reinterpret_cast<int32_t*>(lds);  // [vector][HD + 4]
     constexpr int SROW = HD + 4;
@@ -500,7 +638,7 @@ __device__ inline void prefix_pv_part(const PrefixAttn& a, const Part& p, int8_t
                 for (int h = 0; h < 2; ++h)
                     *reinterpret_cast<uint4*>(sums + (16 * t + c) * SROW + d0 + 4 * h) =
                         make_uint4(o[t][4 * h], o[t][4 * h + 1], o[t][4 * h + 2], o[t][4 * h + 3]);
-        __syncthreads();
+        block_barrier();
         if (kw == 1) return;
 #pragma unroll
         for (int t = 0; t < SUB; ++t)
@@ -520,50 +658,17 @@ __device__ inline void prefix_pv_part(const PrefixAttn& a, const Part& p, int8_t
 }
 
 template <int HD>
-__global__ __launch_bounds__(256, 2) void prefix_pv_kernel(PrefixAttn a) {
-    constexpr int kLds = PvLds<HD, kSub, 1>::kBytes > PvLds<HD, 1, 4>::kBytes ? PvLds<HD, kSub, 1>::kBytes : PvLds<HD, 1, 4>::kBytes;
+__global__ __launch_bounds__(256, 3) void prefix_pv_kernel(PrefixAttn a) {
+    constexpr int kLds = std::max({PvLds<HD, kSub, 1>::kBytes, PvLds<HD, 3, 1>::kBytes, PvLds<HD, 2, 1>::kBytes, PvLds<HD, 1, 2>::kBytes});
     __shared__ __align__(16) int8_t lds[kLds];
     __shared__ __align__(16) ProbRow rows[kTile];
     __shared__ int32_t red[4][kTile], p_sum[kTile];
-    const int tid = threadIdx.x;
     Part p;
     if (!part_of(a, p)) return;
-    const int v = tid & (kTile - 1), share = tid / kTile;
-    uint32_t pair = 0, s = 0;
-    int tail = 0, lim = 0;
-    if (v < p.nv) {
-        int row, head, rem;
-        vector_of(a, p, v, row, head);
-        pair = (uint32_t)row * (uint32_t)a.heads + (uint32_t)head;
-        const int seq = divmod(a.n, row, rem);
-        tail = a.nt_count || p.tail ? tail_of(a, row, p.tail ? p.slot : slot_of(a, seq)) : 0;
-        lim = p.tail ? max(tail, 0) : a.P;
-    }
-    const int lmax = wave_max_i32(lim);
-    if (p.j0 >= lmax) return;  // uniform: every wave's lanes hold all vectors
-    if (v < p.nv) {
-        for (int i = share; i < a.np_count; i += 4) s += (uint32_t)a.psum[(size_t)i * a.pairs + pair];
-        for (int i = share; i < a.nt_count && i * a.rt < tail; i += 4)
-            s += (uint32_t)a.psum[(size_t)(a.np_count + i) * a.pairs + pair];
-    }
-    red[share][v] = (int32_t)s;
-    __syncthreads();
-    if (tid < kTile) {
-        const uint32_t S = (uint32_t)(red[0][tid] + red[1][tid] + red[2][tid] + red[3][tid]);
-        ProbRow r{};
-        r.div = ProbDiv::of(S ? S : 1u, a.prob_frac);
-        r.lim = lim;
-        r.pair = pair;
-        r.uniform = S == 0 ? 1 : 0;
-        const uint32_t keys = (uint32_t)(a.P + max(tail, 0)), one = 1u << a.prob_frac;
-        if (S == 0 && keys) udivmod32(one, keys, recip32(keys), &r.base, &r.extra);
-        rows[tid] = r;
-        p_sum[tid] = 0;
-    }
-    __syncthreads();
-    const int j1 = min(p.j1, lmax);
-    if (p.subs == 1) prefix_pv_part<HD, 1, 4>(a, p, lds, rows, p_sum, j1);
-    else prefix_pv_part<HD, kSub, 1>(a, p, lds, rows, p_sum, j1);
+    if (p.subs == 1) prefix_pv_part<HD, 1, 2>(a, p, lds, rows, p_sum, red);
+    else if (p.subs == 2) prefix_pv_part<HD, 2, 1>(a, p, lds, rows, p_sum, red);
+    else if (p.subs == 3) prefix_pv_part<HD, 3, 1>(a, p, lds, rows, p_sum, red);
+    else prefix_pv_part<HD, kSub, 1>(a, p, lds, rows, p_sum, red);
 }
 
 // The ranges' sums, one rounding (attention.rs:84-86); four dimensions per thread.
@@ -574,19 +679,24 @@ __global__ __launch_bounds__(256) void prefix_out_kernel(PrefixAttn a) {
     int rem;
     const int seq = divmod(a.n, row, rem), tail = tail_of(a, row, slot_of(a, seq));
     uint32_t s[4] = {0, 0, 0, 0};
-    auto add = [&](int range) {
-        const uint4 x = *reinterpret_cast<const uint4*>(a.pout + ((size_t)range * a.pairs + (size_t)row * a.heads) * HD + i);
-        s[0] += x.x;
-        s[1] += x.y;
-        s[2] += x.z;
-        s[3] += x.w;
-    };
-    if (tail >= 0) {
-#pragma unroll 8
-        for (int r = 0; r < a.np_count; ++r) add(r);
-#pragma unroll 4
-        for (int r = 0; r < a.nt_count; ++r)
-            if (r * a.rt < tail) add(a.np_count + r);
+    // the ranges with a key of the row, eight loads in flight
+    const int all = a.np_count + a.nt_count;
+    for (int r0 = 0; tail >= 0 && r0 < all; r0 += 8) {
+        uint4 x[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+            const int r = r0 + k;
+            x[k] = make_uint4(0, 0, 0, 0);
+            if (r < all && (r < a.np_count || (r - a.np_count) * a.rt < tail))
+                x[k] = *reinterpret_cast<const uint4*>(a.pout + ((size_t)r * a.pairs + (size_t)row * a.heads) * HD + i);
+        }
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+            s[0] += x[k].x;
+            s[1] += x[k].y;
+            s[2] += x[k].z;
+            s[3] += x[k].w;
+        }
     }
     uint32_t y[4];
 #pragma unroll
@@ -598,8 +708,9 @@ template <int HD>
 hipError_t prefix_launch(const PrefixAttn& a, const PrefixPlan& pl, hipStream_t st) {
     const unsigned grid = (unsigned)(pl.blocks_p + pl.blocks_t);
     if (grid) {
-        const size_t tab = ((size_t)a.lut_len + 1) * 2;
-        if (a.scale.fast) {
+        const size_t tab = ((size_t)a.lut_len / 8 + 1) * 16;
+        // 2^31 >> lut_shift is past every table
+        if (a.scale.fast && (a.lut_shift & 31) <= 15) {
             prefix_qk_kernel<HD, true, kMaxPass><<<grid, 256, 0, st>>>(a);
             prefix_qk_kernel<HD, true, kExpPass><<<grid, 256, tab, st>>>(a);
         } else {
@@ -649,7 +760,7 @@ int myl_attention_prefix_dev(myl_ctx* ctx, const int16_t* q, size_t n_seqs, size
     if (!q || !out || !exp_lut || !lens) return bad("null operand");
     if (prefix_len && (!k_prefix || !v_prefix)) return bad("null prefix");
     if (max_tail && n_slots && (!k_tail || !v_tail)) return bad("null tail");
-    const uintptr_t ptrs = (uintptr_t)q | (uintptr_t)out | (uintptr_t)k_prefix | (uintptr_t)v_prefix | (uintptr_t)k_tail |
+    const uintptr_t ptrs = (uintptr_t)q | (uintptr_t)out | (uintptr_t)exp_lut | (uintptr_t)k_prefix | (uintptr_t)v_prefix | (uintptr_t)k_tail |
                            (uintptr_t)v_tail | (uintptr_t)workspace;
     if ((ptrs & 15) || ((ldq | ldo | prefix_head_stride | tail_slot_stride | tail_head_stride) & 7))
         return bad("operands must be 16-byte aligned, strides multiples of 8");

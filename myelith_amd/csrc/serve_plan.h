@@ -71,12 +71,12 @@ inline PrefixPlan prefix_plan(const PrefixShape& s, int cus) {
     p.tp = (p.vp + kPrefixTile - 1) / kPrefixTile;
     p.tt = (p.vt + kPrefixTile - 1) / kPrefixTile;
     const int P = (int)s.prefix_len, T = (int)s.max_tail;
-    // Blocks of about three per CU together, ranges of 64 keys at least.
+    // Two blocks per CU (the prefix's and the tails' each), ranges of 64 keys at least.
     auto cut = [&](int keys, int64_t per_range, int& n, int& len) {
         n = len = 0;
         if (keys == 0 || per_range == 0) return;
         const int steps = (keys + 63) / 64;
-        const int64_t want = std::max<int64_t>(1, 3 * cus / per_range);
+        const int64_t want = std::max<int64_t>(1, 2 * cus / per_range);
         const int each = (int)((steps + std::min<int64_t>(want, steps) - 1) / std::min<int64_t>(want, steps));
         len = 64 * each;
         n = (steps + each - 1) / each;
