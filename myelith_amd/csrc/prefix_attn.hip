@@ -29,8 +29,7 @@
 namespace myl {
 namespace {
 
-constexpr int kTile = kPrefixTile;  // vectors of a block
-constexpr int kSub = kTile / 16;    // 16-vector tiles of the matrix instructions
+constexpr int kQkTile = kPrefixQkTile, kPvTile = kPrefixPvTile;  // vectors of a block
 
 // The call, as every kernel sees it.  Row r = seq * rows_per_seq + i attends
 // keys 0 .. P-1 of the prefix, then the first lens[r] of its sequence's tail.
@@ -40,12 +39,16 @@ struct PrefixAttn {
     const int16_t* lut;
     int16_t* out;
     int32_t *pmax, *psum, *pout;  // [range][pair], [range][pair], [range][pair][hd]; pair = row * heads + head
-    uint16_t* pexp;               // [pair][e]: prefix keys, then tail keys from pe on
+    uint16_t *pexp, *texp;        // exp values of the prefix's and the tails' keys (exp_tile)
     size_t ldq, ldo, ph, ts, th;  // strides in elements: q/out rows, prefix heads, tail slots, tail heads
     int64_t mult;
     ScoreScale scale;
-    Divider n, G, tp, np, tt, nt, kvh;
-    int R, heads, P, max_tail, n_slots, vp_count, vt_count, np_count, nt_count, rp, rt, pe, e, blocks_p;
+    Divider n, G, np, nt, kvh;
+    struct Cut {
+        Divider tp, tt;  // tiles of the prefix's and of a sequence's vectors
+        int blocks_p;
+    } qk, pv;
+    int R, heads, P, max_tail, n_slots, vp_count, vt_count, np_count, nt_count, rp, rt, vp16, vt16, pgroups, tgroups;
     uint32_t pairs, lut_len;
     uint8_t shift, lut_shift, prob_frac;
 };
@@ -73,43 +76,54 @@ struct Part {
     int g, v0, nv;         // KV head; first vector, vectors
     int row0;              // row of vector 0 (of the batch or the sequence)
     int range, j0, j1;     // range index among all, keys [j0, j1) of the prefix or the tail
-    int slot;
+    int seq, slot;
     int subs;              // 16-vector tiles with a vector
 };
 // False: nothing to do.  Prefix blocks of one range follow one another on one XCD
 // (block b runs on XCD b % 8), so its L2 serves the range's K and V to all tiles.
-__device__ inline bool part_of(const PrefixAttn& a, Part& p) {
+template <int TILE>
+__device__ inline bool part_of(const PrefixAttn& a, const PrefixAttn::Cut& cut, Part& p) {
     const int b = blockIdx.x;
-    p.tail = b >= a.blocks_p;
+    p.tail = b >= cut.blocks_p;
     if (!p.tail) {
-        const int t = (b & 7) * (a.blocks_p >> 3) + (b >> 3);
+        const int t = (b & 7) * (cut.blocks_p >> 3) + (b >> 3);
         int tile, rng;
-        const int q = divmod(a.tp, t, tile);
+        const int q = divmod(cut.tp, t, tile);
         p.g = divmod(a.np, q, rng);
         if (p.g >= (int)a.kvh.d) return false;
         p.range = rng;
         p.j0 = rng * a.rp;
         p.j1 = min(a.P, p.j0 + a.rp);
-        p.v0 = tile * kTile;
-        p.nv = min(kTile, a.vp_count - p.v0);
+        p.v0 = tile * TILE;
+        p.nv = min(TILE, a.vp_count - p.v0);
         p.row0 = 0;
-        p.slot = 0;
+        p.seq = p.slot = 0;
     } else {
         int tile, rng;
-        int q = divmod(a.tt, b - a.blocks_p, tile);
+        int q = divmod(cut.tt, b - cut.blocks_p, tile);
         q = divmod(a.nt, q, rng);
         const int s = divmod(a.kvh, q, p.g);
         p.range = a.np_count + rng;
         p.j0 = rng * a.rt;
         p.j1 = min(a.max_tail, p.j0 + a.rt);
-        p.v0 = tile * kTile;
-        p.nv = min(kTile, a.vt_count - p.v0);
+        p.v0 = tile * TILE;
+        p.nv = min(TILE, a.vt_count - p.v0);
+        p.seq = s;
         p.row0 = s * (int)a.n.d;
         p.slot = __builtin_amdgcn_readfirstlane(slot_of(a, s));
         if (p.slot < 0) return false;
     }
     p.subs = (p.nv + 15) >> 4;
     return true;
+}
+
+// The exp values lie as the matrix instructions leave them, so that a wave stores (and
+// 16 lanes load) whole lines: [16 vectors][16 keys] blocks of four keys of a vector per
+// lane, entry 64 (key / 4) + 4 vector + key % 4, a vector tile's key groups in a row.
+__device__ inline uint16_t* exp_tile(const PrefixAttn& a, const Part& p, int t) {
+    const size_t tile = (size_t)(p.v0 >> 4) + (size_t)t;
+    if (!p.tail) return a.pexp + ((size_t)p.g * (size_t)a.vp16 + tile) * (size_t)a.pgroups * 256;
+    return a.texp + (((size_t)p.seq * a.kvh.d + (size_t)p.g) * (size_t)a.vt16 + tile) * (size_t)a.tgroups * 256;
 }
 
 // Vector v of the tile: its row and query head.
@@ -156,19 +170,18 @@ __device__ inline int32_t quarters_max(int32_t v) {
 }
 
 // A thread's share of a vector's partials over its ranges (all of the prefix's, its
-// tail's up to `tail` positions, which follow them), kShares threads per vector: eight
+// tail's up to `tail` positions, which follow them), SHARES threads per vector: eight
 // loads in flight.
-constexpr int kShares = 256 / kTile;
-template <class Fold>
+template <int SHARES, class Fold>
 __device__ inline void fold_ranges(const PrefixAttn& a, const int32_t* __restrict__ part, uint32_t pair, int tail, int share,
                                    const Fold& fold) {
     const int all = a.np_count + a.nt_count;
-    for (int i0 = share; i0 < all; i0 += 8 * kShares) {
+    for (int i0 = share; i0 < all; i0 += 8 * SHARES) {
         int32_t x[8];
         bool ok[8];
 #pragma unroll
         for (int k = 0; k < 8; ++k) {
-            const int i = i0 + k * kShares;
+            const int i = i0 + k * SHARES;
             ok[k] = i < all && (i < a.np_count || (i - a.np_count) * a.rt < tail);
             x[k] = ok[k] ? part[(size_t)i * a.pairs + pair] : 0;
         }
@@ -221,13 +234,14 @@ struct TablePiece {
 // where the sums over k come from the matrix cores too (a B operand of 64s, doubled)
 // and start the accumulators, and sum q is one value per lane.  As 256 u + r the score
 // takes 32-bit steps (ScoreScale); other scales take the 64-bit form (FAST false).
-// A wave holds the vectors' planes in registers and streams its groups of K rows
-// from memory to the operands, the next step's loads in flight: no LDS, no barrier.
+// A wave holds the vectors' planes in registers and streams its groups of K rows, the
+// next step's loads in flight; no barrier in the loop.
 // SUBS 16-vector tiles, GU 16-position groups per wave and step.
+constexpr int qk_groups(int subs) { return subs == 1 ? 2 : 1; }
 template <int HD, bool FAST, Pass PASS, int SUBS>
-__device__ inline void prefix_qk_part(const PrefixAttn& a, const Part& p, uint16_t* tab, int32_t (*red)[kTile],
+__device__ inline void prefix_qk_part(const PrefixAttn& a, const Part& p, uint16_t* tab, int8_t* klds, int32_t (*red)[kQkTile],
                                       int32_t* s_max) {
-    constexpr int NS = HD / 64, GU = SUBS == 1 ? 2 : 1;
+    constexpr int NS = HD / 64, GU = qk_groups(SUBS), CH = HD / 8, NI = CH / 4;
     const int tid = threadIdx.x, lane = tid & 63, c = lane & 15, kb = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     TablePiece piece;
@@ -238,13 +252,11 @@ __device__ inline void prefix_qk_part(const PrefixAttn& a, const Part& p, uint16
     uint4 qx[SUBS][NS][2];
 #pragma unroll
     for (int t = 0; t < SUBS; ++t) {
-        // Places past the last vector repeat it: their lanes write the same values to
-        // the same addresses, and no store needs a branch.
+        // places past the last vector repeat it: no branch for them, nothing reads theirs
         int row, head;
         vector_of(a, p, min(16 * t + c, p.nv - 1), row, head);
         lim[t] = p.tail ? max(0, tail_of(a, row, p.slot)) : a.P;
-        const uint32_t pair = (uint32_t)row * (uint32_t)a.heads + (uint32_t)head;
-        eo[t] = a.pexp + (size_t)pair * a.e + (p.tail ? a.pe : 0) + 4 * kb;
+        eo[t] = exp_tile(a, p, t) + 4 * lane;
         const int16_t* qv = a.q + (size_t)row * a.ldq + (size_t)head * HD + 16 * kb;
 #pragma unroll
         for (int s = 0; s < NS; ++s) {
@@ -254,17 +266,19 @@ __device__ inline void prefix_qk_part(const PrefixAttn& a, const Part& p, uint16
     }
     const int16_t* kg = keys_of(a, p, a.kp, a.kt);
     const __amdgpu_buffer_rsrc_t rk = weight_rsrc(kg, (uint32_t)(p.tail ? a.max_tail : a.P) * HD * 2u);
-    const uint32_t klane = (uint32_t)c * HD + 16u * kb;
-    uint4 kx[GU][NS][2];
+    // K rows come in whole lines (CH lanes of 16 bytes a row) and reach the operands' lanes
+    // through the wave's own LDS, chunk x of row r at x ^ (r % CH): in order within a
+    // wave, so without a barrier.  (Loaded straight to the operands, 16 rows per
+    // instruction, they cost a cache access per lane: 1.6 times as long.)
+    const int krow = lane / CH, kch = lane % CH;
+    const uint32_t klane = (uint32_t)krow * HD + 8u * kch;
+    int8_t* const kl_w = klds + wave * GU * 32 * HD;
+    uint4 kx[GU][NI];
     auto load = [&](int j) {
 #pragma unroll
-        for (int g = 0; g < GU; ++g) {
-            const uint32_t at = ((uint32_t)(j + 64 * g) * HD + klane) * 2u;
+        for (int g = 0; g < GU; ++g)
 #pragma unroll
-            for (int s = 0; s < NS; ++s)
-#pragma unroll
-                for (int i = 0; i < 2; ++i) kx[g][s][i] = cload16(rk, at + 128u * s + 16u * i);
-        }
+            for (int i = 0; i < NI; ++i) kx[g][i] = cload16(rk, ((uint32_t)(j + 64 * g + i * (64 / CH)) * HD + klane) * 2u);
     };
     load(p.j0 + 16 * wave);
 #pragma unroll
@@ -279,11 +293,11 @@ __device__ inline void prefix_qk_part(const PrefixAttn& a, const Part& p, uint16
     int32_t mx = INT32_MIN;
     if (PASS == kExpPass) {
         // the maxima over all ranges
-        const int v = tid & (kTile - 1), share = tid / kTile;
+        const int v = tid & (kQkTile - 1), share = tid / kQkTile;
         if (v < p.nv) {
             int row, head;
             vector_of(a, p, v, row, head);
-            fold_ranges(a, a.pmax, (uint32_t)row * (uint32_t)a.heads + (uint32_t)head, vector_tail(a, p, row), share,
+            fold_ranges<256 / kQkTile>(a, a.pmax, (uint32_t)row * (uint32_t)a.heads + (uint32_t)head, vector_tail(a, p, row), share,
                         [&](int32_t x) { mx = max(mx, x); });
         }
         red[share][v] = mx;
@@ -310,7 +324,12 @@ __device__ inline void prefix_qk_part(const PrefixAttn& a, const Part& p, uint16
     }
     if (PASS == kExpPass) {
         block_barrier();
-        if (tid < kTile) s_max[tid] = max(max(red[0][tid], red[1][tid]), max(red[2][tid], red[3][tid]));
+        if (tid < kQkTile) {
+            int32_t v = red[0][tid];
+#pragma unroll
+            for (int i = 1; i < 256 / kQkTile; ++i) v = max(v, red[i][tid]);
+            s_max[tid] = v;
+        }
         block_barrier();  // the table is complete as well
 #pragma unroll
         for (int t = 0; t < SUBS; ++t) m[t] = s_max[min(16 * t + c, p.nv - 1)];
@@ -331,8 +350,21 @@ __device__ inline void prefix_qk_part(const PrefixAttn& a, const Part& p, uint16
 #pragma unroll
         for (int g = 0; g < GU; ++g)
 #pragma unroll
-            for (int s = 0; s < NS; ++s) planes16(kx[g][s], kh[g][s], kl[g][s]);
+            for (int i = 0; i < NI; ++i) {
+                const int row = i * (64 / CH) + krow;
+                *reinterpret_cast<uint4*>(kl_w + g * 32 * HD + row * 2 * HD + ((kch ^ (row & (CH - 1))) << 4)) = kx[g][i];
+            }
         load(j + 64 * GU);
+#pragma unroll
+        for (int g = 0; g < GU; ++g)
+#pragma unroll
+            for (int s = 0; s < NS; ++s) {
+                uint4 x[2];
+#pragma unroll
+                for (int i = 0; i < 2; ++i)
+                    x[i] = *reinterpret_cast<const uint4*>(kl_w + g * 32 * HD + c * 2 * HD + (((8 * s + 2 * kb + i) ^ (c & (CH - 1))) << 4));
+                planes16(x, kh[g][s], kl[g][s]);
+            }
 #pragma unroll
         for (int g = 0; g < GU; ++g) {
             const int jg = j + 64 * g;
@@ -384,7 +416,7 @@ __device__ inline void prefix_qk_part(const PrefixAttn& a, const Part& p, uint16
                     }
                 }
                 if (PASS == kExpPass && (!MASK || jg < j1))
-                    *reinterpret_cast<uint2*>(eo[t] + jg) = make_uint2(ev[0] | (ev[1] << 16), ev[2] | (ev[3] << 16));
+                    *reinterpret_cast<uint2*>(eo[t] + 16 * jg) = make_uint2(ev[0] | (ev[1] << 16), ev[2] | (ev[3] << 16));
             }
         }
     };
@@ -418,13 +450,14 @@ __device__ inline void prefix_qk_part(const PrefixAttn& a, const Part& p, uint16
 template <int HD, bool FAST, Pass PASS>
 __global__ __launch_bounds__(256, 3) void prefix_qk_kernel(PrefixAttn a) {
     extern __shared__ __align__(16) uint16_t tab[];  // kExpPass: the table and a 0
-    __shared__ int32_t red[4][kTile], s_max[kTile];
+    __shared__ __align__(16) int8_t klds[4 * qk_groups(1) * 32 * HD];
+    __shared__ int32_t red[256 / kQkTile][kQkTile], s_max[kQkTile];
     Part p;
-    if (!part_of(a, p)) return;
-    if (p.subs == 1) prefix_qk_part<HD, FAST, PASS, 1>(a, p, tab, red, s_max);
-    else if (p.subs == 2) prefix_qk_part<HD, FAST, PASS, 2>(a, p, tab, red, s_max);
-    else if (p.subs == 3) prefix_qk_part<HD, FAST, PASS, 3>(a, p, tab, red, s_max);
-    else prefix_qk_part<HD, FAST, PASS, kSub>(a, p, tab, red, s_max);
+    if (!part_of<kQkTile>(a, a.qk, p)) return;
+    if (p.subs == 1) prefix_qk_part<HD, FAST, PASS, 1>(a, p, tab, klds, red, s_max);
+    else if (p.subs == 2) prefix_qk_part<HD, FAST, PASS, 2>(a, p, tab, klds, red, s_max);
+    else if (p.subs == 3) prefix_qk_part<HD, FAST, PASS, 3>(a, p, tab, klds, red, s_max);
+    else prefix_qk_part<HD, FAST, PASS, 4>(a, p, tab, klds, red, s_max);
 }
 
 // What a vector's probabilities need.
@@ -455,17 +488,17 @@ template <int HD, int SUB, int KU>
 struct PvLds {
     static constexpr int kKeys = 64 * PvShape<HD>::KW * KU;  // keys of a step
     static constexpr int kChunks = kKeys / 16;
-    static constexpr int kRow = 16 * SUB * 16 + 64;          // bytes of a 16-key chunk of all vectors; 64 spread the banks
+    static constexpr int kRow = 16 * SUB * 16;               // bytes of a 16-key chunk of all vectors
     static constexpr int kPlane = kChunks * kRow;
     static constexpr int kBytes = 4 * kPlane;                // two planes, two steps
 };
 
 template <int HD, int SUB, int KU>
 __device__ inline void prefix_pv_part(const PrefixAttn& a, const Part& p, int8_t* lds, ProbRow* rows, int32_t* p_sum,
-                                      int32_t (*red)[kTile]) {
+                                      int32_t (*red)[kPvTile]) {
     using L = PvLds<HD, SUB, KU>;
     constexpr int DW = PvShape<HD>::DW, KW = PvShape<HD>::KW, CH = L::kChunks;
-    constexpr int ITEMS = (16 * SUB * CH + 255) / 256;
+    constexpr int V = 16 * SUB, ITEMS = (V * CH + 255) / 256;
     const int tid = threadIdx.x, lane = tid & 63, c = lane & 15, kb = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6), dw = wave % DW, kw = wave / DW;
     const int16_t* vg = keys_of(a, p, a.vp, a.vt);
@@ -484,7 +517,7 @@ __device__ inline void prefix_pv_part(const PrefixAttn& a, const Part& p, int8_t
     // the vectors' exp sums over all ranges, and what follows from them
     int j1;
     {
-        const int v = tid & (kTile - 1), share = tid / kTile;
+        const int v = tid & (kPvTile - 1), share = tid / kPvTile;
         uint32_t pair = 0, s = 0;
         int tail = 0, lim = 0;
         if (v < p.nv) {
@@ -496,10 +529,10 @@ __device__ inline void prefix_pv_part(const PrefixAttn& a, const Part& p, int8_t
         }
         j1 = min(p.j1, wave_max_i32(lim));
         if (p.j0 >= j1) return;  // uniform: every wave's lanes hold all vectors
-        if (v < p.nv) fold_ranges(a, a.psum, pair, tail, share, [&](int32_t x) { s += (uint32_t)x; });
+        if (v < p.nv) fold_ranges<256 / kPvTile>(a, a.psum, pair, tail, share, [&](int32_t x) { s += (uint32_t)x; });
         red[share][v] = (int32_t)s;
         block_barrier();
-        if (tid < kTile) {
+        if (tid < kPvTile) {
             const uint32_t S = (uint32_t)(red[0][tid] + red[1][tid] + red[2][tid] + red[3][tid]);
             ProbRow r{};
             r.div = ProbDiv::of(S ? S : 1u, a.prob_frac);
@@ -522,25 +555,24 @@ __device__ inline void prefix_pv_part(const PrefixAttn& a, const Part& p, int8_t
     int32_t psum[ITEMS], lim[ITEMS];
     ProbDiv div[ITEMS];
     const uint16_t* erow[ITEMS];
-    uint4 ex[ITEMS][2];
-    const int koff = p.tail ? a.pe : 0, kfirst = p.tail ? a.P : 0;
+    uint2 ex[ITEMS][4];
+    const int kfirst = p.tail ? a.P : 0;
 #pragma unroll
     for (int i = 0; i < ITEMS; ++i) {
-        const int it = tid + 256 * i, v = it / CH;
+        const int it = tid + 256 * i, v = it % V, ch = it / V;
         psum[i] = 0;
-        lim[i] = v < p.nv ? min(rows[v & (kTile - 1)].lim, j1) - 16 * (it % CH) : 0;
-        div[i] = rows[v & (kTile - 1)].div;
-        erow[i] = a.pexp + (size_t)rows[v & (kTile - 1)].pair * a.e + koff + 16 * (it % CH);
+        lim[i] = ch < CH && v < p.nv ? min(rows[v].lim, j1) - 16 * ch : 0;
+        div[i] = rows[v].div;
+        erow[i] = exp_tile(a, p, v >> 4) + 256 * ch + 4 * (v & 15);
     }
     auto load_e = [&](int j) {
 #pragma unroll
         for (int i = 0; i < ITEMS; ++i) {
-            ex[i][0] = ex[i][1] = make_uint4(0, 0, 0, 0);
-            if (j < lim[i]) {
-                const uint4* e = reinterpret_cast<const uint4*>(erow[i] + j);
-                ex[i][0] = e[0];
-                ex[i][1] = e[1];
-            }
+#pragma unroll
+            for (int k = 0; k < 4; ++k) ex[i][k] = make_uint2(0, 0);
+            if (j < lim[i])
+#pragma unroll
+                for (int k = 0; k < 4; ++k) ex[i][k] = *reinterpret_cast<const uint2*>(erow[i] + 16 * j + 64 * k);
         }
     };
     load_e(p.j0);
@@ -550,9 +582,9 @@ __device__ inline void prefix_pv_part(const PrefixAttn& a, const Part& p, int8_t
         int8_t* pl = ph + L::kPlane;
 #pragma unroll
         for (int i = 0; i < ITEMS; ++i) {
-            const int it = tid + 256 * i, v = it / CH, ch = it % CH;
-            if (it >= 16 * SUB * CH) break;
-            const uint32_t w[8] = {ex[i][0].x, ex[i][0].y, ex[i][0].z, ex[i][0].w, ex[i][1].x, ex[i][1].y, ex[i][1].z, ex[i][1].w};
+            const int it = tid + 256 * i, v = it % V, ch = it / V;
+            if (it >= V * CH) break;
+            const uint32_t w[8] = {ex[i][0].x, ex[i][0].y, ex[i][1].x, ex[i][1].y, ex[i][2].x, ex[i][2].y, ex[i][3].x, ex[i][3].y};
             uint32_t pw[8];
 #pragma unroll
             for (int k = 0; k < 8; ++k) pw[k] = div[i](w[k] & 0xFFFFu) | (div[i](w[k] >> 16) << 16);
@@ -614,7 +646,7 @@ __device__ inline void prefix_pv_part(const PrefixAttn& a, const Part& p, int8_t
 #pragma unroll
     for (int i = 0; i < ITEMS; ++i) {
         const int it = tid + 256 * i;
-        if (it < 16 * SUB * CH) atomicAdd(&p_sum[it / CH], psum[i]);
+        if (it < V * CH) atomicAdd(&p_sum[it % V], psum[i]);
     }
     block_barrier();
     // the key waves' sums meet in LDS (in place of the P planes)
@@ -659,16 +691,16 @@ __device__ inline void prefix_pv_part(const PrefixAttn& a, const Part& p, int8_t
 
 template <int HD>
 __global__ __launch_bounds__(256, 3) void prefix_pv_kernel(PrefixAttn a) {
-    constexpr int kLds = std::max({PvLds<HD, kSub, 1>::kBytes, PvLds<HD, 3, 1>::kBytes, PvLds<HD, 2, 1>::kBytes, PvLds<HD, 1, 2>::kBytes});
+    constexpr int kLds = std::max({PvLds<HD, 4, 1>::kBytes, PvLds<HD, 3, 1>::kBytes, PvLds<HD, 2, 1>::kBytes, PvLds<HD, 1, 2>::kBytes});
     __shared__ __align__(16) int8_t lds[kLds];
-    __shared__ __align__(16) ProbRow rows[kTile];
-    __shared__ int32_t red[4][kTile], p_sum[kTile];
+    __shared__ __align__(16) ProbRow rows[kPvTile];
+    __shared__ int32_t red[4][kPvTile], p_sum[kPvTile];
     Part p;
-    if (!part_of(a, p)) return;
+    if (!part_of<kPvTile>(a, a.pv, p)) return;
     if (p.subs == 1) prefix_pv_part<HD, 1, 2>(a, p, lds, rows, p_sum, red);
     else if (p.subs == 2) prefix_pv_part<HD, 2, 1>(a, p, lds, rows, p_sum, red);
     else if (p.subs == 3) prefix_pv_part<HD, 3, 1>(a, p, lds, rows, p_sum, red);
-    else prefix_pv_part<HD, kSub, 1>(a, p, lds, rows, p_sum, red);
+    else prefix_pv_part<HD, 4, 1>(a, p, lds, rows, p_sum, red);
 }
 
 // The ranges' sums, one rounding (attention.rs:84-86); four dimensions per thread.
@@ -704,20 +736,28 @@ __global__ __launch_bounds__(256) void prefix_out_kernel(PrefixAttn a) {
     *reinterpret_cast<uint2*>(a.out + (size_t)row * a.ldo + i) = make_uint2(y[0] | (y[1] << 16), y[2] | (y[3] << 16));
 }
 
+template <int HD, bool FAST>
+hipError_t prefix_scores(const PrefixAttn& a, unsigned grid, hipStream_t st) {
+    prefix_qk_kernel<HD, FAST, kMaxPass><<<grid, 256, 0, st>>>(a);
+    const size_t tab = ((size_t)a.lut_len / 8 + 1) * 16;
+    if (tab > 24 * 1024) {  // with the K rows' place more than the 64 KiB a launch has by default
+        const hipError_t e = hipFuncSetAttribute((const void*)prefix_qk_kernel<HD, FAST, kExpPass>,
+                                                 hipFuncAttributeMaxDynamicSharedMemorySize, (int)((kPrefixMaxLut / 8 + 1) * 16));
+        if (e != hipSuccess) return e;
+    }
+    prefix_qk_kernel<HD, FAST, kExpPass><<<grid, 256, tab, st>>>(a);
+    return hipGetLastError();
+}
+
 template <int HD>
 hipError_t prefix_launch(const PrefixAttn& a, const PrefixPlan& pl, hipStream_t st) {
-    const unsigned grid = (unsigned)(pl.blocks_p + pl.blocks_t);
+    const unsigned grid = (unsigned)(pl.qk.blocks_p + pl.qk.blocks_t);
     if (grid) {
-        const size_t tab = ((size_t)a.lut_len / 8 + 1) * 16;
         // 2^31 >> lut_shift is past every table
-        if (a.scale.fast && (a.lut_shift & 31) <= 15) {
-            prefix_qk_kernel<HD, true, kMaxPass><<<grid, 256, 0, st>>>(a);
-            prefix_qk_kernel<HD, true, kExpPass><<<grid, 256, tab, st>>>(a);
-        } else {
-            prefix_qk_kernel<HD, false, kMaxPass><<<grid, 256, 0, st>>>(a);
-            prefix_qk_kernel<HD, false, kExpPass><<<grid, 256, tab, st>>>(a);
-        }
-        prefix_pv_kernel<HD><<<grid, 256, 0, st>>>(a);
+        const bool fast = a.scale.fast && (a.lut_shift & 31) <= 15;
+        const hipError_t e = fast ? prefix_scores<HD, true>(a, grid, st) : prefix_scores<HD, false>(a, grid, st);
+        if (e != hipSuccess) return e;
+        prefix_pv_kernel<HD><<<(unsigned)(pl.pv.blocks_p + pl.pv.blocks_t), 256, 0, st>>>(a);
     }
     prefix_out_kernel<HD><<<dim3((unsigned)((a.heads * HD + 1023) / 1024), (unsigned)a.R), 256, 0, st>>>(a);
     return hipGetLastError();
@@ -773,17 +813,20 @@ int myl_attention_prefix_dev(myl_ctx* ctx, const int16_t* q, size_t n_seqs, size
     a.slots = slots; a.lens = lens; a.lut = exp_lut; a.out = out;
     a.pmax = reinterpret_cast<int32_t*>(ws + pl.off_max);
     a.psum = reinterpret_cast<int32_t*>(ws + pl.off_sum);
-    a.pexp = reinterpret_cast<uint16_t*>(ws + pl.off_exp);
+    a.pexp = reinterpret_cast<uint16_t*>(ws + pl.off_pexp);
+    a.texp = reinterpret_cast<uint16_t*>(ws + pl.off_texp);
     a.pout = reinterpret_cast<int32_t*>(ws + pl.off_out);
     a.ldq = ldq; a.ldo = ldo; a.ph = prefix_head_stride; a.ts = tail_slot_stride; a.th = tail_head_stride;
     a.mult = score_mult;
     a.scale = ScoreScale::of(score_mult, score_shift, (int)head_dim);
     auto div = [](size_t d) { return Divider::of((uint32_t)std::max<size_t>(d, 1)); };
     a.n = div(rows_per_seq); a.G = div((size_t)pl.G); a.kvh = div(kv_heads);
-    a.tp = div((size_t)pl.tp); a.np = div((size_t)pl.np); a.tt = div((size_t)pl.tt); a.nt = div((size_t)pl.nt);
+    a.np = div((size_t)pl.np); a.nt = div((size_t)pl.nt);
+    auto cut = [&](const PrefixPlan::Cut& c) { return PrefixAttn::Cut{div((size_t)c.tp), div((size_t)c.tt), (int)c.blocks_p}; };
+    a.qk = cut(pl.qk); a.pv = cut(pl.pv);
     a.R = (int)(n_seqs * rows_per_seq); a.heads = (int)heads; a.P = (int)prefix_len; a.max_tail = (int)max_tail;
     a.n_slots = (int)n_slots; a.vp_count = pl.vp; a.vt_count = pl.vt; a.np_count = pl.np; a.nt_count = pl.nt;
-    a.rp = pl.rp; a.rt = pl.rt; a.pe = pl.pe; a.e = pl.e; a.blocks_p = (int)pl.blocks_p;
+    a.rp = pl.rp; a.rt = pl.rt; a.vp16 = (pl.vp + 15) / 16; a.vt16 = (pl.vt + 15) / 16; a.pgroups = pl.pgroups; a.tgroups = pl.tgroups;
     a.pairs = (uint32_t)pl.pairs; a.lut_len = (uint32_t)lut_len;
     a.shift = score_shift; a.lut_shift = lut_shift; a.prob_frac = prob_frac;
     return ctx->hip(head_dim == 128 ? prefix_launch<128>(a, pl, ctx->stream) : prefix_launch<64>(a, pl, ctx->stream), what);

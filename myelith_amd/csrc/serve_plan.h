@@ -47,20 +47,22 @@ inline const char* prefix_refuse(const PrefixShape& s) {
 }
 
 // The work of a call.  The vectors (query heads of rows) that read one KV head are cut
-// into tiles of at most 64, the keys of the prefix and of the tails into ranges of a
-// multiple of 64; a block takes one tile and one range.  Prefix tiles hold vectors of every row,
-// tail tiles those of one sequence.
-struct PrefixPlan {
-    int G, vp, vt;          // query heads per KV head; vectors per KV head: of all rows, of one sequence
-    int tp, tt;             // tiles of each
-    int np, rp, nt, rt;     // ranges of prefix and tail keys, keys per range
-    int pe, e;              // keys of the prefix rounded up to 64, row stride of the exp values
-    int64_t blocks_p, blocks_t;
-    size_t pairs;           // rows x heads
-    size_t off_max, off_sum, off_exp, off_out, bytes;
-};
+// into tiles, the keys of the prefix and of the tails into ranges of a multiple of 64; a
+// block takes one tile and one range.  Prefix tiles hold vectors of every row, tail
+// tiles those of one sequence.
+constexpr int kPrefixQkTile = 64, kPrefixPvTile = 64;
 
-constexpr int kPrefixTile = 64;
+struct PrefixPlan {
+    int G, vp, vt;       // query heads per KV head; vectors per KV head: of all rows, of one sequence
+    struct Cut {
+        int tp, tt;      // tiles of each
+        int64_t blocks_p, blocks_t;
+    } qk, pv;
+    int np, rp, nt, rt;  // ranges of prefix and tail keys, keys per range
+    int pgroups, tgroups;  // 16-key groups of the prefix and of a tail, rounded up to 64 keys
+    size_t pairs;        // rows x heads
+    size_t off_max, off_sum, off_pexp, off_texp, off_out, bytes;
+};
 
 inline PrefixPlan prefix_plan(const PrefixShape& s, int cus) {
     PrefixPlan p{};
@@ -68,10 +70,10 @@ inline PrefixPlan prefix_plan(const PrefixShape& s, int cus) {
     p.G = (int)(s.heads / s.kv_heads);
     p.vp = (int)(R * p.G);
     p.vt = (int)(s.rows_per_seq * p.G);
-    p.tp = (p.vp + kPrefixTile - 1) / kPrefixTile;
-    p.tt = (p.vt + kPrefixTile - 1) / kPrefixTile;
     const int P = (int)s.prefix_len, T = (int)s.max_tail;
-    // Two blocks per CU (the prefix's and the tails' each), ranges of 64 keys at least.
+    auto tiles = [](int v, int tile) { return (v + tile - 1) / tile; };
+    // Two blocks of the P.V tiles per CU (the prefix's and the tails' each), ranges of
+    // 64 keys at least.
     auto cut = [&](int keys, int64_t per_range, int& n, int& len) {
         n = len = 0;
         if (keys == 0 || per_range == 0) return;
@@ -81,18 +83,25 @@ inline PrefixPlan prefix_plan(const PrefixShape& s, int cus) {
         len = 64 * each;
         n = (steps + each - 1) / each;
     };
-    cut(P, kvh * p.tp, p.np, p.rp);
-    cut(T, kvh * (int64_t)s.n_seqs * p.tt, p.nt, p.rt);
-    p.pe = (P + 63) / 64 * 64;
-    p.e = p.pe + (T + 63) / 64 * 64;
-    p.blocks_p = (kvh * p.tp * p.np + 7) / 8 * 8;
-    p.blocks_t = kvh * (int64_t)s.n_seqs * p.tt * p.nt;
+    cut(P, kvh * tiles(p.vp, kPrefixPvTile), p.np, p.rp);
+    cut(T, kvh * (int64_t)s.n_seqs * tiles(p.vt, kPrefixPvTile), p.nt, p.rt);
+    auto blocks = [&](int tile, PrefixPlan::Cut& c) {
+        c.tp = tiles(p.vp, tile);
+        c.tt = tiles(p.vt, tile);
+        c.blocks_p = (kvh * c.tp * p.np + 7) / 8 * 8;
+        c.blocks_t = kvh * (int64_t)s.n_seqs * c.tt * p.nt;
+    };
+    blocks(kPrefixQkTile, p.qk);
+    blocks(kPrefixPvTile, p.pv);
+    p.pgroups = (P + 63) / 64 * 4;
+    p.tgroups = (T + 63) / 64 * 4;
     p.pairs = (size_t)R * s.heads;
     Layout l;
     const size_t parts = p.pairs * (size_t)(p.np + p.nt);
     p.off_max = l.take(parts, 4);
     p.off_sum = l.take(parts, 4);
-    p.off_exp = l.take(p.pairs * (size_t)p.e, 2);
+    p.off_pexp = l.take((size_t)kvh * (size_t)tiles(p.vp, 16) * (size_t)p.pgroups * 256, 2);
+    p.off_texp = l.take((size_t)(kvh * (int64_t)s.n_seqs) * (size_t)tiles(p.vt, 16) * (size_t)p.tgroups * 256, 2);
     p.off_out = l.take(parts * s.head_dim, 4);
     p.bytes = std::max<size_t>(l.used, 256);  // 0 stands for sizes that a call refuses
     return p;
