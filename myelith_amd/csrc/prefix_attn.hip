@@ -31,6 +31,12 @@ namespace {
 
 constexpr int kQkTile = kPrefixQkTile, kPvTile = kPrefixPvTile;  // vectors of a block
 
+// n / d by the floor of 2^32 / d (at most 2^32 - 1) and one correction.
+struct SmallDiv {
+    uint32_t d, m;
+    static SmallDiv of(size_t d) { return SmallDiv{(uint32_t)d, recip32_u32((uint32_t)d)}; }
+};
+
 // The call, as every kernel sees it.  Row r = seq * rows_per_seq + i attends
 // keys 0 .. P-1 of the prefix, then the first lens[r] of its sequence's tail.
 struct PrefixAttn {
@@ -43,9 +49,9 @@ struct PrefixAttn {
     size_t ldq, ldo, ph, ts, th;  // strides in elements: q/out rows, prefix heads, tail slots, tail heads
     int64_t mult;
     ScoreScale scale;
-    Divider n, G, np, nt, kvh;
+    SmallDiv n, G, np, nt, kvh;
     struct Cut {
-        Divider tp, tt;  // tiles of the prefix's and of a sequence's vectors
+        SmallDiv tp, tt;  // tiles of the prefix's and of a sequence's vectors
         int blocks_p;
     } qk, pv;
     int R, heads, P, max_tail, n_slots, vp_count, vt_count, np_count, nt_count, rp, rt, vp16, vt16, pgroups, tgroups;
@@ -53,11 +59,11 @@ struct PrefixAttn {
     uint8_t shift, lut_shift, prob_frac;
 };
 
-__device__ inline int divmod(const Divider& d, int n, int& rem) {
-    uint32_t q, r;
-    d.divmod((uint32_t)n, q, r);
-    rem = (int)r;
-    return (int)q;
+__device__ inline int divmod(const SmallDiv& d, int n, int& rem) {
+    uint32_t q = __umulhi((uint32_t)n, d.m), r = (uint32_t)n - q * d.d;
+    const bool up = r >= d.d;
+    rem = (int)(up ? r - d.d : r);
+    return (int)(up ? q + 1 : q);
 }
 
 // The slot of sequence s, or -1; tail positions of row r (-1: left out).
@@ -126,11 +132,28 @@ __device__ inline uint16_t* exp_tile(const PrefixAttn& a, const Part& p, int t) 
     return a.texp + (((size_t)p.seq * a.kvh.d + (size_t)p.g) * (size_t)a.vt16 + tile) * (size_t)a.tgroups * 256;
 }
 
-// Vector v of the tile: its row and query head.
-__device__ inline void vector_of(const PrefixAttn& a, const Part& p, int v, int& row, int& head) {
-    int h;
-    row = p.row0 + divmod(a.G, p.v0 + v, h);
-    head = p.g * (int)a.G.d + h;
+// The vectors of a tile, worked out once per block: places past the last vector repeat it.
+template <int TILE>
+struct Vectors {
+    size_t q[TILE];      // element offset of the query vector
+    uint32_t pair[TILE];
+    int32_t lim[TILE];   // keys of this part (the prefix, or the sequence's tail) that it attends
+    int32_t tail[TILE];  // TAILS: tail positions of its row, -1: left out
+};
+template <int TILE, bool TAILS>
+__device__ inline void vectors_of(const PrefixAttn& a, const Part& p, int hd, Vectors<TILE>& vs) {
+    const int v = threadIdx.x;
+    if (v < TILE) {
+        int h, rem;
+        const int row = p.row0 + divmod(a.G, p.v0 + min(v, p.nv - 1), h), head = p.g * (int)a.G.d + h;
+        vs.q[v] = (size_t)row * a.ldq + (size_t)(head * hd);
+        vs.pair[v] = (uint32_t)row * (uint32_t)a.heads + (uint32_t)head;
+        int tail = 0;
+        if (p.tail) tail = tail_of(a, row, p.slot);
+        else if (TAILS && a.nt_count) tail = tail_of(a, row, slot_of(a, divmod(a.n, row, rem)));
+        vs.lim[v] = p.tail ? max(tail, 0) : a.P;
+        vs.tail[v] = tail;
+    }
 }
 
 __device__ inline const int16_t* keys_of(const PrefixAttn& a, const Part& p, const int16_t* prefix, const int16_t* tail) {
@@ -191,13 +214,6 @@ __device__ inline void fold_ranges(const PrefixAttn& a, const int32_t* __restric
     }
 }
 
-// Tail positions of the row of a vector, for its statistics.
-__device__ inline int vector_tail(const PrefixAttn& a, const Part& p, int row) {
-    if (a.nt_count == 0) return 0;
-    int rem;
-    return tail_of(a, row, p.tail ? p.slot : slot_of(a, divmod(a.n, row, rem)));
-}
-
 enum Pass { kMaxPass, kExpPass };
 
 // The exp table's copy in LDS, eight entries per load: entries past the table are 0 (one at
@@ -237,33 +253,24 @@ struct TablePiece {
 // A wave holds the vectors' planes in registers and streams its groups of K rows, the
 // next step's loads in flight; no barrier in the loop.
 // SUBS 16-vector tiles, GU 16-position groups per wave and step.
+// The larger of two signed 64-bit values.  The comparison goes to a scalar pair: the second
+// v_cndmask_b32 of one VCC costs about 35 cycles (measured; with the pair, 5).
+__device__ inline int64_t max64(int64_t x, int64_t y) {
+    uint64_t m;
+    asm("v_cmp_gt_i64_e64 %0, %1, %2\n\ts_nop 1" : "=s"(m) : "v"(x), "v"(y));
+    int32_t hi, lo;
+    asm("v_cndmask_b32_e64 %0, %1, %2, %3" : "=v"(hi) : "v"((int32_t)(y >> 32)), "v"((int32_t)(x >> 32)), "s"(m));
+    asm("v_cndmask_b32_e64 %0, %1, %2, %3" : "=v"(lo) : "v"((int32_t)y), "v"((int32_t)x), "s"(m));
+    return (int64_t)(((uint64_t)(uint32_t)hi << 32) | (uint32_t)lo);
+}
+
 constexpr int qk_groups(int subs) { return subs == 1 ? 2 : 1; }
 template <int HD, bool FAST, Pass PASS, int SUBS>
-__device__ inline void prefix_qk_part(const PrefixAttn& a, const Part& p, uint16_t* tab, int8_t* klds, int32_t (*red)[kQkTile],
-                                      int32_t* s_max) {
+__device__ inline void prefix_qk_part(const PrefixAttn& a, const Part& p, Vectors<kQkTile>& vs, uint16_t* tab, int8_t* klds,
+                                      int32_t (*red)[kQkTile], int32_t* s_max) {
     constexpr int NS = HD / 64, GU = qk_groups(SUBS), CH = HD / 8, NI = CH / 4;
     const int tid = threadIdx.x, lane = tid & 63, c = lane & 15, kb = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    TablePiece piece;
-    if (PASS == kExpPass) piece.load(a, 8 * tid);
-    uint16_t* eo[SUBS];
-    int lim[SUBS];  // keys of this range that the vector attends end here
-    int lmax = 0, lmin = 0x7FFFFFFF;
-    uint4 qx[SUBS][NS][2];
-#pragma unroll
-    for (int t = 0; t < SUBS; ++t) {
-        // places past the last vector repeat it: no branch for them, nothing reads theirs
-        int row, head;
-        vector_of(a, p, min(16 * t + c, p.nv - 1), row, head);
-        lim[t] = p.tail ? max(0, tail_of(a, row, p.slot)) : a.P;
-        eo[t] = exp_tile(a, p, t) + 4 * lane;
-        const int16_t* qv = a.q + (size_t)row * a.ldq + (size_t)head * HD + 16 * kb;
-#pragma unroll
-        for (int s = 0; s < NS; ++s) {
-            qx[t][s][0] = *reinterpret_cast<const uint4*>(qv + 64 * s);
-            qx[t][s][1] = *reinterpret_cast<const uint4*>(qv + 64 * s + 8);
-        }
-    }
     const int16_t* kg = keys_of(a, p, a.kp, a.kt);
     const __amdgpu_buffer_rsrc_t rk = weight_rsrc(kg, (uint32_t)(p.tail ? a.max_tail : a.P) * HD * 2u);
     // K rows come in whole lines (CH lanes of 16 bytes a row) and reach the operands' lanes
@@ -280,11 +287,31 @@ __device__ inline void prefix_qk_part(const PrefixAttn& a, const Part& p, uint16
 #pragma unroll
             for (int i = 0; i < NI; ++i) kx[g][i] = cload16(rk, ((uint32_t)(j + 64 * g + i * (64 / CH)) * HD + klane) * 2u);
     };
-    load(p.j0 + 16 * wave);
+    int j = p.j0 + 16 * wave;
+    load(j);
+    TablePiece piece;
+    if (PASS == kExpPass) piece.load(a, 8 * tid);
+    vectors_of<kQkTile, PASS == kExpPass>(a, p, HD, vs);
+    block_barrier();
+    uint16_t* eo[SUBS];
+    int lim[SUBS];  // keys of this range that the vector attends end here
+    int lmax = 0, lmin = 0x7FFFFFFF;
+    // the vectors once per block, in whole lines, into the K rows' place
+    constexpr int QI = (16 * SUBS * CH + 255) / 256;
+    uint4 qs[QI];
+#pragma unroll
+    for (int i = 0; i < QI; ++i) {
+        const int v = (tid + 256 * i) / CH;
+        qs[i] = *reinterpret_cast<const uint4*>(a.q + vs.q[min(v, kQkTile - 1)] + 8 * (tid % CH));
+    }
 #pragma unroll
     for (int t = 0; t < SUBS; ++t) {
+        // tiles past the last one repeat it: the same values to the same addresses
+        const int tile = min(t, p.subs - 1), v = 16 * tile + c;
+        lim[t] = vs.lim[v];
         lmax = max(lmax, lim[t]);
         lmin = min(lmin, lim[t]);
+        eo[t] = exp_tile(a, p, tile) + 4 * lane;
     }
     lmax = wave_max_i32(lmax);
     lmin = min(p.j1, ~wave_max_i32(~lmin));
@@ -294,12 +321,7 @@ __device__ inline void prefix_qk_part(const PrefixAttn& a, const Part& p, uint16
     if (PASS == kExpPass) {
         // the maxima over all ranges
         const int v = tid & (kQkTile - 1), share = tid / kQkTile;
-        if (v < p.nv) {
-            int row, head;
-            vector_of(a, p, v, row, head);
-            fold_ranges<256 / kQkTile>(a, a.pmax, (uint32_t)row * (uint32_t)a.heads + (uint32_t)head, vector_tail(a, p, row), share,
-                        [&](int32_t x) { mx = max(mx, x); });
-        }
+        fold_ranges<256 / kQkTile>(a, a.pmax, vs.pair[v], vs.tail[v], share, [&](int32_t x) { mx = max(mx, x); });
         red[share][v] = mx;
         piece.store(a, 8 * tid, tab);
         for (uint32_t i0 = 8 * tid + 8192; i0 <= a.lut_len; i0 += 8192) {
@@ -307,32 +329,43 @@ __device__ inline void prefix_qk_part(const PrefixAttn& a, const Part& p, uint16
             piece.store(a, i0, tab);
         }
     }
+#pragma unroll
+    for (int i = 0; i < QI; ++i) {
+        const int v = (tid + 256 * i) / CH;
+        if (v < 16 * SUBS) *reinterpret_cast<uint4*>(klds + v * 2 * HD + (((tid % CH) ^ (v & (CH - 1))) << 4)) = qs[i];
+    }
+    block_barrier();
     v4i32_t qh[SUBS][NS], ql[SUBS][NS];
     int32_t qsum[SUBS], m[SUBS];
 #pragma unroll
     for (int t = 0; t < SUBS; ++t) {
         qsum[t] = 0;
+        const int v = 16 * min(t, p.subs - 1) + c;
 #pragma unroll
         for (int s = 0; s < NS; ++s) {
-            planes16(qx[t][s], qh[t][s], ql[t][s]);
-            const uint32_t w[8] = {qx[t][s][0].x, qx[t][s][0].y, qx[t][s][0].z, qx[t][s][0].w,
-                                   qx[t][s][1].x, qx[t][s][1].y, qx[t][s][1].z, qx[t][s][1].w};
+            uint4 x[2];
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+                x[i] = *reinterpret_cast<const uint4*>(klds + v * 2 * HD + (((8 * s + 2 * kb + i) ^ (c & (CH - 1))) << 4));
+            planes16(x, qh[t][s], ql[t][s]);
+            const uint32_t w[8] = {x[0].x, x[0].y, x[0].z, x[0].w, x[1].x, x[1].y, x[1].z, x[1].w};
 #pragma unroll
             for (int i = 0; i < 8; ++i) qsum[t] = sum_pairs(w[i], qsum[t]);
         }
         qsum[t] = 128 * quarters_sum(qsum[t]);
     }
     if (PASS == kExpPass) {
-        block_barrier();
         if (tid < kQkTile) {
             int32_t v = red[0][tid];
 #pragma unroll
             for (int i = 1; i < 256 / kQkTile; ++i) v = max(v, red[i][tid]);
             s_max[tid] = v;
         }
-        block_barrier();  // the table is complete as well
+    }
+    block_barrier();  // the vectors are read, the table is complete
+    if (PASS == kExpPass) {
 #pragma unroll
-        for (int t = 0; t < SUBS; ++t) m[t] = s_max[min(16 * t + c, p.nv - 1)];
+        for (int t = 0; t < SUBS; ++t) m[t] = s_max[16 * min(t, p.subs - 1) + c];
     }
     // kMaxPass: the largest dot as u * 2^32 + r (FAST), or the largest score; kExpPass: the sum
     int64_t top[SUBS];
@@ -344,7 +377,7 @@ __device__ inline void prefix_qk_part(const PrefixAttn& a, const Part& p, uint16
     }
     const v4i32_t sixty4 = {0x40404040, 0x40404040, 0x40404040, 0x40404040}, zero = {0, 0, 0, 0};
     // MASK: the step holds keys past some vector's (or the range's) end
-    auto step = [&](int j, auto mask) {
+    auto step = [&](auto mask) {
         constexpr bool MASK = decltype(mask)::value;
         v4i32_t kh[GU][NS], kl[GU][NS];
 #pragma unroll
@@ -387,6 +420,7 @@ __device__ inline void prefix_qk_part(const PrefixAttn& a, const Part& p, uint16
                     ll = __builtin_amdgcn_mfma_i32_16x16x64_i8(kl[g][s], ql[t][s], ll, 0, 0, 0);
                 }
                 uint32_t ev[4];
+                int64_t key[4];
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
                     const int32_t lo = ll[i] + qsum[t];
@@ -395,9 +429,7 @@ __device__ inline void prefix_qk_part(const PrefixAttn& a, const Part& p, uint16
                     const bool ok = !MASK || jg + 4 * kb + i < min(lim[t], j1);
                     if (PASS == kMaxPass) {
                         if (FAST) {
-                            const int64_t key = (int64_t)(((uint64_t)(uint32_t)u << 32) | r);
-                            const bool up = ok & (key > top[t]);
-                            top[t] = up ? key : top[t];
+                            key[i] = (int64_t)(((uint64_t)(uint32_t)(ok ? u : INT32_MIN) << 32) | r);
                         } else {
                             const int64_t dot = 256 * (int64_t)u + (int64_t)r;
                             const int32_t z = (int32_t)rshift_round64(wmul64(dot, a.mult), a.shift);
@@ -415,21 +447,21 @@ __device__ inline void prefix_qk_part(const PrefixAttn& a, const Part& p, uint16
                         best[t] += (int32_t)ev[i];
                     }
                 }
+                if (PASS == kMaxPass && FAST) top[t] = max64(top[t], max64(max64(key[0], key[1]), max64(key[2], key[3])));
                 if (PASS == kExpPass && (!MASK || jg < j1))
                     *reinterpret_cast<uint2*>(eo[t] + 16 * jg) = make_uint2(ev[0] | (ev[1] << 16), ev[2] | (ev[3] << 16));
             }
         }
     };
-    int j = p.j0 + 16 * wave;
-    for (; j + 64 * (GU - 1) + 16 <= lmin; j += 64 * GU) step(j, std::false_type{});
-    for (; j < j1; j += 64 * GU) step(j, std::true_type{});
+    for (; j + 64 * (GU - 1) + 16 <= lmin; j += 64 * GU) step(std::false_type{});
+    for (; j < j1; j += 64 * GU) step(std::true_type{});
     // the block's value per vector
     block_barrier();
 #pragma unroll
     for (int t = 0; t < SUBS; ++t) {
         int32_t v = best[t];
         if (PASS == kMaxPass) {
-            if (FAST) v = top[t] == INT64_MIN ? INT32_MIN : a.scale((int32_t)(top[t] >> 32), (uint32_t)top[t]);
+            if (FAST) v = (int32_t)(top[t] >> 32) == INT32_MIN ? INT32_MIN : a.scale((int32_t)(top[t] >> 32), (uint32_t)top[t]);
             v = quarters_max(v);
         } else {
             v = quarters_sum(v);
@@ -438,9 +470,7 @@ __device__ inline void prefix_qk_part(const PrefixAttn& a, const Part& p, uint16
     }
     block_barrier();
     if (tid < p.nv) {
-        int row, head;
-        vector_of(a, p, tid, row, head);
-        const size_t o = (size_t)p.range * a.pairs + (uint32_t)row * (uint32_t)a.heads + (uint32_t)head;
+        const size_t o = (size_t)p.range * a.pairs + vs.pair[tid];
         const int32_t r0 = red[0][tid], r1 = red[1][tid], r2 = red[2][tid], r3 = red[3][tid];
         if (PASS == kMaxPass) a.pmax[o] = max(max(r0, r1), max(r2, r3));
         else a.psum[o] = r0 + r1 + r2 + r3;
@@ -451,22 +481,20 @@ template <int HD, bool FAST, Pass PASS>
 __global__ __launch_bounds__(256, 3) void prefix_qk_kernel(PrefixAttn a) {
     extern __shared__ __align__(16) uint16_t tab[];  // kExpPass: the table and a 0
     __shared__ __align__(16) int8_t klds[4 * qk_groups(1) * 32 * HD];
+    __shared__ Vectors<kQkTile> vs;
     __shared__ int32_t red[256 / kQkTile][kQkTile], s_max[kQkTile];
     Part p;
     if (!part_of<kQkTile>(a, a.qk, p)) return;
-    if (p.subs == 1) prefix_qk_part<HD, FAST, PASS, 1>(a, p, tab, klds, red, s_max);
-    else if (p.subs == 2) prefix_qk_part<HD, FAST, PASS, 2>(a, p, tab, klds, red, s_max);
-    else if (p.subs == 3) prefix_qk_part<HD, FAST, PASS, 3>(a, p, tab, klds, red, s_max);
-    else prefix_qk_part<HD, FAST, PASS, 4>(a, p, tab, klds, red, s_max);
+    if (p.subs == 1) prefix_qk_part<HD, FAST, PASS, 1>(a, p, vs, tab, klds, red, s_max);
+    else if (p.subs == 2) prefix_qk_part<HD, FAST, PASS, 2>(a, p, vs, tab, klds, red, s_max);
+    else prefix_qk_part<HD, FAST, PASS, 4>(a, p, vs, tab, klds, red, s_max);
 }
 
 // What a vector's probabilities need.
 struct ProbRow {
     ProbDiv div;
     uint32_t base, extra;  // S = 0: the uniform split (softmax.rs:42-48), 1 more for keys below `extra`
-    int32_t uniform, lim;
-    uint32_t pair;
-    int32_t pad[3];
+    int32_t uniform, pad;
 };
 
 // sum p_j v_j of a tile's vectors over a range, HD dimensions: the dimensions are the
@@ -494,8 +522,8 @@ struct PvLds {
 };
 
 template <int HD, int SUB, int KU>
-__device__ inline void prefix_pv_part(const PrefixAttn& a, const Part& p, int8_t* lds, ProbRow* rows, int32_t* p_sum,
-                                      int32_t (*red)[kPvTile]) {
+__device__ inline void prefix_pv_part(const PrefixAttn& a, const Part& p, const Vectors<kPvTile>& vs, int8_t* lds, ProbRow* rows,
+                                      int32_t* p_sum, int32_t (*red)[kPvTile]) {
     using L = PvLds<HD, SUB, KU>;
     constexpr int DW = PvShape<HD>::DW, KW = PvShape<HD>::KW, CH = L::kChunks;
     constexpr int V = 16 * SUB, ITEMS = (V * CH + 255) / 256;
@@ -515,31 +543,20 @@ __device__ inline void prefix_pv_part(const PrefixAttn& a, const Part& p, int8_t
     };
     load_v(p.j0);
     // the vectors' exp sums over all ranges, and what follows from them
-    int j1;
+    const int v0 = tid & (kPvTile - 1), share = tid / kPvTile;
+    const int j1 = min(p.j1, wave_max_i32(vs.lim[v0]));
+    if (p.j0 >= j1) return;  // uniform: every wave's lanes hold all vectors
     {
-        const int v = tid & (kPvTile - 1), share = tid / kPvTile;
-        uint32_t pair = 0, s = 0;
-        int tail = 0, lim = 0;
-        if (v < p.nv) {
-            int row, head;
-            vector_of(a, p, v, row, head);
-            pair = (uint32_t)row * (uint32_t)a.heads + (uint32_t)head;
-            tail = vector_tail(a, p, row);
-            lim = p.tail ? max(tail, 0) : a.P;
-        }
-        j1 = min(p.j1, wave_max_i32(lim));
-        if (p.j0 >= j1) return;  // uniform: every wave's lanes hold all vectors
-        if (v < p.nv) fold_ranges<256 / kPvTile>(a, a.psum, pair, tail, share, [&](int32_t x) { s += (uint32_t)x; });
-        red[share][v] = (int32_t)s;
+        uint32_t s = 0;
+        fold_ranges<256 / kPvTile>(a, a.psum, vs.pair[v0], vs.tail[v0], share, [&](int32_t x) { s += (uint32_t)x; });
+        red[share][v0] = (int32_t)s;
         block_barrier();
         if (tid < kPvTile) {
             const uint32_t S = (uint32_t)(red[0][tid] + red[1][tid] + red[2][tid] + red[3][tid]);
             ProbRow r{};
             r.div = ProbDiv::of(S ? S : 1u, a.prob_frac);
-            r.lim = lim;
-            r.pair = pair;
-            r.uniform = S == 0 && v < p.nv ? 1 : 0;
-            const uint32_t keys = (uint32_t)(a.P + max(tail, 0)), one = 1u << a.prob_frac;
+            r.uniform = S == 0 ? 1 : 0;
+            const uint32_t keys = (uint32_t)(a.P + max(vs.tail[tid], 0)), one = 1u << a.prob_frac;
             if (S == 0 && keys) udivmod32(one, keys, recip32(keys), &r.base, &r.extra);
             rows[tid] = r;
             p_sum[tid] = 0;
@@ -561,9 +578,9 @@ __device__ inline void prefix_pv_part(const PrefixAttn& a, const Part& p, int8_t
     for (int i = 0; i < ITEMS; ++i) {
         const int it = tid + 256 * i, v = it % V, ch = it / V;
         psum[i] = 0;
-        lim[i] = ch < CH && v < p.nv ? min(rows[v].lim, j1) - 16 * ch : 0;
+        lim[i] = ch < CH ? min(vs.lim[v], j1) - 16 * ch : 0;
         div[i] = rows[v].div;
-        erow[i] = exp_tile(a, p, v >> 4) + 256 * ch + 4 * (v & 15);
+        erow[i] = exp_tile(a, p, min(v >> 4, p.subs - 1)) + 256 * ch + 4 * (v & 15);  // tiles past the last repeat it
     }
     auto load_e = [&](int j) {
 #pragma unroll
@@ -682,7 +699,7 @@ __device__ inline void prefix_pv_part(const PrefixAttn& a, const Part& p, int8_t
         const int v = 16 * t + c;
         if (v >= p.nv) continue;
         const uint32_t add = 128u * (uint32_t)p_sum[v];
-        int32_t* dst = a.pout + ((size_t)p.range * a.pairs + rows[v].pair) * HD + d0;
+        int32_t* dst = a.pout + ((size_t)p.range * a.pairs + vs.pair[v]) * HD + d0;
 #pragma unroll
         for (int h = 0; h < 2; ++h)
             *reinterpret_cast<uint4*>(dst + 4 * h) = make_uint4(o[t][4 * h] + add, o[t][4 * h + 1] + add, o[t][4 * h + 2] + add, o[t][4 * h + 3] + add);
@@ -691,16 +708,18 @@ __device__ inline void prefix_pv_part(const PrefixAttn& a, const Part& p, int8_t
 
 template <int HD>
 __global__ __launch_bounds__(256, 3) void prefix_pv_kernel(PrefixAttn a) {
-    constexpr int kLds = std::max({PvLds<HD, 4, 1>::kBytes, PvLds<HD, 3, 1>::kBytes, PvLds<HD, 2, 1>::kBytes, PvLds<HD, 1, 2>::kBytes});
+    constexpr int kLds = std::max({PvLds<HD, 4, 1>::kBytes, PvLds<HD, 2, 1>::kBytes, PvLds<HD, 1, 2>::kBytes});
     __shared__ __align__(16) int8_t lds[kLds];
     __shared__ __align__(16) ProbRow rows[kPvTile];
+    __shared__ Vectors<kPvTile> vs;
     __shared__ int32_t red[4][kPvTile], p_sum[kPvTile];
     Part p;
     if (!part_of<kPvTile>(a, a.pv, p)) return;
-    if (p.subs == 1) prefix_pv_part<HD, 1, 2>(a, p, lds, rows, p_sum, red);
-    else if (p.subs == 2) prefix_pv_part<HD, 2, 1>(a, p, lds, rows, p_sum, red);
-    else if (p.subs == 3) prefix_pv_part<HD, 3, 1>(a, p, lds, rows, p_sum, red);
-    else prefix_pv_part<HD, 4, 1>(a, p, lds, rows, p_sum, red);
+    vectors_of<kPvTile, true>(a, p, HD, vs);
+    block_barrier();
+    if (p.subs == 1) prefix_pv_part<HD, 1, 2>(a, p, vs, lds, rows, p_sum, red);
+    else if (p.subs == 2) prefix_pv_part<HD, 2, 1>(a, p, vs, lds, rows, p_sum, red);
+    else prefix_pv_part<HD, 4, 1>(a, p, vs, lds, rows, p_sum, red);
 }
 
 // The ranges' sums, one rounding (attention.rs:84-86); four dimensions per thread.
@@ -819,7 +838,7 @@ int myl_attention_prefix_dev(myl_ctx* ctx, const int16_t* q, size_t n_seqs, size
     a.ldq = ldq; a.ldo = ldo; a.ph = prefix_head_stride; a.ts = tail_slot_stride; a.th = tail_head_stride;
     a.mult = score_mult;
     a.scale = ScoreScale::of(score_mult, score_shift, (int)head_dim);
-    auto div = [](size_t d) { return Divider::of((uint32_t)std::max<size_t>(d, 1)); };
+    auto div = [](size_t d) { return SmallDiv::of(std::max<size_t>(d, 1)); };
     a.n = div(rows_per_seq); a.G = div((size_t)pl.G); a.kvh = div(kv_heads);
     a.np = div((size_t)pl.np); a.nt = div((size_t)pl.nt);
     auto cut = [&](const PrefixPlan::Cut& c) { return PrefixAttn::Cut{div((size_t)c.tp), div((size_t)c.tt), (int)c.blocks_p}; };
