@@ -236,6 +236,19 @@ MYL_FN int32_t softmax_div_round_pos(int32_t num, int32_t s, uint32_t m) {
     return (int32_t)q;
 }
 
+// n / d and n % d of index arithmetic by m = floor(2^32 / d) (at most 2^32 - 1), worked out on
+// the host, and one correction; 0 <= n < 2^31.
+struct SmallDiv {
+    uint32_t d, m;
+    static SmallDiv of(size_t d) { return SmallDiv{(uint32_t)d, recip32_u32((uint32_t)d)}; }
+};
+MYL_FN int divmod(const SmallDiv& d, int n, int& rem) {
+    const uint32_t q = (uint32_t)(((uint64_t)(uint32_t)n * d.m) >> 32), r = (uint32_t)n - q * d.d;
+    const bool up = r >= d.d;
+    rem = (int)(up ? r - d.d : r);
+    return (int)(up ? q + 1 : q);
+}
+
 // Unsigned 32-bit n % d without a hardware divide (small loops only: LUT row
 // selection pos % n_pos, done once per launch).
 MYL_FN uint32_t umod32_slow(uint32_t n, uint32_t d) {

@@ -31,12 +31,6 @@ namespace {
 
 constexpr int kQkTile = kPrefixQkTile, kPvTile = kPrefixPvTile;  // vectors of a block
 
-// n / d by the floor of 2^32 / d (at most 2^32 - 1) and one correction.
-struct SmallDiv {
-    uint32_t d, m;
-    static SmallDiv of(size_t d) { return SmallDiv{(uint32_t)d, recip32_u32((uint32_t)d)}; }
-};
-
 // The call, as every kernel sees it.  Row r = seq * rows_per_seq + i attends
 // keys 0 .. P-1 of the prefix, then the first lens[r] of its sequence's tail.
 struct PrefixAttn {
@@ -58,13 +52,6 @@ struct PrefixAttn {
     uint32_t pairs, lut_len;
     uint8_t shift, lut_shift, prob_frac;
 };
-
-__device__ inline int divmod(const SmallDiv& d, int n, int& rem) {
-    uint32_t q = __umulhi((uint32_t)n, d.m), r = (uint32_t)n - q * d.d;
-    const bool up = r >= d.d;
-    rem = (int)(up ? r - d.d : r);
-    return (int)(up ? q + 1 : q);
-}
 
 // The slot of sequence s, or -1; tail positions of row r (-1: left out).
 __device__ inline int slot_of(const PrefixAttn& a, int s) {

@@ -107,4 +107,45 @@ inline PrefixPlan prefix_plan(const PrefixShape& s, int cus) {
     return p;
 }
 
+// ---- draft verification -------------------------------------------------------
+
+constexpr size_t kVerifyMaxVocab = (size_t)1 << 20, kVerifyMaxDrafts = 1024, kVerifyMaxLut = 32768;
+constexpr size_t kVerifyMaxRows = 65535;
+constexpr int kVerifyChunk = 8192;  // values of a row per block
+
+struct VerifyShape {
+    size_t n_seqs, k, vocab, lut_len;
+};
+
+inline const char* verify_refuse(const VerifyShape& s) {
+    if (s.vocab == 0 || s.vocab > kVerifyMaxVocab) return "the vocabulary must hold 1 to 2^20 tokens";
+    if (s.k > kVerifyMaxDrafts || s.n_seqs > kVerifyMaxRows || s.n_seqs * (2 * s.k + 1) > kVerifyMaxRows)
+        return "too many drafts (1024 a sequence) or rows (65535)";
+    if (s.lut_len > kVerifyMaxLut) return "the exp table must hold 1 to 32768 entries";
+    return nullptr;
+}
+
+// bins: how far below its maximum a logit can lie and have a weight, at four table entries a
+// step; words: pairs of 16-bit counters for them.
+struct VerifyPlan {
+    int chunks;
+    uint32_t bins, words;
+    size_t off_stat, off_max, off_counts, off_sums, bytes;
+};
+
+inline VerifyPlan verify_plan(const VerifyShape& s) {
+    VerifyPlan p{};
+    p.chunks = (int)((s.vocab + kVerifyChunk - 1) / kVerifyChunk);
+    p.bins = (uint32_t)((s.lut_len + 3) / 4);
+    p.words = (p.bins + 1) / 2;
+    const size_t rows = s.n_seqs * (2 * s.k + 1), c = (size_t)p.chunks;
+    Layout l;
+    p.off_stat = l.take(rows, 16);
+    p.off_max = l.take(rows * c, 4);
+    p.off_counts = l.take(rows * c * p.words, 4);
+    p.off_sums = l.take(std::max(s.n_seqs * c * (kVerifyChunk / 256), rows * c), 8);
+    p.bytes = std::max<size_t>(l.used, 256);
+    return p;
+}
+
 }  // namespace myl
