@@ -130,7 +130,7 @@ inline const char* verify_refuse(const VerifyShape& s) {
 struct VerifyPlan {
     int chunks;
     uint32_t bins, words;
-    size_t off_stat, off_max, off_counts, off_sums, bytes;
+    size_t off_stat, off_max, off_counts, off_sums, off_first, bytes;
 };
 
 inline VerifyPlan verify_plan(const VerifyShape& s) {
@@ -144,6 +144,7 @@ inline VerifyPlan verify_plan(const VerifyShape& s) {
     p.off_max = l.take(rows * c, 4);
     p.off_counts = l.take(rows * c * p.words, 4);
     p.off_sums = l.take(std::max(s.n_seqs * c * (kVerifyChunk / 256), rows * c), 8);
+    p.off_first = l.take(s.n_seqs, 4);
     p.bytes = std::max<size_t>(l.used, 256);
     return p;
 }

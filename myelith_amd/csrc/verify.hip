@@ -50,6 +50,7 @@ struct Verify {
     uint32_t* counts;      // [rows][chunks][words]
     uint64_t* sums;        // [sequences][chunks][kVerifyChunk / 256]
     uint64_t* keys;        // greedy: [rows][chunks]
+    int32_t* first;        // [sequences] accepted drafts
 };
 
 struct RowStat {
@@ -58,7 +59,9 @@ struct RowStat {
     uint64_t s;  // the sum of the weights
 };
 
-constexpr int kBlk = 256, kGroups = kVerifyChunk / 1024;  // threads; quads of a thread in a chunk
+constexpr int kBlk = 256, kWeightThreads = 1024;
+template <int THREADS>
+constexpr int kGroups = kVerifyChunk / (4 * THREADS);  // quads of a thread in a chunk
 
 // Four consecutive values of a row: rows start at any 4-byte address.
 typedef int32_t RowQuad __attribute__((ext_vector_type(4), aligned(4)));
@@ -88,11 +91,12 @@ __device__ inline const int32_t* row_of(const Verify& a, int r) {
     return rem < n ? a.draft + (size_t)(r - T) * a.ldd : nullptr;
 }
 
-// A thread's quads of a chunk, kGroups of them 1024 values apart: f(i, quad, values of it in the row).
-__device__ inline void load_chunk(const int32_t* __restrict__ z, int V, int c0, RowQuad (&v)[kGroups], int (&n)[kGroups]) {
+// A thread's quads of a chunk, 4 THREADS values apart, and how many values of each lie in the row.
+template <int THREADS>
+__device__ inline void load_chunk(const int32_t* __restrict__ z, int V, int c0, RowQuad (&v)[kGroups<THREADS>], int (&n)[kGroups<THREADS>]) {
 #pragma unroll
-    for (int q = 0; q < kGroups; ++q) {
-        const int i = c0 + q * 1024 + 4 * (int)threadIdx.x;
+    for (int q = 0; q < kGroups<THREADS>; ++q) {
+        const int i = c0 + q * 4 * THREADS + 4 * (int)threadIdx.x;
         n[q] = min(max(V - i, 0), 4);
         if (n[q] == 4) v[q] = *reinterpret_cast<const RowQuad*>(z + i);
         else
@@ -107,16 +111,16 @@ __global__ __launch_bounds__(kBlk) void verify_count_kernel(Verify a) {
     const int c = blockIdx.x, r = blockIdx.y, tid = threadIdx.x;
     const int32_t* z = row_of(a, r);
     if (!z) return;
-    RowQuad v[kGroups];
-    int n[kGroups];
-    load_chunk(z, a.V, c * kVerifyChunk, v, n);
+    RowQuad v[kGroups<kBlk>];
+    int n[kGroups<kBlk>];
+    load_chunk<kBlk>(z, a.V, c * kVerifyChunk, v, n);
     for (uint32_t i = tid; i < a.words * 2; i += kBlk) cnt[i] = 0;
     int32_t mx = INT32_MIN;
 #pragma unroll
-    for (int q = 0; q < kGroups; ++q) mx = max(max(mx, max(v[q][0], v[q][1])), max(v[q][2], v[q][3]));
+    for (int q = 0; q < kGroups<kBlk>; ++q) mx = max(max(mx, max(v[q][0], v[q][1])), max(v[q][2], v[q][3]));
     mx = block_max_i32_dpp(mx, red);  // its barrier also publishes the cleared counters
 #pragma unroll
-    for (int q = 0; q < kGroups; ++q) {
+    for (int q = 0; q < kGroups<kBlk>; ++q) {
         // a value that fills the wave's quads is counted once: the lanes' adds to one counter follow one another
         const int32_t first = __builtin_amdgcn_readfirstlane(v[q][0]);
         if (__all(n[q] == 4 && v[q][0] == first && v[q][1] == first && v[q][2] == first && v[q][3] == first)) {
@@ -137,30 +141,64 @@ __global__ __launch_bounds__(kBlk) void verify_count_kernel(Verify a) {
     if (tid == 0) a.cmax[(size_t)r * a.chunks + c] = mx;
 }
 
+// The weights of the bins in LDS, by a block of THREADS: the first entries are on their way
+// while the block loads what else it needs.  A barrier follows before they are read.
+template <int THREADS>
+struct BinWeights {
+    static constexpr int kEach = 1024 / THREADS;
+    uint32_t w[kEach];
+    __device__ inline void load(const Verify& a) {
+#pragma unroll
+        for (int i = 0; i < kEach; ++i) w[i] = weight_below(a, threadIdx.x + i * THREADS);
+    }
+    __device__ inline void store(const Verify& a, uint16_t* wt) const {
+#pragma unroll
+        for (int i = 0; i < kEach; ++i)
+            if (threadIdx.x + i * THREADS < a.bins) wt[threadIdx.x + i * THREADS] = (uint16_t)w[i];
+        for (uint32_t i = threadIdx.x + 1024; i < a.bins; i += THREADS) wt[i] = (uint16_t)weight_below(a, i);
+    }
+};
+
 // A wave per chunk: its counts against the table, shifted by how far its maximum is below the row's.
-__global__ __launch_bounds__(kBlk) void verify_sum_kernel(Verify a) {
-    __shared__ uint64_t red[kBlk / 64];
+// 16 waves: with four, 19 chunks of a row came one after another (13.7 us for 264 rows of 152064, now 5.8).
+constexpr int kSumThreads = 1024;
+__global__ __launch_bounds__(kSumThreads) void verify_sum_kernel(Verify a) {
+    extern __shared__ uint16_t wt[];
+    __shared__ uint64_t red[kSumThreads / 64];
     const int r = blockIdx.x, tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
     if (!row_of(a, r)) return;
     const int32_t* cm = a.cmax + (size_t)r * a.chunks;
+    BinWeights<kSumThreads> bw;
+    bw.load(a);
     int32_t mx = INT32_MIN;
     for (int c = lane; c < a.chunks; c += 64) mx = max(mx, cm[c]);
+    bw.store(a, wt);
     mx = wave_max_i32(mx);
+    __syncthreads();
     uint64_t s = 0;
-    for (int c = w; c < a.chunks; c += kBlk / 64) {
+    for (int c = w; c < a.chunks; c += kSumThreads / 64) {
         const uint32_t d = (uint32_t)mx - (uint32_t)cm[c];
         if (d >= a.bins) continue;
         const uint32_t* n = a.counts + ((size_t)r * a.chunks + c) * a.words;
-#pragma unroll 4
-        for (uint32_t i = lane; i < a.words; i += 64) {
-            const uint32_t two = n[i];
-            s += (uint64_t)(two & 0xFFFFu) * weight_below(a, d + 2 * i) + (uint64_t)(two >> 16) * weight_below(a, d + 2 * i + 1);
+        for (uint32_t i0 = lane; i0 < a.words; i0 += 8 * 64) {
+            uint32_t two[8];
+#pragma unroll
+            for (int k = 0; k < 8; ++k) two[k] = i0 + 64 * k < a.words ? n[i0 + 64 * k] : 0;
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+                const uint32_t at = d + 2 * (i0 + 64 * k);
+                if (two[k] & 0xFFFFu) s += (uint64_t)(two[k] & 0xFFFFu) * (at < a.bins ? wt[at] : 0u);
+                if (two[k] >> 16) s += (uint64_t)(two[k] >> 16) * (at + 1 < a.bins ? wt[at + 1] : 0u);
+            }
         }
     }
     s = wave_sum_u64(s);
     if (lane == 0) red[w] = s;
     __syncthreads();
-    if (tid == 0) a.stat[r] = RowStat{mx, 0, red[0] + red[1] + red[2] + red[3]};
+    if (w == 0) {
+        s = wave_sum_u64(lane < kSumThreads / 64 ? red[lane] : 0);
+        if (lane == 0) a.stat[r] = RowStat{mx, 0, s};
+    }
 }
 
 // How a sequence's drafts end: the accepted ones, and the weights of the next
@@ -173,8 +211,8 @@ struct Ending {
     int64_t not_j;
 };
 
-// Whole block: every draft is tested at once, the first that fails ends them.
-__device__ inline Ending verify_ending(const Verify& a, int b, int* s_first) {
+// The first draft that fails, all tested at once by the whole block.
+__device__ inline int verify_first(const Verify& a, int b, int* s_first) {
     const int T = a.B * (a.k + 1), nd = drafts_of(a, b);
     if (threadIdx.x == 0) *s_first = nd;
     __syncthreads();
@@ -195,8 +233,13 @@ __device__ inline Ending verify_ending(const Verify& a, int b, int* s_first) {
         if (!ok) atomicMin(s_first, i);
     }
     __syncthreads();
+    return *s_first;
+}
+
+__device__ inline Ending verify_ending(const Verify& a, int b, int first) {
+    const int T = a.B * (a.k + 1), nd = drafts_of(a, b);
     Ending e{};
-    e.n = *s_first;
+    e.n = first;
     const int tr = b * (a.k + 1) + e.n, dr = b * a.k + e.n;
     const RowStat p = a.stat[tr];
     e.prow = a.target + (size_t)tr * a.ldt;
@@ -225,23 +268,42 @@ __device__ inline uint64_t ending_weight(const Verify& a, const Ending& e, int j
     return x > y ? x - y : 0;
 }
 
-// The next token's weights, summed over every 256 values (a wave's quads): Grid (chunks, sequences).
-__global__ __launch_bounds__(kBlk) void verify_weight_kernel(Verify a) {
+// The next token's weights, summed over every 256 values (a wave's quads).  Grid (chunks,
+// sequences).  Both rows' quads are loaded together and the table waits in LDS: a lookup
+// and a load of q per value that has a weight, one after another, took longer (24 sequences:
+// 15.9 us, now 9.4), as did 256 threads, which come to eight wave sums each (12.7).
+__global__ __launch_bounds__(kWeightThreads) void verify_weight_kernel(Verify a) {
+    extern __shared__ uint16_t wt[];
     __shared__ int s_first;
     const int c = blockIdx.x, b = blockIdx.y, tid = threadIdx.x;
-    const Ending e = verify_ending(a, b, &s_first);
-    RowQuad v[kGroups];
-    int n[kGroups];
-    load_chunk(e.prow, a.V, c * kVerifyChunk, v, n);
+    BinWeights<kWeightThreads> bw;
+    bw.load(a);
+    const int first = verify_first(a, b, &s_first);
+    const Ending e = verify_ending(a, b, first);
+    RowQuad v[kGroups<kWeightThreads>], u[kGroups<kWeightThreads>];
+    int n[kGroups<kWeightThreads>];
+    load_chunk<kWeightThreads>(e.prow, a.V, c * kVerifyChunk, v, n);
+    if (e.qrow) load_chunk<kWeightThreads>(e.qrow, a.V, c * kVerifyChunk, u, n);
+    bw.store(a, wt);
+    __syncthreads();
+    if (c == 0 && tid == 0) a.first[b] = first;
     uint64_t* out = a.sums + ((size_t)b * a.chunks + c) * (kVerifyChunk / 256);
+    auto at = [&](int32_t m, int32_t z) -> uint64_t {
+        const uint32_t below = (uint32_t)m - (uint32_t)z;
+        return below < a.bins ? wt[below] : 0u;
+    };
 #pragma unroll
-    for (int q = 0; q < kGroups; ++q) {
+    for (int q = 0; q < kGroups<kWeightThreads>; ++q) {
         uint64_t s = 0;
 #pragma unroll
-        for (int k = 0; k < 4; ++k)
-            if (k < n[q]) s += ending_weight(a, e, c * kVerifyChunk + q * 1024 + 4 * tid + k, v[q][k]);
+        for (int k = 0; k < 4; ++k) {
+            uint64_t p = at(e.pm, v[q][k]);
+            if (k >= n[q] || c * kVerifyChunk + q * 4 * kWeightThreads + 4 * tid + k == e.not_j) p = 0;
+            const uint64_t x = p * e.Q, y = e.qrow ? at(e.qm, u[q][k]) * e.P : 0;
+            s += x > y ? x - y : 0;
+        }
         s = wave_sum_u64(s);
-        if ((tid & 63) == 0) out[q * 4 + (tid >> 6)] = s;
+        if ((tid & 63) == 0) out[q * (kWeightThreads / 64) + (tid >> 6)] = s;
     }
 }
 
@@ -313,7 +375,7 @@ __device__ inline int64_t first_max(const int32_t* z, int V, uint64_t* red) {
 }
 
 __global__ __launch_bounds__(kBlk) void verify_pick_kernel(Verify a) {
-    __shared__ int s_first, s_pick;
+    __shared__ int s_pick;
     __shared__ myl_u128 red[kBlk];
     const int b = blockIdx.x, tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
     // each thread: `per` of the sequence's sums, in order (at most 2^20 / 256 / kBlk = 16)
@@ -322,7 +384,7 @@ __global__ __launch_bounds__(kBlk) void verify_pick_kernel(Verify a) {
     const uint64_t r = a.randoms[(size_t)b * (a.k + 1) + a.k];
     myl_u128 own = 0;
     for (int i = 0; i < per; ++i) own += tid * per + i < groups ? sums[tid * per + i] : 0;
-    Ending e = verify_ending(a, b, &s_first);
+    Ending e = verify_ending(a, b, a.first[b]);
     red[tid] = own;
     __syncthreads();
     // running totals of the 256 shares: 64 lanes of each wave, four shares each
@@ -402,13 +464,13 @@ __global__ __launch_bounds__(kBlk) void verify_max_kernel(Verify a) {
     const int c = blockIdx.x, r = blockIdx.y, tid = threadIdx.x;
     const int32_t* z = row_of(a, r);
     if (!z) return;
-    RowQuad v[kGroups];
-    int n[kGroups];
-    load_chunk(z, a.V, c * kVerifyChunk, v, n);
+    RowQuad v[kGroups<kBlk>];
+    int n[kGroups<kBlk>];
+    load_chunk<kBlk>(z, a.V, c * kVerifyChunk, v, n);
     int32_t best = INT32_MIN;
     int at = -1;
 #pragma unroll
-    for (int q = 0; q < kGroups; ++q)
+    for (int q = 0; q < kGroups<kBlk>; ++q)
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
             const bool up = (e < n[q]) & ((v[q][e] > best) | (at < 0));
@@ -499,6 +561,7 @@ int myl_verify_drafts_dev(myl_ctx* ctx, const int32_t* target, size_t ldt, const
     a.counts = reinterpret_cast<uint32_t*>(ws + pl.off_counts);
     a.sums = reinterpret_cast<uint64_t*>(ws + pl.off_sums);
     a.keys = reinterpret_cast<uint64_t*>(ws + pl.off_sums);
+    a.first = reinterpret_cast<int32_t*>(ws + pl.off_first);
     const unsigned T = (unsigned)(a.B * (a.k + 1)), rows = T + (draft ? (unsigned)(a.B * a.k) : 0u), chunks = (unsigned)pl.chunks;
     if (!exp_lut) {
         verify_max_kernel<<<dim3(chunks, T), kBlk, 0, st>>>(a);
@@ -506,8 +569,8 @@ int myl_verify_drafts_dev(myl_ctx* ctx, const int32_t* target, size_t ldt, const
         return ctx->hip(hipGetLastError(), what);
     }
     verify_count_kernel<<<dim3(chunks, rows), kBlk, (size_t)pl.words * 8, st>>>(a);
-    verify_sum_kernel<<<rows, kBlk, 0, st>>>(a);
-    verify_weight_kernel<<<dim3(chunks, (unsigned)a.B), kBlk, 0, st>>>(a);
+    verify_sum_kernel<<<rows, kSumThreads, (size_t)pl.bins * 2, st>>>(a);
+    verify_weight_kernel<<<dim3(chunks, (unsigned)a.B), kWeightThreads, (size_t)pl.bins * 2, st>>>(a);
     verify_pick_kernel<<<a.B, kBlk, 0, st>>>(a);
     return ctx->hip(hipGetLastError(), what);
 }
