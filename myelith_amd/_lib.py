@@ -89,7 +89,7 @@ SIGNATURES: dict[str, tuple] = {
     "myl_argmax_dev": (INT, [P, P, sz, sz, sz, P]),
     "myl_sample_dev": (INT, [P, P, sz, sz, sz, P, P, P]),
     "myl_logsoftmax_dev": (INT, [P, P, sz, sz, sz, P, sz, P, P]),
-    "myl_linear_w8a16_adapters_workspace": (sz, [P, sz, sz, sz, sz]),
+    "myl_linear_w8a16_adapters_workspace": (sz, [P, sz, sz, sz, sz, sz]),
     "myl_linear_w8a16_adapters_dev": (INT, [P, P, sz, sz, P, sz, sz, P, u8, u8, P, P, P, P, u8, P, P, sz, sz, P, sz, P, sz]),
     "myl_attention_prefix_workspace": (sz, [P, sz, sz, sz, sz, sz, sz, sz]),
     "myl_attention_prefix_dev": (INT, [P, P, sz, sz, sz, sz, sz, sz, P, P, sz, sz, P, P, sz, sz, sz, sz, P, P, i64, u8,

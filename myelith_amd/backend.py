@@ -385,7 +385,8 @@ class RocmBackend:
 
     def linear_w8a16_adapters_workspace(self, x, W, A):
         """A workspace for linear_w8a16_adapters_dev on operands of these shapes."""
-        n = lib().myl_linear_w8a16_adapters_workspace(self._h, x.shape[0], W.shape[0], x.shape[1], A.shape[1])
+        n = lib().myl_linear_w8a16_adapters_workspace(self._h, x.shape[0], W.shape[0], x.shape[1], A.shape[1],
+                                                      A.shape[0])
         return self._new_workspace(n, x.device, "linear_w8a16_adapters_dev")
 
     def linear_w8a16_adapters_dev(self, x, W, w_shifts, act_frac: int, ids, A, a_shifts, mid_frac: int, B, b_shifts,
@@ -409,7 +410,7 @@ class RocmBackend:
             out = torch.empty((M, N), dtype=torch.int16, device=x.device)
         _need_dev(what, x.device, out=(out, "int16", None))
         _need(tuple(out.shape) == (M, N) and _strides(out)[1] in (0, 1), f"{what}: out must be [M x N]")
-        ws = self._workspace(lib().myl_linear_w8a16_adapters_workspace(self._h, M, N, K, rank), x.device, workspace)
+        ws = self._workspace(lib().myl_linear_w8a16_adapters_workspace(self._h, M, N, K, rank, n), x.device, workspace)
         rc = lib().myl_linear_w8a16_adapters_dev(
             self._h, x.data_ptr(), M, _strides(x)[0] or K, W.data_ptr(), N, K, w_shifts.data_ptr(), act_frac, out_frac,
             None if out_frac_pc is None else out_frac_pc.data_ptr(), ids.data_ptr(), A.data_ptr(), a_shifts.data_ptr(),

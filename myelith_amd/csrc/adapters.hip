@@ -5,80 +5,444 @@
 //   d[m] = linear_w8a16(u[m], B[id], b_shifts[id], mid_frac, out_frac)   [N]
 //   out[m] = clamp_i16(linear_w8a16(x[m], W, w_shifts, act_frac, out_frac) + d[m])
 // with id = ids[m]; a row whose id is outside [0, n_adapters) has d = 0.
+//
+//   adapters_down_kernel  rows of one adapter together, x A over slices of K: exact i64 sums
+//   linear_w8a16          the shared product into out
+//   adapters_up_kernel    u from the slices' sums, u B, added to out
+//
+// Both run on the int8 matrix cores over the byte planes x = 256 hi + lo' + 128
+// (gemm_mfma.h), the sums of the weights from a third product with a vector of ones.
 #include "abi_internal.h"
 #include "gemm_dispatch.h"
+#include "qk_planes.h"
+#include "serve_plan.h"
 
 #include <algorithm>
 #include <string>
 
 namespace myl {
-
-// One wave per (row, rank index).
-__global__ __launch_bounds__(64) void adapters_down_kernel(const int16_t* __restrict__ x, int ldx, int K,
-                                                           const int32_t* __restrict__ ids, int n_adapters, int rank,
-                                                           const int8_t* __restrict__ A,
-                                                           const uint8_t* __restrict__ a_shifts, uint8_t act_frac,
-                                                           uint8_t mid_frac, int16_t* __restrict__ u) {
-    const int m = blockIdx.x, j = blockIdx.y;
-    const int id = ids[m];
-    if (id < 0 || id >= n_adapters) return;
-    const int16_t* xr = x + (size_t)m * ldx;
-    const int8_t* a = A + ((size_t)id * rank + j) * K;
-    int64_t acc = 0;
-    for (int k = threadIdx.x; k < K; k += 64) acc += (int32_t)xr[k] * (int32_t)a[k];
-    acc = wave_sum_i64(acc);
-    if (threadIdx.x == 0)
-        u[(size_t)m * rank + j] =
-            clamp_i16_i64(rescale64(acc, (uint8_t)(a_shifts[(size_t)id * rank + j] + act_frac), mid_frac));
-}
-
-// One thread per output.
-__global__ __launch_bounds__(256) void adapters_up_kernel(const int16_t* __restrict__ u, const int32_t* __restrict__ ids,
-                                                          int n_adapters, int rank, const int8_t* __restrict__ B,
-                                                          const uint8_t* __restrict__ b_shifts, uint8_t mid_frac,
-                                                          uint8_t out_frac, const uint8_t* __restrict__ out_frac_pc,
-                                                          int N, int16_t* __restrict__ out, int ldo) {
-    const int m = blockIdx.y, n = blockIdx.x * 256 + threadIdx.x;
-    const int id = ids[m];
-    if (n >= N || id < 0 || id >= n_adapters) return;
-    const int8_t* b = B + ((size_t)id * N + n) * rank;
-    int32_t acc = 0;
-    for (int j = 0; j < rank; ++j) acc += (int32_t)u[(size_t)m * rank + j] * (int32_t)b[j];
-    const int16_t d = clamp_i16_i64(rescale64(acc, (uint8_t)(b_shifts[(size_t)id * N + n] + mid_frac),
-                                              out_frac_pc ? out_frac_pc[n] : out_frac));
-    int16_t* o = out + (size_t)m * ldo + n;
-    *o = clamp_i16((int32_t)*o + (int32_t)d);
-}
-
-__global__ __launch_bounds__(256) void adapters_clear_kernel(unsigned long long* __restrict__ p, size_t n) {
-    for (size_t i = (size_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (size_t)gridDim.x * 256) p[i] = 0;
-}
-
 namespace {
 
-constexpr size_t kMaxRank = 256;               // |sum B u| <= 2^7 2^15 2^8 = 2^30
-constexpr size_t kAccElems = (size_t)512 << 10;  // products with more outputs do not split K
-
-// The workspace: the shared product's byte planes and split-K sums, and u.
-struct Space {
-    int8_t* planes = nullptr;
-    unsigned long long* acc = nullptr;
-    size_t planes_bytes = 0, acc_elems = 0, bytes = 0;
-    int16_t* u = nullptr;
-    static Space of(void* base, size_t M, size_t N, size_t K, size_t rank) {
-        Carve c{(char*)base};
-        Space s;
-        if (M >= 2) {
-            s.planes_bytes = 2 * M * K;
-            s.acc_elems = M * N <= kAccElems ? M * N : 0;
-            s.planes = c.take<int8_t>(s.planes_bytes);
-            s.acc = c.take<unsigned long long>(std::max<size_t>(s.acc_elems, 1));
-        }
-        s.u = c.take<int16_t>(M * rank);
-        s.bytes = c.used ? c.used : 256;  // 0 stands for sizes that a call refuses
-        return s;
-    }
+// The rows of one adapter among a window's: up to 64 of them for the kernel that adds u B.
+struct TileRows {
+    int32_t id, rows;  // rows 0: nothing to do
+    uint8_t at[64];    // places in the window
 };
+static_assert(sizeof(TileRows) == kAdapterTileBytes);
+
+struct Adapters {
+    const int16_t* x;
+    const int32_t* ids;
+    const int8_t *A, *B;
+    const uint8_t *a_shifts, *b_shifts, *out_frac_pc;
+    int16_t* out;
+    int64_t* part;    // [split][M][rank_pad]
+    TileRows* tiles;  // [window][slot]
+    uint64_t* acc;    // cleared for the shared product
+    size_t acc_elems, ldx, ldo, b_bytes;
+    int M, N, K, rank, rank_pad, n, splits, per_wave, units, n_chunk;
+    SmallDiv slots;
+    uint8_t act_frac, mid_frac, out_frac;
+};
+
+// Rows of A, B and x start anywhere.
+typedef uint32_t Bytes16 __attribute__((ext_vector_type(4), aligned(1)));
+typedef uint32_t Halves8 __attribute__((ext_vector_type(4), aligned(2)));
+typedef uint32_t Bytes8 __attribute__((ext_vector_type(2), aligned(1)));
+
+__device__ inline v4i32_t operand(const Bytes16& v) { return v4i32_t{(int)v[0], (int)v[1], (int)v[2], (int)v[3]}; }
+// 16 int16 as their byte planes.
+__device__ inline void planes16(const Halves8 (&x)[2], v4i32_t& h, v4i32_t& l) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const uint32_t a = x[i >> 1][2 * (i & 1)], b = x[i >> 1][2 * (i & 1) + 1];
+        h[i] = (int)__builtin_amdgcn_perm(b, a, 0x07050301u);
+        l[i] = (int)(__builtin_amdgcn_perm(b, a, 0x06040200u) ^ 0x80808080u);
+    }
+}
+__device__ inline v4i32_t mfma(const v4i32_t& a, const v4i32_t& b, const v4i32_t& c) {
+    return __builtin_amdgcn_mfma_i32_16x16x64_i8(a, b, c, 0, 0, 0);
+}
+
+// ---- tiles of rows ---------------------------------------------------------------
+
+struct Grouping {
+    alignas(16) int32_t id[kAdapterWindow];
+    uint64_t leads[4];
+    int32_t tile_id, first, rows[4];
+    uint8_t at[16];
+};
+
+// Tile t of window w: a row's number among its adapter's rows in the window is a count of
+// equal ids before it, every 16th of them leads a tile, and tiles are numbered in the order
+// of the rows that lead them.  Each block works its tile out: a launch to sort the rows
+// first would take longer than the at most 256 compares of a thread.  Returns the tile's
+// rows (0: no such tile), their places in s.at and its adapter in s.tile_id; `full`, if not
+// null, gets 64 rows from the first tile of each 64.
+__device__ inline int group_rows(const Adapters& a, int w, int t, Grouping& s, TileRows* full) {
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int rows = min(kAdapterWindow, a.M - w * kAdapterWindow);
+    int id = tid < rows ? a.ids[(size_t)w * kAdapterWindow + tid] : -1;
+    if ((uint32_t)id >= (uint32_t)a.n) id = -1;
+    s.id[tid] = id;
+    if (tid == 0) s.tile_id = -1;
+    __syncthreads();
+    int c = 0;
+    if (64 * wave < rows) {
+        for (int i = 0; i < 64 * wave; i += 4) {
+            const int4 q = *reinterpret_cast<const int4*>(&s.id[i]);
+            c += (q.x == id) + (q.y == id) + (q.z == id) + (q.w == id);
+        }
+        const int own = min(64, rows - 64 * wave);
+        for (int i = 0; i < own; ++i) c += __builtin_amdgcn_readlane(id, i) == id && i < lane;
+    }
+    const bool lead = id >= 0 && (c & 15) == 0;
+    const uint64_t b = __ballot(lead);
+    if (lane == 0) s.leads[wave] = b;
+    __syncthreads();
+    int mine = __popcll(b & ((1ull << lane) - 1ull));
+    for (int v = 0; v < wave; ++v) mine += __popcll(s.leads[v]);
+    if (lead && mine == t) {
+        s.tile_id = id;
+        s.first = c;
+    }
+    __syncthreads();
+    const int tile_id = s.tile_id, first = s.first;
+    if (tile_id < 0) {
+        if (full && tid == 0) full->rows = 0;
+        return 0;
+    }
+    const bool member = id == tile_id && c >= first;
+    if (member && c < first + 16) s.at[c - first] = (uint8_t)tid;
+    if (full && (first & 63) == 0 && member && c < first + 64) full->at[c - first] = (uint8_t)tid;
+    const uint64_t m = __ballot(member);
+    if (lane == 0) s.rows[wave] = __popcll(m);
+    __syncthreads();
+    const int all = s.rows[0] + s.rows[1] + s.rows[2] + s.rows[3];
+    if (full && tid == 0) {
+        full->id = tile_id;
+        full->rows = (first & 63) == 0 ? min(all, 64) : 0;
+    }
+    return min(all, 16);
+}
+
+// ---- x A --------------------------------------------------------------------------
+
+// Grid (windows x slots, rank groups, splits of K); 256 threads.  Lane l holds row l % 16 of
+// A and of x at 16 (l / 16) of each 64 of K: two matrix steps use up a line of A.  A wave
+// loads the next unit while it multiplies one.
+template <int RT>
+__global__ __launch_bounds__(256, 2) void adapters_down_kernel(Adapters a) {
+    __shared__ Grouping s;
+    __shared__ int64_t red[4][RT][4][64];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const size_t block = ((size_t)blockIdx.z * gridDim.y + blockIdx.y) * gridDim.x + blockIdx.x;
+    for (size_t i = block * 256 + tid; i < a.acc_elems; i += (size_t)gridDim.x * gridDim.y * gridDim.z * 256) a.acc[i] = 0;
+    int t;
+    const int w = divmod(a.slots, (int)blockIdx.x, t);
+    const int rows = group_rows(a, w, t, s, blockIdx.y == 0 && blockIdx.z == 0 ? a.tiles + blockIdx.x : nullptr);
+    if (rows == 0) return;
+    const int col = lane & 15, kq = lane >> 4;
+    const size_t row = (size_t)w * kAdapterWindow + s.at[min(col, rows - 1)];
+    const int16_t* x = a.x + row * a.ldx + 16 * kq;
+    const int8_t* A[RT];
+    const int j0 = 16 * RT * (int)blockIdx.y;
+#pragma unroll
+    for (int r = 0; r < RT; ++r)
+        A[r] = a.A + ((size_t)s.tile_id * (size_t)a.rank + (size_t)min(j0 + 16 * r + col, a.rank - 1)) * (size_t)a.K + 16 * kq;
+
+    struct Unit {
+        Halves8 x[2][2];
+        Bytes16 a[2][RT];
+    };
+    const v4i32_t one = {0x01010101, 0x01010101, 0x01010101, 0x01010101};
+    v4i32_t hi[RT], lo[RT], ones[RT];
+#pragma unroll
+    for (int r = 0; r < RT; ++r) hi[r] = lo[r] = ones[r] = v4i32_t{0, 0, 0, 0};
+    auto load = [&](Unit& v, int u) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const size_t k = (size_t)u * kAdapterUnit + 64 * h;
+#pragma unroll
+            for (int r = 0; r < RT; ++r) v.a[h][r] = *reinterpret_cast<const Bytes16*>(A[r] + k);
+            v.x[h][0] = *reinterpret_cast<const Halves8*>(x + k);
+            v.x[h][1] = *reinterpret_cast<const Halves8*>(x + k + 8);
+        }
+    };
+    auto multiply = [&](const Unit& v) {
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            v4i32_t xh, xl;
+            planes16(v.x[h], xh, xl);
+#pragma unroll
+            for (int r = 0; r < RT; ++r) {
+                const v4i32_t w8 = operand(v.a[h][r]);
+                hi[r] = mfma(w8, xh, hi[r]);
+                lo[r] = mfma(w8, xl, lo[r]);
+                ones[r] = mfma(w8, one, ones[r]);
+            }
+        }
+    };
+    const int64_t first = ((int64_t)blockIdx.z * 4 + wave) * a.per_wave;
+    const int u0 = (int)min(first, (int64_t)a.units), u1 = (int)min(first + a.per_wave, (int64_t)a.units);
+    const int whole = min(u1, a.K / kAdapterUnit);
+    if (u0 < whole) {
+        Unit v, next;
+        load(v, u0);
+        int u = u0;
+        for (; u + 2 <= whole; u += 2) {
+            load(next, u + 1);
+            multiply(v);
+            load(v, min(u + 2, whole - 1));
+            multiply(next);
+        }
+        if (u < whole) multiply(v);
+    }
+    if (u0 < u1 && whole < u1) {  // the end of K: zero weights past it
+        Unit v;
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+            const int k = whole * kAdapterUnit + 64 * h, left = a.K - k - 16 * kq;
+#pragma unroll
+            for (int r = 0; r < RT; ++r) v.a[h][r] = Bytes16{0, 0, 0, 0};
+            v.x[h][0] = v.x[h][1] = Halves8{0, 0, 0, 0};
+            if (left >= 16) {
+#pragma unroll
+                for (int r = 0; r < RT; ++r) v.a[h][r] = *reinterpret_cast<const Bytes16*>(A[r] + k);
+                v.x[h][0] = *reinterpret_cast<const Halves8*>(x + k);
+                v.x[h][1] = *reinterpret_cast<const Halves8*>(x + k + 8);
+            } else {
+#pragma unroll
+                for (int e = 0; e < 15; ++e)
+                    if (e < left) {
+#pragma unroll
+                        for (int r = 0; r < RT; ++r) v.a[h][r][e >> 2] |= (uint32_t)(uint8_t)A[r][k + e] << (8 * (e & 3));
+                        v.x[h][e >> 3][(e & 7) >> 1] |= (uint32_t)(uint16_t)x[k + e] << (16 * (e & 1));
+                    }
+            }
+        }
+        multiply(v);
+    }
+#pragma unroll
+    for (int r = 0; r < RT; ++r)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) red[wave][r][e][lane] = (int64_t)hi[r][e] * 256 + (int64_t)lo[r][e] + (int64_t)ones[r][e] * 128;
+    __syncthreads();
+    // lane l: row l % 16 of the tile, rank rows 4 (l / 16) .. + 3
+    for (int r = wave; r < RT; r += 4) {
+        const int j = j0 + 16 * r + 4 * kq;
+        if (col >= rows || j >= a.rank_pad) continue;
+        int64_t* p = a.part + ((size_t)blockIdx.z * (size_t)a.M + row) * (size_t)a.rank_pad + j;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) p[e] = red[0][r][e][lane] + red[1][r][e][lane] + red[2][r][e][lane] + red[3][r][e][lane];
+    }
+}
+
+// ---- u B --------------------------------------------------------------------------
+
+// The 16 bytes from p on, those at `end` and behind it zero.
+__device__ inline v4i32_t bytes_until(const int8_t* p, const int8_t* end) {
+    uint64_t v[2] = {0, 0};
+#pragma nounroll
+    for (int e = 0; e < 8; ++e) {
+        if (p + e < end) v[0] |= (uint64_t)(uint8_t)p[e] << (8 * e);
+        if (p + e + 8 < end) v[1] |= (uint64_t)(uint8_t)p[e + 8] << (8 * e);
+    }
+    return v4i32_t{(int)v[0], (int)(v[0] >> 32), (int)v[1], (int)(v[1] >> 32)};
+}
+
+// 32 columns of B as the rows of two matrix operands, in an order that leaves a lane eight
+// columns that follow one another: column n0 + 8 (l / 16) + 4 q + e of row l % 16 in register
+// e of product q.  With them the lane's shifts.
+template <int KB>
+struct Columns {
+    v4i32_t w8[2][KB];
+    Bytes8 frac, to;
+};
+
+typedef short Short2 __attribute__((ext_vector_type(2)));
+
+// Grid (windows x slots, chunks of columns); 256 threads, KB steps of 64 of the rank.  The
+// rows' u lie in LDS as byte planes, zero from the rank on.  A wave loads the next columns
+// while it works on some, and all rows' outputs before it multiplies.
+template <int KB>
+__global__ __launch_bounds__(256) void adapters_up_kernel(Adapters a) {
+    constexpr int stride = 64 * KB + 16, quads = 16 * KB;
+    __shared__ __align__(16) int8_t plane[2][64 * stride];
+    __shared__ size_t place[64];
+    const TileRows* tile = a.tiles + blockIdx.x;
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), col = lane & 15, kq = lane >> 4;
+    const int at0 = tile->at[tid & 63], at1 = tile->at[tid / quads];
+    const int rows = __builtin_amdgcn_readfirstlane(tile->rows), id = __builtin_amdgcn_readfirstlane(tile->id);
+    if (rows == 0) return;
+    const int begin = (int)blockIdx.y * a.n_chunk, end = min(a.N, begin + a.n_chunk), subs = (rows + 15) >> 4;
+    const int8_t *B = a.B + (size_t)id * (size_t)a.N * (size_t)a.rank, *b_end = a.B + a.b_bytes;
+    const uint8_t* bs = a.b_shifts + (size_t)id * (size_t)a.N;
+
+    auto fetch = [&](Columns<KB>& c, int n0) {
+        const int8_t* b = B + (size_t)n0 * (size_t)a.rank;
+        if (n0 + 32 <= a.N && b + 31 * a.rank + 64 * KB <= b_end) {
+#pragma unroll
+            for (int q = 0; q < 2; ++q) {
+                const uint32_t off = (uint32_t)((8 * (col >> 2) + 4 * q + (col & 3)) * a.rank + 16 * kq);
+#pragma unroll
+                for (int k = 0; k < KB; ++k) c.w8[q][k] = operand(*reinterpret_cast<const Bytes16*>(b + off + 64 * k));
+            }
+            c.frac = *reinterpret_cast<const Bytes8*>(bs + n0 + 8 * kq);
+            if (a.out_frac_pc) c.to = *reinterpret_cast<const Bytes8*>(a.out_frac_pc + n0 + 8 * kq);
+        } else {
+#pragma unroll
+            for (int q = 0; q < 2; ++q) {
+                const int8_t* p = b + min(8 * (col >> 2) + 4 * q + (col & 3), a.N - 1 - n0) * a.rank + 16 * kq;
+#pragma unroll
+                for (int k = 0; k < KB; ++k) c.w8[q][k] = bytes_until(p + 64 * k, b_end);
+            }
+            c.frac = c.to = Bytes8{0, 0};
+#pragma nounroll
+            for (int e = 0; e < 4; ++e) {
+                const int n = min(n0 + 8 * kq + e, a.N - 1), m = min(n0 + 8 * kq + 4 + e, a.N - 1);
+                c.frac[0] |= (uint32_t)bs[n] << (8 * e);
+                c.frac[1] |= (uint32_t)bs[m] << (8 * e);
+                if (a.out_frac_pc) {
+                    c.to[0] |= (uint32_t)a.out_frac_pc[n] << (8 * e);
+                    c.to[1] |= (uint32_t)a.out_frac_pc[m] << (8 * e);
+                }
+            }
+        }
+        if (!a.out_frac_pc) c.to = Bytes8{a.out_frac * 0x01010101u, a.out_frac * 0x01010101u};
+    };
+    Columns<KB> cur, next;
+    int n0 = begin + 64 * wave;
+    if (n0 < end) fetch(cur, n0);
+
+    int t;
+    const size_t base = (size_t)divmod(a.slots, (int)blockIdx.x, t) * kAdapterWindow;
+    const int place0 = __shfl(at0, min(lane, rows - 1), 64);
+    if (tid < 64) place[tid] = (base + (size_t)place0) * a.ldo;
+    for (int i = tid, at = at1; i < rows * quads; i += 256) {
+        const int r = i / quads, j = 4 * (i % quads);
+        if (i != tid) at = tile->at[r];
+        uint32_t h = 0, l = 0;
+        if (j < a.rank) {
+            const int64_t* p = a.part + (base + (size_t)at) * (size_t)a.rank_pad + j;
+            int64_t sum[4] = {0, 0, 0, 0};
+#pragma unroll 4
+            for (int k = 0; k < a.splits; ++k)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) sum[e] += p[(size_t)k * (size_t)a.M * (size_t)a.rank_pad + e];
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                if (j + e < a.rank) {
+                    const uint8_t frac = (uint8_t)(a.a_shifts[(size_t)id * (size_t)a.rank + j + e] + a.act_frac);
+                    const uint32_t u = (uint16_t)clamp_i16_i64(rescale64(sum[e], frac, a.mid_frac));
+                    h |= (u >> 8) << (8 * e);
+                    l |= ((u & 255u) ^ 128u) << (8 * e);
+                }
+        }
+        *reinterpret_cast<uint32_t*>(&plane[0][r * stride + j]) = h;
+        *reinterpret_cast<uint32_t*>(&plane[1][r * stride + j]) = l;
+    }
+    __syncthreads();
+    v4i32_t one[KB];  // ones below the rank
+#pragma unroll
+    for (int b = 0; b < KB; ++b)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const int left = min(max(a.rank - 64 * b - 16 * kq - 4 * e, 0), 4);
+            one[b][e] = left == 0 ? 0 : 0x01010101 >> (8 * (4 - left));
+        }
+    size_t at[4];  // the lane's rows
+#pragma unroll
+    for (int u = 0; u < 4; ++u) at[u] = place[16 * u + col] + (size_t)(8 * kq);
+    // rows 16 u .. of u B: the products of the lane's row and eight columns
+    auto product = [&](const Columns<KB>& c, const v4i32_t (&sums)[2], int u, int32_t (&v)[8]) {
+        v4i32_t hi[2], lo[2];
+#pragma unroll
+        for (int q = 0; q < 2; ++q) {
+            hi[q] = v4i32_t{0, 0, 0, 0};
+            lo[q] = sums[q];
+        }
+#pragma unroll
+        for (int b = 0; b < KB; ++b) {
+            const int i = (16 * u + col) * stride + 64 * b + 16 * kq;
+            const v4i32_t uh = *reinterpret_cast<const v4i32_t*>(&plane[0][i]), ul = *reinterpret_cast<const v4i32_t*>(&plane[1][i]);
+#pragma unroll
+            for (int q = 0; q < 2; ++q) {
+                hi[q] = mfma(c.w8[q][b], uh, hi[q]);
+                lo[q] = mfma(c.w8[q][b], ul, lo[q]);
+            }
+        }
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = (int32_t)((uint32_t)hi[e >> 2][e & 3] << 8) + lo[e >> 2][e & 3];
+    };
+    while (n0 < end) {
+        const int n2 = n0 + (((n0 - begin) & 32) ? 224 : 32);
+        const bool inside = n0 + 32 <= a.N;
+        Halves8 old[4];
+        if (inside) {
+#pragma unroll
+            for (int u = 0; u < 4; ++u)
+                if (u < subs) old[u] = *reinterpret_cast<const Halves8*>(a.out + at[u] + n0);
+        }
+        if (n2 < end) fetch(next, n2);
+        uint32_t sh[8];
+        bool small = true;  // the rounding shift is 1 to 30: 32-bit steps
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            sh[e] = ((cur.frac[e >> 2] >> (8 * (e & 3))) + a.mid_frac - (cur.to[e >> 2] >> (8 * (e & 3)))) & 255u;
+            small &= sh[e] - 1u < 30u;
+        }
+        v4i32_t sums[2];
+#pragma unroll
+        for (int q = 0; q < 2; ++q) {
+            sums[q] = v4i32_t{0, 0, 0, 0};
+#pragma unroll
+            for (int b = 0; b < KB; ++b) sums[q] = mfma(cur.w8[q][b], one[b], sums[q]);
+            sums[q] <<= 7;
+        }
+        if (inside && __all(small)) {
+            int32_t half[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) half[e] = (int32_t)(1u << (sh[e] - 1u)) - 1;
+#pragma unroll
+            for (int u = 0; u < 4; ++u) {
+                if (u >= subs) break;
+                int32_t v[8];
+                product(cur, sums, u, v);
+#pragma unroll
+                for (int p = 0; p < 4; ++p) {
+                    int32_t d[2];
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        const int e = 2 * p + i;
+                        d[i] = (v[e] + half[e] + (int32_t)(((uint32_t)v[e] >> sh[e]) & 1u)) >> sh[e];
+                    }
+                    const Short2 add = __builtin_amdgcn_cvt_pk_i16(d[0], d[1]);  // clamps
+                    const uint32_t was = old[u][p];  // a bit cast of a vector's element takes element 0
+                    old[u][p] = __builtin_bit_cast(uint32_t, __builtin_elementwise_add_sat(add, __builtin_bit_cast(Short2, was)));
+                }
+                if (16 * u + col < rows) *reinterpret_cast<Halves8*>(a.out + at[u] + n0) = old[u];
+            }
+        } else {
+#pragma nounroll
+            for (int u = 0; u < subs; ++u) {
+                int32_t v[8];
+                product(cur, sums, u, v);
+                int16_t* o = a.out + place[16 * u + col] + n0 + 8 * kq;
+#pragma unroll
+                for (int e = 0; e < 8; ++e)
+                    if (16 * u + col < rows && n0 + 8 * kq + e < a.N)
+                        o[e] = clamp_i16((int32_t)o[e] + (int32_t)clamp_i16_i64(rescale64(v[e], (uint8_t)sh[e], 0)));
+            }
+        }
+        cur = next;
+        n0 = n2;
+    }
+}
+
+__global__ __launch_bounds__(256) void adapters_clear_kernel(uint64_t* __restrict__ p, size_t n) {
+    for (size_t i = (size_t)blockIdx.x * 256 + threadIdx.x; i < n; i += (size_t)gridDim.x * 256) p[i] = 0;
+}
 
 }  // namespace
 }  // namespace myl
@@ -87,9 +451,10 @@ using namespace myl;
 
 extern "C" {
 
-size_t myl_linear_w8a16_adapters_workspace(const myl_ctx* ctx, size_t M, size_t N, size_t K, size_t rank) {
-    if (!ctx || !fits_int(M) || !fits_int(N) || !fits_int(K) || rank > kMaxRank) return 0;
-    return Space::of(nullptr, M, N, K, rank).bytes;
+size_t myl_linear_w8a16_adapters_workspace(const myl_ctx* ctx, size_t M, size_t N, size_t K, size_t rank, size_t n_adapters) {
+    const AdapterShape s{M, N, K, rank, n_adapters};
+    if (!ctx || adapter_refuse(s)) return 0;
+    return adapter_plan(s, ctx->prop.multiProcessorCount).bytes;
 }
 
 int myl_linear_w8a16_adapters_dev(myl_ctx* ctx, const int16_t* x, size_t M, size_t ldx, const int8_t* W, size_t N,
@@ -101,42 +466,55 @@ int myl_linear_w8a16_adapters_dev(myl_ctx* ctx, const int16_t* x, size_t M, size
     if (!ctx) return MYL_E_INVALID;
     const char* what = "linear_w8a16_adapters_dev";
     auto bad = [&](const char* why) { return ctx->fail(MYL_E_INVALID, std::string(what) + ": " + why); };
-    if (K == 0) return bad("K must be > 0");
+    const AdapterShape s{M, N, K, rank, n_adapters};
+    if (const char* why = adapter_refuse(s)) return bad(why);
     if (ldx < K || ldo < N) return bad("leading dimension too small");
-    if (!fits_int(M) || !fits_int(N) || !fits_int(K) || !fits_int(ldx) || !fits_int(ldo) || !fits_int(n_adapters))
-        return bad("shape too large");
-    if (n_adapters > 0 && (rank == 0 || rank > kMaxRank)) return bad("rank must be 1 to 256");
+    if (!fits_int(ldx) || !fits_int(ldo)) return bad("leading dimension too large");
     if (M == 0 || N == 0) return MYL_OK;
     if (!x || !W || !w_shifts || !out) return bad("null operand");
     if (n_adapters > 0 && (!ids || !A || !a_shifts || !B || !b_shifts)) return bad("null adapter operand");
-    if (n_adapters == 0) rank = 0;
-    const Space s = Space::of(workspace, M, N, K, rank);
-    if (!workspace || workspace_bytes < s.bytes) return bad("workspace too small (myl_linear_w8a16_adapters_workspace)");
+    const AdapterPlan p = adapter_plan(s, ctx->prop.multiProcessorCount);
+    if (!workspace || workspace_bytes < p.bytes) return bad("workspace too small (myl_linear_w8a16_adapters_workspace)");
     if ((uintptr_t)workspace & 15) return bad("workspace must be 16-byte aligned");
     const DeviceGuard guard(ctx->device);
     const hipStream_t st = ctx->stream;
+    char* ws = static_cast<char*>(workspace);
     MmCtx mm;
-    mm.cus = ctx->prop.multiProcessorCount > 0 ? ctx->prop.multiProcessorCount : 1;
-    mm.planes = s.planes;
-    mm.planes_bytes = s.planes_bytes;
-    mm.acc = s.acc;
-    mm.acc_elems = s.acc_elems;
-    if (s.acc_elems) {
-        adapters_clear_kernel<<<(unsigned)std::min<size_t>((s.acc_elems + 255) / 256, 1024), 256, 0, st>>>(s.acc, s.acc_elems);
-        if (int rc = ctx->hip(hipGetLastError(), what)) return rc;
+    mm.cus = std::max(ctx->prop.multiProcessorCount, 1);
+    if (M >= 2) {
+        mm.planes = reinterpret_cast<int8_t*>(ws + p.off_planes);
+        mm.planes_bytes = p.planes_bytes;
+        mm.acc = reinterpret_cast<unsigned long long*>(ws + p.off_acc);
+        mm.acc_elems = p.acc_elems;
     }
+    Adapters a{};
+    a.acc = reinterpret_cast<uint64_t*>(mm.acc);
+    a.acc_elems = p.acc_elems;
+    if (n_adapters > 0) {
+        a.x = x; a.ids = ids; a.A = A; a.B = B; a.a_shifts = a_shifts; a.b_shifts = b_shifts; a.out_frac_pc = out_frac_pc;
+        a.out = out;
+        a.part = reinterpret_cast<int64_t*>(ws + p.off_part);
+        a.tiles = reinterpret_cast<TileRows*>(ws + p.off_tiles);
+        a.ldx = ldx; a.ldo = ldo; a.b_bytes = n_adapters * N * rank;
+        a.M = (int)M; a.N = (int)N; a.K = (int)K; a.rank = (int)rank; a.rank_pad = p.rank_pad; a.n = (int)n_adapters;
+        a.splits = p.splits; a.per_wave = p.per_wave; a.units = (int)((K + kAdapterUnit - 1) / kAdapterUnit); a.n_chunk = p.n_chunk;
+        a.slots = SmallDiv::of((size_t)p.slots);
+        a.act_frac = act_frac; a.mid_frac = mid_frac; a.out_frac = out_frac;
+        const dim3 grid((unsigned)(p.windows * p.slots), (unsigned)p.rank_groups, (unsigned)p.splits);
+        if (p.rank_tiles == 1) adapters_down_kernel<1><<<grid, 256, 0, st>>>(a);
+        else if (p.rank_tiles == 2) adapters_down_kernel<2><<<grid, 256, 0, st>>>(a);
+        else adapters_down_kernel<4><<<grid, 256, 0, st>>>(a);
+    } else if (p.acc_elems) {
+        adapters_clear_kernel<<<(unsigned)std::min<size_t>((p.acc_elems + 255) / 256, 1024), 256, 0, st>>>(a.acc, a.acc_elems);
+    }
+    if (int rc = ctx->hip(hipGetLastError(), what)) return rc;
     int rc = ctx->hip(linear_w8a16(x, (int)M, (int)ldx, W, (int)N, (int)K, w_shifts, act_frac, out_frac, out_frac_pc, out,
                                    (int)ldo, st, &mm), what);
     if (rc || n_adapters == 0) return rc;
-    for (size_t m0 = 0; m0 < M; m0 += 65535) {  // the grid's y range
-        const int rows = (int)std::min<size_t>(M - m0, 65535);
-        adapters_down_kernel<<<dim3(rows, (unsigned)rank), 64, 0, st>>>(x + m0 * ldx, (int)ldx, (int)K, ids + m0, (int)n_adapters,
-                                                                        (int)rank, A, a_shifts, act_frac, mid_frac,
-                                                                        s.u + m0 * rank);
-        adapters_up_kernel<<<dim3((unsigned)((N + 255) / 256), rows), 256, 0, st>>>(
-            s.u + m0 * rank, ids + m0, (int)n_adapters, (int)rank, B, b_shifts, mid_frac, out_frac, out_frac_pc, (int)N,
-            out + m0 * ldo, (int)ldo);
-    }
+    const dim3 grid((unsigned)(p.windows * p.slots), (unsigned)p.n_chunks);
+    if (p.rank_pad <= 64) adapters_up_kernel<1><<<grid, 256, 0, st>>>(a);
+    else if (p.rank_pad == 128) adapters_up_kernel<2><<<grid, 256, 0, st>>>(a);
+    else adapters_up_kernel<4><<<grid, 256, 0, st>>>(a);
     return ctx->hip(hipGetLastError(), what);
 }
 
