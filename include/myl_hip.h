@@ -232,7 +232,8 @@ int myl_logsoftmax_dev(myl_ctx* ctx, const int32_t* logits, size_t M, size_t n, 
  * id = ids[m].  A row whose id is outside [0, n_adapters) has no adapter (d = 0).
  * A [n_adapters x rank x K], a_shifts [n_adapters x rank], B [n_adapters x N x
  * rank], b_shifts [n_adapters x N]; rank is at most 256 (an adapter of lower
- * rank is padded with zero rows of A and zero columns of B), M at most 2^23. */
+ * rank is padded with zero rows of A and zero columns of B), M at most 2^23, N and K
+ * at most 2^30. */
 size_t myl_linear_w8a16_adapters_workspace(const myl_ctx* ctx, size_t M, size_t N, size_t K, size_t rank,
                                            size_t n_adapters);
 int myl_linear_w8a16_adapters_dev(myl_ctx* ctx, const int16_t* x, size_t M, size_t ldx, const int8_t* W, size_t N,

@@ -37,18 +37,18 @@ struct Adapters {
     const uint8_t *a_shifts, *b_shifts, *out_frac_pc;
     int16_t* out;
     int64_t* part;    // [split][M][rank_pad]
-    TileRows* tiles;  // [window][slot]
+    TileRows* tiles;  // [window][up_tiles]
     uint64_t* acc;    // cleared for the shared product
     size_t acc_elems, ldx, ldo, b_bytes;
-    int M, N, K, rank, rank_pad, n, splits, per_wave, units, n_chunk;
-    SmallDiv slots;
+    int M, N, K, rank, rank_pad, n, splits, per_wave, units, n_chunk, tile_count;
+    SmallDiv down_tiles, up_tiles;
     uint8_t act_frac, mid_frac, out_frac;
 };
 
 // Rows of A, B and x start anywhere.
 typedef uint32_t Bytes16 __attribute__((ext_vector_type(4), aligned(1)));
 typedef uint32_t Halves8 __attribute__((ext_vector_type(4), aligned(2)));
-typedef uint32_t Bytes8 __attribute__((ext_vector_type(2), aligned(1)));
+typedef uint32_t Halves2 __attribute__((aligned(2)));
 
 __device__ inline v4i32_t operand(const Bytes16& v) { return v4i32_t{(int)v[0], (int)v[1], (int)v[2], (int)v[3]}; }
 // 16 int16 as their byte planes.
@@ -68,8 +68,8 @@ __device__ inline v4i32_t mfma(const v4i32_t& a, const v4i32_t& b, const v4i32_t
 
 struct Grouping {
     alignas(16) int32_t id[kAdapterWindow];
-    uint64_t leads[4];
-    int32_t tile_id, first, rows[4];
+    uint64_t leads[4], leads64[4];
+    int32_t tile_id, first, up, rows[4];
     uint8_t at[16];
 };
 
@@ -77,9 +77,10 @@ struct Grouping {
 // equal ids before it, every 16th of them leads a tile, and tiles are numbered in the order
 // of the rows that lead them.  Each block works its tile out: a launch to sort the rows
 // first would take longer than the at most 256 compares of a thread.  Returns the tile's
-// rows (0: no such tile), their places in s.at and its adapter in s.tile_id; `full`, if not
-// null, gets 64 rows from the first tile of each 64.
-__device__ inline int group_rows(const Adapters& a, int w, int t, Grouping& s, TileRows* full) {
+// rows (0: no such tile), their places in s.at and its adapter in s.tile_id; `up`, if not
+// null, are the window's tiles of 64 rows, to be written: each by the block whose tile's first
+// row leads it, those that stay empty by the blocks of their number.
+__device__ inline int group_rows(const Adapters& a, int w, int t, Grouping& s, TileRows* up) {
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int rows = min(kAdapterWindow, a.M - w * kAdapterWindow);
     int id = tid < rows ? a.ids[(size_t)w * kAdapterWindow + tid] : -1;
@@ -89,46 +90,56 @@ __device__ inline int group_rows(const Adapters& a, int w, int t, Grouping& s, T
     __syncthreads();
     int c = 0;
     if (64 * wave < rows) {
+#pragma unroll 8
         for (int i = 0; i < 64 * wave; i += 4) {
             const int4 q = *reinterpret_cast<const int4*>(&s.id[i]);
             c += (q.x == id) + (q.y == id) + (q.z == id) + (q.w == id);
         }
-        const int own = min(64, rows - 64 * wave);
-        for (int i = 0; i < own; ++i) c += __builtin_amdgcn_readlane(id, i) == id && i < lane;
+        for (int i0 = 0; i0 < min(64, rows - 64 * wave); i0 += 16)
+#pragma unroll
+            for (int i = 0; i < 16; ++i) c += __builtin_amdgcn_readlane(id, i0 + i) == id && i0 + i < lane;
     }
     const bool lead = id >= 0 && (c & 15) == 0;
-    const uint64_t b = __ballot(lead);
-    if (lane == 0) s.leads[wave] = b;
+    const uint64_t b = __ballot(lead), b64 = __ballot(lead && (c & 63) == 0), below = (1ull << lane) - 1ull;
+    if (lane == 0) {
+        s.leads[wave] = b;
+        s.leads64[wave] = b64;
+    }
     __syncthreads();
-    int mine = __popcll(b & ((1ull << lane) - 1ull));
-    for (int v = 0; v < wave; ++v) mine += __popcll(s.leads[v]);
+    int mine = __popcll(b & below), mine64 = __popcll(b64 & below);
+    for (int v = 0; v < wave; ++v) {
+        mine += __popcll(s.leads[v]);
+        mine64 += __popcll(s.leads64[v]);
+    }
     if (lead && mine == t) {
         s.tile_id = id;
         s.first = c;
+        s.up = (c & 63) == 0 ? mine64 : -1;
     }
+    if (up && tid == 0 && t < (int)a.up_tiles.d &&
+        t >= __popcll(s.leads64[0]) + __popcll(s.leads64[1]) + __popcll(s.leads64[2]) + __popcll(s.leads64[3]))
+        up[t].rows = 0;
     __syncthreads();
     const int tile_id = s.tile_id, first = s.first;
-    if (tile_id < 0) {
-        if (full && tid == 0) full->rows = 0;
-        return 0;
-    }
+    if (tile_id < 0) return 0;
+    TileRows* full = up && s.up >= 0 ? up + s.up : nullptr;
     const bool member = id == tile_id && c >= first;
     if (member && c < first + 16) s.at[c - first] = (uint8_t)tid;
-    if (full && (first & 63) == 0 && member && c < first + 64) full->at[c - first] = (uint8_t)tid;
+    if (full && member && c < first + 64) full->at[c - first] = (uint8_t)tid;
     const uint64_t m = __ballot(member);
     if (lane == 0) s.rows[wave] = __popcll(m);
     __syncthreads();
     const int all = s.rows[0] + s.rows[1] + s.rows[2] + s.rows[3];
     if (full && tid == 0) {
         full->id = tile_id;
-        full->rows = (first & 63) == 0 ? min(all, 64) : 0;
+        full->rows = min(all, 64);
     }
     return min(all, 16);
 }
 
 // ---- x A --------------------------------------------------------------------------
 
-// Grid (windows x slots, rank groups, splits of K); 256 threads.  Lane l holds row l % 16 of
+// Grid (windows x down_tiles, rank groups, splits of K); 256 threads.  Lane l holds row l % 16 of
 // A and of x at 16 (l / 16) of each 64 of K: two matrix steps use up a line of A.  A wave
 // loads the next unit while it multiplies one.
 template <int RT>
@@ -139,8 +150,8 @@ __global__ __launch_bounds__(256, 2) void adapters_down_kernel(Adapters a) {
     const size_t block = ((size_t)blockIdx.z * gridDim.y + blockIdx.y) * gridDim.x + blockIdx.x;
     for (size_t i = block * 256 + tid; i < a.acc_elems; i += (size_t)gridDim.x * gridDim.y * gridDim.z * 256) a.acc[i] = 0;
     int t;
-    const int w = divmod(a.slots, (int)blockIdx.x, t);
-    const int rows = group_rows(a, w, t, s, blockIdx.y == 0 && blockIdx.z == 0 ? a.tiles + blockIdx.x : nullptr);
+    const int w = divmod(a.down_tiles, (int)blockIdx.x, t);
+    const int rows = group_rows(a, w, t, s, blockIdx.y == 0 && blockIdx.z == 0 ? a.tiles + (size_t)w * a.up_tiles.d : nullptr);
     if (rows == 0) return;
     const int col = lane & 15, kq = lane >> 4;
     const size_t row = (size_t)w * kAdapterWindow + s.at[min(col, rows - 1)];
@@ -251,97 +262,102 @@ __device__ inline v4i32_t bytes_until(const int8_t* p, const int8_t* end) {
     return v4i32_t{(int)v[0], (int)(v[0] >> 32), (int)v[1], (int)(v[1] >> 32)};
 }
 
-// 32 columns of B as the rows of two matrix operands, in an order that leaves a lane eight
-// columns that follow one another: column n0 + 8 (l / 16) + 4 q + e of row l % 16 in register
-// e of product q.  With them the lane's shifts.
+// 64 columns of B as the rows of four matrix operands, and the shifts of the two columns
+// (n0 + 2 (l % 32) and the next) whose outputs the lane adds to.
 template <int KB>
 struct Columns {
-    v4i32_t w8[2][KB];
-    Bytes8 frac, to;
+    v4i32_t w8[4][KB];
+    uint8_t frac[2], to[2];
 };
 
+constexpr uint32_t kUpGrid = 32768;  // tiles in the second dimension of the grid
 typedef short Short2 __attribute__((ext_vector_type(2)));
 
-// Grid (windows x slots, chunks of columns); 256 threads, KB steps of 64 of the rank.  The
-// rows' u lie in LDS as byte planes, zero from the rank on.  A wave loads the next columns
-// while it works on some, and all rows' outputs before it multiplies.
+// Grid (chunks of columns, tiles, 32768s of tiles); 256 threads, KB steps of 64 of the rank.
+// Chunks are the first dimension: tiles that stay empty do not leave an XCD idle.  The
+// rows' u lie in LDS as byte planes, zero from the rank on.  A wave works on 16 rows and 64
+// columns at a time: the products go through LDS, so that a load or store of out takes two
+// whole lines and a lane has two columns' shifts.  It loads the next columns and the next
+// rows' outputs before it multiplies.
 template <int KB>
-__global__ __launch_bounds__(256) void adapters_up_kernel(Adapters a) {
-    constexpr int stride = 64 * KB + 16, quads = 16 * KB;
+__global__ __launch_bounds__(256, KB == 1 ? 3 : KB == 2 ? 2 : 1) void adapters_up_kernel(Adapters a) {
+    constexpr int stride = 64 * KB + 16;
     __shared__ __align__(16) int8_t plane[2][64 * stride];
+    __shared__ __align__(16) int32_t product[4][16 * 68];
     __shared__ size_t place[64];
-    const TileRows* tile = a.tiles + blockIdx.x;
+    const int tile_index = (int)(blockIdx.z * kUpGrid + blockIdx.y);
+    if (tile_index >= a.tile_count) return;
+    const TileRows* tile = a.tiles + tile_index;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), col = lane & 15, kq = lane >> 4;
-    const int at0 = tile->at[tid & 63], at1 = tile->at[tid / quads];
+    const int pair = 2 * (lane & 31), odd = lane >> 5;  // its columns; its rows are odd, odd + 2, ..
+    const int at0 = tile->at[lane];
     const int rows = __builtin_amdgcn_readfirstlane(tile->rows), id = __builtin_amdgcn_readfirstlane(tile->id);
     if (rows == 0) return;
-    const int begin = (int)blockIdx.y * a.n_chunk, end = min(a.N, begin + a.n_chunk), subs = (rows + 15) >> 4;
+    const int begin = (int)blockIdx.x * a.n_chunk, end = min(a.N, begin + a.n_chunk), subs = (rows + 15) >> 4;
     const int8_t *B = a.B + (size_t)id * (size_t)a.N * (size_t)a.rank, *b_end = a.B + a.b_bytes;
     const uint8_t* bs = a.b_shifts + (size_t)id * (size_t)a.N;
+    int t;
+    const size_t base = (size_t)divmod(a.up_tiles, tile_index, t) * kAdapterWindow;
 
     auto fetch = [&](Columns<KB>& c, int n0) {
         const int8_t* b = B + (size_t)n0 * (size_t)a.rank;
-        if (n0 + 32 <= a.N && b + 31 * a.rank + 64 * KB <= b_end) {
+        if (n0 + 64 <= a.N && b + 63 * a.rank + 64 * KB <= b_end) {
 #pragma unroll
-            for (int q = 0; q < 2; ++q) {
-                const uint32_t off = (uint32_t)((8 * (col >> 2) + 4 * q + (col & 3)) * a.rank + 16 * kq);
+            for (int q = 0; q < 4; ++q)
 #pragma unroll
-                for (int k = 0; k < KB; ++k) c.w8[q][k] = operand(*reinterpret_cast<const Bytes16*>(b + off + 64 * k));
-            }
-            c.frac = *reinterpret_cast<const Bytes8*>(bs + n0 + 8 * kq);
-            if (a.out_frac_pc) c.to = *reinterpret_cast<const Bytes8*>(a.out_frac_pc + n0 + 8 * kq);
+                for (int k = 0; k < KB; ++k)
+                    c.w8[q][k] = operand(*reinterpret_cast<const Bytes16*>(b + (uint32_t)((16 * q + col) * a.rank + 16 * kq) + 64 * k));
         } else {
 #pragma unroll
-            for (int q = 0; q < 2; ++q) {
-                const int8_t* p = b + min(8 * (col >> 2) + 4 * q + (col & 3), a.N - 1 - n0) * a.rank + 16 * kq;
+            for (int q = 0; q < 4; ++q)
 #pragma unroll
-                for (int k = 0; k < KB; ++k) c.w8[q][k] = bytes_until(p + 64 * k, b_end);
-            }
-            c.frac = c.to = Bytes8{0, 0};
-#pragma nounroll
-            for (int e = 0; e < 4; ++e) {
-                const int n = min(n0 + 8 * kq + e, a.N - 1), m = min(n0 + 8 * kq + 4 + e, a.N - 1);
-                c.frac[0] |= (uint32_t)bs[n] << (8 * e);
-                c.frac[1] |= (uint32_t)bs[m] << (8 * e);
-                if (a.out_frac_pc) {
-                    c.to[0] |= (uint32_t)a.out_frac_pc[n] << (8 * e);
-                    c.to[1] |= (uint32_t)a.out_frac_pc[m] << (8 * e);
-                }
-            }
+                for (int k = 0; k < KB; ++k) c.w8[q][k] = bytes_until(b + min(16 * q + col, a.N - 1 - n0) * a.rank + 16 * kq + 64 * k, b_end);
         }
-        if (!a.out_frac_pc) c.to = Bytes8{a.out_frac * 0x01010101u, a.out_frac * 0x01010101u};
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const int n = min(n0 + pair + i, a.N - 1);
+            c.frac[i] = bs[n];
+            c.to[i] = a.out_frac_pc ? a.out_frac_pc[n] : a.out_frac;
+        }
     };
     Columns<KB> cur, next;
+    uint32_t old[8] = {}, ahead[8] = {};  // out at the lane's rows and columns, of these 16 rows and the next
+    auto outputs = [&](uint32_t (&o)[8], auto&& place_of, int n0) {
+        if (n0 + 64 <= a.N)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) o[i] = *reinterpret_cast<const Halves2*>(a.out + place_of(2 * i + odd) + n0 + pair);
+    };
     int n0 = begin + 64 * wave;
-    if (n0 < end) fetch(cur, n0);
+    if (n0 < end) {
+        fetch(cur, n0);
+        outputs(old, [&](int r) { return (base + (size_t)__shfl(at0, min(r, rows - 1), 64)) * a.ldo; }, n0);
+    }
 
-    int t;
-    const size_t base = (size_t)divmod(a.slots, (int)blockIdx.x, t) * kAdapterWindow;
     const int place0 = __shfl(at0, min(lane, rows - 1), 64);
     if (tid < 64) place[tid] = (base + (size_t)place0) * a.ldo;
-    for (int i = tid, at = at1; i < rows * quads; i += 256) {
-        const int r = i / quads, j = 4 * (i % quads);
-        if (i != tid) at = tile->at[r];
-        uint32_t h = 0, l = 0;
-        if (j < a.rank) {
-            const int64_t* p = a.part + (base + (size_t)at) * (size_t)a.rank_pad + j;
-            int64_t sum[4] = {0, 0, 0, 0};
+    const int quads = __builtin_ctz((unsigned)a.rank_pad) - 2;  // a row's fours of the rank, as a shift
+    for (int i = tid; i < rows << quads; i += 256) {
+        const int r = i >> quads, j = 4 * (i & ((1 << quads) - 1));
+        const int64_t* p = a.part + (base + (size_t)tile->at[r]) * (size_t)a.rank_pad + j;
+        int64_t sum[4] = {0, 0, 0, 0};
 #pragma unroll 4
-            for (int k = 0; k < a.splits; ++k)
+        for (int k = 0; k < a.splits; ++k)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) sum[e] += p[(size_t)k * (size_t)a.M * (size_t)a.rank_pad + e];
+            for (int e = 0; e < 4; ++e) sum[e] += p[(size_t)k * (size_t)a.M * (size_t)a.rank_pad + e];
+        uint32_t h = 0, l = 0;
 #pragma unroll
-            for (int e = 0; e < 4; ++e)
-                if (j + e < a.rank) {
-                    const uint8_t frac = (uint8_t)(a.a_shifts[(size_t)id * (size_t)a.rank + j + e] + a.act_frac);
-                    const uint32_t u = (uint16_t)clamp_i16_i64(rescale64(sum[e], frac, a.mid_frac));
-                    h |= (u >> 8) << (8 * e);
-                    l |= ((u & 255u) ^ 128u) << (8 * e);
-                }
-        }
+        for (int e = 0; e < 4; ++e)
+            if (j + e < a.rank) {
+                const uint8_t frac = (uint8_t)(a.a_shifts[(size_t)id * (size_t)a.rank + j + e] + a.act_frac);
+                const uint32_t u = (uint16_t)clamp_i16_i64(rescale64(sum[e], frac, a.mid_frac));
+                h |= (u >> 8) << (8 * e);
+                l |= ((u & 255u) ^ 128u) << (8 * e);
+            }
         *reinterpret_cast<uint32_t*>(&plane[0][r * stride + j]) = h;
         *reinterpret_cast<uint32_t*>(&plane[1][r * stride + j]) = l;
     }
+    for (int r = tid >> 2, j = a.rank_pad + 16 * (tid & 3); j < 64 * KB; j += 64)
+        *reinterpret_cast<v4i32_t*>(&plane[0][r * stride + j]) = *reinterpret_cast<v4i32_t*>(&plane[1][r * stride + j]) = v4i32_t{0, 0, 0, 0};
     __syncthreads();
     v4i32_t one[KB];  // ones below the rank
 #pragma unroll
@@ -351,89 +367,73 @@ __global__ __launch_bounds__(256) void adapters_up_kernel(Adapters a) {
             const int left = min(max(a.rank - 64 * b - 16 * kq - 4 * e, 0), 4);
             one[b][e] = left == 0 ? 0 : 0x01010101 >> (8 * (4 - left));
         }
-    size_t at[4];  // the lane's rows
-#pragma unroll
-    for (int u = 0; u < 4; ++u) at[u] = place[16 * u + col] + (size_t)(8 * kq);
-    // rows 16 u .. of u B: the products of the lane's row and eight columns
-    auto product = [&](const Columns<KB>& c, const v4i32_t (&sums)[2], int u, int32_t (&v)[8]) {
-        v4i32_t hi[2], lo[2];
-#pragma unroll
-        for (int q = 0; q < 2; ++q) {
-            hi[q] = v4i32_t{0, 0, 0, 0};
-            lo[q] = sums[q];
-        }
-#pragma unroll
-        for (int b = 0; b < KB; ++b) {
-            const int i = (16 * u + col) * stride + 64 * b + 16 * kq;
-            const v4i32_t uh = *reinterpret_cast<const v4i32_t*>(&plane[0][i]), ul = *reinterpret_cast<const v4i32_t*>(&plane[1][i]);
-#pragma unroll
-            for (int q = 0; q < 2; ++q) {
-                hi[q] = mfma(c.w8[q][b], uh, hi[q]);
-                lo[q] = mfma(c.w8[q][b], ul, lo[q]);
-            }
-        }
-#pragma unroll
-        for (int e = 0; e < 8; ++e) v[e] = (int32_t)((uint32_t)hi[e >> 2][e & 3] << 8) + lo[e >> 2][e & 3];
-    };
     while (n0 < end) {
-        const int n2 = n0 + (((n0 - begin) & 32) ? 224 : 32);
-        const bool inside = n0 + 32 <= a.N;
-        Halves8 old[4];
-        if (inside) {
-#pragma unroll
-            for (int u = 0; u < 4; ++u)
-                if (u < subs) old[u] = *reinterpret_cast<const Halves8*>(a.out + at[u] + n0);
-        }
+        const int n2 = n0 + 256;
         if (n2 < end) fetch(next, n2);
-        uint32_t sh[8];
-        bool small = true;  // the rounding shift is 1 to 30: 32-bit steps
+        uint32_t sh[2], half[2];
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            sh[e] = ((cur.frac[e >> 2] >> (8 * (e & 3))) + a.mid_frac - (cur.to[e >> 2] >> (8 * (e & 3)))) & 255u;
-            small &= sh[e] - 1u < 30u;
+        for (int i = 0; i < 2; ++i) {
+            sh[i] = (uint32_t)(uint8_t)(cur.frac[i] + a.mid_frac - cur.to[i]);
+            half[i] = (1u << ((sh[i] - 1u) & 31u)) - 1u;
         }
-        v4i32_t sums[2];
+        // 32-bit steps where the rounding shifts are 1 to 30
+        const bool fast = n0 + 64 <= a.N && __all(sh[0] - 1u < 30u && sh[1] - 1u < 30u);
+        v4i32_t sums[4];
 #pragma unroll
-        for (int q = 0; q < 2; ++q) {
+        for (int q = 0; q < 4; ++q) {
             sums[q] = v4i32_t{0, 0, 0, 0};
 #pragma unroll
             for (int b = 0; b < KB; ++b) sums[q] = mfma(cur.w8[q][b], one[b], sums[q]);
             sums[q] <<= 7;
         }
-        if (inside && __all(small)) {
-            int32_t half[8];
-#pragma unroll
-            for (int e = 0; e < 8; ++e) half[e] = (int32_t)(1u << (sh[e] - 1u)) - 1;
-#pragma unroll
-            for (int u = 0; u < 4; ++u) {
-                if (u >= subs) break;
-                int32_t v[8];
-                product(cur, sums, u, v);
-#pragma unroll
-                for (int p = 0; p < 4; ++p) {
-                    int32_t d[2];
-#pragma unroll
-                    for (int i = 0; i < 2; ++i) {
-                        const int e = 2 * p + i;
-                        d[i] = (v[e] + half[e] + (int32_t)(((uint32_t)v[e] >> sh[e]) & 1u)) >> sh[e];
-                    }
-                    const Short2 add = __builtin_amdgcn_cvt_pk_i16(d[0], d[1]);  // clamps
-                    const uint32_t was = old[u][p];  // a bit cast of a vector's element takes element 0
-                    old[u][p] = __builtin_bit_cast(uint32_t, __builtin_elementwise_add_sat(add, __builtin_bit_cast(Short2, was)));
-                }
-                if (16 * u + col < rows) *reinterpret_cast<Halves8*>(a.out + at[u] + n0) = old[u];
-            }
-        } else {
 #pragma nounroll
-            for (int u = 0; u < subs; ++u) {
-                int32_t v[8];
-                product(cur, sums, u, v);
-                int16_t* o = a.out + place[16 * u + col] + n0 + 8 * kq;
+        for (int u = 0; u < subs; ++u) {
+            const size_t* places = place + 16 * u;
+            if (u + 1 < subs) outputs(ahead, [&](int r) { return places[16 + r]; }, n0);
+            else if (n2 < end) outputs(ahead, [&](int r) { return place[r]; }, n2);
+            v4i32_t hi[4], lo[4];
 #pragma unroll
-                for (int e = 0; e < 8; ++e)
-                    if (16 * u + col < rows && n0 + 8 * kq + e < a.N)
-                        o[e] = clamp_i16((int32_t)o[e] + (int32_t)clamp_i16_i64(rescale64(v[e], (uint8_t)sh[e], 0)));
+            for (int q = 0; q < 4; ++q) {
+                hi[q] = v4i32_t{0, 0, 0, 0};
+                lo[q] = sums[q];
             }
+#pragma unroll
+            for (int b = 0; b < KB; ++b) {
+                const int i = (16 * u + col) * stride + 64 * b + 16 * kq;
+                const v4i32_t uh = *reinterpret_cast<const v4i32_t*>(&plane[0][i]), ul = *reinterpret_cast<const v4i32_t*>(&plane[1][i]);
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    hi[q] = mfma(cur.w8[q][b], uh, hi[q]);
+                    lo[q] = mfma(cur.w8[q][b], ul, lo[q]);
+                }
+            }
+            int32_t* v = product[wave];  // [16 rows][64 columns], the wave's own
+#pragma unroll
+            for (int q = 0; q < 4; ++q) *reinterpret_cast<v4i32_t*>(&v[col * 68 + 16 * q + 4 * kq]) = (hi[q] << 8) + lo[q];
+            asm volatile("" ::: "memory");
+            if (fast) {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const int r = 2 * i + odd;
+                    const int2 w = *reinterpret_cast<const int2*>(&v[r * 68 + pair]);
+                    const int32_t d0 = (int32_t)((uint32_t)w.x + half[0] + (((uint32_t)w.x >> sh[0]) & 1u)) >> sh[0];
+                    const int32_t d1 = (int32_t)((uint32_t)w.y + half[1] + (((uint32_t)w.y >> sh[1]) & 1u)) >> sh[1];
+                    const Short2 sum = __builtin_elementwise_add_sat(Short2(__builtin_amdgcn_cvt_pk_i16(d0, d1)), __builtin_bit_cast(Short2, old[i]));
+                    if (16 * u + r < rows) *reinterpret_cast<Halves2*>(a.out + places[r] + n0 + pair) = __builtin_bit_cast(uint32_t, sum);
+                }
+            } else {
+#pragma nounroll
+                for (int r = odd; r < min(16, rows - 16 * u); r += 2)
+#pragma unroll
+                    for (int i = 0; i < 2; ++i)
+                        if (n0 + pair + i < a.N) {
+                            int16_t* o = a.out + places[r] + n0 + pair + i;
+                            *o = clamp_i16((int32_t)*o + (int32_t)clamp_i16_i64(rescale64(v[r * 68 + pair + i], (uint8_t)sh[i], 0)));
+                        }
+            }
+            asm volatile("" ::: "memory");
+#pragma unroll
+            for (int i = 0; i < 8; ++i) old[i] = ahead[i];
         }
         cur = next;
         n0 = n2;
@@ -498,9 +498,11 @@ int myl_linear_w8a16_adapters_dev(myl_ctx* ctx, const int16_t* x, size_t M, size
         a.ldx = ldx; a.ldo = ldo; a.b_bytes = n_adapters * N * rank;
         a.M = (int)M; a.N = (int)N; a.K = (int)K; a.rank = (int)rank; a.rank_pad = p.rank_pad; a.n = (int)n_adapters;
         a.splits = p.splits; a.per_wave = p.per_wave; a.units = (int)((K + kAdapterUnit - 1) / kAdapterUnit); a.n_chunk = p.n_chunk;
-        a.slots = SmallDiv::of((size_t)p.slots);
+        a.down_tiles = SmallDiv::of((size_t)p.down_tiles);
+        a.up_tiles = SmallDiv::of((size_t)p.up_tiles);
+        a.tile_count = p.windows * p.up_tiles;
         a.act_frac = act_frac; a.mid_frac = mid_frac; a.out_frac = out_frac;
-        const dim3 grid((unsigned)(p.windows * p.slots), (unsigned)p.rank_groups, (unsigned)p.splits);
+        const dim3 grid((unsigned)(p.windows * p.down_tiles), (unsigned)p.rank_groups, (unsigned)p.splits);
         if (p.rank_tiles == 1) adapters_down_kernel<1><<<grid, 256, 0, st>>>(a);
         else if (p.rank_tiles == 2) adapters_down_kernel<2><<<grid, 256, 0, st>>>(a);
         else adapters_down_kernel<4><<<grid, 256, 0, st>>>(a);
@@ -511,7 +513,8 @@ int myl_linear_w8a16_adapters_dev(myl_ctx* ctx, const int16_t* x, size_t M, size
     int rc = ctx->hip(linear_w8a16(x, (int)M, (int)ldx, W, (int)N, (int)K, w_shifts, act_frac, out_frac, out_frac_pc, out,
                                    (int)ldo, st, &mm), what);
     if (rc || n_adapters == 0) return rc;
-    const dim3 grid((unsigned)(p.windows * p.slots), (unsigned)p.n_chunks);
+    const unsigned tiles = (unsigned)a.tile_count;
+    const dim3 grid((unsigned)p.n_chunks, std::min(tiles, kUpGrid), (tiles + kUpGrid - 1) / kUpGrid);
     if (p.rank_pad <= 64) adapters_up_kernel<1><<<grid, 256, 0, st>>>(a);
     else if (p.rank_pad == 128) adapters_up_kernel<2><<<grid, 256, 0, st>>>(a);
     else adapters_up_kernel<4><<<grid, 256, 0, st>>>(a);

@@ -27,6 +27,7 @@ struct Layout {
 
 constexpr size_t kAdapterMaxRank = 256;               // |sum B u| <= 2^7 2^15 2^8 = 2^30
 constexpr size_t kAdapterMaxRows = (size_t)1 << 23;   // a block per slot, 256 threads each, below 2^32
+constexpr size_t kAdapterMaxSide = (size_t)1 << 30;
 constexpr size_t kAdapterAccElems = (size_t)512 << 10;  // products with more outputs do not split K
 constexpr int kAdapterWindow = 256, kAdapterUnit = 128;
 
@@ -36,19 +37,21 @@ struct AdapterShape {
 
 inline const char* adapter_refuse(const AdapterShape& s) {
     if (s.K == 0) return "K must be > 0";
-    if (s.M > kAdapterMaxRows || s.N > kInt || s.K > kInt || s.n > kInt) return "shape too large (2^23 rows, 2^31 - 1 otherwise)";
+    if (s.M > kAdapterMaxRows || s.N > kAdapterMaxSide || s.K > kAdapterMaxSide || s.n > kInt)
+        return "shape too large (2^23 rows, 2^30 columns, 2^31 - 1 adapters)";
     if (s.n > 0 && (s.rank == 0 || s.rank > kAdapterMaxRank)) return "rank must be 1 to 256";
     return nullptr;
 }
 
-// The rows of one adapter within a window of 256 rows, 16 at a time, are a tile of x A:
-// slots tiles at most in a window.  A block takes a tile, 16 rank_tiles rows of A and
-// 4 per_wave units of 128 of K (a quarter each wave).  The rows of an adapter, 64 at a
-// time, with n_chunk columns are a block of u B.
+// The rows of one adapter within a window of 256 rows, 16 at a time, are a tile of x A: at
+// most down_tiles in a window.  A block takes a tile, 16 rank_tiles rows of A and 4 per_wave
+// units of 128 of K (a quarter each wave).  64 at a time they are a tile of u B: at most
+// up_tiles in a window; a block takes one and n_chunk columns.
 struct AdapterPlan {
-    int windows, slots, rank_tiles, rank_groups, splits, per_wave, n_chunk, n_chunks, rank_pad;
+    int windows, down_tiles, up_tiles, rank_tiles, rank_groups, splits, per_wave, n_chunk, n_chunks, rank_pad;
     size_t planes_bytes, acc_elems, off_planes, off_acc, off_part, off_tiles, bytes;
 };
+constexpr int64_t kAdapterMaxChunk = (int64_t)1 << 20;
 constexpr size_t kAdapterTileBytes = 72;  // adapter, rows, and their 64 places in the window
 
 inline AdapterPlan adapter_plan(const AdapterShape& s, int cus) {
@@ -63,7 +66,8 @@ inline AdapterPlan adapter_plan(const AdapterShape& s, int cus) {
     if (s.M && s.N && s.n) {
         const int w = (int)std::min<size_t>(s.M, kAdapterWindow), d = (int)std::min<size_t>(s.n, (size_t)w);
         p.windows = (int)((s.M + kAdapterWindow - 1) / kAdapterWindow);
-        p.slots = d + (w - d) / 16;
+        p.down_tiles = d + (w - d) / 16;
+        p.up_tiles = d + (w - d) / 64;
         const int tiles = (int)(s.rank + 15) / 16;
         p.rank_tiles = tiles <= 2 ? tiles : 4;
         p.rank_groups = (tiles + p.rank_tiles - 1) / p.rank_tiles;
@@ -71,17 +75,16 @@ inline AdapterPlan adapter_plan(const AdapterShape& s, int cus) {
         while (p.rank_pad < (int)s.rank) p.rank_pad *= 2;
         auto up = [](int64_t a, int64_t b) { return (a + b - 1) / b; };
         // Two blocks per CU, a unit per wave at least; a wave's i32 sums hold 2^17 products.
-        const int64_t units = up((int64_t)s.K, kAdapterUnit), blocks = (int64_t)p.windows * p.slots * p.rank_groups;
+        const int64_t units = up((int64_t)s.K, kAdapterUnit), blocks = (int64_t)p.windows * p.down_tiles * p.rank_groups;
         const int64_t want = std::max(std::min(up(2 * (int64_t)cus, blocks), up(units, 4)), up(units, 4 * 512));
         p.per_wave = (int)up(units, 4 * want);
         p.splits = (int)up(units, 4 * (int64_t)p.per_wave);
-        // Eight blocks per CU, 256 columns at least.
-        const int64_t rows = (int64_t)p.windows * (d + (w - d) / 64);
-        const int64_t cols = std::max(up((int64_t)s.N, up(8 * (int64_t)cus, rows)), up((int64_t)s.N, 65535));
-        p.n_chunk = (int)std::min<int64_t>(up(cols, 256) * 256, (int64_t)1 << 22);
+        // Four blocks per CU (2003 rows: 55 us; eight: 62), 256 columns at least.
+        const int64_t cols = up((int64_t)s.N, up(4 * (int64_t)cus, (int64_t)p.windows * p.up_tiles));
+        p.n_chunk = (int)std::min<int64_t>(up(cols, 256) * 256, kAdapterMaxChunk);
         p.n_chunks = (int)up((int64_t)s.N, p.n_chunk);
         p.off_part = l.take((size_t)p.splits * s.M * (size_t)p.rank_pad, 8);
-        p.off_tiles = l.take((size_t)p.windows * (size_t)p.slots, kAdapterTileBytes);
+        p.off_tiles = l.take((size_t)p.windows * (size_t)p.up_tiles, kAdapterTileBytes);
     }
     p.bytes = std::max<size_t>(l.used, 256);  // 0 stands for sizes that a call refuses
     return p;
