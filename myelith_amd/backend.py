@@ -377,6 +377,9 @@ class RocmBackend:
             ws.record_stream(torch.cuda.ExternalStream(stream, device=device))
         return ws
 
+    def _need_here(self, what: str, device) -> None:
+        _need(device.type == "cuda" and device.index == self._device_id, f"{what}: the operands must be on device {self._device_id}")
+
     @staticmethod
     def _new_workspace(nbytes: int, device, what: str):
         import torch
@@ -410,6 +413,7 @@ class RocmBackend:
             out = torch.empty((M, N), dtype=torch.int16, device=x.device)
         _need_dev(what, x.device, out=(out, "int16", None))
         _need(tuple(out.shape) == (M, N) and _strides(out)[1] in (0, 1), f"{what}: out must be [M x N]")
+        self._need_here(what, x.device)
         ws = self._workspace(lib().myl_linear_w8a16_adapters_workspace(self._h, M, N, K, rank, n), x.device, workspace)
         rc = lib().myl_linear_w8a16_adapters_dev(
             self._h, x.data_ptr(), M, _strides(x)[0] or K, W.data_ptr(), N, K, w_shifts.data_ptr(), act_frac, out_frac,
@@ -468,13 +472,15 @@ class RocmBackend:
               f"{what}: the positions of a KV head follow one another")
         _need(ps == _strides(v_prefix) and ts == _strides(v_tail), f"{what}: keys and values have the same strides")
         max_tail = T if max_tail is None else max_tail
+        ldq, ldo = rows_of(q, "q"), rows_of(out, "out")
+        self._need_here(what, dev)
         ws = self._workspace(lib().myl_attention_prefix_workspace(self._h, n_seqs, rows_per_seq, H, KH, hd, P, max_tail),
                              dev, workspace)
         rc = lib().myl_attention_prefix_dev(
-            self._h, q.data_ptr(), n_seqs, rows_per_seq, rows_of(q, "q"), H, KH, hd, k_prefix.data_ptr(), v_prefix.data_ptr(),
+            self._h, q.data_ptr(), n_seqs, rows_per_seq, ldq, H, KH, hd, k_prefix.data_ptr(), v_prefix.data_ptr(),
             P, ps[0] or P * hd, k_tail.data_ptr(), v_tail.data_ptr(), S, ts[0] or KH * T * hd, ts[1] or T * hd, max_tail,
             None if slots is None else slots.data_ptr(), lens.data_ptr(), score_mult, score_shift, exp_lut.data_ptr(),
-            exp_lut.numel(), lut_shift, prob_frac, out.data_ptr(), rows_of(out, "out"), ws.data_ptr(),
+            exp_lut.numel(), lut_shift, prob_frac, out.data_ptr(), ldo, ws.data_ptr(),
             ws.numel() * ws.element_size())
         if rc:
             self.check(rc, what)
@@ -520,10 +526,11 @@ class RocmBackend:
             out = torch.empty((B, k1), dtype=torch.int64, device=dev) if out is None else out
         _need_dev(what, dev, accepted=(accepted, "int32", (B,)), out=(out, "int64", (B, k1)))
         lut_len = 0 if exp_lut is None else exp_lut.numel()
+        ldt, ldd = rows_of(target, "target", k1), V if draft is None or k == 0 else rows_of(draft, "draft", k)
+        self._need_here(what, dev)
         ws = self._workspace(lib().myl_verify_drafts_workspace(self._h, B, k, V, lut_len), dev, workspace)
         rc = lib().myl_verify_drafts_dev(
-            self._h, target.data_ptr(), rows_of(target, "target", k1), None if draft is None or k == 0 else draft.data_ptr(),
-            V if draft is None or k == 0 else rows_of(draft, "draft", k), B, k, V, tokens.data_ptr(),
+            self._h, target.data_ptr(), ldt, None if draft is None or k == 0 else draft.data_ptr(), ldd, B, k, V, tokens.data_ptr(),
             None if n_draft is None else n_draft.data_ptr(), None if randoms is None else randoms.data_ptr(),
             None if exp_lut is None else exp_lut.data_ptr(), lut_len, accepted.data_ptr(), out.data_ptr(), ws.data_ptr(),
             ws.numel() * ws.element_size())

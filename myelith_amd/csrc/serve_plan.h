@@ -39,7 +39,10 @@ inline const char* adapter_refuse(const AdapterShape& s) {
     if (s.K == 0) return "K must be > 0";
     if (s.M > kAdapterMaxRows || s.N > kAdapterMaxSide || s.K > kAdapterMaxSide || s.n > kInt)
         return "shape too large (2^23 rows, 2^30 columns, 2^31 - 1 adapters)";
-    if (s.n > 0 && (s.rank == 0 || s.rank > kAdapterMaxRank)) return "rank must be 1 to 256";
+    if (s.n == 0) return nullptr;
+    if (s.rank == 0 || s.rank > kAdapterMaxRank) return "rank must be 1 to 256";
+    const size_t most = (size_t)1 << 47;  // bytes of A and B
+    if (s.n > most / (s.K * s.rank) || (s.N > 0 && s.n > most / (s.N * s.rank))) return "adapters larger than the address space";
     return nullptr;
 }
 

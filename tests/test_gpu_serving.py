@@ -417,3 +417,261 @@ def test_refusals(backend, exp_lut):
     with pytest.raises(ValueError, match="table"):
         backend.verify_drafts_dev(z, tok, rnd, exp_lut=torch.zeros(32769, dtype=torch.int16, device="cuda"))
     assert att().shape == (2, 4, 64)  # the context is as good as before
+
+
+# ---- many rows, long offsets --------------------------------------------------------------
+
+@pytest.mark.parametrize("M,N,K,rank,n", [(1500, 520, 64, 8, 300), (257, 70, 130, 12, 2), (1030, 33, 96, 70, 17)])
+def test_adapters_many_rows(backend, M, N, K, rank, n):
+    """Several windows of rows, adapters with rows in each, more columns than a block takes at once."""
+    case(f"adapters many rows M={M} N={N} K={K} rank={rank} n={n}")
+    s = adapter_inputs(M, M, N, K, rank, n)
+    same(run_adapters(backend, s), want_adapters(s), "many rows")
+    s["ids"] = np.repeat(rng(5).integers(-1, n, M // 50 + 1), 50)[:M].astype(np.int32)
+    same(run_adapters(backend, s), want_adapters(s), "runs")
+
+
+def test_adapters_past_4_gib(backend):
+    """Adapters whose rows lie more than 2^32 bytes into A."""
+    import torch
+    case("adapters past 4 GiB")
+    n, rank, K = 270, 256, 65472
+    ids = [269, 0, 260]
+    s = adapter_inputs(51, 3, 8, K, 1, n, ids)
+    A = torch.empty((n, rank, K), dtype=torch.int8, device="cuda")
+    for i in ids:
+        A[i].random_(-128, 128)
+    s.update(A=A, a_shifts=np.full((n, rank), 14, np.uint8), B=rng(6).integers(-128, 128, (n, 8, rank)).astype(np.int8),
+             b_shifts=np.full((n, 8), 10, np.uint8))
+    got = run_adapters(backend, s)
+    keep = dict(s, A=np.stack([A[i].cpu().numpy() for i in ids]), ids=np.arange(3))
+    for name in ("a_shifts", "B", "b_shifts"):
+        keep[name] = s[name][ids]
+    same(got, want_adapters(keep), "past 4 GiB")
+
+
+def test_attention_past_4_gib(backend, exp_lut):
+    """Prefix heads, tail slots and rows of queries and outputs more than 2^32 bytes apart."""
+    import torch
+    case("attention past 4 GiB")
+    P, T, far = 70, 40, 1 << 30
+    kv = torch.empty(2 * far + (1 << 21), dtype=torch.int16, device="cuda")
+    rows = torch.zeros(2 * far + (1 << 21), dtype=torch.int16, device="cuda")
+    s = attention_inputs(52, 3, 1, P, T, 4, 2, 64, slots=[2, 0, 1])
+    s["kt"], s["vp"] = s["kt"][:3], s["kp"]
+    s["vt"] = s["kt"]
+    prefix = kv.as_strided((2, P, 64), (2 * far, 64, 1))
+    tails = kv.as_strided((3, 2, T, 64), (far, T * 64, 64, 1), 1 << 20)
+    q, out = (rows.as_strided((3, 4, 64), (far, 64, 1), at) for at in (0, 1 << 20))
+    for t, v in ((prefix, s["kp"]), (tails, s["kt"]), (q, s["q"])):
+        t.copy_(gpu(v))
+    got = backend.attention_prefix_dev(q, prefix, prefix, tails, tails, gpu(s["lens"]), s["mult"], s["shift"], gpu(exp_lut), 6, 14,
+                                       slots=gpu(s["slots"]), out=out)
+    torch.cuda.synchronize()
+    same(got, ref.attention(**s, lut=exp_lut), "past 4 GiB")
+    assert int(torch.count_nonzero(rows)) == int(torch.count_nonzero(q)) + int(torch.count_nonzero(out))
+
+
+def test_verify_past_4_gib(backend, exp_lut):
+    import torch
+    case("drafts past 4 GiB")
+    s = verify_inputs(53, 2, 1, 9000)
+    far = 1 << 29
+    buf = torch.empty(3 * far + (1 << 20), dtype=torch.int32, device="cuda")
+    target = buf.as_strided((2, 2, 9000), (2 * far, far, 1))
+    draft = buf.as_strided((2, 1, 9000), (3 * far, 3 * far, 1), 1 << 16)
+    target.copy_(gpu(s["target"]))
+    draft.copy_(gpu(s["draft"]))
+    got = backend.verify_drafts_dev(target, gpu(s["tokens"]), gpu(s["randoms"].view(np.int64)), exp_lut=gpu(exp_lut), draft=draft)
+    torch.cuda.synchronize()
+    want = ref.verify(**s, lut=exp_lut)
+    same(got[0], want[0], "accepted")
+    same(got[1], want[1], "tokens")
+
+
+# ---- a serving step: the operators together -----------------------------------------------
+
+class Step:
+    """A projection with adapters, attention behind the shared prefix, logits and the check of
+    the drafts, for seqs sequences of k drafts; one workspace serves all calls in turn."""
+
+    def __init__(self, backend, exp_lut, seqs=5, k=3, seed=61):
+        import torch
+        self.b, self.lut, self.k, self.seqs = backend, exp_lut, k, seqs
+        H, hd, V, rows = 14, 64, 1500, seqs * (k + 1)
+        r = rng(seed)
+        self.ad = adapter_inputs(seed, rows, H * hd, 448, 16, 4, np.repeat(r.integers(-1, 4, seqs), k + 1))
+        self.at = attention_inputs(seed + 1, seqs, k + 1, 150, 33, H, 2, hd)
+        self.Wv = r.integers(-128, 128, (V, H * hd)).astype(np.int8)
+        self.v_shifts = np.full(V, 9, np.uint8)
+        self.d = {n: gpu(v) for n, v in [*self.ad.items(), *self.at.items(), ("Wv", self.Wv), ("v_shifts", self.v_shifts)]
+                  if isinstance(v, np.ndarray)}
+        self.table = gpu(exp_lut)
+        self.proj = torch.empty((rows, H * hd), dtype=torch.int16, device="cuda")
+        self.mix = torch.empty((rows, H, hd), dtype=torch.int16, device="cuda")
+        self.logits = torch.empty((rows, V), dtype=torch.int32, device="cuda")
+        self.accepted = torch.empty(seqs, dtype=torch.int32, device="cuda")
+        self.tokens = torch.empty((seqs, k + 1), dtype=torch.int64, device="cuda")
+        self.target = self.logits.view(seqs, k + 1, V)
+        d = self.d
+        spaces = [backend.linear_w8a16_adapters_workspace(d["x"], d["W"], d["A"]),
+                  backend.attention_prefix_workspace(self.mix, d["kp"], d["kt"], k + 1),
+                  backend.verify_drafts_workspace(self.target, self.table)]
+        self.ws = dirty(max(spaces, key=lambda t: t.numel()))
+        self.new_inputs(seed)
+
+    def new_inputs(self, seed):
+        import torch
+        r = rng(seed)
+        self.ad["x"] = gauss16(r, self.ad["x"].shape, 2000)
+        self.at["lens"] = (r.integers(0, 30, (self.seqs, 1)) + np.arange(self.k + 1)).reshape(-1).astype(np.int32)
+        drafts = r.integers(0, 1500, (self.seqs, self.k)).astype(np.int64)
+        self.randoms = r.integers(0, 2**64, (self.seqs, self.k + 1), dtype=np.uint64)
+        for name, v in (("x", self.ad["x"]), ("lens", self.at["lens"]), ("drafts", drafts), ("randoms", self.randoms.view(np.int64))):
+            if name in self.d:
+                self.d[name].copy_(gpu(v))
+            else:
+                self.d[name] = gpu(v)
+        torch.cuda.synchronize()
+
+    def project_and_attend(self):
+        d, b = self.d, self.b
+        b.linear_w8a16_adapters_dev(d["x"], d["W"], d["w_shifts"], 10, d["ids"], d["A"], d["a_shifts"], 10, d["B"], d["b_shifts"], 10,
+                                    out=self.proj, workspace=self.ws)
+        b.attention_prefix_dev(self.proj.view(self.mix.shape), d["kp"], d["vp"], d["kt"], d["vt"], d["lens"], self.at["mult"],
+                               self.at["shift"], self.table, 6, 14, rows_per_seq=self.k + 1, slots=d["slots"], out=self.mix, workspace=self.ws)
+
+    def to_logits(self):
+        """And a first draft that the target is fond of."""
+        self.b.logits_dev(self.mix.view(self.proj.shape), self.d["Wv"], self.d["v_shifts"], 10, 6, out=self.logits)
+        self.d["drafts"][:, 0] = self.target[:, 0].argmax(-1)
+
+    def check_drafts(self):
+        self.b.verify_drafts_dev(self.target, self.d["drafts"], self.d["randoms"], exp_lut=self.table, accepted=self.accepted,
+                                 out=self.tokens, workspace=self.ws)
+
+    def check(self, what):
+        """Every stage against its plain form (the logits, which other tests check, as they are)."""
+        import torch
+        torch.cuda.synchronize()
+        proj = want_adapters(self.ad)
+        same(self.proj, proj, f"{what}: projection")
+        same(self.mix, ref.attention(**dict(self.at, q=proj.reshape(self.mix.shape)), lut=self.lut), f"{what}: attention")
+        z = self.target.cpu().numpy()
+        want = ref.verify(z, self.d["drafts"].cpu().numpy(), self.randoms, lut=self.lut)
+        same(self.accepted, want[0], f"{what}: accepted")
+        same(self.tokens, want[1], f"{what}: tokens")
+        return want
+
+
+def test_serving_step(backend, exp_lut):
+    case("serving step")
+    step = Step(backend, exp_lut)
+    for turn in range(3):
+        case(f"serving step, turn {turn}")
+        step.project_and_attend()
+        step.to_logits()
+        step.check_drafts()
+        accepted, tokens = step.check(f"turn {turn}")
+        assert ((tokens >= 0).sum(1) == accepted + 1).all()
+        step.new_inputs(70 + turn)
+
+
+def test_serving_step_captured(backend, exp_lut):
+    """Two captured graphs on one workspace, replayed several times with eager work, new inputs
+    and synchronisations between."""
+    import torch
+    case("serving step captured")
+    step = Step(backend, exp_lut, seed=62)
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    try:
+        with torch.cuda.stream(stream):
+            backend.use_torch_stream()
+            step.project_and_attend()
+            step.to_logits()
+            step.check_drafts()
+        torch.cuda.synchronize()
+        graphs = []
+        for part in (step.project_and_attend, step.check_drafts):
+            g = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(g, stream=stream):
+                part()
+            graphs.append(g)
+        torch.cuda.synchronize()
+        for turn in range(4):
+            case(f"replay {turn}")
+            step.new_inputs(80 + turn)
+            step.ws.fill_(turn + 1)
+            for t in (step.proj, step.mix, step.logits, step.accepted, step.tokens):
+                t.fill_(-7)
+            torch.cuda.synchronize()
+            with torch.cuda.stream(stream):
+                backend.use_torch_stream()
+                graphs[0].replay()
+                step.to_logits()
+                graphs[1].replay()
+                torch.cuda.synchronize()
+            step.check(f"replay {turn}")
+    finally:
+        torch.cuda.synchronize()
+        backend.use_torch_stream()
+
+
+def test_two_steps_at_once(backend, exp_lut):
+    """Two contexts on two streams of their own, each with its workspace, side by side."""
+    import torch
+    from myelith_amd.backend import RocmBackend
+    case("two steps at once")
+    other = RocmBackend(0)
+    try:
+        steps = [Step(backend, exp_lut, seed=63), Step(other, exp_lut, seqs=9, k=1, seed=64)]
+        streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+        torch.cuda.synchronize()
+        for s, stream in zip(steps, streams):
+            with torch.cuda.stream(stream):
+                s.b.use_torch_stream()
+        for _ in range(10):
+            for s, stream in zip(steps, streams):
+                with torch.cuda.stream(stream):
+                    s.project_and_attend()
+                    s.to_logits()
+                    s.check_drafts()
+        for i, s in enumerate(steps):
+            s.check(f"step {i}")
+    finally:
+        torch.cuda.synchronize()
+        backend.use_torch_stream()
+        other.close()
+
+
+def test_calls_without_workspace_or_outputs(backend, exp_lut):
+    """The calls' own workspaces and outputs, on the context's stream and on another than torch's."""
+    import torch
+    case("own workspaces")
+    s, t, v = adapter_inputs(65, 9, 70, 96, 8, 3), attention_inputs(66, 3, 2, 90, 20, 4, 2, 64), verify_inputs(67, 3, 2, 700)
+    da, dt = ({k: gpu(x) if isinstance(x, np.ndarray) else x for k, x in y.items()} for y in (s, t))
+    z, tok, rnd, table = gpu(v["target"]), gpu(v["tokens"]), gpu(v["randoms"].view(np.int64)), gpu(exp_lut)
+    draft = gpu(v["draft"])
+    side = torch.cuda.Stream()
+    try:
+        for where in ("torch's stream", "another stream"):
+            torch.cuda.synchronize()
+            if where == "another stream":
+                with torch.cuda.stream(side):
+                    backend.use_torch_stream()
+            for _ in range(3):  # the memory of a call that has ended may be handed to the next
+                a = backend.linear_w8a16_adapters_dev(da["x"], da["W"], da["w_shifts"], 10, da["ids"], da["A"], da["a_shifts"], 10,
+                                                      da["B"], da["b_shifts"], 10)
+                b = backend.attention_prefix_dev(dt["q"], dt["kp"], dt["vp"], dt["kt"], dt["vt"], dt["lens"], dt["mult"], dt["shift"],
+                                                 table, 6, 14, rows_per_seq=2, slots=dt["slots"])
+                c = backend.verify_drafts_dev(z, tok, rnd, exp_lut=table, draft=draft)
+            torch.cuda.synchronize()
+            same(a, want_adapters(s), where)
+            same(b, ref.attention(**t, lut=exp_lut), where)
+            want = ref.verify(**v, lut=exp_lut)
+            same(c[0], want[0], where)
+            same(c[1], want[1], where)
+    finally:
+        torch.cuda.synchronize()
+        backend.use_torch_stream()
