@@ -39,18 +39,22 @@ def _need(ok, what: str) -> None:
 
 
 def _need_dev(what: str, device, **tensors) -> None:
-    """name=(tensor, dtype name, shape): on the device, of that type and shape (-1:
-    any size), its elements in order (strides are the caller's to check where shape is None)."""
+    """name=(tensor, dtype name, shape): on the device, of that type and shape, its
+    elements in order (strides are the caller's to check where shape is None)."""
+    import torch
     for name, (t, dtype, shape) in tensors.items():
-        if t.device != device or str(t.dtype) != "torch." + dtype:
+        if t.device != device or t.dtype is not getattr(torch, dtype):
             raise ValueError(f"{what}: {name} must be {dtype} on {device}")
-        if shape is not None and not (tuple(t.shape) == shape and t.is_contiguous()):
+        if shape is not None and not (t.shape == shape and t.is_contiguous()):
             raise ValueError(f"{what}: {name} must be contiguous {list(shape)}, not {list(t.shape)}")
 
 
 def _strides(t):
     """The strides that an element's place depends on (0 for dimensions of one element or none)."""
-    return tuple(st if n > 1 else 0 for st, n in zip(t.stride(), t.shape)) if t.numel() else (0,) * t.ndim
+    st, shape = t.stride(), t.shape
+    if 0 in shape:
+        return (0,) * len(st)
+    return tuple(s if n > 1 else 0 for s, n in zip(st, shape)) if 1 in shape else st
 
 
 class RocmBackend:
@@ -364,21 +368,23 @@ class RocmBackend:
         return out
 
     # ---- a serving step: adapters, a shared prefix, drafted tokens ---------------
-    def _workspace(self, nbytes: int, device, workspace):
-        """The caller's workspace, or one for this call alone (the allocator keeps
-        it until the context's stream has passed it)."""
+    def _workspace(self, device, workspace, size_of, *sizes):
+        """The caller's workspace (the call checks its size), or one for this call
+        alone (the allocator keeps it until the context's stream has passed it)."""
         if workspace is not None:
-            _need(workspace.device == device and workspace.is_contiguous(), "workspace: contiguous, on the operands' device")
+            if workspace.device != device or not workspace.is_contiguous():
+                raise ValueError("workspace: contiguous, on the operands' device")
             return workspace
         import torch
-        ws = torch.empty(max(nbytes, 1), dtype=torch.uint8, device=device)
+        ws = torch.empty(max(size_of(self._h, *sizes), 1), dtype=torch.uint8, device=device)
         stream = lib().myl_stream(self._h) or 0
         if stream != torch.cuda.current_stream(device).cuda_stream:
             ws.record_stream(torch.cuda.ExternalStream(stream, device=device))
         return ws
 
     def _need_here(self, what: str, device) -> None:
-        _need(device.type == "cuda" and device.index == self._device_id, f"{what}: the operands must be on device {self._device_id}")
+        if device.type != "cuda" or device.index != self._device_id:
+            raise ValueError(f"{what}: the operands must be on device {self._device_id}")
 
     @staticmethod
     def _new_workspace(nbytes: int, device, what: str):
@@ -405,20 +411,24 @@ class RocmBackend:
         _need_dev(what, x.device, x=(x, "int16", None), W=(W, "int8", (N, K)), w_shifts=(w_shifts, "uint8", (N,)),
                   ids=(ids, "int32", (M,)), A=(A, "int8", (n, rank, K)), a_shifts=(a_shifts, "uint8", (n, rank)),
                   B=(B, "int8", (n, N, rank)), b_shifts=(b_shifts, "uint8", (n, N)))
-        _need(_strides(x)[1] in (0, 1), f"{what}: the elements of a row of x follow one another")
+        ldx, step = _strides(x)
+        if step not in (0, 1):
+            raise ValueError(f"{what}: the elements of a row of x follow one another")
         if out_frac_pc is not None:
             _need_dev(what, x.device, out_frac_pc=(out_frac_pc, "uint8", (N,)))
         if out is None:
             import torch
             out = torch.empty((M, N), dtype=torch.int16, device=x.device)
         _need_dev(what, x.device, out=(out, "int16", None))
-        _need(tuple(out.shape) == (M, N) and _strides(out)[1] in (0, 1), f"{what}: out must be [M x N]")
+        ldo, step = _strides(out)
+        if out.shape != (M, N) or step not in (0, 1):
+            raise ValueError(f"{what}: out must be [M x N]")
         self._need_here(what, x.device)
-        ws = self._workspace(lib().myl_linear_w8a16_adapters_workspace(self._h, M, N, K, rank, n), x.device, workspace)
+        ws = self._workspace(x.device, workspace, lib().myl_linear_w8a16_adapters_workspace, M, N, K, rank, n)
         rc = lib().myl_linear_w8a16_adapters_dev(
-            self._h, x.data_ptr(), M, _strides(x)[0] or K, W.data_ptr(), N, K, w_shifts.data_ptr(), act_frac, out_frac,
+            self._h, x.data_ptr(), M, ldx or K, W.data_ptr(), N, K, w_shifts.data_ptr(), act_frac, out_frac,
             None if out_frac_pc is None else out_frac_pc.data_ptr(), ids.data_ptr(), A.data_ptr(), a_shifts.data_ptr(),
-            mid_frac, B.data_ptr(), b_shifts.data_ptr(), n, rank, out.data_ptr(), _strides(out)[0] or N,
+            mid_frac, B.data_ptr(), b_shifts.data_ptr(), n, rank, out.data_ptr(), ldo or N,
             ws.data_ptr(), ws.numel() * ws.element_size())
         if rc:
             self.check(rc, what)
@@ -445,10 +455,12 @@ class RocmBackend:
         KH, P = k_prefix.shape[:2]
         S, _, T = k_tail.shape[:3]
         dev = q.device
-        _need(rows_per_seq > 0 and R % rows_per_seq == 0, f"{what}: rows must be a multiple of rows_per_seq")
-        _need(k_prefix.shape == v_prefix.shape == (KH, P, hd) and k_tail.shape == v_tail.shape == (S, KH, T, hd),
-              f"{what}: prefix [kv_heads x P x hd], tails [slots x kv_heads x capacity x hd]")
-        _need(max_tail is None or 0 <= max_tail <= T, f"{what}: max_tail is at most the tails' capacity")
+        if rows_per_seq <= 0 or R % rows_per_seq:
+            raise ValueError(f"{what}: rows must be a multiple of rows_per_seq")
+        if not (k_prefix.shape == v_prefix.shape == (KH, P, hd) and k_tail.shape == v_tail.shape == (S, KH, T, hd)):
+            raise ValueError(f"{what}: prefix [kv_heads x P x hd], tails [slots x kv_heads x capacity x hd]")
+        if max_tail is not None and not 0 <= max_tail <= T:
+            raise ValueError(f"{what}: max_tail is at most the tails' capacity")
         _need_dev(what, dev, q=(q, "int16", None), k_prefix=(k_prefix, "int16", None), v_prefix=(v_prefix, "int16", None),
                   k_tail=(k_tail, "int16", None), v_tail=(v_tail, "int16", None), lens=(lens, "int32", (R,)),
                   exp_lut=(exp_lut, "int16", (exp_lut.numel(),)))
@@ -456,26 +468,30 @@ class RocmBackend:
         if slots is not None:
             _need_dev(what, dev, slots=(slots, "int32", (n_seqs,)))
         else:
-            _need(S >= n_seqs, f"{what}: fewer tails than sequences")
+            if not (S >= n_seqs):
+                raise ValueError(f"{what}: fewer tails than sequences")
         if out is None:
             import torch
             out = torch.empty((R, H, hd), dtype=torch.int16, device=dev)
         _need_dev(what, dev, out=(out, "int16", None))
-        _need(out.shape == q.shape, f"{what}: out must have q's shape")
+        if out.shape != q.shape:
+            raise ValueError(f"{what}: out must have q's shape")
 
         def rows_of(t, name):
-            _need(_strides(t)[1] in (0, hd) and _strides(t)[2] in (0, 1), f"{what}: the heads of a row of {name} follow one another")
-            return _strides(t)[0] or H * hd
+            row, head, one = _strides(t)
+            if head not in (0, hd) or one not in (0, 1):
+                raise ValueError(f"{what}: the heads of a row of {name} follow one another")
+            return row or H * hd
 
         ps, ts = _strides(k_prefix), _strides(k_tail)
-        _need(ps[1] in (0, hd) and ps[2] in (0, 1) and ts[2] in (0, hd) and ts[3] in (0, 1),
-              f"{what}: the positions of a KV head follow one another")
-        _need(ps == _strides(v_prefix) and ts == _strides(v_tail), f"{what}: keys and values have the same strides")
+        if not (ps[1] in (0, hd) and ps[2] in (0, 1) and ts[2] in (0, hd) and ts[3] in (0, 1)):
+            raise ValueError(f"{what}: the positions of a KV head follow one another")
+        if ps != _strides(v_prefix) or ts != _strides(v_tail):
+            raise ValueError(f"{what}: keys and values have the same strides")
         max_tail = T if max_tail is None else max_tail
         ldq, ldo = rows_of(q, "q"), rows_of(out, "out")
         self._need_here(what, dev)
-        ws = self._workspace(lib().myl_attention_prefix_workspace(self._h, n_seqs, rows_per_seq, H, KH, hd, P, max_tail),
-                             dev, workspace)
+        ws = self._workspace(dev, workspace, lib().myl_attention_prefix_workspace, n_seqs, rows_per_seq, H, KH, hd, P, max_tail)
         rc = lib().myl_attention_prefix_dev(
             self._h, q.data_ptr(), n_seqs, rows_per_seq, ldq, H, KH, hd, k_prefix.data_ptr(), v_prefix.data_ptr(),
             P, ps[0] or P * hd, k_tail.data_ptr(), v_tail.data_ptr(), S, ts[0] or KH * T * hd, ts[1] or T * hd, max_tail,
@@ -504,19 +520,23 @@ class RocmBackend:
         what = "verify_drafts_dev"
         B, k1, V = target.shape
         dev, k = target.device, k1 - 1
-        _need(k >= 0, f"{what}: target must be [B x k+1 x V]")
+        if k < 0:
+            raise ValueError(f"{what}: target must be [B x k+1 x V]")
         _need_dev(what, dev, target=(target, "int32", None), tokens=(tokens, "int64", (B, k)))
 
         def rows_of(t, name, n):
             seq, row, one = _strides(t)
-            _need(one in (0, 1) and (not seq or not row or seq == n * row), f"{what}: the rows of {name} are evenly spaced")
+            if one not in (0, 1) or (seq and row and seq != n * row):
+                raise ValueError(f"{what}: the rows of {name} are evenly spaced")
             return row or seq or V
 
         if exp_lut is not None:
-            _need(randoms is not None, f"{what}: random numbers are needed unless the check is greedy")
+            if randoms is None:
+                raise ValueError(f"{what}: random numbers are needed unless the check is greedy")
             _need_dev(what, dev, exp_lut=(exp_lut, "int16", (exp_lut.numel(),)), randoms=(randoms, "int64", (B, k1)))
         if draft is not None:
-            _need(tuple(draft.shape) == (B, k, V), f"{what}: draft must be [B x k x V]")
+            if draft.shape != (B, k, V):
+                raise ValueError(f"{what}: draft must be [B x k x V]")
             _need_dev(what, dev, draft=(draft, "int32", None))
         if n_draft is not None:
             _need_dev(what, dev, n_draft=(n_draft, "int32", (B,)))
@@ -528,7 +548,7 @@ class RocmBackend:
         lut_len = 0 if exp_lut is None else exp_lut.numel()
         ldt, ldd = rows_of(target, "target", k1), V if draft is None or k == 0 else rows_of(draft, "draft", k)
         self._need_here(what, dev)
-        ws = self._workspace(lib().myl_verify_drafts_workspace(self._h, B, k, V, lut_len), dev, workspace)
+        ws = self._workspace(dev, workspace, lib().myl_verify_drafts_workspace, B, k, V, lut_len)
         rc = lib().myl_verify_drafts_dev(
             self._h, target.data_ptr(), ldt, None if draft is None or k == 0 else draft.data_ptr(), ldd, B, k, V, tokens.data_ptr(),
             None if n_draft is None else n_draft.data_ptr(), None if randoms is None else randoms.data_ptr(),

@@ -11,6 +11,7 @@
 //                          as 16 bits, and the ranges' sums of them
 //   prefix_pv_kernel       p_j from e_j and S, sum p_j v_j over each range
 //   prefix_out_kernel      the sums over the ranges, rounded and clamped
+// With few keys one launch does it all (prefix_short_kernel).
 // The prefix is read once for 64 vectors of any rows: their tiles and the
 // tails' tiles (vectors of one sequence) run side by side in every launch.
 #include "abi_internal.h"
@@ -29,6 +30,7 @@
 namespace myl {
 namespace {
 
+constexpr int kShortThreads = 512;
 constexpr int kQkTile = kPrefixQkTile, kPvTile = kPrefixPvTile;  // vectors of a block
 
 // The call, as every kernel sees it.  Row r = seq * rows_per_seq + i attends
@@ -48,6 +50,7 @@ struct PrefixAttn {
         SmallDiv tp, tt;  // tiles of the prefix's and of a sequence's vectors
         int blocks_p;
     } qk, pv;
+    int short_cap;                // keys that a block of prefix_short_kernel has room for
     int R, heads, P, max_tail, n_slots, vp_count, vt_count, np_count, nt_count, rp, rt, vp16, vt16, pgroups, tgroups;
     uint32_t pairs, lut_len;
     uint8_t shift, lut_shift, prob_frac;
@@ -147,10 +150,11 @@ __device__ inline const int16_t* keys_of(const PrefixAttn& a, const Part& p, con
     return uniform_ptr(p.tail ? tail + (size_t)p.slot * a.ts + (size_t)p.g * a.th : prefix + (size_t)p.g * a.ph);
 }
 
-__device__ inline int32_t sum_pairs(uint32_t w, int32_t acc) {
+__device__ inline int32_t dot_pairs(uint32_t w, uint32_t x, int32_t acc) {
     typedef short __attribute__((ext_vector_type(2))) s2;
-    return __builtin_amdgcn_sdot2(__builtin_bit_cast(s2, w), s2{1, 1}, acc, false);
+    return __builtin_amdgcn_sdot2(__builtin_bit_cast(s2, w), __builtin_bit_cast(s2, x), acc, false);
 }
+__device__ inline int32_t sum_pairs(uint32_t w, int32_t acc) { return dot_pairs(w, 0x00010001u, acc); }
 // 8 int16 as their byte planes x = 256 hi + lo' + 128.
 __device__ inline void planes8(const uint4& x, uint32_t* h, uint32_t* l) {
     h[0] = __builtin_amdgcn_perm(x.y, x.x, 0x07050301u);
@@ -240,17 +244,6 @@ struct TablePiece {
 // A wave holds the vectors' planes in registers and streams its groups of K rows, the
 // next step's loads in flight; no barrier in the loop.
 // SUBS 16-vector tiles, GU 16-position groups per wave and step.
-// The larger of two signed 64-bit values.  The comparison goes to a scalar pair: the second
-// v_cndmask_b32 of one VCC costs about 35 cycles (measured; with the pair, 5).
-__device__ inline int64_t max64(int64_t x, int64_t y) {
-    uint64_t m;
-    asm("v_cmp_gt_i64_e64 %0, %1, %2\n\ts_nop 1" : "=s"(m) : "v"(x), "v"(y));
-    int32_t hi, lo;
-    asm("v_cndmask_b32_e64 %0, %1, %2, %3" : "=v"(hi) : "v"((int32_t)(y >> 32)), "v"((int32_t)(x >> 32)), "s"(m));
-    asm("v_cndmask_b32_e64 %0, %1, %2, %3" : "=v"(lo) : "v"((int32_t)y), "v"((int32_t)x), "s"(m));
-    return (int64_t)(((uint64_t)(uint32_t)hi << 32) | (uint32_t)lo);
-}
-
 constexpr int qk_groups(int subs) { return subs == 1 ? 2 : 1; }
 template <int HD, bool FAST, Pass PASS, int SUBS>
 __device__ inline void prefix_qk_part(const PrefixAttn& a, const Part& p, Vectors<kQkTile>& vs, uint16_t* tab, int8_t* klds,
@@ -434,7 +427,7 @@ __device__ inline void prefix_qk_part(const PrefixAttn& a, const Part& p, Vector
                         best[t] += (int32_t)ev[i];
                     }
                 }
-                if (PASS == kMaxPass && FAST) top[t] = max64(top[t], max64(max64(key[0], key[1]), max64(key[2], key[3])));
+                if (PASS == kMaxPass && FAST) top[t] = max(top[t], max(max(key[0], key[1]), max(key[2], key[3])));
                 if (PASS == kExpPass && (!MASK || jg < j1))
                     *reinterpret_cast<uint2*>(eo[t] + 16 * jg) = make_uint2(ev[0] | (ev[1] << 16), ev[2] | (ev[3] << 16));
             }
@@ -742,6 +735,99 @@ __global__ __launch_bounds__(256) void prefix_out_kernel(PrefixAttn a) {
     *reinterpret_cast<uint2*>(a.out + (size_t)row * a.ldo + i) = make_uint2(y[0] | (y[1] << 16), y[2] | (y[3] << 16));
 }
 
+// ---- few keys: one launch ---------------------------------------------------------
+
+// A block per row and KV head does all of it: scores of the row's query heads (at most 8, of
+// the 15 of qk_planes_wave) with all keys into LDS, a wave per head for the softmax,
+// P.V with a pair of dimensions and every so-many-th eight keys per thread.  The keys are
+// read for every row instead of every 64 vectors, but nothing waits for another launch.
+template <int HD>
+__global__ __launch_bounds__(kShortThreads) void prefix_short_kernel(PrefixAttn a) {
+    constexpr int PAIRS = HD / 2, STREAMS = kShortThreads / PAIRS, WAVES = kShortThreads / 64;
+    static_assert(WAVES >= (int)kPrefixShortHeads);
+    extern __shared__ __align__(16) int32_t z[];  // [G][cap] scores, [G][cap] probabilities, [G][HD] sums
+    const int G = (int)a.G.d, cap = a.short_cap;
+    uint16_t* ps = reinterpret_cast<uint16_t*>(z + G * cap);
+    int32_t* acc = reinterpret_cast<int32_t*>(ps + G * cap);
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    int g, rem;
+    const int row = divmod(a.kvh, (int)blockIdx.x, g), slot = slot_of(a, divmod(a.n, row, rem));
+    const int tail = __builtin_amdgcn_readfirstlane(tail_of(a, row, slot)), L = tail < 0 ? 0 : a.P + tail;
+    int16_t* out = a.out + (size_t)row * a.ldo + (size_t)(g * G * HD);
+    for (int i = tid; i < G * HD; i += kShortThreads) acc[i] = 0;
+    const size_t toff = (size_t)max(slot, 0) * a.ts + (size_t)g * a.th, poff = (size_t)g * a.ph;
+    const int16_t* q = a.q + (size_t)row * a.ldq + (size_t)(g * G * HD);
+    const int gp = tail < 0 ? 0 : (a.P + 15) >> 4, groups = gp + (max(tail, 0) + 15) / 16;
+    for (int i = wave; i < groups; i += WAVES) {
+        if (i < gp) qk_planes_wave<HD>(a.P, 16 * i, a.kp + poff, q, G, a.mult, a.shift, z, (size_t)cap);
+        else qk_planes_wave<HD>(tail, 16 * (i - gp), a.kt + toff, q, G, a.mult, a.shift, z + a.P, (size_t)cap);
+    }
+    __syncthreads();
+    if (const int h = wave; h < G && L > 0) {
+        int32_t* zh = z + h * cap;
+        int32_t m = INT32_MIN;
+        for (int j = lane; j < L; j += 64) m = max(m, zh[j]);
+        m = wave_max_i32(m);
+        uint32_t s = 0;
+        for (int j = lane; j < L; j += 64) {  // sat_sub and the lookup of softmax.rs:12-38
+            const uint32_t i = min((uint32_t)m - (uint32_t)zh[j], 0x7FFFFFFFu) >> (a.lut_shift & 31u);
+            const int32_t e = i < a.lut_len ? max((int32_t)a.lut[i], 0) : 0;
+            zh[j] = e;
+            s += (uint32_t)e;
+        }
+        s = (uint32_t)wave_sum_i32((int32_t)s);
+        const ProbDiv div = ProbDiv::of(s ? s : 1u, a.prob_frac);
+        uint32_t base = 0, extra = 0;
+        if (s == 0) udivmod32(1u << a.prob_frac, (uint32_t)L, recip32((uint32_t)L), &base, &extra);
+        for (int j = lane; j < ((L + 7) & ~7); j += 64) {
+            const uint32_t p = j >= L ? 0u : s ? div((uint32_t)zh[j]) : base + ((uint32_t)j < extra ? 1u : 0u);
+            ps[h * cap + j] = (uint16_t)p;
+        }
+    }
+    __syncthreads();
+    // dimensions 2 dp, + 1; the probabilities are at most 2^14, so pairs of keys fit v_dot2
+    const int dp = tid % PAIRS, stream = tid / PAIRS;
+    const int16_t *vp = a.vp + poff + 2 * dp, *vt = a.vt + toff + 2 * dp;
+    if (L > 0) {
+        int32_t s0[kPrefixShortHeads], s1[kPrefixShortHeads];
+#pragma unroll
+        for (int h = 0; h < (int)kPrefixShortHeads; ++h) s0[h] = s1[h] = 0;
+        for (int j0 = 8 * stream; j0 < L; j0 += 8 * STREAMS) {
+            uint32_t v[8];
+#pragma unroll
+            for (int k = 0; k < 8; ++k) {
+                const int j = min(j0 + k, L - 1);
+                v[k] = *reinterpret_cast<const uint32_t*>((j < a.P ? vp : vt) + (size_t)(j < a.P ? j : j - a.P) * HD);
+            }
+            uint32_t w0[4], w1[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                w0[k] = __builtin_amdgcn_perm(v[2 * k + 1], v[2 * k], 0x05040100u);
+                w1[k] = __builtin_amdgcn_perm(v[2 * k + 1], v[2 * k], 0x07060302u);
+            }
+#pragma unroll
+            for (int h = 0; h < (int)kPrefixShortHeads; ++h) {
+                if (h >= G) break;
+                const uint4 p4 = *reinterpret_cast<const uint4*>(ps + h * cap + j0);
+                const uint32_t p[4] = {p4.x, p4.y, p4.z, p4.w};
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    s0[h] = dot_pairs(w0[k], p[k], s0[h]);
+                    s1[h] = dot_pairs(w1[k], p[k], s1[h]);
+                }
+            }
+        }
+#pragma unroll
+        for (int h = 0; h < (int)kPrefixShortHeads; ++h) {
+            if (h >= G) break;
+            atomicAdd(&acc[h * HD + 2 * dp], s0[h]);
+            atomicAdd(&acc[h * HD + 2 * dp + 1], s1[h]);
+        }
+    }
+    __syncthreads();
+    for (int i = tid; i < G * HD; i += kShortThreads) out[i] = clamp_i16(rshift_round32(acc[i], a.prob_frac));
+}
+
 template <int HD, bool FAST>
 hipError_t prefix_scores(const PrefixAttn& a, unsigned grid, hipStream_t st) {
     prefix_qk_kernel<HD, FAST, kMaxPass><<<grid, 256, 0, st>>>(a);
@@ -757,6 +843,10 @@ hipError_t prefix_scores(const PrefixAttn& a, unsigned grid, hipStream_t st) {
 
 template <int HD>
 hipError_t prefix_launch(const PrefixAttn& a, const PrefixPlan& pl, hipStream_t st) {
+    if (pl.short_cap) {
+        prefix_short_kernel<HD><<<(unsigned)(a.R * (int)a.kvh.d), kShortThreads, prefix_short_lds(pl.G, pl.short_cap, HD), st>>>(a);
+        return hipGetLastError();
+    }
     const unsigned grid = (unsigned)(pl.qk.blocks_p + pl.qk.blocks_t);
     if (grid) {
         // 2^31 >> lut_shift is past every table
@@ -830,6 +920,7 @@ int myl_attention_prefix_dev(myl_ctx* ctx, const int16_t* q, size_t n_seqs, size
     a.np = div((size_t)pl.np); a.nt = div((size_t)pl.nt);
     auto cut = [&](const PrefixPlan::Cut& c) { return PrefixAttn::Cut{div((size_t)c.tp), div((size_t)c.tt), (int)c.blocks_p}; };
     a.qk = cut(pl.qk); a.pv = cut(pl.pv);
+    a.short_cap = pl.short_cap;
     a.R = (int)(n_seqs * rows_per_seq); a.heads = (int)heads; a.P = (int)prefix_len; a.max_tail = (int)max_tail;
     a.n_slots = (int)n_slots; a.vp_count = pl.vp; a.vt_count = pl.vt; a.np_count = pl.np; a.nt_count = pl.nt;
     a.rp = pl.rp; a.rt = pl.rt; a.vp16 = (pl.vp + 15) / 16; a.vt16 = (pl.vt + 15) / 16; a.pgroups = pl.pgroups; a.tgroups = pl.tgroups;

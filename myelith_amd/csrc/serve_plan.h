@@ -123,7 +123,12 @@ inline const char* prefix_refuse(const PrefixShape& s) {
 // tiles those of one sequence.
 constexpr int kPrefixQkTile = 64, kPrefixPvTile = 64;
 
+constexpr size_t kPrefixShortHeads = 8, kPrefixShortWork = 320 * 128;  // heads of a KV head; keys x head_dim
+// LDS of a block that does a row's heads by itself: scores, probabilities, sums.
+inline size_t prefix_short_lds(int G, int cap, size_t hd) { return (size_t)G * ((size_t)cap * 6 + hd * 4); }
+
 struct PrefixPlan {
+    int short_cap;         // > 0: one launch, blocks with room for so many keys; nothing below is used
     int G, vp, vt;       // query heads per KV head; vectors per KV head: of all rows, of one sequence
     struct Cut {
         int tp, tt;      // tiles of each
@@ -135,6 +140,16 @@ struct PrefixPlan {
     size_t off_max, off_sum, off_pexp, off_texp, off_out, bytes;
 };
 
+// One launch with a block per row and KV head, which reads its keys for itself, or four
+// launches that share the keys between rows.  Measured with seven heads per KV head, one /
+// four launches: 320 keys of 128 18.1 / 22.4 us for one row, 18.6 / 24.3 for 16, 46.1 / 47.4
+// for 256 rows of four KV heads; 512 keys 25.3 / 22.9, 25.7 / 25.0, 69.2 / 46.5; 512 keys of 64
+// 18.1 / 21.9, 18.5 / 22.8, and 24.8 / 30.7 for 256 rows of two KV heads.  A wave does one head.
+inline bool prefix_short(const PrefixShape& s, int cus) {
+    const size_t blocks = s.n_seqs * s.rows_per_seq * s.kv_heads, keys = s.prefix_len + s.max_tail;
+    return keys > 0 && s.heads / s.kv_heads <= kPrefixShortHeads && blocks <= 4 * (size_t)cus && keys * s.head_dim <= kPrefixShortWork;
+}
+
 inline PrefixPlan prefix_plan(const PrefixShape& s, int cus) {
     PrefixPlan p{};
     const int64_t R = (int64_t)(s.n_seqs * s.rows_per_seq), kvh = (int64_t)s.kv_heads;
@@ -142,6 +157,11 @@ inline PrefixPlan prefix_plan(const PrefixShape& s, int cus) {
     p.vp = (int)(R * p.G);
     p.vt = (int)(s.rows_per_seq * p.G);
     const int P = (int)s.prefix_len, T = (int)s.max_tail;
+    if (prefix_short(s, cus)) {
+        p.short_cap = (P + T + 63) / 64 * 64;
+        p.bytes = 256;
+        return p;
+    }
     auto tiles = [](int v, int tile) { return (v + tile - 1) / tile; };
     // Two blocks of the P.V tiles per CU (the prefix's and the tails' each), ranges of
     // 64 keys at least.

@@ -419,6 +419,48 @@ def test_refusals(backend, exp_lut):
     assert att().shape == (2, 4, 64)  # the context is as good as before
 
 
+# ---- the form that shares the keys between rows, at the sizes that one launch takes with fewer heads ----
+
+@pytest.mark.parametrize("seqs,rows,prefix,tail,H,KH,hd", [
+    (1, 1, 1, 0, 9, 1, 64), (1, 1, 0, 1, 10, 1, 64), (1, 1, 1, 1, 18, 2, 128), (2, 1, 15, 3, 18, 2, 64), (2, 1, 16, 16, 36, 4, 128),
+    (3, 1, 17, 33, 9, 1, 64), (5, 2, 63, 65, 20, 2, 64), (4, 1, 64, 64, 18, 2, 128), (9, 1, 65, 5, 36, 4, 128), (1, 8, 127, 129, 9, 1, 128),
+    (700, 1, 40, 9, 14, 2, 64)])
+def test_attention_many_heads_or_rows(backend, exp_lut, seqs, rows, prefix, tail, H, KH, hd):
+    case(f"attention {seqs}x{rows} prefix={prefix} tail={tail} heads={H}/{KH} hd={hd}")
+    s = attention_inputs(prefix + tail, seqs, rows, prefix, tail, H, KH, hd)
+    same(run_attention(backend, s, exp_lut), ref.attention(**s, lut=exp_lut), "attention")
+
+
+@pytest.mark.parametrize("prefix,tail", [(50, 20), (0, 20), (50, 0), (0, 0)])
+def test_attention_many_heads_left_out_and_bad_slots(backend, exp_lut, prefix, tail):
+    case(f"attention many heads left out prefix={prefix} tail={tail}")
+    s = attention_inputs(24, 7, 2, prefix, tail, 18, 2, 64, slots=[3, 3, -1, 8, 0, 2**31 - 1, -2**31])
+    s["lens"] = np.array([0, tail, -1, 2, 1, tail + 5, 2**31 - 1, -2**31, tail, -7, 3, 0, 1, -1], np.int32)
+    same(run_attention(backend, s, exp_lut), ref.attention(**s, lut=exp_lut), "left out")
+
+
+@pytest.mark.parametrize("H", [8, 18])
+@pytest.mark.parametrize("mult,shift,lut_shift,prob_frac", [(2896, 30, 0, 8), (1, 9, 3, 0), (-4096, 22, 6, 14), (1 << 30, 40, 6, 14),
+                                                           (0, 21, 6, 14), (3, 0, 31, 13), (2896, 63, 6, 14)])
+def test_attention_scales_of_both_forms(backend, exp_lut, H, mult, shift, lut_shift, prob_frac):
+    case(f"attention scales H={H} {mult} {shift} {lut_shift} {prob_frac}")
+    s = attention_inputs(25, 3, 2, 70, 30, H, 2, 128)
+    s.update(mult=mult, shift=shift, lut_shift=lut_shift, prob_frac=prob_frac)
+    same(run_attention(backend, s, exp_lut), ref.attention(**s, lut=exp_lut), "scales")
+
+
+@pytest.mark.parametrize("H", [8, 18])
+@pytest.mark.parametrize("table", ["one", "negative", "zero", "long"])
+def test_attention_tables_of_both_forms(backend, H, table):
+    """Tables of one entry, with negative entries, without weight (a uniform split), and of 32768."""
+    case(f"attention table {table} H={H}")
+    lut = {"one": np.array([5], np.int16), "negative": rng(7).integers(-300, 300, 500).astype(np.int16), "zero": np.zeros(3, np.int16),
+           "long": rng(8).integers(0, 32768, 32768).astype(np.int16)}[table]
+    s = attention_inputs(26, 3, 2, 70, 30, H, 2, 64)
+    s.update(lut_shift=0 if table == "long" else 3)
+    same(run_attention(backend, s, lut), ref.attention(**s, lut=lut), table)
+
+
 # ---- many rows, long offsets --------------------------------------------------------------
 
 @pytest.mark.parametrize("M,N,K,rank,n", [(1500, 520, 64, 8, 300), (257, 70, 130, 12, 2), (1030, 33, 96, 70, 17)])
@@ -495,13 +537,13 @@ class Step:
     """A projection with adapters, attention behind the shared prefix, logits and the check of
     the drafts, for seqs sequences of k drafts; one workspace serves all calls in turn."""
 
-    def __init__(self, backend, exp_lut, seqs=5, k=3, seed=61):
+    def __init__(self, backend, exp_lut, seqs=5, k=3, seed=61, prefix=150):
         import torch
         self.b, self.lut, self.k, self.seqs = backend, exp_lut, k, seqs
         H, hd, V, rows = 14, 64, 1500, seqs * (k + 1)
         r = rng(seed)
         self.ad = adapter_inputs(seed, rows, H * hd, 448, 16, 4, np.repeat(r.integers(-1, 4, seqs), k + 1))
-        self.at = attention_inputs(seed + 1, seqs, k + 1, 150, 33, H, 2, hd)
+        self.at = attention_inputs(seed + 1, seqs, k + 1, prefix, 33, H, 2, hd)
         self.Wv = r.integers(-128, 128, (V, H * hd)).astype(np.int8)
         self.v_shifts = np.full(V, 9, np.uint8)
         self.d = {n: gpu(v) for n, v in [*self.ad.items(), *self.at.items(), ("Wv", self.Wv), ("v_shifts", self.v_shifts)]
@@ -564,9 +606,10 @@ class Step:
         return want
 
 
-def test_serving_step(backend, exp_lut):
+@pytest.mark.parametrize("prefix", [150, 900])
+def test_serving_step(backend, exp_lut, prefix):
     case("serving step")
-    step = Step(backend, exp_lut)
+    step = Step(backend, exp_lut, prefix=prefix)
     for turn in range(3):
         case(f"serving step, turn {turn}")
         step.project_and_attend()
@@ -577,12 +620,13 @@ def test_serving_step(backend, exp_lut):
         step.new_inputs(70 + turn)
 
 
-def test_serving_step_captured(backend, exp_lut):
+@pytest.mark.parametrize("prefix", [150, 900])
+def test_serving_step_captured(backend, exp_lut, prefix):
     """Two captured graphs on one workspace, replayed several times with eager work, new inputs
     and synchronisations between."""
     import torch
     case("serving step captured")
-    step = Step(backend, exp_lut, seed=62)
+    step = Step(backend, exp_lut, seed=62, prefix=prefix)
     stream = torch.cuda.Stream()
     stream.wait_stream(torch.cuda.current_stream())
     try:
@@ -625,7 +669,7 @@ def test_two_steps_at_once(backend, exp_lut):
     case("two steps at once")
     other = RocmBackend(0)
     try:
-        steps = [Step(backend, exp_lut, seed=63), Step(other, exp_lut, seqs=9, k=1, seed=64)]
+        steps = [Step(backend, exp_lut, seed=63), Step(other, exp_lut, seqs=9, k=1, seed=64, prefix=1200)]
         streams = [torch.cuda.Stream(), torch.cuda.Stream()]
         torch.cuda.synchronize()
         for s, stream in zip(steps, streams):

@@ -74,6 +74,12 @@ static void adapters(AdapterShape s, int cus) {
 static void prefix(PrefixShape s, int cus) {
     if (prefix_refuse(s)) return;
     const PrefixPlan p = prefix_plan(s, cus);
+    if (p.short_cap) {
+        const size_t keys = s.prefix_len + s.max_tail;
+        CHECK(keys > 0 && (size_t)p.short_cap >= keys && p.short_cap % 64 == 0 && p.G <= 8 && p.bytes == 256 &&
+              prefix_short_lds(p.G, p.short_cap, s.head_dim) <= 65536 && s.n_seqs * s.rows_per_seq * s.kv_heads <= 4 * (size_t)cus, "short: %zu keys", keys);
+        return;
+    }
     const int64_t P = (int64_t)s.prefix_len, T = (int64_t)s.max_tail, R = (int64_t)(s.n_seqs * s.rows_per_seq);
     auto ranges = [&](int64_t keys, int n, int len, bool any) {
         if (keys == 0 || !any) return CHECK(n == 0, "ranges without keys"), void();
