@@ -258,8 +258,9 @@ int myl_linear_w8a16_adapters_dev(myl_ctx* ctx, const int16_t* x, size_t M, size
  * The keys' order for softmax_int's uniform split is prefix, then tail.  Query
  * head h reads KV head h / (heads / kv_heads).  head_dim is 64 or 128
  * (MYL_E_UNSUPPORTED otherwise), prob_frac at most 14, prefix_len + max_tail at
- * most 65536, heads and rows at most 65535 each; negative exp table entries
- * count as 0.  Pointers are 16-byte aligned, strides (in elements) multiples of 8. */
+ * most 65536, heads and rows at most 65535 each and 2^22 together, the exp table
+ * 1 to 32768 entries; negative ones count as 0.  Pointers to int16 and the
+ * workspace are 16-byte aligned, strides (in elements) multiples of 8. */
 size_t myl_attention_prefix_workspace(const myl_ctx* ctx, size_t n_seqs, size_t rows_per_seq, size_t heads,
                                       size_t kv_heads, size_t head_dim, size_t prefix_len, size_t max_tail);
 int myl_attention_prefix_dev(myl_ctx* ctx, const int16_t* q, size_t n_seqs, size_t rows_per_seq, size_t ldq,
@@ -292,8 +293,8 @@ int myl_attention_prefix_dev(myl_ctx* ctx, const int16_t* q, size_t n_seqs, size
  *   accepted [n_seqs]: drafts accepted            out      [n_seqs x (k + 1)]: the
  *            accepted drafts, the next token, then -1
  * A drafted token outside the vocabulary is rejected.  vocab is at most 2^20,
- * k at most 1024 (0 samples a token per row), the table at most 32768 entries
- * (trailing zeros left off make it faster). */
+ * k at most 1024 (0 samples a token per row), n_seqs (2 k + 1) at most 65535,
+ * the table at most 32768 entries (trailing zeros left off make it faster). */
 size_t myl_verify_drafts_workspace(const myl_ctx* ctx, size_t n_seqs, size_t k, size_t vocab, size_t lut_len);
 int myl_verify_drafts_dev(myl_ctx* ctx, const int32_t* target, size_t ldt, const int32_t* draft, size_t ldd,
                           size_t n_seqs, size_t k, size_t vocab, const int64_t* tokens, const int32_t* n_draft,

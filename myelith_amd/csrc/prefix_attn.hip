@@ -242,7 +242,11 @@ struct TablePiece {
 // and start the accumulators, and sum q is one value per lane.  As 256 u + r the score
 // takes 32-bit steps (ScoreScale); other scales take the 64-bit form (FAST false).
 // A wave holds the vectors' planes in registers and streams its groups of K rows, the
-// next step's loads in flight; no barrier in the loop.
+// next step's loads in flight; no barrier in the loop.  Bound by issue (each instruction takes
+// about four cycles beside the matrix instructions): 64 rows of 28 heads by 30000 keys of
+// 128 take 45 us for the maxima (1.2 POP/s) and 73 for the exp values, whose table lookup and
+// store come on top.  Tiles of 32 vectors took 1.5 times as long, two steps of K in flight or
+// operands read a step ahead as long or longer (236 registers; spills).
 // SUBS 16-vector tiles, GU 16-position groups per wave and step.
 constexpr int qk_groups(int subs) { return subs == 1 ? 2 : 1; }
 template <int HD, bool FAST, Pass PASS, int SUBS>
@@ -485,7 +489,8 @@ struct ProbRow {
 // modulo 2^32, and the whole sum fits 32 bits (serve_plan.h).  V is turned in registers:
 // lane l loads dimensions 2 (l % 16), + 1 of the 16 keys of its block l / 16 and
 // gathers each dimension's bytes of four keys with v_perm, which is the A operand.
-// The p planes pass through LDS, two steps' places in turn, one barrier a step.
+// The p planes pass through LDS, two steps' places in turn, one barrier a step.  Bound by
+// issue like the scores: 65 us at 64 rows of 28 heads by 30000 keys of 128.
 template <int HD>
 struct PvShape {
     static constexpr int DW = HD / 32;  // waves side by side over the dimensions
@@ -740,7 +745,9 @@ __global__ __launch_bounds__(256) void prefix_out_kernel(PrefixAttn a) {
 // A block per row and KV head does all of it: scores of the row's query heads (at most 8, of
 // the 15 of qk_planes_wave) with all keys into LDS, a wave per head for the softmax,
 // P.V with a pair of dimensions and every so-many-th eight keys per thread.  The keys are
-// read for every row instead of every 64 vectors, but nothing waits for another launch.
+// read for every row instead of every 64 vectors, but nothing waits for another launch: 9.1 us
+// for 2 rows of 14 heads by 131 keys of 64, where four launches took 19.  Bound by the chain
+// of loads, softmax and sums in a block; the adds into acc are of integers, in any order.
 template <int HD>
 __global__ __launch_bounds__(kShortThreads) void prefix_short_kernel(PrefixAttn a) {
     constexpr int PAIRS = HD / 2, STREAMS = kShortThreads / PAIRS, WAVES = kShortThreads / 64;

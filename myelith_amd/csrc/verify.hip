@@ -21,7 +21,9 @@
 // follow (verify_sum_kernel).  Many blocks share a row, so that few rows fill the chip too.
 // The row that decides the next token is read a second time, chunk by chunk
 // (verify_weight_kernel), and the group of 256 values with the token a third
-// (verify_pick_kernel).
+// (verify_pick_kernel).  24 sequences of up to 5 drafts (about 150 rows, 88 MB), vocabulary
+// 152064: 19.4 us for the count (4.5 TB/s), 5.6, 9.5 and 5.9 for the others, 40 in all; one
+// block per row, with a pass for the maximum and one for the sum, took 355.
 #include "abi_internal.h"
 #include "ops.h"
 #include "serve_plan.h"
