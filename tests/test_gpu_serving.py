@@ -719,3 +719,20 @@ def test_calls_without_workspace_or_outputs(backend, exp_lut):
     finally:
         torch.cuda.synchronize()
         backend.use_torch_stream()
+
+
+def test_adapters_odd_addresses(backend):
+    """Adapters, shifts and rows that start anywhere; an odd K and rank."""
+    import torch
+    case("adapters odd addresses")
+    s = adapter_inputs(71, 37, 333, 1031, 5, 6)
+
+    def shifted(a):
+        t = torch.zeros(a.size + 3, dtype=torch.from_numpy(a[:0].copy()).dtype, device="cuda")
+        t[1:1 + a.size] = gpu(a).reshape(-1)
+        return t[1:1 + a.size].view(a.shape)
+
+    d = dict(s, **{k: shifted(s[k]) for k in ("x", "A", "a_shifts", "B", "b_shifts")})
+    pc = rng(9).integers(7, 13, 333).astype(np.uint8)
+    same(run_adapters(backend, d), want_adapters(s), "odd addresses")
+    same(run_adapters(backend, d, pc=pc), want_adapters(s, pc=pc), "odd addresses, per-channel output scale")
