@@ -163,14 +163,20 @@ inline PrefixPlan prefix_plan(const PrefixShape& s, int cus) {
         return p;
     }
     auto tiles = [](int v, int tile) { return (v + tile - 1) / tile; };
-    // Two blocks of the P.V tiles per CU (the prefix's and the tails' each), ranges of
-    // 64 keys at least.
+    // Two blocks of the P.V tiles per CU (the prefix's and the tails' each), but at least two
+    // steps of 64 keys a range, and e of them where there are 7 (e - 1)^2 or more: each range costs
+    // every later launch a partial result per vector, each step costs its block.  us a call at
+    // ranges of at least 1 / 2 / 4 / 8 steps: 64 rows, 1000 keys 53 / 40 / 41; one row, 16000
+    // keys - / 45 / 35 / 32; four rows, 30000 keys 56 / 55 / 52 / 47; 24 rows, 4000 keys 43 / 42 / 38
+    // / 46 (3: 36).
     auto cut = [&](int keys, int64_t per_range, int& n, int& len) {
         n = len = 0;
         if (keys == 0 || per_range == 0) return;
         const int steps = (keys + 63) / 64;
         const int64_t want = std::max<int64_t>(1, 2 * cus / per_range);
-        const int each = (int)((steps + std::min<int64_t>(want, steps) - 1) / std::min<int64_t>(want, steps));
+        int each = (int)((steps + std::min<int64_t>(want, steps) - 1) / std::min<int64_t>(want, steps)), least = 2;
+        while (7 * least * least < steps) ++least;
+        each = std::max(each, least);
         len = 64 * each;
         n = (steps + each - 1) / each;
     };
