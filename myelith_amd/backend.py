@@ -369,18 +369,23 @@ class RocmBackend:
 
     # ---- a serving step: adapters, a shared prefix, drafted tokens ---------------
     def _workspace(self, device, workspace, size_of, *sizes):
-        """The caller's workspace (the call checks its size), or one for this call
-        alone (the allocator keeps it until the context's stream has passed it)."""
+        """The caller's workspace (the call checks its size), or one for this call alone."""
         if workspace is not None:
             if workspace.device != device or not workspace.is_contiguous():
                 raise ValueError("workspace: contiguous, on the operands' device")
             return workspace
+        return self._empty(max(size_of(self._h, *sizes), 1), "uint8", device)
+
+    def _empty(self, shape, dtype: str, device):
+        """A tensor that a call writes: its memory is handed on only when the
+        context's stream has passed the call."""
         import torch
-        ws = torch.empty(max(size_of(self._h, *sizes), 1), dtype=torch.uint8, device=device)
-        stream = lib().myl_stream(self._h) or 0
-        if stream != torch.cuda.current_stream(device).cuda_stream:
-            ws.record_stream(torch.cuda.ExternalStream(stream, device=device))
-        return ws
+        t = torch.empty(shape, dtype=getattr(torch, dtype), device=device)
+        if device.type == "cuda":
+            stream = lib().myl_stream(self._h) or 0
+            if stream != torch.cuda.current_stream(device).cuda_stream:
+                t.record_stream(torch.cuda.ExternalStream(stream, device=device))
+        return t
 
     def _need_here(self, what: str, device) -> None:
         if device.type != "cuda" or device.index != self._device_id:
@@ -417,8 +422,7 @@ class RocmBackend:
         if out_frac_pc is not None:
             _need_dev(what, x.device, out_frac_pc=(out_frac_pc, "uint8", (N,)))
         if out is None:
-            import torch
-            out = torch.empty((M, N), dtype=torch.int16, device=x.device)
+            out = self._empty((M, N), "int16", x.device)
         _need_dev(what, x.device, out=(out, "int16", None))
         ldo, step = _strides(out)
         if out.shape != (M, N) or step not in (0, 1):
@@ -471,8 +475,7 @@ class RocmBackend:
             if not (S >= n_seqs):
                 raise ValueError(f"{what}: fewer tails than sequences")
         if out is None:
-            import torch
-            out = torch.empty((R, H, hd), dtype=torch.int16, device=dev)
+            out = self._empty((R, H, hd), "int16", dev)
         _need_dev(what, dev, out=(out, "int16", None))
         if out.shape != q.shape:
             raise ValueError(f"{what}: out must have q's shape")
@@ -540,10 +543,10 @@ class RocmBackend:
             _need_dev(what, dev, draft=(draft, "int32", None))
         if n_draft is not None:
             _need_dev(what, dev, n_draft=(n_draft, "int32", (B,)))
-        if accepted is None or out is None:
-            import torch
-            accepted = torch.empty(B, dtype=torch.int32, device=dev) if accepted is None else accepted
-            out = torch.empty((B, k1), dtype=torch.int64, device=dev) if out is None else out
+        if accepted is None:
+            accepted = self._empty(B, "int32", dev)
+        if out is None:
+            out = self._empty((B, k1), "int64", dev)
         _need_dev(what, dev, accepted=(accepted, "int32", (B,)), out=(out, "int64", (B, k1)))
         lut_len = 0 if exp_lut is None else exp_lut.numel()
         ldt, ldd = rows_of(target, "target", k1), V if draft is None or k == 0 else rows_of(draft, "draft", k)

@@ -736,3 +736,27 @@ def test_adapters_odd_addresses(backend):
     pc = rng(9).integers(7, 13, 333).astype(np.uint8)
     same(run_adapters(backend, d), want_adapters(s), "odd addresses")
     same(run_adapters(backend, d, pc=pc), want_adapters(s, pc=pc), "odd addresses, per-channel output scale")
+
+
+def test_one_context_on_two_streams(backend, exp_lut):
+    """Calls of one context on two streams, side by side, each step with its workspace."""
+    import torch
+    case("one context on two streams")
+    steps = [Step(backend, exp_lut, seed=72), Step(backend, exp_lut, seqs=3, k=2, seed=73, prefix=800)]
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    try:
+        for s in steps:
+            s.project_and_attend()
+            s.to_logits()
+        torch.cuda.synchronize()
+        for _ in range(10):
+            for s, stream in zip(steps, streams):
+                with torch.cuda.stream(stream):
+                    backend.use_torch_stream()
+                    s.project_and_attend()
+                    s.check_drafts()
+        for i, s in enumerate(steps):
+            s.check(f"step {i}")
+    finally:
+        torch.cuda.synchronize()
+        backend.use_torch_stream()
