@@ -50,11 +50,22 @@ def _need_dev(what: str, device, **tensors) -> None:
 
 
 def _strides(t):
-    """The strides that an element's place depends on (0 for dimensions of one element or none)."""
+    """The strides that an element's place depends on (None for dimensions of one element or
+    none, whose stride says nothing)."""
     st, shape = t.stride(), t.shape
     if 0 in shape:
-        return (0,) * len(st)
-    return tuple(s if n > 1 else 0 for s, n in zip(st, shape)) if 1 in shape else st
+        return (None,) * len(st)
+    return tuple(s if n > 1 else None for s, n in zip(st, shape)) if 1 in shape else st
+
+
+def _apart(what: str, name: str, stride, dense: int) -> int:
+    """The stride of a dimension, `dense` where it says nothing.  0 is refused: an expanded
+    tensor owns fewer elements than a kernel would take it for."""
+    if stride is None:
+        return dense
+    if stride == 0:
+        raise ValueError(f"{what}: {name} must not be expanded (a stride of 0)")
+    return stride
 
 
 class RocmBackend:
@@ -417,7 +428,8 @@ class RocmBackend:
                   ids=(ids, "int32", (M,)), A=(A, "int8", (n, rank, K)), a_shifts=(a_shifts, "uint8", (n, rank)),
                   B=(B, "int8", (n, N, rank)), b_shifts=(b_shifts, "uint8", (n, N)))
         ldx, step = _strides(x)
-        if step not in (0, 1):
+        ldx = _apart(what, "x", ldx, K)
+        if step not in (None, 1):
             raise ValueError(f"{what}: the elements of a row of x follow one another")
         if out_frac_pc is not None:
             _need_dev(what, x.device, out_frac_pc=(out_frac_pc, "uint8", (N,)))
@@ -425,14 +437,15 @@ class RocmBackend:
             out = self._empty((M, N), "int16", x.device)
         _need_dev(what, x.device, out=(out, "int16", None))
         ldo, step = _strides(out)
-        if out.shape != (M, N) or step not in (0, 1):
+        ldo = _apart(what, "out", ldo, N)
+        if out.shape != (M, N) or step not in (None, 1):
             raise ValueError(f"{what}: out must be [M x N]")
         self._need_here(what, x.device)
         ws = self._workspace(x.device, workspace, lib().myl_linear_w8a16_adapters_workspace, M, N, K, rank, n)
         rc = lib().myl_linear_w8a16_adapters_dev(
-            self._h, x.data_ptr(), M, ldx or K, W.data_ptr(), N, K, w_shifts.data_ptr(), act_frac, out_frac,
+            self._h, x.data_ptr(), M, ldx, W.data_ptr(), N, K, w_shifts.data_ptr(), act_frac, out_frac,
             None if out_frac_pc is None else out_frac_pc.data_ptr(), ids.data_ptr(), A.data_ptr(), a_shifts.data_ptr(),
-            mid_frac, B.data_ptr(), b_shifts.data_ptr(), n, rank, out.data_ptr(), ldo or N,
+            mid_frac, B.data_ptr(), b_shifts.data_ptr(), n, rank, out.data_ptr(), ldo,
             ws.data_ptr(), ws.numel() * ws.element_size())
         if rc:
             self.check(rc, what)
@@ -482,22 +495,24 @@ class RocmBackend:
 
         def rows_of(t, name):
             row, head, one = _strides(t)
-            if head not in (0, hd) or one not in (0, 1):
+            if head not in (None, hd) or one not in (None, 1):
                 raise ValueError(f"{what}: the heads of a row of {name} follow one another")
-            return row or H * hd
+            return _apart(what, name, row, H * hd)
 
         ps, ts = _strides(k_prefix), _strides(k_tail)
-        if not (ps[1] in (0, hd) and ps[2] in (0, 1) and ts[2] in (0, hd) and ts[3] in (0, 1)):
+        if not (ps[1] in (None, hd) and ps[2] in (None, 1) and ts[2] in (None, hd) and ts[3] in (None, 1)):
             raise ValueError(f"{what}: the positions of a KV head follow one another")
         if ps != _strides(v_prefix) or ts != _strides(v_tail):
             raise ValueError(f"{what}: keys and values have the same strides")
+        p_head, t_head = _apart(what, "prefix", ps[0], P * hd), _apart(what, "tails", ts[1], T * hd)
+        t_slot = KH * T * hd if ts[0] is None else ts[0]  # 0: the slots share one tail
         max_tail = T if max_tail is None else max_tail
         ldq, ldo = rows_of(q, "q"), rows_of(out, "out")
         self._need_here(what, dev)
         ws = self._workspace(dev, workspace, lib().myl_attention_prefix_workspace, n_seqs, rows_per_seq, H, KH, hd, P, max_tail)
         rc = lib().myl_attention_prefix_dev(
             self._h, q.data_ptr(), n_seqs, rows_per_seq, ldq, H, KH, hd, k_prefix.data_ptr(), v_prefix.data_ptr(),
-            P, ps[0] or P * hd, k_tail.data_ptr(), v_tail.data_ptr(), S, ts[0] or KH * T * hd, ts[1] or T * hd, max_tail,
+            P, p_head, k_tail.data_ptr(), v_tail.data_ptr(), S, t_slot, t_head, max_tail,
             None if slots is None else slots.data_ptr(), lens.data_ptr(), score_mult, score_shift, exp_lut.data_ptr(),
             exp_lut.numel(), lut_shift, prob_frac, out.data_ptr(), ldo, ws.data_ptr(),
             ws.numel() * ws.element_size())
@@ -529,9 +544,9 @@ class RocmBackend:
 
         def rows_of(t, name, n):
             seq, row, one = _strides(t)
-            if one not in (0, 1) or (seq and row and seq != n * row):
+            if one not in (None, 1) or (None not in (seq, row) and seq != n * row):
                 raise ValueError(f"{what}: the rows of {name} are evenly spaced")
-            return row or seq or V
+            return _apart(what, name, seq if row is None else row, V)
 
         if exp_lut is not None:
             if randoms is None:
