@@ -392,11 +392,33 @@ class RocmBackend:
         context's stream has passed the call."""
         import torch
         t = torch.empty(shape, dtype=getattr(torch, dtype), device=device)
-        if device.type == "cuda":
-            stream = lib().myl_stream(self._h) or 0
-            if stream != torch.cuda.current_stream(device).cuda_stream:
-                t.record_stream(torch.cuda.ExternalStream(stream, device=device))
+        stream = self._other_stream(device)
+        if stream is not None:
+            t.record_stream(stream)
         return t
+
+    def _other_stream(self, device):
+        """The context's stream where it is not torch's current one."""
+        import torch
+        if device.type != "cuda":
+            return None
+        stream = lib().myl_stream(self._h) or 0
+        if stream == torch.cuda.current_stream(device).cuda_stream:
+            return None
+        return torch.cuda.ExternalStream(stream, device=device)
+
+    def _after_last_use(self, what: str, device) -> None:
+        """Behind a call's allocations, before its launch: the last use of their memory may
+        still be queued on torch's current stream, so the context's stream waits for it."""
+        import torch
+        stream = self._other_stream(device)
+        if stream is None:
+            return
+        with torch.cuda.stream(stream):
+            captured = torch.cuda.is_current_stream_capturing()
+        if captured != torch.cuda.is_current_stream_capturing():
+            raise ValueError(f"{what}: while one of torch's stream and the context's is captured, outputs and workspace are the caller's")
+        stream.wait_stream(torch.cuda.current_stream(device))
 
     def _need_here(self, what: str, device) -> None:
         if device.type != "cuda" or device.index != self._device_id:
@@ -433,7 +455,8 @@ class RocmBackend:
             raise ValueError(f"{what}: the elements of a row of x follow one another")
         if out_frac_pc is not None:
             _need_dev(what, x.device, out_frac_pc=(out_frac_pc, "uint8", (N,)))
-        if out is None:
+        made = out is None
+        if made:
             out = self._empty((M, N), "int16", x.device)
         _need_dev(what, x.device, out=(out, "int16", None))
         ldo, step = _strides(out)
@@ -442,6 +465,8 @@ class RocmBackend:
             raise ValueError(f"{what}: out must be [M x N]")
         self._need_here(what, x.device)
         ws = self._workspace(x.device, workspace, lib().myl_linear_w8a16_adapters_workspace, M, N, K, rank, n)
+        if made or workspace is None:
+            self._after_last_use(what, x.device)
         rc = lib().myl_linear_w8a16_adapters_dev(
             self._h, x.data_ptr(), M, ldx, W.data_ptr(), N, K, w_shifts.data_ptr(), act_frac, out_frac,
             None if out_frac_pc is None else out_frac_pc.data_ptr(), ids.data_ptr(), A.data_ptr(), a_shifts.data_ptr(),
@@ -487,7 +512,8 @@ class RocmBackend:
         else:
             if not (S >= n_seqs):
                 raise ValueError(f"{what}: fewer tails than sequences")
-        if out is None:
+        made = out is None
+        if made:
             out = self._empty((R, H, hd), "int16", dev)
         _need_dev(what, dev, out=(out, "int16", None))
         if out.shape != q.shape:
@@ -510,6 +536,8 @@ class RocmBackend:
         ldq, ldo = rows_of(q, "q"), rows_of(out, "out")
         self._need_here(what, dev)
         ws = self._workspace(dev, workspace, lib().myl_attention_prefix_workspace, n_seqs, rows_per_seq, H, KH, hd, P, max_tail)
+        if made or workspace is None:
+            self._after_last_use(what, dev)
         rc = lib().myl_attention_prefix_dev(
             self._h, q.data_ptr(), n_seqs, rows_per_seq, ldq, H, KH, hd, k_prefix.data_ptr(), v_prefix.data_ptr(),
             P, p_head, k_tail.data_ptr(), v_tail.data_ptr(), S, t_slot, t_head, max_tail,
@@ -558,6 +586,7 @@ class RocmBackend:
             _need_dev(what, dev, draft=(draft, "int32", None))
         if n_draft is not None:
             _need_dev(what, dev, n_draft=(n_draft, "int32", (B,)))
+        made = accepted is None or out is None
         if accepted is None:
             accepted = self._empty(B, "int32", dev)
         if out is None:
@@ -567,6 +596,8 @@ class RocmBackend:
         ldt, ldd = rows_of(target, "target", k1), V if draft is None or k == 0 else rows_of(draft, "draft", k)
         self._need_here(what, dev)
         ws = self._workspace(dev, workspace, lib().myl_verify_drafts_workspace, B, k, V, lut_len)
+        if made or workspace is None:
+            self._after_last_use(what, dev)
         rc = lib().myl_verify_drafts_dev(
             self._h, target.data_ptr(), ldt, None if draft is None or k == 0 else draft.data_ptr(), ldd, B, k, V, tokens.data_ptr(),
             None if n_draft is None else n_draft.data_ptr(), None if randoms is None else randoms.data_ptr(),

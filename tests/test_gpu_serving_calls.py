@@ -8,7 +8,7 @@ import pytest
 
 import serving_ref as ref
 from conftest import case
-from test_gpu_serving import (adapter_inputs, attention_inputs, dirty, exp_lut, gpu, rng, run_adapters, run_attention,  # noqa: F401
+from test_gpu_serving import (adapter_inputs, attention_inputs, exp_lut, gauss16, gpu, rng, run_adapters, run_attention,  # noqa: F401
                               same, verify_inputs, want_adapters)
 
 pytestmark = pytest.mark.gpu
@@ -22,3 +22,71 @@ def test_tails_that_all_slots_share(backend, exp_lut, prefix):
     s["kt"][:], s["vt"][:] = s["kt"][:1], s["vt"][:1]
     d = dict(s, kt=gpu(s["kt"][:1]).expand(s["kt"].shape), vt=gpu(s["vt"][:1]).expand(s["vt"].shape))
     same(run_attention(backend, d, exp_lut), ref.attention(**s, lut=exp_lut), "shared tail")
+
+
+def test_allocated_memory_still_in_use_on_torchs_stream(backend):
+    """A temporary that torch's queued kernels still read is freed just before a call on
+    another stream, which takes its memory for the output."""
+    import torch
+    case("memory in use on torch's stream")
+    M, N = 64, 16384
+    s = adapter_inputs(82, M, N, 64, 8, 3)
+    d = {k: gpu(v) if isinstance(v, np.ndarray) else v for k, v in s.items()}
+    args = (d["x"], d["W"], d["w_shifts"], 10, d["ids"], d["A"], d["a_shifts"], 10, d["B"], d["b_shifts"], 10)
+    ws = backend.linear_w8a16_adapters_workspace(d["x"], d["W"], d["A"])
+    a = torch.ones((8192, 8192), dtype=torch.float32, device="cuda")
+    product = torch.empty_like(a)
+    side = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    try:
+        with torch.cuda.stream(side):
+            backend.use_torch_stream()
+        for turn in range(3):
+            torch.cuda.empty_cache()
+            seen = torch.empty((M, N), dtype=torch.int16, device="cuda")
+            temporary = torch.full((M, N), 1000 + turn, dtype=torch.int16, device="cuda")
+            torch.cuda.synchronize()
+            for _ in range(4):  # some ten milliseconds each
+                torch.mm(a, a, out=product)
+            seen.copy_(temporary)
+            place = temporary.data_ptr()
+            del temporary
+            out = backend.linear_w8a16_adapters_dev(*args, workspace=ws)
+            torch.cuda.synchronize()
+            assert out.data_ptr() == place  # the memory is the temporary's
+            assert (seen == 1000 + turn).all()
+            same(out, want_adapters(s), f"turn {turn}")
+            del out, seen
+    finally:
+        torch.cuda.synchronize()
+        backend.use_torch_stream()
+
+
+def test_allocating_in_a_capture_of_both_streams(backend):
+    """The context's stream forked off the captured one: memory and launch are the graph's."""
+    import torch
+    case("capture of two streams")
+    s = adapter_inputs(83, 20, 90, 128, 8, 4)
+    d = {k: gpu(v) if isinstance(v, np.ndarray) else v for k, v in s.items()}
+    main, side = torch.cuda.Stream(), torch.cuda.Stream()
+    torch.cuda.synchronize()
+    try:
+        with torch.cuda.stream(side):
+            backend.use_torch_stream()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=main):
+            side.wait_stream(main)
+            out = backend.linear_w8a16_adapters_dev(d["x"], d["W"], d["w_shifts"], 10, d["ids"], d["A"], d["a_shifts"], 10, d["B"],
+                                                    d["b_shifts"], 10)
+            main.wait_stream(side)
+        for turn in range(4):
+            s["x"] = gauss16(rng(84 + turn), s["x"].shape, 2000)
+            d["x"].copy_(gpu(s["x"]))
+            out.fill_(-7)
+            torch.cuda.synchronize()
+            g.replay()
+            torch.cuda.synchronize()
+            same(out, want_adapters(s), f"replay {turn}")
+    finally:
+        torch.cuda.synchronize()
+        backend.use_torch_stream()

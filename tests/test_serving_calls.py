@@ -3,6 +3,8 @@ library is replaced by a recorder, so that the operands' addresses, strides and
 sizes can be held against the memory that the tensors own."""
 from __future__ import annotations
 
+import contextlib
+
 import pytest
 import torch
 
@@ -91,3 +93,109 @@ def test_dimensions_of_one_element_take_the_dense_stride(recorded):
                                       randoms=torch.zeros((1, 2), dtype=torch.int64), draft=odd(torch.int32, (1, 1, 50), (0, 0, 1))))
     args = log[-1][1]
     assert (args[2], args[4]) == (60, 50)
+
+
+# ---- the streams of memory that a call allocates ------------------------------------------
+
+class OnGpu(torch.Tensor):
+    """A CPU tensor that says it is on the GPU."""
+    device = property(lambda self: torch.device("cuda", 0))
+    recorded = []
+
+    def record_stream(self, stream):
+        OnGpu.recorded.append((self.data_ptr(), stream.cuda_stream))
+
+
+class FakeStream:
+    log, torchs, captured = None, 7, ()  # captured: handles
+
+    def __init__(self, handle, device=None):
+        self.cuda_stream = handle
+
+    def wait_stream(self, other):
+        self.log.append(("wait", self.cuda_stream, other.cuda_stream))
+
+
+@pytest.fixture
+def streams(recorded, monkeypatch):
+    """The recorded backend on stream 9 with torch on stream 7; allocations and waits are recorded too."""
+    b, log = recorded
+    from myelith_amd import backend
+    entries = backend.lib()
+    entries.myl_stream = lambda ctx: 9
+    empty = torch.empty
+
+    def allocate(shape, dtype=None, device=None):
+        log.append(("empty", shape))
+        return empty(shape, dtype=dtype).as_subclass(OnGpu)
+    monkeypatch.setattr(torch, "empty", allocate)
+    current = []
+
+    @contextlib.contextmanager
+    def on(stream):
+        current.append(stream)
+        yield
+        current.pop()
+    monkeypatch.setattr(torch.cuda, "current_stream", lambda device=None: current[-1] if current else FakeStream(FakeStream.torchs))
+    monkeypatch.setattr(torch.cuda, "stream", on)
+    monkeypatch.setattr(torch.cuda, "ExternalStream", FakeStream)
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: torch.cuda.current_stream().cuda_stream in FakeStream.captured)
+    monkeypatch.setattr(FakeStream, "log", log)
+    monkeypatch.setattr(OnGpu, "recorded", [])
+    return b, log
+
+
+def on_gpu(args):
+    return {k: v.as_subclass(OnGpu) if isinstance(v, torch.Tensor) else v for k, v in args.items()}
+
+
+def calls_of(b):
+    """Each call with its arguments, and its outputs as the caller would give them."""
+    i16 = lambda *s: torch.zeros(s, dtype=torch.int16)
+    space = dict(workspace=torch.zeros(256, dtype=torch.uint8))
+    return [(b.linear_w8a16_adapters_dev, on_gpu(adapter_args()), on_gpu(dict(space, out=i16(3, 5)))),
+            (b.attention_prefix_dev, on_gpu(attention_args()), on_gpu(dict(space, out=i16(4, 4, 64)))),
+            (b.verify_drafts_dev, on_gpu(verify_args()),
+             on_gpu(dict(space, accepted=torch.zeros(2, dtype=torch.int32), out=torch.zeros((2, 4), dtype=torch.int64))))]
+
+
+def test_allocated_memory_is_written_after_its_last_use(streams):
+    """torch hands out memory whose last use is queued on its current stream: a context on
+    another stream waits for that, after the call's allocations and before its launch."""
+    b, log = streams
+    for call, args, given in calls_of(b):
+        for left_out in [given, *([k] for k in given)]:
+            log.clear()
+            OnGpu.recorded.clear()
+            call(**args, **{k: v for k, v in given.items() if k not in left_out})
+            kinds = [e[0] if e[0] in ("empty", "wait") else "launch" for e in log if not e[0].endswith("_workspace")]
+            assert kinds == ["empty"] * len(left_out) + ["wait", "launch"], (call.__name__, list(left_out), kinds)
+            assert ("wait", 9, 7) in log and [s for _, s in OnGpu.recorded] == [9] * len(left_out)
+        log.clear()
+        call(**args, **given)
+        assert len(log) == 1, log  # nothing allocated, nothing to wait for
+
+
+def test_allocating_on_torchs_stream_waits_for_nothing(streams, monkeypatch):
+    b, log = streams
+    monkeypatch.setattr(FakeStream, "torchs", 9)
+    for call, args, given in calls_of(b):
+        log.clear()
+        call(**args)
+        assert not [e for e in log if e[0] == "wait"] and not OnGpu.recorded
+
+
+@pytest.mark.parametrize("captured", [(7,), (9,), (7, 9)])
+def test_allocating_while_one_stream_is_captured_is_refused(streams, monkeypatch, captured):
+    """The memory or the launch alone would be the graph's; both in one capture are."""
+    b, log = streams
+    monkeypatch.setattr(FakeStream, "captured", captured)
+    for call, args, given in calls_of(b):
+        log.clear()
+        if len(captured) == 2:
+            call(**args)
+        else:
+            with pytest.raises(ValueError, match="captured"):
+                call(**args)
+            assert not [e for e in log if e[0].endswith("_dev")]
+        call(**args, **given)
