@@ -27,6 +27,15 @@ namespace myl {
 
 inline int xvec_ok(const int16_t* x, int ldx) { return (((uintptr_t)x & 15) == 0) && (ldx % 8 == 0); }
 
+template <typename WT, class Epi>
+inline hipError_t gemv_generic(const int16_t* x, int M, int ldx, const WT* W, int N, int K, const Epi& epi, hipStream_t st) {
+    for (int64_t m0 = 0; m0 < M; m0 += kGridRows) {
+        const int rows = std::min(M - (int)m0, kGridRows);
+        gemv_generic_kernel<WT, Epi><<<dim3((N + 255) / 256, rows), 256, 0, st>>>(x + (size_t)m0 * ldx, rows, ldx, W, N, K, epi.offset_m((int)m0));
+    }
+    return hipGetLastError();
+}
+
 template <int R, int MT, int U, class Epi>
 inline hipError_t launch_i8(const int16_t* x, int M, int ldx, const int8_t* W, int N, int K, const Epi& epi,
                             hipStream_t st) {
@@ -251,11 +260,7 @@ template <class Epi>
 inline hipError_t gemv_i8(const int16_t* x, int M, int ldx, const int8_t* W, int N, int K, const Epi& epi,
                           hipStream_t st, const MmCtx* mm) {
     const bool fast = (K % 16 == 0) && (((uintptr_t)W & 15) == 0) && K < 131072;
-    if (!fast) {
-        dim3 grid((N + 255) / 256, M);
-        gemv_generic_kernel<int8_t, Epi><<<grid, 256, 0, st>>>(x, M, ldx, W, N, K, epi);
-        return hipGetLastError();
-    }
+    if (!fast) return gemv_generic(x, M, ldx, W, N, K, epi, st);
     // More than one activation row: the int8 matrix cores (16-byte aligned
     // rows).  Up to 64 rows are one tile row, so the weights stream once; the
     // multi-row GEMV below reached only ~0.6 TB/s at 8 rows on MI355X.
@@ -286,11 +291,7 @@ template <class Epi>
 inline hipError_t gemv_i16(const int16_t* x, int M, int ldx, const int16_t* W, int N, int K, const Epi& epi,
                            hipStream_t st, const MmCtx* mm = nullptr) {
     const bool fast = (K % 8 == 0) && (((uintptr_t)W & 15) == 0) && K <= 8192;
-    if (!fast) {
-        dim3 grid((N + 255) / 256, M);
-        gemv_generic_kernel<int16_t, Epi><<<grid, 256, 0, st>>>(x, M, ldx, W, N, K, epi);
-        return hipGetLastError();
-    }
+    if (!fast) return gemv_generic(x, M, ldx, W, N, K, epi, st);
     // 2-32 rows: the weight stream (gemm_rows.h; 5 rows of the 7B head: 164 us, 350
     // in the LDS tiles below).
     if (M > 1 && xvec_ok(x, ldx) && mm) {

@@ -757,7 +757,10 @@ inline int mm2_tiles(int M, int N) {
 
 
 inline hipError_t split_planes(const int16_t* x, int M, int ldx, int K, int8_t* Ap, hipStream_t st) {
-    split_planes_kernel<><<<dim3((K / 8 + 255) / 256, M), 256, 0, st>>>(x, M, ldx, K, Ap);
+    for (int64_t m0 = 0; m0 < M; m0 += kGridRows) {
+        const int rows = std::min(M - (int)m0, kGridRows);
+        split_planes_kernel<><<<dim3((K / 8 + 255) / 256, rows), 256, 0, st>>>(x + (size_t)m0 * ldx, rows, ldx, K, Ap + (size_t)(2 * m0) * K);
+    }
     return hipGetLastError();
 }
 

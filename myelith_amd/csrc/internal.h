@@ -21,6 +21,10 @@ struct MmCtx {
     size_t planes_bytes = 0;
 };
 
+// A grid's second dimension is at most this: kernels that take a row there are
+// launched in pieces.
+constexpr int kGridRows = 65535;
+
 // y[m][r] = clamp_i16(rescale_i64(W[r].x[m], w_shifts[r] + act_frac, out_frac_pc ? out_frac_pc[r] : out_frac))
 hipError_t linear_w8a16(const int16_t* x, int M, int ldx, const int8_t* W, int N, int K, const uint8_t* w_shifts,
                         uint8_t act_frac, uint8_t out_frac, const uint8_t* out_frac_pc, int16_t* out, int ldo,

@@ -90,3 +90,51 @@ def test_allocating_in_a_capture_of_both_streams(backend):
     finally:
         torch.cuda.synchronize()
         backend.use_torch_stream()
+
+
+# ---- more rows than a grid's second dimension holds -----------------------------------------
+
+def want_adapters_by_id(s, out_frac=10):
+    """want_adapters, the rows of an adapter together."""
+    out = ref.linear(s["x"], s["W"], s["w_shifts"], 10, out_frac)
+    for a in range(s["A"].shape[0]):
+        rows = np.flatnonzero(s["ids"] == a)
+        u = ref.linear(s["x"][rows], s["A"][a], s["a_shifts"][a], 10, 10)
+        out[rows] += ref.linear(u, s["B"][a], s["b_shifts"][a], 10, out_frac)
+    return ref.clamp16(out).astype(np.int16)
+
+
+@pytest.mark.parametrize("M,N,K", [(65600, 5, 64), (65600, 3, 33), (65535, 2, 16), (65536, 7, 192), (131200, 2, 17)])
+def test_adapters_past_65535_rows(backend, M, N, K):
+    """Rows of byte planes (K a multiple of 64), of the plain sums (K 33, 17) and of the tiles between."""
+    case(f"adapters M={M} N={N} K={K}")
+    s = adapter_inputs(M + K, M, N, K, 4, 6)
+    same(run_adapters(backend, s), want_adapters_by_id(s), "many rows")
+
+
+@pytest.mark.parametrize("K", [64, 33])
+def test_products_past_65535_rows(backend, K):
+    """The projection itself and the sums it is made of."""
+    case(f"products past 65535 rows K={K}")
+    r = rng(K)
+    x, W = gauss16(r, (65700, K), 2000), r.integers(-128, 128, (3, K)).astype(np.int8)
+    shifts = np.array([8, 9, 10], np.uint8)
+    same(backend.linear_w8a16_dev(gpu(x), gpu(W), gpu(shifts), 10, 10), ref.linear(x, W, shifts, 10, 10).astype(np.int16), "projection")
+    same(backend.dot_i8_i16_dev(gpu(x), gpu(W)), ref.dots(x, W), "sums")
+
+
+def test_adapters_planes_past_4_gib(backend):
+    """Rows whose byte planes lie more than 2^32 bytes into the workspace."""
+    import torch
+    case("adapters planes past 4 GiB")
+    M, N, K = 131400, 6, 16448
+    assert 2 * M * K > 2**32
+    few = adapter_inputs(85, 40, N, K, 4, 3)
+    x = torch.empty((M, K), dtype=torch.int16, device="cuda")
+    x.random_(-3000, 3001)
+    ids = rng(86).integers(-1, 4, M)
+    got = run_adapters(backend, dict(few, x=x, ids=ids.astype(np.int32))).cpu().numpy()
+    at = np.unique(np.concatenate([rng(87).integers(0, M, 300), [0, 65534, 65535, 65536, 131069, 131070, 131071, M - 1]]))
+    keep = dict(few, x=x[torch.from_numpy(at).cuda()].cpu().numpy(), ids=ids[at])
+    bad = np.flatnonzero((got[at] != want_adapters_by_id(keep)).any(1))
+    assert not bad.size, at[bad]
