@@ -580,6 +580,8 @@ class RocmBackend:
             if randoms is None:
                 raise ValueError(f"{what}: random numbers are needed unless the check is greedy")
             _need_dev(what, dev, exp_lut=(exp_lut, "int16", (exp_lut.numel(),)), randoms=(randoms, "int64", (B, k1)))
+            if not exp_lut.numel():  # it has no address: the call would be the greedy one
+                raise ValueError(f"{what}: the exp table must hold 1 to 32768 entries")
         if draft is not None:
             if draft.shape != (B, k, V):
                 raise ValueError(f"{what}: draft must be [B x k x V]")

@@ -199,3 +199,14 @@ def test_allocating_while_one_stream_is_captured_is_refused(streams, monkeypatch
                 call(**args)
             assert not [e for e in log if e[0].endswith("_dev")]
         call(**args, **given)
+
+
+# ---- arguments that would arrive as something else ------------------------------------------
+
+def test_an_empty_table_is_not_the_greedy_check(recorded):
+    """An empty tensor has no address, and no table means greedy."""
+    b, log = recorded
+    with pytest.raises(ValueError, match="table"):
+        b.verify_drafts_dev(**verify_args(exp_lut=torch.zeros(0, dtype=torch.int16)))
+    b.verify_drafts_dev(**verify_args(exp_lut=None, randoms=None))
+    assert log[-1][1][11:13] == (None, 0)  # table, entries
