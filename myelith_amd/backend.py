@@ -49,6 +49,13 @@ def _need_dev(what: str, device, **tensors) -> None:
             raise ValueError(f"{what}: {name} must be contiguous {list(shape)}, not {list(t.shape)}")
 
 
+def _need_bytes(what: str, **values) -> None:
+    """Numbers that the library takes as uint8, which would keep the low bits of others."""
+    for name, v in values.items():
+        if not 0 <= v <= 255:
+            raise ValueError(f"{what}: {name} must be 0 to 255, not {v}")
+
+
 def _strides(t):
     """The strides that an element's place depends on (None for dimensions of one element or
     none, whose stride says nothing)."""
@@ -443,6 +450,7 @@ class RocmBackend:
         [n x rank x K] with a_shifts uint8 [n x rank], B int8 [n x N x rank]
         with b_shifts uint8 [n x N] (include/myl_hip.h states the arithmetic)."""
         what = "linear_w8a16_adapters_dev"
+        _need_bytes(what, act_frac=act_frac, mid_frac=mid_frac, out_frac=out_frac)
         M, K = x.shape
         N = W.shape[0]
         n, rank = A.shape[:2]
@@ -493,6 +501,9 @@ class RocmBackend:
         max_tail, by default the capacity; negative: the row is left out and
         its output is zero).  include/myl_hip.h states the arithmetic."""
         what = "attention_prefix_dev"
+        _need_bytes(what, score_shift=score_shift, lut_shift=lut_shift, prob_frac=prob_frac)
+        if not -2**63 <= score_mult < 2**63:
+            raise ValueError(f"{what}: score_mult must be an int64, not {score_mult}")
         R, H, hd = q.shape
         KH, P = k_prefix.shape[:2]
         S, _, T = k_tail.shape[:3]

@@ -210,3 +210,19 @@ def test_an_empty_table_is_not_the_greedy_check(recorded):
         b.verify_drafts_dev(**verify_args(exp_lut=torch.zeros(0, dtype=torch.int16)))
     b.verify_drafts_dev(**verify_args(exp_lut=None, randoms=None))
     assert log[-1][1][11:13] == (None, 0)  # table, entries
+
+
+def test_scalars_outside_their_type_are_refused(recorded):
+    """A C byte would keep the low bits of them: 270 fractional bits would be 14."""
+    b, log = recorded
+    cases = [(b.linear_w8a16_adapters_dev, adapter_args, ("act_frac", "mid_frac", "out_frac"), (-1, 256, 2**40)),
+             (b.attention_prefix_dev, attention_args, ("score_shift", "lut_shift", "prob_frac"), (-1, 256, 270)),
+             (b.attention_prefix_dev, attention_args, ("score_mult",), (-2**63 - 1, 2**63, 2**64))]
+    for call, args, names, values in cases:
+        for name in names:
+            for v in values:
+                with pytest.raises(ValueError, match=name):
+                    call(**args(**{name: v}))
+    b.linear_w8a16_adapters_dev(**adapter_args(act_frac=0, mid_frac=255, out_frac=255))
+    b.attention_prefix_dev(**attention_args(score_mult=-2**63, score_shift=255, lut_shift=0, prob_frac=0))
+    assert len([e for e in log if e[0].endswith("_dev")]) == 2
