@@ -219,7 +219,9 @@ int myl_logsoftmax_dev(myl_ctx* ctx, const int32_t* logits, size_t M, size_t n, 
  * forms keep nothing between calls: their scratch is the caller's `workspace`
  * (device memory, 16-byte aligned, of at least the bytes that the matching
  * *_workspace function names; it returns 0 for sizes the call refuses), whose
- * contents before and after a call mean nothing.  So they can be captured into
+ * contents before and after a call mean nothing.  The bytes named for some sizes
+ * serve every call none of whose sizes is larger (for attention, with the same
+ * heads, KV heads and head_dim).  So they can be captured into
  * HIP graphs, and calls on different contexts and streams run at once as long
  * as each has its own workspace.  Operands and outputs do not overlap unless
  * stated. */

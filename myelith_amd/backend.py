@@ -438,7 +438,7 @@ class RocmBackend:
         return torch.empty(nbytes, dtype=torch.uint8, device=device)
 
     def linear_w8a16_adapters_workspace(self, x, W, A):
-        """A workspace for linear_w8a16_adapters_dev on operands of these shapes."""
+        """A workspace for linear_w8a16_adapters_dev on operands of these shapes, and on smaller ones."""
         n = lib().myl_linear_w8a16_adapters_workspace(self._h, x.shape[0], W.shape[0], x.shape[1], A.shape[1],
                                                       A.shape[0])
         return self._new_workspace(n, x.device, "linear_w8a16_adapters_dev")
@@ -484,10 +484,11 @@ class RocmBackend:
             self.check(rc, what)
         return out
 
-    def attention_prefix_workspace(self, q, k_prefix, k_tail, rows_per_seq: int = 1):
-        """A workspace for attention_prefix_dev on operands of these shapes."""
+    def attention_prefix_workspace(self, q, k_prefix, k_tail, rows_per_seq: int = 1, max_tail=None):
+        """A workspace for attention_prefix_dev on operands of these shapes, and on smaller ones."""
         n = lib().myl_attention_prefix_workspace(self._h, q.shape[0] // max(1, rows_per_seq), rows_per_seq, q.shape[1],
-                                                 k_prefix.shape[0], q.shape[2], k_prefix.shape[1], k_tail.shape[2])
+                                                 k_prefix.shape[0], q.shape[2], k_prefix.shape[1],
+                                                 k_tail.shape[2] if max_tail is None else max_tail)
         return self._new_workspace(n, q.device, "attention_prefix_dev")
 
     def attention_prefix_dev(self, q, k_prefix, v_prefix, k_tail, v_tail, lens, score_mult: int, score_shift: int,
@@ -560,7 +561,7 @@ class RocmBackend:
         return out
 
     def verify_drafts_workspace(self, target, exp_lut=None, draft=None):
-        """A workspace for verify_drafts_dev on operands of these shapes."""
+        """A workspace for verify_drafts_dev on operands of these shapes, and on smaller ones."""
         n = lib().myl_verify_drafts_workspace(self._h, target.shape[0], target.shape[1] - 1, target.shape[2],
                                               0 if exp_lut is None else exp_lut.numel())
         return self._new_workspace(n, target.device, "verify_drafts_dev")

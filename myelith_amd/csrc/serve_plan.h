@@ -13,7 +13,9 @@ namespace myl {
 
 constexpr size_t kInt = 0x7FFFFFFF;
 
-// Pieces of a workspace in 256-byte steps.
+// Pieces of a workspace in 256-byte steps.  A piece has room for every call none of whose
+// sizes is larger, so that a program keeps the workspace of its largest step: where fewer
+// rows or keys are cut into more parts, the room is a bound that grows with the sizes.
 struct Layout {
     size_t used = 0;
     size_t take(size_t n, size_t each) {
@@ -57,6 +59,14 @@ struct AdapterPlan {
 constexpr int64_t kAdapterMaxChunk = (int64_t)1 << 20;
 constexpr size_t kAdapterTileBytes = 72;  // adapter, rows, and their 64 places in the window
 
+// M x splits of any smaller call, which adapter_plan bounds by max(min(up(2 CUs, blocks),
+// units / 4), units / 2048): M up(2 CUs, blocks) <= M + 2 CUs M / blocks, and blocks is at
+// least 1 and at least M / 16 (a tile for 16 rows).
+inline size_t adapter_most_parts(const AdapterShape& s, int cus) {
+    const size_t units = (s.K + kAdapterUnit - 1) / kAdapterUnit;
+    return std::max(std::min(s.M + 2 * (size_t)cus * std::min<size_t>(s.M, 16), s.M * ((units + 3) / 4)), s.M * ((units + 4 * 512 - 1) / (4 * 512)));
+}
+
 inline AdapterPlan adapter_plan(const AdapterShape& s, int cus) {
     AdapterPlan p{};
     Layout l;
@@ -64,7 +74,7 @@ inline AdapterPlan adapter_plan(const AdapterShape& s, int cus) {
         p.planes_bytes = 2 * s.M * s.K;
         p.acc_elems = s.M * s.N <= kAdapterAccElems ? s.M * s.N : 0;
         p.off_planes = l.take(p.planes_bytes, 1);
-        p.off_acc = l.take(std::max<size_t>(p.acc_elems, 1), 8);
+        p.off_acc = l.take(std::max<size_t>(std::min(s.M * s.N, kAdapterAccElems), 1), 8);
     }
     if (s.M && s.N && s.n) {
         const int w = (int)std::min<size_t>(s.M, kAdapterWindow), d = (int)std::min<size_t>(s.n, (size_t)w);
@@ -87,7 +97,7 @@ inline AdapterPlan adapter_plan(const AdapterShape& s, int cus) {
         const int64_t cols = up((int64_t)s.N, up(4 * (int64_t)cus, (int64_t)p.windows * p.up_tiles));
         p.n_chunk = (int)std::min<int64_t>(up(cols, 256) * 256, kAdapterMaxChunk);
         p.n_chunks = (int)up((int64_t)s.N, p.n_chunk);
-        p.off_part = l.take((size_t)p.splits * s.M * (size_t)p.rank_pad, 8);
+        p.off_part = l.take(adapter_most_parts(s, cus) * (size_t)p.rank_pad, 8);
         p.off_tiles = l.take((size_t)p.windows * (size_t)p.up_tiles, kAdapterTileBytes);
     }
     p.bytes = std::max<size_t>(l.used, 256);  // 0 stands for sizes that a call refuses
@@ -150,6 +160,23 @@ inline bool prefix_short(const PrefixShape& s, int cus) {
     return keys > 0 && s.heads / s.kv_heads <= kPrefixShortHeads && blocks <= 4 * (size_t)cus && keys * s.head_dim <= kPrefixShortWork;
 }
 
+// How many steps of 64 keys a range takes at least.
+inline int prefix_least_steps(int steps) {
+    int least = 2;
+    while (7 * least * least < steps) ++least;
+    return least;
+}
+
+// Vectors x ranges of any smaller call, `vectors` (of one KV head, or of one sequence and KV head)
+// in each of `groups`: at most as many ranges as the steps allow (the most with the least
+// steps of a range, or one less, which stop at 7 (least - 1)^2 steps), and at most
+// 2 CUs / (groups ceil(vectors / 64)) of them, or one.
+inline size_t prefix_most_parts(size_t vectors, size_t groups, size_t keys, int cus) {
+    const int steps = (int)((keys + 63) / 64), least = prefix_least_steps(steps);
+    const size_t ranges = (size_t)std::max((steps + least - 1) / least, least > 2 ? 7 * (least - 1) : 0);
+    return std::min(vectors * groups * ranges, std::max(vectors * groups, std::min<size_t>(vectors, kPrefixPvTile) * 2 * (size_t)cus));
+}
+
 inline PrefixPlan prefix_plan(const PrefixShape& s, int cus) {
     PrefixPlan p{};
     const int64_t R = (int64_t)(s.n_seqs * s.rows_per_seq), kvh = (int64_t)s.kv_heads;
@@ -174,9 +201,8 @@ inline PrefixPlan prefix_plan(const PrefixShape& s, int cus) {
         if (keys == 0 || per_range == 0) return;
         const int steps = (keys + 63) / 64;
         const int64_t want = std::max<int64_t>(1, 2 * cus / per_range);
-        int each = (int)((steps + std::min<int64_t>(want, steps) - 1) / std::min<int64_t>(want, steps)), least = 2;
-        while (7 * least * least < steps) ++least;
-        each = std::max(each, least);
+        int each = (int)((steps + std::min<int64_t>(want, steps) - 1) / std::min<int64_t>(want, steps));
+        each = std::max(each, prefix_least_steps(steps));
         len = 64 * each;
         n = (steps + each - 1) / each;
     };
@@ -194,7 +220,8 @@ inline PrefixPlan prefix_plan(const PrefixShape& s, int cus) {
     p.tgroups = (T + 63) / 64 * 4;
     p.pairs = (size_t)R * s.heads;
     Layout l;
-    const size_t parts = p.pairs * (size_t)(p.np + p.nt);
+    const size_t parts = prefix_most_parts((size_t)p.vp, s.kv_heads, s.prefix_len, cus) +
+                         prefix_most_parts((size_t)p.vt, s.kv_heads * s.n_seqs, s.max_tail, cus);
     p.off_max = l.take(parts, 4);
     p.off_sum = l.take(parts, 4);
     p.off_pexp = l.take((size_t)kvh * (size_t)tiles(p.vp, 16) * (size_t)p.pgroups * 256, 2);

@@ -8,7 +8,7 @@ import pytest
 
 import serving_ref as ref
 from conftest import case
-from test_gpu_serving import (adapter_inputs, attention_inputs, exp_lut, gauss16, gpu, rng, run_adapters, run_attention,  # noqa: F401
+from test_gpu_serving import (adapter_inputs, attention_inputs, dirty, exp_lut, gauss16, gpu, rng, run_adapters, run_attention,  # noqa: F401
                               same, verify_inputs, want_adapters)
 
 pytestmark = pytest.mark.gpu
@@ -138,3 +138,33 @@ def test_adapters_planes_past_4_gib(backend):
     keep = dict(few, x=x[torch.from_numpy(at).cuda()].cpu().numpy(), ids=ids[at])
     bad = np.flatnonzero((got[at] != want_adapters_by_id(keep)).any(1))
     assert not bad.size, at[bad]
+
+
+# ---- a workspace kept from the largest step ----------------------------------------------------
+
+@pytest.mark.parametrize("rows", [114, 113, 100, 57, 16, 3, 1])
+def test_adapters_in_the_workspace_of_more_rows(backend, rows):
+    case(f"adapters workspace kept, {rows} rows")
+    s = adapter_inputs(88, 120, 4608, 3584, 16, 24)
+    d = {k: gpu(v) if isinstance(v, np.ndarray) else v for k, v in s.items()}
+    ws = dirty(backend.linear_w8a16_adapters_workspace(d["x"], d["W"], d["A"]))
+    got = backend.linear_w8a16_adapters_dev(d["x"][:rows], d["W"], d["w_shifts"], 10, d["ids"][:rows], d["A"], d["a_shifts"], 10, d["B"],
+                                            d["b_shifts"], 10, workspace=ws)
+    same(got, want_adapters(dict(s, x=s["x"][:rows], ids=s["ids"][:rows])), "fewer rows")
+
+
+@pytest.mark.parametrize("seqs,tail", [(1, 1856), (1, 1792), (2, 1792), (2, 450), (1, 448), (2, 0)])
+def test_attention_in_the_workspace_of_longer_tails(backend, exp_lut, seqs, tail):
+    """The workspace of two sequences at the tails' capacity, for fewer and for shorter tails."""
+    case(f"attention workspace kept, {seqs} sequences, tails of {tail}")
+    s = attention_inputs(89, 2, 1, 1000, 1856, 28, 4, 128)
+    d = {k: gpu(v) if isinstance(v, np.ndarray) else v for k, v in s.items()}
+    ws = dirty(backend.attention_prefix_workspace(d["q"], d["kp"], d["kt"]))
+    s.update(q=s["q"][:seqs], lens=np.minimum(s["lens"][:seqs], tail), slots=s["slots"][:seqs], max_tail=tail)
+    got = backend.attention_prefix_dev(d["q"][:seqs], d["kp"], d["vp"], d["kt"], d["vt"], gpu(s["lens"]), s["mult"], s["shift"], gpu(exp_lut), 6, 14,
+                                       slots=gpu(s["slots"]), max_tail=tail, workspace=ws)
+    same(got, ref.attention(**s, lut=exp_lut), "shorter tails")
+    own = backend.attention_prefix_workspace(d["q"][:seqs], d["kp"], d["kt"], max_tail=tail)
+    assert own.numel() <= ws.numel()
+    same(backend.attention_prefix_dev(d["q"][:seqs], d["kp"], d["vp"], d["kt"], d["vt"], gpu(s["lens"]), s["mult"], s["shift"], gpu(exp_lut), 6, 14,
+                                      slots=gpu(s["slots"]), max_tail=tail, workspace=dirty(own)), ref.attention(**s, lut=exp_lut), "own workspace")
