@@ -208,11 +208,14 @@ __device__ inline void fold_ranges(const PrefixAttn& a, const int32_t* __restric
 enum Pass { kMaxPass, kExpPass };
 
 // The exp table's copy in LDS, eight entries per load: entries past the table are 0 (one at
-// least follows it), negative ones count as 0.
+// least follows it), negative ones count as 0.  An odd last entry is loaded by itself: the
+// words' loads return 0 from it on.
 struct TablePiece {
     uint4 x[4];
+    uint32_t last;
     __device__ inline void load(const PrefixAttn& a, uint32_t i0) {
-        const __amdgpu_buffer_rsrc_t rl = weight_rsrc(a.lut, (a.lut_len * 2u + 3u) & ~3u);
+        const __amdgpu_buffer_rsrc_t rl = weight_rsrc(a.lut, prefix_table_bytes(a.lut_len));
+        last = (uint16_t)a.lut[a.lut_len - 1u];
 #pragma unroll
         for (int k = 0; k < 4; ++k) x[k] = cload16(rl, 2u * (i0 + 2048u * k));
     }
@@ -224,6 +227,7 @@ struct TablePiece {
             uint32_t w[4] = {x[k].x, x[k].y, x[k].z, x[k].w};
 #pragma unroll
             for (int b = 0; b < 4; ++b) {
+                if (i + 2 * b + 1 == a.lut_len) w[b] = last;
                 const uint32_t lo = i + 2 * b < a.lut_len && !(w[b] & 0x8000u) ? w[b] & 0xFFFFu : 0u;
                 const uint32_t hi = i + 2 * b + 1 < a.lut_len && !(w[b] >> 31) ? w[b] & 0xFFFF0000u : 0u;
                 w[b] = lo | hi;

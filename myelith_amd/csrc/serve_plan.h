@@ -137,6 +137,9 @@ constexpr size_t kPrefixShortHeads = 8, kPrefixShortWork = 320 * 128;  // heads 
 // LDS of a block that does a row's heads by itself: scores, probabilities, sums.
 inline size_t prefix_short_lds(int G, int cap, size_t hd) { return (size_t)G * ((size_t)cap * 6 + hd * 4); }
 
+// The whole words of an exp table, which wide loads may touch: not an odd last entry.
+constexpr uint32_t prefix_table_bytes(uint32_t lut_len) { return lut_len / 2 * 4; }
+
 struct PrefixPlan {
     int short_cap;         // > 0: one launch, blocks with room for so many keys; nothing below is used
     int G, vp, vt;       // query heads per KV head; vectors per KV head: of all rows, of one sequence

@@ -168,3 +168,25 @@ def test_attention_in_the_workspace_of_longer_tails(backend, exp_lut, seqs, tail
     assert own.numel() <= ws.numel()
     same(backend.attention_prefix_dev(d["q"][:seqs], d["kp"], d["vp"], d["kt"], d["vt"], gpu(s["lens"]), s["mult"], s["shift"], gpu(exp_lut), 6, 14,
                                       slots=gpu(s["slots"]), max_tail=tail, workspace=dirty(own)), ref.attention(**s, lut=exp_lut), "own workspace")
+
+
+@pytest.mark.parametrize("entries", [1, 2, 3, 7, 8, 9, 15, 17, 2047, 2049, 2661, 8191, 8193, 16385, 32767])
+def test_tables_that_end_inside_a_load(backend, entries):
+    """The last entry counts and what lies behind it does not, wherever the table ends."""
+    case(f"attention table of {entries}")
+    import torch
+    lut = rng(entries).integers(1, 32768, entries).astype(np.int16)
+    behind = torch.full((entries + 64,), 32767, dtype=torch.int16, device="cuda")
+    behind[:entries] = gpu(lut)
+    s = attention_inputs(90, 3, 1, 500, 40, 18, 2, 64)
+    s["lut_shift"] = 0
+    # a scale at which some score lies at the table's last entry and others behind it
+    spread = np.abs(ref.dots(s["q"].reshape(-1, 64), s["kp"].reshape(-1, 64))).max()
+    s["mult"] = max(1, int(entries * 2.0**s["shift"] / spread))
+    without = np.append(lut[:-1], 0).astype(np.int16)
+    while ((want := ref.attention(**s, lut=lut)) == ref.attention(**s, lut=without)).all():
+        s["mult"] += 1
+    d = {k: gpu(v) if isinstance(v, np.ndarray) else v for k, v in s.items()}
+    got = backend.attention_prefix_dev(d["q"], d["kp"], d["vp"], d["kt"], d["vt"], d["lens"], s["mult"], s["shift"], behind[:entries],
+                                       s["lut_shift"], 14, slots=d["slots"])
+    same(got, want, f"{entries} entries")

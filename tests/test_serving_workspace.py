@@ -95,3 +95,25 @@ def test_a_workspace_serves_every_smaller_call(tmp_path):
     r = subprocess.run([str(exe)], capture_output=True, text=True, timeout=600)
     assert r.returncode == 0, (r.stdout[-3000:], r.stderr[-3000:])
     assert int(re.match(r"checked (\d+) bad 0", r.stdout.strip().splitlines()[-1]).group(1)) > 300000
+
+
+TABLE = r"""
+#include "serve_plan.h"
+#include <cstdio>
+int main() {
+    for (uint32_t n = 1; n <= myl::kPrefixMaxLut; ++n) {
+        const uint32_t b = myl::prefix_table_bytes(n);
+        if (b % 4 || b > 2 * n || b + 2 < 2 * n) return std::printf("%u entries: %u bytes\n", n, b), 1;
+    }
+}
+"""
+
+
+@pytest.mark.skipif(shutil.which("g++") is None, reason="g++ absent")
+def test_wide_loads_of_a_table_end_inside_it(tmp_path):
+    """The exp table is read by whole words, which cover all but an odd last entry."""
+    src, exe = tmp_path / "t.cpp", tmp_path / "t"
+    src.write_text(TABLE)
+    subprocess.run(["g++", "-std=c++17", "-I", str(CSRC), str(src), "-o", str(exe)], check=True, capture_output=True, timeout=300)
+    r = subprocess.run([str(exe)], capture_output=True, text=True, timeout=60)
+    assert r.returncode == 0, r.stdout
