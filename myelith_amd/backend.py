@@ -450,7 +450,8 @@ class RocmBackend:
         [n x rank x K] with a_shifts uint8 [n x rank], B int8 [n x N x rank]
         with b_shifts uint8 [n x N] (include/myl_hip.h states the arithmetic)."""
         what = "linear_w8a16_adapters_dev"
-        _need_bytes(what, act_frac=act_frac, mid_frac=mid_frac, out_frac=out_frac)
+        if (act_frac | mid_frac | out_frac) >> 8:
+            _need_bytes(what, act_frac=act_frac, mid_frac=mid_frac, out_frac=out_frac)
         M, K = x.shape
         N = W.shape[0]
         n, rank = A.shape[:2]
@@ -502,7 +503,8 @@ class RocmBackend:
         max_tail, by default the capacity; negative: the row is left out and
         its output is zero).  include/myl_hip.h states the arithmetic."""
         what = "attention_prefix_dev"
-        _need_bytes(what, score_shift=score_shift, lut_shift=lut_shift, prob_frac=prob_frac)
+        if (score_shift | lut_shift | prob_frac) >> 8:
+            _need_bytes(what, score_shift=score_shift, lut_shift=lut_shift, prob_frac=prob_frac)
         if not -2**63 <= score_mult < 2**63:
             raise ValueError(f"{what}: score_mult must be an int64, not {score_mult}")
         R, H, hd = q.shape
@@ -540,7 +542,8 @@ class RocmBackend:
         ps, ts = _strides(k_prefix), _strides(k_tail)
         if not (ps[1] in (None, hd) and ps[2] in (None, 1) and ts[2] in (None, hd) and ts[3] in (None, 1)):
             raise ValueError(f"{what}: the positions of a KV head follow one another")
-        if ps != _strides(v_prefix) or ts != _strides(v_tail):
+        if (k_prefix.stride() != v_prefix.stride() and ps != _strides(v_prefix)) or \
+                (k_tail.stride() != v_tail.stride() and ts != _strides(v_tail)):
             raise ValueError(f"{what}: keys and values have the same strides")
         p_head, t_head = _apart(what, "prefix", ps[0], P * hd), _apart(what, "tails", ts[1], T * hd)
         t_slot = KH * T * hd if ts[0] is None else ts[0]  # 0: the slots share one tail
