@@ -44,18 +44,6 @@ struct DeviceGuard {
     DeviceGuard& operator=(const DeviceGuard&) = delete;
 };
 
-// Pieces of a workspace the caller gave (256-byte steps); with base null, only the sizes are added up.
-struct Carve {
-    char* base;
-    size_t used = 0;
-    template <class T>
-    T* take(size_t n) {
-        const size_t off = used;
-        used += (n * sizeof(T) + 255) & ~(size_t)255;
-        return base ? reinterpret_cast<T*>(base + off) : nullptr;
-    }
-};
-
 inline bool fits_int(size_t v) { return v <= (size_t)INT32_MAX; }
 
 // Looks up, with `device` current, the device address of the scratch array of

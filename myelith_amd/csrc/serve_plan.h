@@ -88,7 +88,7 @@ inline AdapterPlan adapter_plan(const AdapterShape& s, int cus) {
         while (p.rank_pad < (int)s.rank) p.rank_pad *= 2;
         auto up = [](int64_t a, int64_t b) { return (a + b - 1) / b; };
         // Two blocks per CU (61 rows, rank 64, K 18944: 14.7 us; four: 16.6), a unit per wave at
-        // least; a wave's i32 sums hold 2^17 products.
+        // least and 512 at most: its i32 sums hold 2^16 products of up to 2^14.
         const int64_t units = up((int64_t)s.K, kAdapterUnit), blocks = (int64_t)p.windows * p.down_tiles * p.rank_groups;
         const int64_t want = std::max(std::min(up(2 * (int64_t)cus, blocks), up(units, 4)), up(units, 4 * 512));
         p.per_wave = (int)up(units, 4 * want);

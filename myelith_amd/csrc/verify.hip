@@ -395,7 +395,7 @@ __global__ __launch_bounds__(kBlk) void verify_pick_kernel(Verify a) {
     for (int k = 0; k < 4; ++k) four[k] = red[4 * lane + k];
     {
         const myl_u128 t = four[0] + four[1] + four[2] + four[3];
-        // 128-bit scan as two words: the low 63 bits and the rest
+        // 128-bit scan as two words, the low 56 bits (64 of them stay below 2^62) and the rest
         const uint64_t mask = (1ull << 56) - 1;
         const uint64_t lo = wave_scan_u64((uint64_t)t & mask, lane), hi = wave_scan_u64((uint64_t)(t >> 56), lane);
         const myl_u128 inc = ((myl_u128)hi << 56) + lo;
