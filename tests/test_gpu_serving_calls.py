@@ -8,7 +8,7 @@ import pytest
 
 import serving_ref as ref
 from conftest import case
-from test_gpu_serving import (adapter_inputs, attention_inputs, dirty, exp_lut, gauss16, gpu, rng, run_adapters, run_attention,  # noqa: F401
+from test_gpu_serving import (Step, adapter_inputs, attention_inputs, dirty, exp_lut, gauss16, gpu, rng, run_adapters, run_attention,  # noqa: F401
                               same, verify_inputs, want_adapters)
 
 pytestmark = pytest.mark.gpu
@@ -190,3 +190,60 @@ def test_tables_that_end_inside_a_load(backend, entries):
     got = backend.attention_prefix_dev(d["q"], d["kp"], d["vp"], d["kt"], d["vt"], d["lens"], s["mult"], s["shift"], behind[:entries],
                                        s["lut_shift"], 14, slots=d["slots"])
     same(got, want, f"{entries} entries")
+
+
+# ---- steps side by side ---------------------------------------------------------------------------
+
+def junk(step):
+    """Nothing that a step wrote before is left."""
+    for t in (step.proj, step.mix, step.accepted, step.tokens):
+        t.fill_(-7)
+    dirty(step.ws)
+
+
+@pytest.mark.parametrize("contexts", [1, 2])
+def test_each_of_two_streams_writes_all_of_its_outputs(backend, exp_lut, contexts):
+    """Two steps on two streams, of one context or of one each: the last round starts from
+    outputs and workspaces that hold nothing of the rounds before."""
+    import torch
+    from myelith_amd.backend import RocmBackend
+    case(f"two streams, {contexts} contexts")
+    other = backend if contexts == 1 else RocmBackend(0)
+    try:
+        steps = [Step(backend, exp_lut, seed=91), Step(other, exp_lut, seqs=4, k=2, seed=92, prefix=900)]
+        streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+        for s in steps:
+            s.project_and_attend()
+            s.to_logits()
+        torch.cuda.synchronize()
+        for turn in range(6):
+            case(f"round {turn}")
+            if turn in (0, 5):
+                torch.cuda.synchronize()
+                for s in steps:
+                    junk(s)
+                torch.cuda.synchronize()
+            for s, stream in zip(steps, streams):
+                with torch.cuda.stream(stream):
+                    if contexts == 1 or turn == 0:
+                        s.b.use_torch_stream()
+                    s.project_and_attend()
+                    s.check_drafts()
+        for i, s in enumerate(steps):
+            s.check(f"step {i}")
+    finally:
+        torch.cuda.synchronize()
+        backend.use_torch_stream()
+        if other is not backend:
+            other.close()
+
+
+# ---- a request's prompt behind the prefix ----------------------------------------------------------
+
+@pytest.mark.parametrize("seqs,rows,prefix,H,KH,hd", [(1, 300, 500, 14, 2, 64), (2, 150, 130, 8, 2, 128), (3, 257, 0, 3, 1, 64)])
+def test_attention_prompts(backend, exp_lut, seqs, rows, prefix, H, KH, hd):
+    """Hundreds of rows of a sequence, each attending its own position and all before it."""
+    case(f"attention prompts {seqs}x{rows} behind {prefix}")
+    s = attention_inputs(93, seqs, rows, prefix, rows + 20, H, KH, hd)
+    s["lens"] = (np.array([[0], [20], [7]][:seqs]) + 1 + np.arange(rows)).reshape(-1).astype(np.int32)
+    same(run_attention(backend, s, exp_lut), ref.attention(**s, lut=exp_lut), "prompts")
