@@ -261,8 +261,12 @@ int myl_linear_w8a16_adapters_dev(myl_ctx* ctx, const int16_t* x, size_t M, size
  * head h reads KV head h / (heads / kv_heads).  head_dim is 64 or 128
  * (MYL_E_UNSUPPORTED otherwise), prob_frac at most 14, prefix_len + max_tail at
  * most 65536, heads and rows at most 65535 each and 2^22 together, the exp table
- * 1 to 32768 entries; negative ones count as 0.  Pointers to int16 and the
- * workspace are 16-byte aligned, strides (in elements) multiples of 8. */
+ * 1 to 32768 entries; negative ones count as 0 (trailing zeros left off make it
+ * faster).  Pointers to int16 and the workspace are 16-byte aligned, strides (in
+ * elements) multiples of 8; a tail_slot_stride of 0 gives all slots one tail.
+ * Except where the keys are few, the workspace holds an exp value of 2 bytes per
+ * row, head and key: 1 GB for a prompt of 2048 rows of 28 heads behind 6000 keys.
+ * Fewer rows per call take less. */
 size_t myl_attention_prefix_workspace(const myl_ctx* ctx, size_t n_seqs, size_t rows_per_seq, size_t heads,
                                       size_t kv_heads, size_t head_dim, size_t prefix_len, size_t max_tail);
 int myl_attention_prefix_dev(myl_ctx* ctx, const int16_t* q, size_t n_seqs, size_t rows_per_seq, size_t ldq,
@@ -285,10 +289,17 @@ int myl_attention_prefix_dev(myl_ctx* ctx, const int16_t* q, size_t n_seqs, size
  *   floor(r_k W / 2^64) < w_0 + ... + w_j,  W = sum w_j,
  * where w_j = p_j of row i behind the last draft, and max(0, p_j Q - q_j P) of
  * row i where draft i was rejected (p_j if that leaves nothing; the row's first
- * maximum if P = 0).  So the tokens follow the target's probabilities whatever
- * was drafted.  exp_lut = NULL checks greedily: draft i is accepted when it is
- * the first maximum of row i (sampling.rs:8-18), the next token is the row's
- * first maximum; draft and randoms are not read.
+ * maximum if P = 0).  With random numbers that are uniform and independent of
+ * the drafts the tokens follow the target's probabilities p_j / P
+ *   - with draft logits: where each draft was drawn from their weights q_j, as
+ *     this call draws a token per row with k = 0;
+ *   - with draft = NULL: whatever was drafted, and however.
+ * Drafts of another choice handed over with their logits (the draft's argmax, or
+ * a token of myl_sample_dev, whose weights are z_j - min z + 1) bias the tokens, with
+ * no error.  Nor are the p_j the weights by which myl_sample_dev draws.
+ * exp_lut = NULL checks greedily: draft i is accepted when it is the first
+ * maximum of row i (sampling.rs:8-18), the next token is the row's first maximum;
+ * draft and randoms are not read.
  *   target   [n_seqs * (k + 1)] rows (stride ldt): row b (k + 1) + i follows draft i - 1
  *   draft    [n_seqs * k] rows (stride ldd)       tokens   [n_seqs x k]
  *   n_draft  [n_seqs], clamped to 0 .. k (NULL: k) randoms  [n_seqs x (k + 1)]

@@ -575,7 +575,9 @@ class RocmBackend:
         [B x k+1 x V] logits, tokens int64 [B x k], randoms uint64 [B x k+1]
         (torch int64 tensors hold the bits), draft int32 [B x k x V] logits or
         None (drafts without probabilities), n_draft int32 [B] or None (k each);
-        exp_lut None checks greedily (randoms may be None).  Returns (accepted
+        exp_lut None checks greedily (randoms may be None).  Drafts that were not
+        drawn from the weights of `draft` (as this call draws with k = 0) are
+        handed over without it: their tokens would be biased.  Returns (accepted
         int32 [B], out int64 [B x k+1]: accepted drafts, the next token, -1).
         include/myl_hip.h states the arithmetic."""
         what = "verify_drafts_dev"

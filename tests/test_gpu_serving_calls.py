@@ -247,3 +247,37 @@ def test_attention_prompts(backend, exp_lut, seqs, rows, prefix, H, KH, hd):
     s = attention_inputs(93, seqs, rows, prefix, rows + 20, H, KH, hd)
     s["lens"] = (np.array([[0], [20], [7]][:seqs]) + 1 + np.arange(rows)).reshape(-1).astype(np.int32)
     same(run_attention(backend, s, exp_lut), ref.attention(**s, lut=exp_lut), "prompts")
+
+
+# ---- the tokens' distribution ---------------------------------------------------------------------
+
+@pytest.mark.parametrize("drafted", ["sampled", "argmax"])
+def test_tokens_follow_the_target(backend, exp_lut, drafted):
+    """Drafts that the call itself draws from the draft's logits (no drafts: a token per row), or
+    the draft's argmax handed over without probabilities; then their check.  Counts of n
+    independent tokens lie within 6 deviations sqrt(n p (1 - p)) of n p."""
+    import torch
+    case(f"tokens follow the target, {drafted} drafts")
+    B, V = 20000, 11
+    r = rng(94)
+    zt = r.integers(-150, 150, V).astype(np.int32)
+    zd = (zt + r.integers(-60, 61, V)).astype(np.int32)
+    table = gpu(exp_lut)
+    target = gpu(zt).expand(B, 2, V).contiguous()
+    draft = gpu(zd).expand(B, 1, V).contiguous()
+    rnd = gpu(r.integers(0, 2**64, (B, 3), dtype=np.uint64).view(np.int64))
+    none = torch.zeros((B, 0), dtype=torch.int64, device="cuda")
+    if drafted == "sampled":
+        accepted, tokens = backend.verify_drafts_dev(draft, none, rnd[:, :1].contiguous(), exp_lut=table)
+        assert not accepted.any()
+    else:
+        tokens = backend.argmax_dev(draft.view(B, V)).view(B, 1)
+    accepted, out = backend.verify_drafts_dev(target, tokens, rnd[:, 1:].contiguous(), exp_lut=table,
+                                              draft=draft if drafted == "sampled" else None)
+    p = ref.row_weights(zt, exp_lut) / ref.row_weights(zt, exp_lut).sum()
+    accepted, out = accepted.cpu().numpy(), out.cpu().numpy()
+    assert 0.1 < accepted.mean() < 0.95
+    for what, got in (("first tokens", out[:, 0]), ("tokens behind an accepted draft", out[accepted == 1, 1])):
+        n = got.size
+        count = np.bincount(got, minlength=V)
+        assert (np.abs(count - n * p) <= 6 * np.sqrt(n * p * (1 - p))).all(), (what, count / n, p)
