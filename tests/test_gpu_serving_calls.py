@@ -8,7 +8,7 @@ import pytest
 
 import serving_ref as ref
 from conftest import case
-from test_gpu_serving import (Step, adapter_inputs, attention_inputs, dirty, exp_lut, gauss16, gpu, rng, run_adapters, run_attention,  # noqa: F401
+from test_gpu_serving import (Step, adapter_inputs, attention_inputs, dirty, exp_lut, gauss16, gpu, rng, run_adapters, run_attention, run_verify,  # noqa: F401
                               same, verify_inputs, want_adapters)
 
 pytestmark = pytest.mark.gpu
@@ -281,3 +281,81 @@ def test_tokens_follow_the_target(backend, exp_lut, drafted):
         n = got.size
         count = np.bincount(got, minlength=V)
         assert (np.abs(count - n * p) <= 6 * np.sqrt(n * p * (1 - p))).all(), (what, count / n, p)
+
+
+# ---- the largest sizes ------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("prefix,tail", [(65536, 0), (0, 65536), (65000, 536), (1, 65535)])
+def test_attention_of_65536_keys(backend, exp_lut, prefix, tail):
+    case(f"attention of {prefix} + {tail} keys")
+    s = attention_inputs(95, 1, 2, prefix, tail, 2, 1, 64)
+    s["lens"] = np.array([tail, max(tail - 1, 0)], np.int32)
+    same(run_attention(backend, s, exp_lut), ref.attention(**s, lut=exp_lut), "65536 keys")
+    flat = np.full(32768, 32767, np.int16)  # the exp sums at their largest
+    s.update(mult=0)
+    same(run_attention(backend, s, flat), ref.attention(**s, lut=flat), "65536 keys, large entries")
+
+
+@pytest.mark.parametrize("B,k,V", [(1, 1, 1 << 20), (31, 1024, 5), (65535, 0, 2), (21845, 1, 3)])
+def test_verify_at_the_largest_sizes(backend, exp_lut, B, k, V):
+    case(f"verify B={B} k={k} V={V}")
+    s = verify_inputs(96, B, k, V)
+    for draft, lut in ((s["draft"], exp_lut), (None, exp_lut), (None, None)):
+        got, want = run_verify(backend, dict(s, draft=draft), lut), ref.verify(lut=lut, **dict(s, draft=draft))
+        same(got[0], want[0], "accepted")
+        same(got[1], want[1], "tokens")
+
+
+def test_verify_accepts_1024_drafts(backend, exp_lut):
+    case("verify 1024 drafts accepted")
+    s = verify_inputs(97, 3, 1024, 6)
+    s["draft"] = s["target"][:, :1024].copy()
+    s["randoms"][:, :1024] = 2**64 - 1
+    s["tokens"] = s["target"][:, :1024].argmax(2).astype(np.int64)
+    s["tokens"][1, 1023] = -1
+    s["n_draft"] = np.array([1024, 1024, 1000], np.int32)
+    got, want = run_verify(backend, s, exp_lut), ref.verify(lut=exp_lut, **s)
+    assert want[0].tolist() == [1024, 1023, 1000]
+    same(got[0], want[0], "accepted")
+    same(got[1], want[1], "tokens")
+
+
+@pytest.mark.parametrize("M,N,K,rank,n", [(3, 1100003, 16, 3, 2), (2, 70, 262144 + 48, 5, 2), (1, 40, 131072, 256, 3)])
+def test_adapters_wide_and_deep(backend, M, N, K, rank, n):
+    case(f"adapters M={M} N={N} K={K} rank={rank}")
+    s = adapter_inputs(98, M, N, K, rank, n)
+    same(run_adapters(backend, s), want_adapters(s), "wide or deep")
+
+
+@pytest.mark.parametrize("H", [8, 18])
+def test_attention_captured_with_the_whole_table(backend, H):
+    """The table as luts.exp_lut() makes it takes more LDS than a launch has by default."""
+    import torch
+    from myelith_amd.luts import exp_lut as whole
+    case(f"attention captured, whole table, {H} heads")
+    s = attention_inputs(99, 3, 1, 400, 30, H, 1, 64)
+    d = {k: gpu(v) if isinstance(v, np.ndarray) else v for k, v in s.items()}
+    lut = whole()
+    table, out = gpu(lut), torch.empty_like(d["q"])
+    ws = backend.attention_prefix_workspace(d["q"], d["kp"], d["kt"])
+    stream = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    try:
+        with torch.cuda.stream(stream):
+            backend.use_torch_stream()
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=stream):
+            backend.attention_prefix_dev(d["q"], d["kp"], d["vp"], d["kt"], d["vt"], d["lens"], s["mult"], s["shift"], table, 6, 14,
+                                         slots=d["slots"], out=out, workspace=ws)
+        for turn in range(4):
+            s["q"] = gauss16(rng(100 + turn), s["q"].shape, 2048)
+            d["q"].copy_(gpu(s["q"]))
+            out.fill_(-7)
+            dirty(ws)
+            torch.cuda.synchronize()
+            g.replay()
+            torch.cuda.synchronize()
+            same(out, ref.attention(**s, lut=lut), f"replay {turn}")
+    finally:
+        torch.cuda.synchronize()
+        backend.use_torch_stream()
