@@ -13,7 +13,7 @@
 // Both run on the int8 matrix cores over the byte planes x = 256 hi + lo' + 128
 // (gemm_mfma.h), the sums of the weights from a third product with a vector of ones.
 // The shared product takes most of the time: 61 rows, N 3584, K 18944, rank 64, 32 adapters:
-// x A 14.7 us, W x 36, u B 7.6; 2003 rows, N 18944, K 3584, rank 16: 14, 306, 55.
+// x A 13.8 us, W x 36, u B 7.8; 2003 rows, N 18944, K 3584, rank 16: 14, 321, 54.
 #include "abi_internal.h"
 #include "gemm_dispatch.h"
 #include "qk_planes.h"
@@ -143,8 +143,8 @@ __device__ inline int group_rows(const Adapters& a, int w, int t, Grouping& s, T
 
 // Grid (windows x down_tiles, rank groups, splits of K); 256 threads.  Lane l holds row l % 16 of
 // A and of x at 16 (l / 16) of each 64 of K: two matrix steps use up a line of A.  A wave
-// loads the next unit while it multiplies one.  Bound by reading A: 38.8 MB in 14.7 us (61 rows,
-// rank 64, 32 adapters, K 18944; 2.6 TB/s with the latency of ids, grouping and first loads).
+// loads the next unit while it multiplies one.  Bound by reading A: 38.8 MB in 13.8 us (61 rows,
+// rank 64, 32 adapters, K 18944; 2.8 TB/s with the latency of ids, grouping and first loads).
 // A wave per (row, rank) read A once per row: 91 us.
 template <int RT>
 __global__ __launch_bounds__(256, 2) void adapters_down_kernel(Adapters a) {
