@@ -78,6 +78,8 @@ def _apart(what: str, name: str, stride, dense: int) -> int:
 class RocmBackend:
     """One HIP context on one device (rocm.rs:41-60)."""
 
+    _own_stream = None  # the context's, until a caller's takes its place
+
     def __init__(self, device_id: int = 0):
         h = C.c_void_p()
         rc = lib().myl_init(device_id, C.byref(h))
@@ -85,6 +87,7 @@ class RocmBackend:
             raise MylError(f"RocmBackend::init({device_id}) failed with status {rc}")
         self._h = h
         self._device_id = device_id
+        self._own_stream = lib().myl_stream(h)
         # models and MoE layers on this context: closed before it is destroyed,
         # whatever order the interpreter finalises them in
         self._owned = weakref.WeakSet()
@@ -386,41 +389,41 @@ class RocmBackend:
         return out
 
     # ---- a serving step: adapters, a shared prefix, drafted tokens ---------------
-    def _workspace(self, device, workspace, size_of, *sizes):
+    def _workspace(self, device, workspace, stream, size_of, *sizes):
         """The caller's workspace (the call checks its size), or one for this call alone."""
         if workspace is not None:
             if workspace.device != device or not workspace.is_contiguous():
                 raise ValueError("workspace: contiguous, on the operands' device")
             return workspace
-        return self._empty(max(size_of(self._h, *sizes), 1), "uint8", device)
+        return self._empty(max(size_of(self._h, *sizes), 1), "uint8", device, stream)
 
-    def _empty(self, shape, dtype: str, device):
-        """A tensor that a call writes: its memory is handed on only when the
-        context's stream has passed the call."""
+    @staticmethod
+    def _empty(shape, dtype: str, device, stream):
+        """A tensor that a call writes: its memory is handed on only when `stream`
+        (_other_stream) has passed the call."""
         import torch
         t = torch.empty(shape, dtype=getattr(torch, dtype), device=device)
-        stream = self._other_stream(device)
         if stream is not None:
             t.record_stream(stream)
         return t
 
     def _other_stream(self, device):
-        """The context's stream where it is not torch's current one."""
+        """The context's stream where nothing orders it with torch's current one: not if
+        they are the same, nor for the null stream and the context's own, which HIP makes
+        wait for each other."""
         import torch
         if device.type != "cuda":
             return None
-        stream = lib().myl_stream(self._h) or 0
-        if stream == torch.cuda.current_stream(device).cuda_stream:
+        stream, torchs = lib().myl_stream(self._h) or 0, torch.cuda.current_stream(device).cuda_stream
+        if stream == torchs or (torchs == 0 and stream == self._own_stream):
             return None
         return torch.cuda.ExternalStream(stream, device=device)
 
-    def _after_last_use(self, what: str, device) -> None:
+    @staticmethod
+    def _after_last_use(what: str, device, stream) -> None:
         """Behind a call's allocations, before its launch: the last use of their memory may
         still be queued on torch's current stream, so the context's stream waits for it."""
         import torch
-        stream = self._other_stream(device)
-        if stream is None:
-            return
         with torch.cuda.stream(stream):
             captured = torch.cuda.is_current_stream_capturing()
         if captured != torch.cuda.is_current_stream_capturing():
@@ -464,18 +467,18 @@ class RocmBackend:
             raise ValueError(f"{what}: the elements of a row of x follow one another")
         if out_frac_pc is not None:
             _need_dev(what, x.device, out_frac_pc=(out_frac_pc, "uint8", (N,)))
-        made = out is None
-        if made:
-            out = self._empty((M, N), "int16", x.device)
+        stream = self._other_stream(x.device) if out is None or workspace is None else None
+        if out is None:
+            out = self._empty((M, N), "int16", x.device, stream)
         _need_dev(what, x.device, out=(out, "int16", None))
         ldo, step = _strides(out)
         ldo = _apart(what, "out", ldo, N)
         if out.shape != (M, N) or step not in (None, 1):
             raise ValueError(f"{what}: out must be [M x N]")
         self._need_here(what, x.device)
-        ws = self._workspace(x.device, workspace, lib().myl_linear_w8a16_adapters_workspace, M, N, K, rank, n)
-        if made or workspace is None:
-            self._after_last_use(what, x.device)
+        ws = self._workspace(x.device, workspace, stream, lib().myl_linear_w8a16_adapters_workspace, M, N, K, rank, n)
+        if stream is not None:
+            self._after_last_use(what, x.device, stream)
         rc = lib().myl_linear_w8a16_adapters_dev(
             self._h, x.data_ptr(), M, ldx, W.data_ptr(), N, K, w_shifts.data_ptr(), act_frac, out_frac,
             None if out_frac_pc is None else out_frac_pc.data_ptr(), ids.data_ptr(), A.data_ptr(), a_shifts.data_ptr(),
@@ -526,9 +529,9 @@ class RocmBackend:
         else:
             if not (S >= n_seqs):
                 raise ValueError(f"{what}: fewer tails than sequences")
-        made = out is None
-        if made:
-            out = self._empty((R, H, hd), "int16", dev)
+        stream = self._other_stream(dev) if out is None or workspace is None else None
+        if out is None:
+            out = self._empty((R, H, hd), "int16", dev, stream)
         _need_dev(what, dev, out=(out, "int16", None))
         if out.shape != q.shape:
             raise ValueError(f"{what}: out must have q's shape")
@@ -550,9 +553,9 @@ class RocmBackend:
         max_tail = T if max_tail is None else max_tail
         ldq, ldo = rows_of(q, "q"), rows_of(out, "out")
         self._need_here(what, dev)
-        ws = self._workspace(dev, workspace, lib().myl_attention_prefix_workspace, n_seqs, rows_per_seq, H, KH, hd, P, max_tail)
-        if made or workspace is None:
-            self._after_last_use(what, dev)
+        ws = self._workspace(dev, workspace, stream, lib().myl_attention_prefix_workspace, n_seqs, rows_per_seq, H, KH, hd, P, max_tail)
+        if stream is not None:
+            self._after_last_use(what, dev, stream)
         rc = lib().myl_attention_prefix_dev(
             self._h, q.data_ptr(), n_seqs, rows_per_seq, ldq, H, KH, hd, k_prefix.data_ptr(), v_prefix.data_ptr(),
             P, p_head, k_tail.data_ptr(), v_tail.data_ptr(), S, t_slot, t_head, max_tail,
@@ -605,18 +608,18 @@ class RocmBackend:
             _need_dev(what, dev, draft=(draft, "int32", None))
         if n_draft is not None:
             _need_dev(what, dev, n_draft=(n_draft, "int32", (B,)))
-        made = accepted is None or out is None
+        stream = self._other_stream(dev) if accepted is None or out is None or workspace is None else None
         if accepted is None:
-            accepted = self._empty(B, "int32", dev)
+            accepted = self._empty(B, "int32", dev, stream)
         if out is None:
-            out = self._empty((B, k1), "int64", dev)
+            out = self._empty((B, k1), "int64", dev, stream)
         _need_dev(what, dev, accepted=(accepted, "int32", (B,)), out=(out, "int64", (B, k1)))
         lut_len = 0 if exp_lut is None else exp_lut.numel()
         ldt, ldd = rows_of(target, "target", k1), V if draft is None or k == 0 else rows_of(draft, "draft", k)
         self._need_here(what, dev)
-        ws = self._workspace(dev, workspace, lib().myl_verify_drafts_workspace, B, k, V, lut_len)
-        if made or workspace is None:
-            self._after_last_use(what, dev)
+        ws = self._workspace(dev, workspace, stream, lib().myl_verify_drafts_workspace, B, k, V, lut_len)
+        if stream is not None:
+            self._after_last_use(what, dev, stream)
         rc = lib().myl_verify_drafts_dev(
             self._h, target.data_ptr(), ldt, None if draft is None or k == 0 else draft.data_ptr(), ldd, B, k, V, tokens.data_ptr(),
             None if n_draft is None else n_draft.data_ptr(), None if randoms is None else randoms.data_ptr(),

@@ -24,11 +24,13 @@ def test_tails_that_all_slots_share(backend, exp_lut, prefix):
     same(run_attention(backend, d, exp_lut), ref.attention(**s, lut=exp_lut), "shared tail")
 
 
-def test_allocated_memory_still_in_use_on_torchs_stream(backend):
+@pytest.mark.parametrize("torchs", ["null", "side"])
+@pytest.mark.parametrize("context", ["own", "side"])
+def test_allocated_memory_still_in_use_on_torchs_stream(backend, torchs, context):
     """A temporary that torch's queued kernels still read is freed just before a call on
     another stream, which takes its memory for the output."""
     import torch
-    case("memory in use on torch's stream")
+    case(f"memory in use on torch's {torchs} stream, the context on its {context} one")
     M, N = 64, 16384
     s = adapter_inputs(82, M, N, 64, 8, 3)
     d = {k: gpu(v) if isinstance(v, np.ndarray) else v for k, v in s.items()}
@@ -36,27 +38,28 @@ def test_allocated_memory_still_in_use_on_torchs_stream(backend):
     ws = backend.linear_w8a16_adapters_workspace(d["x"], d["W"], d["A"])
     a = torch.ones((8192, 8192), dtype=torch.float32, device="cuda")
     product = torch.empty_like(a)
-    side = torch.cuda.Stream()
+    current = torch.cuda.default_stream() if torchs == "null" else torch.cuda.Stream()
     torch.cuda.synchronize()
     try:
-        with torch.cuda.stream(side):
-            backend.use_torch_stream()
+        with torch.cuda.stream(torch.cuda.default_stream() if context == "own" else torch.cuda.Stream()):
+            backend.use_torch_stream()  # the null stream leaves a context its own
         for turn in range(3):
-            torch.cuda.empty_cache()
-            seen = torch.empty((M, N), dtype=torch.int16, device="cuda")
-            temporary = torch.full((M, N), 1000 + turn, dtype=torch.int16, device="cuda")
-            torch.cuda.synchronize()
-            for _ in range(4):  # some ten milliseconds each
-                torch.mm(a, a, out=product)
-            seen.copy_(temporary)
-            place = temporary.data_ptr()
-            del temporary
-            out = backend.linear_w8a16_adapters_dev(*args, workspace=ws)
-            torch.cuda.synchronize()
-            assert out.data_ptr() == place  # the memory is the temporary's
-            assert (seen == 1000 + turn).all()
-            same(out, want_adapters(s), f"turn {turn}")
-            del out, seen
+            with torch.cuda.stream(current):
+                torch.cuda.empty_cache()
+                seen = torch.empty((M, N), dtype=torch.int16, device="cuda")
+                temporary = torch.full((M, N), 1000 + turn, dtype=torch.int16, device="cuda")
+                torch.cuda.synchronize()
+                for _ in range(4):  # some ten milliseconds each
+                    torch.mm(a, a, out=product)
+                seen.copy_(temporary)
+                place = temporary.data_ptr()
+                del temporary
+                out = backend.linear_w8a16_adapters_dev(*args, workspace=ws)
+                torch.cuda.synchronize()
+                assert out.data_ptr() == place  # the memory is the temporary's
+                assert (seen == 1000 + turn).all()
+                same(out, want_adapters(s), f"turn {turn}")
+                del out, seen
     finally:
         torch.cuda.synchronize()
         backend.use_torch_stream()
@@ -203,8 +206,8 @@ def junk(step):
 
 @pytest.mark.parametrize("contexts", [1, 2])
 def test_each_of_two_streams_writes_all_of_its_outputs(backend, exp_lut, contexts):
-    """Two steps on two streams, of one context or of one each: the last round starts from
-    outputs and workspaces that hold nothing of the rounds before."""
+    """Two steps on two streams, of one context or of one each: the last turn starts from
+    outputs and workspaces that hold nothing of the turns before."""
     import torch
     from myelith_amd.backend import RocmBackend
     case(f"two streams, {contexts} contexts")
@@ -217,7 +220,7 @@ def test_each_of_two_streams_writes_all_of_its_outputs(backend, exp_lut, context
             s.to_logits()
         torch.cuda.synchronize()
         for turn in range(6):
-            case(f"round {turn}")
+            case(f"turn {turn}")
             if turn in (0, 5):
                 torch.cuda.synchronize()
                 for s in steps:

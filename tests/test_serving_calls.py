@@ -159,10 +159,14 @@ def calls_of(b):
              on_gpu(dict(space, accepted=torch.zeros(2, dtype=torch.int32), out=torch.zeros((2, 4), dtype=torch.int64))))]
 
 
-def test_allocated_memory_is_written_after_its_last_use(streams):
+@pytest.mark.parametrize("torchs,own", [(7, 3), (7, 9), (0, 3)])
+def test_allocated_memory_is_written_after_its_last_use(streams, monkeypatch, torchs, own):
     """torch hands out memory whose last use is queued on its current stream: a context on
-    another stream waits for that, after the call's allocations and before its launch."""
+    another stream waits for that, after the call's allocations and before its launch.  (The
+    context's own stream and the null stream wait for each other by themselves.)"""
     b, log = streams
+    monkeypatch.setattr(FakeStream, "torchs", torchs)
+    b._own_stream = own
     for call, args, given in calls_of(b):
         for left_out in [given, *([k] for k in given)]:
             log.clear()
@@ -170,15 +174,18 @@ def test_allocated_memory_is_written_after_its_last_use(streams):
             call(**args, **{k: v for k, v in given.items() if k not in left_out})
             kinds = [e[0] if e[0] in ("empty", "wait") else "launch" for e in log if not e[0].endswith("_workspace")]
             assert kinds == ["empty"] * len(left_out) + ["wait", "launch"], (call.__name__, list(left_out), kinds)
-            assert ("wait", 9, 7) in log and [s for _, s in OnGpu.recorded] == [9] * len(left_out)
+            assert ("wait", 9, torchs) in log and [s for _, s in OnGpu.recorded] == [9] * len(left_out)
         log.clear()
         call(**args, **given)
         assert len(log) == 1, log  # nothing allocated, nothing to wait for
 
 
-def test_allocating_on_torchs_stream_waits_for_nothing(streams, monkeypatch):
+@pytest.mark.parametrize("torchs,own", [(9, 3), (0, 9)])
+def test_allocating_on_an_ordered_stream_waits_for_nothing(streams, monkeypatch, torchs, own):
+    """torch's stream itself, and the context's own stream beside the null stream."""
     b, log = streams
-    monkeypatch.setattr(FakeStream, "torchs", 9)
+    monkeypatch.setattr(FakeStream, "torchs", torchs)
+    b._own_stream = own
     for call, args, given in calls_of(b):
         log.clear()
         call(**args)
