@@ -412,7 +412,7 @@ class RocmBackend:
         they are the same, nor for the null stream and the context's own, which HIP makes
         wait for each other."""
         import torch
-        if device.type != "cuda":
+        if device.type != "cuda" or device.index != self._device_id:  # the call will be refused
             return None
         stream, torchs = lib().myl_stream(self._h) or 0, torch.cuda.current_stream(device).cuda_stream
         if stream == torchs or (torchs == 0 and stream == self._own_stream):
@@ -424,11 +424,13 @@ class RocmBackend:
         """Behind a call's allocations, before its launch: the last use of their memory may
         still be queued on torch's current stream, so the context's stream waits for it."""
         import torch
-        with torch.cuda.stream(stream):
-            captured = torch.cuda.is_current_stream_capturing()
-        if captured != torch.cuda.is_current_stream_capturing():
+        torchs, captured = torch.cuda.current_stream(device), []
+        for s in (stream, torchs):
+            with torch.cuda.stream(s):  # its device's, whatever the current device
+                captured.append(torch.cuda.is_current_stream_capturing())
+        if captured[0] != captured[1]:
             raise ValueError(f"{what}: while one of torch's stream and the context's is captured, outputs and workspace are the caller's")
-        stream.wait_stream(torch.cuda.current_stream(device))
+        stream.wait_stream(torchs)
 
     def _need_here(self, what: str, device) -> None:
         if device.type != "cuda" or device.index != self._device_id:

@@ -208,6 +208,12 @@ def test_allocating_while_one_stream_is_captured_is_refused(streams, monkeypatch
         call(**args, **given)
 
 
+def test_another_devices_memory_is_not_tied_to_the_stream(streams):
+    """Operands on another device than the context's are refused; what was allocated there is freed as usual."""
+    b, log = streams
+    assert b._other_stream(torch.device("cuda", 1)) is None and b._other_stream(torch.device("cuda", 0)) is not None
+
+
 # ---- arguments that would arrive as something else ------------------------------------------
 
 def test_an_empty_table_is_not_the_greedy_check(recorded):
