@@ -314,6 +314,101 @@ int myl_verify_drafts_dev(myl_ctx* ctx, const int32_t* target, size_t ldt, const
                           const uint64_t* randoms, const int16_t* exp_lut, size_t lut_len, int32_t* accepted,
                           int64_t* out, void* workspace, size_t workspace_bytes);
 
+/* ---- a serving step over a paged cache ----------------------------------------
+ * No counterparts in the reference, whose cache is one row of positions per
+ * sequence (kv_cache.rs); each step is a reference primitive.  As for the serving
+ * calls above: scratch is the caller's workspace, the calls can be captured
+ * into HIP graphs, and calls on different contexts and streams run at once as
+ * long as each has its own workspace (and no call reads pages that another writes).
+ *
+ * A cache is n_pages pages of page_size positions (1 to 65536) of the keys, and as many of
+ * the values, int16.  Position off of page p, KV head h: head_dim consecutive elements at
+ *   p * page_stride + h * head_stride + off * pos_stride
+ * in elements, multiples of 8, the same for keys and values; so [page][head][position]
+ * and [page][position][head] both do.  A sequence's positions lie in the pages that its
+ * row of `tables` (n_seqs rows of table_len int32, table_stride apart) names in turn:
+ * position pos in page tables[seq][pos / page_size], at pos % page_size.  Sequences may
+ * share pages.  An id outside [0, n_pages) names no page.  Pointers to int16 and uint8 and
+ * the workspace are 16-byte aligned; head_dim is 64 or 128 (MYL_E_UNSUPPORTED
+ * otherwise). */
+
+/* Norms of each query and key head (rmsnorm.rs:61-161 over head_dim values, whose x_shifts
+ * are all one and so leave the result): gamma and gamma_shifts [head_dim] of the
+ * queries and of the keys (both NULL: those stay as they are), inv_n_q20 =
+ * 2^20 / head_dim (0 to 2^20), results at q_out_frac and k_out_frac. */
+typedef struct myl_head_norm {
+    const int8_t* q_gamma;
+    const uint8_t* q_gamma_shifts;
+    const int8_t* k_gamma;
+    const uint8_t* k_gamma_shifts;
+    const int16_t* rsqrt_lut;
+    size_t rsqrt_len;
+    int64_t inv_n_q20;
+    uint8_t lut_input_shift, lut_output_frac, q_out_frac, k_out_frac;
+} myl_head_norm;
+
+/* New rows into a paged cache: row r is position positions[r] of sequence seqs[r]
+ * (seqs NULL: sequence r).  q [rows] rows of heads x head_dim, k and v of kv_heads x
+ * head_dim, row strides ldq, ldk, ldv (multiples of 8; the three parts of one
+ * product's rows, say).  In turn:
+ *   bias   [(heads + 2 kv_heads) x head_dim] of q, k and v, with bias_shifts:
+ *          add_bias_i16 (linear.rs:132-145) at q_frac, k_frac, v_frac; NULL: none
+ *   norm   rmsnorm of each query and key head; NULL: none
+ *   rope   queries and keys by the tables' row positions[r] % (lut_len / (head_dim / 2))
+ *          (rope.rs:17-59; cos_lut, sin_lut of lut_len entries, rope_frac)
+ * then queries go to q_out (row stride ldo; q itself with ldo = ldq is allowed), keys and
+ * values to the position's place in the pages.  A row whose position is negative or
+ * whose sequence is outside [0, n_seqs) is left out: nothing of it is written.  A
+ * position past the table or on no page keeps its query only.  Rows of one call name
+ * different places; of two with the same place, either may be what stays.  heads
+ * may be 0 (keys and values alone). */
+int myl_kv_append_paged_dev(myl_ctx* ctx, const int16_t* q, size_t ldq, const int16_t* k, size_t ldk, const int16_t* v,
+                            size_t ldv, size_t rows, size_t heads, size_t kv_heads, size_t head_dim, const int16_t* bias,
+                            const uint8_t* bias_shifts, uint8_t q_frac, uint8_t k_frac, uint8_t v_frac,
+                            const myl_head_norm* norm, const int16_t* cos_lut, const int16_t* sin_lut, size_t lut_len,
+                            uint8_t rope_frac, const int32_t* positions, const int32_t* seqs, const int32_t* tables,
+                            size_t n_seqs, size_t table_len, size_t table_stride, int16_t* k_pages, int16_t* v_pages,
+                            size_t n_pages, size_t page_size, size_t page_stride, size_t head_stride, size_t pos_stride,
+                            int16_t* q_out, size_t ldo);
+
+/* Attention (attention.rs:42-90) of each sequence's newest rows over its pages: row
+ * r = s * rows_per_seq + i of sequence s attends positions 0 .. lens[r] - 1 (at most
+ * max_len, which is at most table_len * page_size and 131072) that lie on a page; drafted rows
+ * of one sequence take rising lens.  q, out [n_seqs * rows_per_seq] rows of heads x
+ * head_dim, row strides ldq, ldo (multiples of 8).  A row with no key, also of a lens of 0
+ * or below, gives zero.  Query head h reads KV head h / (heads / kv_heads).
+ * prob_frac is at most 14, heads and rows at most 65535 each and 2^22 together, the exp
+ * table 1 to 32768 entries; negative ones count as 0.  A max_len close to the longest
+ * row's keeps the launch small; the workspace holds a score of 4 bytes per
+ * row, head and position below max_len. */
+size_t myl_attention_paged_workspace(const myl_ctx* ctx, size_t n_seqs, size_t rows_per_seq, size_t heads,
+                                     size_t kv_heads, size_t head_dim, size_t max_len);
+int myl_attention_paged_dev(myl_ctx* ctx, const int16_t* q, size_t n_seqs, size_t rows_per_seq, size_t ldq,
+                            size_t heads, size_t kv_heads, size_t head_dim, const int16_t* k_pages,
+                            const int16_t* v_pages, size_t n_pages, size_t page_size, size_t page_stride,
+                            size_t head_stride, size_t pos_stride, const int32_t* tables, size_t table_len,
+                            size_t table_stride, const int32_t* lens, size_t max_len, int64_t score_mult,
+                            uint8_t score_shift, const int16_t* exp_lut, size_t lut_len, uint8_t lut_shift,
+                            uint8_t prob_frac, int16_t* out, size_t ldo, void* workspace, size_t workspace_bytes);
+
+/* Log probabilities of given tokens, the entropy and the most likely alternatives of rows of
+ * Q6 logits (row stride ldz), in Q16.  With m = max z, e_j = exp_lut[(m - z_j) << 2]
+ * (0 past the table and for negative entries) and S = sum e_j, as in myl_logsoftmax_dev:
+ *   logprobs[r][i]   (z_t - m) 2^10 - ln_q16(S) of token t = tokens[r][i]; 0 where t is
+ *                    outside the vocabulary
+ *   entropy[r]       -sum p_j ln p_j: ln_q16(S) + RNE(2^10 sum e_j (m - z_j) / S)
+ *   top_tokens, top_logprobs [rows x top_n]: the largest logits in turn, of equal ones the
+ *                    lowest index first, with the log probability as above
+ * S = 0 is taken as 1 for ln_q16, with an entropy of 0.  tokens and logprobs
+ * [rows x n_tokens]; n_tokens and top_n may be 0 and entropy NULL.  rows is at most
+ * 65535, vocab 2^20, n_tokens 65536, top_n 32, the table 32768 entries (trailing zeros
+ * left off make it faster). */
+size_t myl_logprobs_workspace(const myl_ctx* ctx, size_t rows, size_t vocab, size_t top_n, size_t lut_len);
+int myl_logprobs_dev(myl_ctx* ctx, const int32_t* logits, size_t rows, size_t vocab, size_t ldz, const int16_t* exp_lut,
+                     size_t lut_len, const int64_t* tokens, size_t n_tokens, size_t top_n, int64_t* logprobs,
+                     int64_t* entropy, int64_t* top_tokens, int64_t* top_logprobs, void* workspace,
+                     size_t workspace_bytes);
+
 /* ======================================================================
  * 3. Device-resident model (runtime/src/model.rs, kv_cache.rs)
  * ==================================================================== */

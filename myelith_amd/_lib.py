@@ -51,6 +51,13 @@ class Luts(C.Structure):
                 ("exp_len", sz), ("cos", P), ("sin", P), ("rope_len", sz)]
 
 
+class HeadNormArgs(C.Structure):
+    """myl_head_norm (include/myl_hip.h)."""
+    _fields_ = [("q_gamma", P), ("q_gamma_shifts", P), ("k_gamma", P), ("k_gamma_shifts", P), ("rsqrt_lut", P),
+                ("rsqrt_len", sz), ("inv_n_q20", i64), ("lut_input_shift", u8), ("lut_output_frac", u8),
+                ("q_out_frac", u8), ("k_out_frac", u8)]
+
+
 # name -> (restype, argtypes); the exported symbol set of include/myl_hip.h.
 SIGNATURES: dict[str, tuple] = {
     "myl_backend_name": (C.c_char_p, []),
@@ -96,6 +103,13 @@ SIGNATURES: dict[str, tuple] = {
                                        P, sz, u8, u8, P, sz, P, sz]),
     "myl_verify_drafts_workspace": (sz, [P, sz, sz, sz, sz]),
     "myl_verify_drafts_dev": (INT, [P, P, sz, P, sz, sz, sz, sz, P, P, P, P, sz, P, P, P, sz]),
+    "myl_kv_append_paged_dev": (INT, [P, P, sz, P, sz, P, sz, sz, sz, sz, sz, P, P, u8, u8, u8, P, P, P, sz, u8, P, P, P,
+                                      sz, sz, sz, P, P, sz, sz, sz, sz, sz, P, sz]),
+    "myl_attention_paged_workspace": (sz, [P, sz, sz, sz, sz, sz, sz]),
+    "myl_attention_paged_dev": (INT, [P, P, sz, sz, sz, sz, sz, sz, P, P, sz, sz, sz, sz, sz, P, sz, sz, P, sz, i64, u8,
+                                      P, sz, u8, u8, P, sz, P, sz]),
+    "myl_logprobs_workspace": (sz, [P, sz, sz, sz, sz]),
+    "myl_logprobs_dev": (INT, [P, P, sz, sz, sz, P, sz, P, sz, sz, P, P, P, P, P, sz]),
     "myl_model_create_synthetic": (INT, [P, C.POINTER(SynthSpec), C.POINTER(Luts), C.POINTER(P)]),
     "myl_model_destroy": (None, [P]),
     "myl_model_reset": (INT, [P]),

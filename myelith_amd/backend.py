@@ -18,7 +18,7 @@ import weakref
 
 import numpy as np
 
-from ._lib import MYL_E_INVALID, lib
+from ._lib import MYL_E_INVALID, HeadNormArgs, lib
 
 
 class MylError(RuntimeError):
@@ -73,6 +73,33 @@ def _apart(what: str, name: str, stride, dense: int) -> int:
     if stride == 0:
         raise ValueError(f"{what}: {name} must not be expanded (a stride of 0)")
     return stride
+
+
+class HeadNorm:
+    """Norms of each query and key head for kv_append_paged_dev, as a program keeps them
+    beside a layer's weights: gamma int8 and shifts uint8 [head_dim] of the queries and
+    of the keys (None: those have no norm), the rsqrt table int16, 2^20 / head_dim, and the
+    fractional bits of the results."""
+
+    def __init__(self, q_gamma, q_gamma_shifts, k_gamma, k_gamma_shifts, rsqrt_lut, lut_input_shift: int, lut_output_frac: int,
+                 inv_n_q20: int, q_out_frac: int, k_out_frac: int):
+        what = "HeadNorm"
+        _need_bytes(what, lut_input_shift=lut_input_shift, lut_output_frac=lut_output_frac, q_out_frac=q_out_frac,
+                    k_out_frac=k_out_frac)
+        if not 0 <= inv_n_q20 <= 1 << 20:
+            raise ValueError(f"{what}: inv_n_q20 must be 0 to 2^20, not {inv_n_q20}")
+        self.device = rsqrt_lut.device
+        given = [t for t in (q_gamma, k_gamma) if t is not None]
+        if (q_gamma is None) != (q_gamma_shifts is None) or (k_gamma is None) != (k_gamma_shifts is None) or not given:
+            raise ValueError(f"{what}: gamma and its shifts, of the queries, the keys or both")
+        self.head_dim = given[0].numel()
+        n = (self.head_dim,)
+        _need_dev(what, self.device, rsqrt_lut=(rsqrt_lut, "int16", (rsqrt_lut.numel(),)),
+                  **{k: (t, d, n) for k, t, d in (("q_gamma", q_gamma, "int8"), ("q_gamma_shifts", q_gamma_shifts, "uint8"),
+                                                  ("k_gamma", k_gamma, "int8"), ("k_gamma_shifts", k_gamma_shifts, "uint8")) if t is not None})
+        self.tensors = (q_gamma, q_gamma_shifts, k_gamma, k_gamma_shifts, rsqrt_lut)
+        ptr = [None if t is None else t.data_ptr() for t in self.tensors]
+        self.args = HeadNormArgs(*ptr, rsqrt_lut.numel(), inv_n_q20, lut_input_shift, lut_output_frac, q_out_frac, k_out_frac)
 
 
 class RocmBackend:
@@ -630,3 +657,191 @@ class RocmBackend:
         if rc:
             self.check(rc, what)
         return accepted, out
+
+    # ---- a serving step over a paged cache --------------------------------------
+    @staticmethod
+    def _rows_of(what: str, name: str, t, inner: int) -> int:
+        """The row stride of [rows x heads x hd] whose heads follow one another."""
+        row, head, one = _strides(t)
+        if head not in (None, t.shape[2]) or one not in (None, 1):
+            raise ValueError(f"{what}: the heads of a row of {name} follow one another")
+        return _apart(what, name, row, inner)
+
+    @staticmethod
+    def _pages_of(what: str, k_pages, v_pages, tables):
+        """(page, head, position) strides of [pages x kv_heads x page_size x hd] tensors, and
+        the table rows' stride."""
+        n, KH, page, hd = k_pages.shape
+        if v_pages.shape != k_pages.shape:
+            raise ValueError(f"{what}: k_pages and v_pages [pages x kv_heads x page_size x hd]")
+        _need_dev(what, k_pages.device, k_pages=(k_pages, "int16", None), v_pages=(v_pages, "int16", None), tables=(tables, "int32", None))
+        st = _strides(k_pages)
+        if k_pages.stride() != v_pages.stride() and st != _strides(v_pages):
+            raise ValueError(f"{what}: keys and values have the same strides")
+        if st[3] not in (None, 1):
+            raise ValueError(f"{what}: the elements of a position follow one another")
+        if tables.dim() != 2:
+            raise ValueError(f"{what}: tables must be [sequences x pages of each]")
+        row, one = _strides(tables)
+        if one not in (None, 1):
+            raise ValueError(f"{what}: the entries of a sequence's table follow one another")
+        return (_apart(what, "pages", st[0], KH * page * hd), _apart(what, "pages", st[1], page * hd), _apart(what, "pages", st[2], hd),
+                _apart(what, "tables", row, tables.shape[1]))
+
+    def kv_append_paged_dev(self, q, k, v, positions, k_pages, v_pages, tables, cos_lut, sin_lut, rope_frac: int, seqs=None,
+                            bias=None, bias_shifts=None, q_frac: int = 0, k_frac: int = 0, v_frac: int = 0, norm=None, q_out=None):
+        """New rows into a paged cache: q int16 [rows x heads x hd], k and v
+        [rows x kv_heads x hd], positions int32 [rows] (negative: the row is left out) of
+        sequences seqs int32 [rows] (None: row r is sequence r), k_pages and v_pages int16
+        [pages x kv_heads x page_size x hd] (any strides between positions, heads and
+        pages), tables int32 [sequences x pages of each], cos_lut and sin_lut int16
+        [positions x hd / 2], bias int16 and bias_shifts uint8 [(heads + 2 kv_heads) hd] or
+        None, norm a HeadNorm or None.  Returns q_out, the rotated queries; it may be q
+        itself.  include/myl_hip.h states the arithmetic."""
+        what = "kv_append_paged_dev"
+        if (rope_frac | q_frac | k_frac | v_frac) >> 8:
+            _need_bytes(what, rope_frac=rope_frac, q_frac=q_frac, k_frac=k_frac, v_frac=v_frac)
+        R, H, hd = q.shape
+        KH, page = k_pages.shape[1:3]
+        dev = q.device
+        if not (k.shape == v.shape == (R, KH, hd) and k_pages.shape[3] == hd):
+            raise ValueError(f"{what}: q [rows x heads x hd], k and v [rows x kv_heads x hd], pages of those heads")
+        strides = self._pages_of(what, k_pages, v_pages, tables)
+        _need_dev(what, dev, q=(q, "int16", None), k=(k, "int16", None), v=(v, "int16", None), k_pages=(k_pages, "int16", None),
+                  positions=(positions, "int32", (R,)), cos_lut=(cos_lut, "int16", (cos_lut.shape[0], hd // 2)),
+                  sin_lut=(sin_lut, "int16", cos_lut.shape))
+        if seqs is not None:
+            _need_dev(what, dev, seqs=(seqs, "int32", (R,)))
+        if (bias is None) != (bias_shifts is None):
+            raise ValueError(f"{what}: bias and bias_shifts go together")
+        if bias is not None:
+            n = ((H + 2 * KH) * hd,)
+            _need_dev(what, dev, bias=(bias, "int16", n), bias_shifts=(bias_shifts, "uint8", n))
+        if norm is not None and (norm.device != dev or norm.head_dim != hd):
+            raise ValueError(f"{what}: norm must be of head_dim values on {dev}")
+        stream = self._other_stream(dev) if q_out is None else None
+        if q_out is None:
+            q_out = self._empty((R, H, hd), "int16", dev, stream)
+        _need_dev(what, dev, q_out=(q_out, "int16", None))
+        if q_out.shape != q.shape:
+            raise ValueError(f"{what}: q_out must have q's shape")
+        ldq, ldo = self._rows_of(what, "q", q, H * hd), self._rows_of(what, "q_out", q_out, H * hd)
+        ldk, ldv = self._rows_of(what, "k", k, KH * hd), self._rows_of(what, "v", v, KH * hd)
+        self._need_here(what, dev)
+        if stream is not None:
+            self._after_last_use(what, dev, stream)
+        rc = lib().myl_kv_append_paged_dev(
+            self._h, q.data_ptr(), ldq, k.data_ptr(), ldk, v.data_ptr(), ldv, R, H, KH, hd,
+            None if bias is None else bias.data_ptr(), None if bias is None else bias_shifts.data_ptr(), q_frac, k_frac, v_frac,
+            None if norm is None else C.byref(norm.args), cos_lut.data_ptr(), sin_lut.data_ptr(), cos_lut.numel(), rope_frac,
+            positions.data_ptr(), None if seqs is None else seqs.data_ptr(), tables.data_ptr(), tables.shape[0], tables.shape[1],
+            strides[3], k_pages.data_ptr(), v_pages.data_ptr(), k_pages.shape[0], page, *strides[:3], q_out.data_ptr(), ldo)
+        if rc:
+            self.check(rc, what)
+        return q_out
+
+    def attention_paged_workspace(self, q, k_pages, max_len: int, rows_per_seq: int = 1):
+        """A workspace for attention_paged_dev on operands of these shapes, and on fewer rows or keys."""
+        n = lib().myl_attention_paged_workspace(self._h, q.shape[0] // max(1, rows_per_seq), rows_per_seq, q.shape[1],
+                                                k_pages.shape[1], q.shape[2], max_len)
+        return self._new_workspace(n, q.device, "attention_paged_dev")
+
+    def attention_paged_dev(self, q, k_pages, v_pages, tables, lens, score_mult: int, score_shift: int, exp_lut, lut_shift: int,
+                            prob_frac: int, rows_per_seq: int = 1, max_len=None, out=None, workspace=None):
+        """Attention of each sequence's newest rows over a paged cache, int16 throughout: q
+        and out [rows x heads x hd], rows_per_seq rows of each sequence in turn; k_pages
+        and v_pages [pages x kv_heads x page_size x hd] (any strides between positions,
+        heads and pages); tables int32 [sequences x pages of each].  Row r attends the first
+        lens[r] positions of its sequence (at most max_len, by default all that the table
+        names) that lie on a page; without any its output is zero.  include/myl_hip.h
+        states the arithmetic."""
+        what = "attention_paged_dev"
+        if (score_shift | lut_shift | prob_frac) >> 8:
+            _need_bytes(what, score_shift=score_shift, lut_shift=lut_shift, prob_frac=prob_frac)
+        if not -2**63 <= score_mult < 2**63:
+            raise ValueError(f"{what}: score_mult must be an int64, not {score_mult}")
+        R, H, hd = q.shape
+        n_pages, KH, page = k_pages.shape[:3]
+        dev = q.device
+        if k_pages.shape[3] != hd:
+            raise ValueError(f"{what}: pages of q's head_dim")
+        strides = self._pages_of(what, k_pages, v_pages, tables)
+        n_seqs, table_len = tables.shape
+        if rows_per_seq <= 0 or R != n_seqs * rows_per_seq:
+            raise ValueError(f"{what}: rows_per_seq rows for each of the tables' sequences")
+        most = table_len * page
+        if max_len is None:
+            max_len = most
+        elif not 0 <= max_len <= most:
+            raise ValueError(f"{what}: max_len is at most what the tables name")
+        _need_dev(what, dev, q=(q, "int16", None), k_pages=(k_pages, "int16", None), lens=(lens, "int32", (R,)),
+                  exp_lut=(exp_lut, "int16", (exp_lut.numel(),)))
+        stream = self._other_stream(dev) if out is None or workspace is None else None
+        if out is None:
+            out = self._empty((R, H, hd), "int16", dev, stream)
+        _need_dev(what, dev, out=(out, "int16", None))
+        if out.shape != q.shape:
+            raise ValueError(f"{what}: out must have q's shape")
+        ldq, ldo = self._rows_of(what, "q", q, H * hd), self._rows_of(what, "out", out, H * hd)
+        self._need_here(what, dev)
+        ws = self._workspace(dev, workspace, stream, lib().myl_attention_paged_workspace, n_seqs, rows_per_seq, H, KH, hd, max_len)
+        if stream is not None:
+            self._after_last_use(what, dev, stream)
+        rc = lib().myl_attention_paged_dev(
+            self._h, q.data_ptr(), n_seqs, rows_per_seq, ldq, H, KH, hd, k_pages.data_ptr(), v_pages.data_ptr(), n_pages, page,
+            *strides[:3], tables.data_ptr(), table_len, strides[3], lens.data_ptr(), max_len, score_mult, score_shift,
+            exp_lut.data_ptr(), exp_lut.numel(), lut_shift, prob_frac, out.data_ptr(), ldo, ws.data_ptr(),
+            ws.numel() * ws.element_size())
+        if rc:
+            self.check(rc, what)
+        return out
+
+    def logprobs_workspace(self, logits, exp_lut, top_n: int = 0):
+        """A workspace for logprobs_dev on operands of these shapes, and on smaller ones."""
+        n = lib().myl_logprobs_workspace(self._h, logits.shape[0], logits.shape[1], top_n, exp_lut.numel())
+        return self._new_workspace(n, logits.device, "logprobs_dev")
+
+    def logprobs_dev(self, logits, tokens, exp_lut, top_n: int = 0, logprobs=None, entropy=None, top_tokens=None, top_logprobs=None,
+                     workspace=None):
+        """Log probabilities of given tokens, entropy and the top_n most likely alternatives
+        of logit rows, Q16 int64: logits int32 [rows x V], tokens int64 [rows] or
+        [rows x n] (one outside the vocabulary gives 0), exp_lut int16.  Returns
+        (logprobs of tokens' shape, entropy [rows], top_tokens and top_logprobs
+        [rows x top_n]); include/myl_hip.h states the arithmetic."""
+        what = "logprobs_dev"
+        R, V = logits.shape
+        dev = logits.device
+        T = tokens.shape[1] if tokens.dim() == 2 else 1
+        if tokens.dim() not in (1, 2):
+            raise ValueError(f"{what}: tokens must be [rows] or [rows x n]")
+        if top_n < 0:
+            raise ValueError(f"{what}: top_n must not be negative")
+        _need_dev(what, dev, logits=(logits, "int32", None), tokens=(tokens, "int64", (R, *tokens.shape[1:])),
+                  exp_lut=(exp_lut, "int16", (exp_lut.numel(),)))
+        ldz, one = _strides(logits)
+        if one not in (None, 1):
+            raise ValueError(f"{what}: the logits of a row follow one another")
+        ldz = _apart(what, "logits", ldz, V)
+        left_out = logprobs is None or entropy is None or top_tokens is None or top_logprobs is None
+        stream = self._other_stream(dev) if left_out or workspace is None else None
+        if logprobs is None:
+            logprobs = self._empty(tokens.shape, "int64", dev, stream)
+        if entropy is None:
+            entropy = self._empty(R, "int64", dev, stream)
+        if top_tokens is None:
+            top_tokens = self._empty((R, top_n), "int64", dev, stream)
+        if top_logprobs is None:
+            top_logprobs = self._empty((R, top_n), "int64", dev, stream)
+        _need_dev(what, dev, logprobs=(logprobs, "int64", tokens.shape), entropy=(entropy, "int64", (R,)),
+                  top_tokens=(top_tokens, "int64", (R, top_n)), top_logprobs=(top_logprobs, "int64", (R, top_n)))
+        self._need_here(what, dev)
+        ws = self._workspace(dev, workspace, stream, lib().myl_logprobs_workspace, R, V, top_n, exp_lut.numel())
+        if stream is not None:
+            self._after_last_use(what, dev, stream)
+        rc = lib().myl_logprobs_dev(
+            self._h, logits.data_ptr(), R, V, ldz, exp_lut.data_ptr(), exp_lut.numel(), tokens.data_ptr(), T, top_n,
+            logprobs.data_ptr(), entropy.data_ptr(), top_tokens.data_ptr(), top_logprobs.data_ptr(), ws.data_ptr(),
+            ws.numel() * ws.element_size())
+        if rc:
+            self.check(rc, what)
+        return logprobs, entropy, top_tokens, top_logprobs

@@ -34,6 +34,9 @@ SOURCES = {  # source -> is HIP device code
     "adapters.hip": True,
     "prefix_attn.hip": True,
     "verify.hip": True,
+    "paged_append.hip": True,
+    "paged_attn.hip": True,
+    "logprobs.hip": True,
     "abi.cpp": False,
     "artifact.cpp": False,
 }

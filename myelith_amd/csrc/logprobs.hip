@@ -1,0 +1,229 @@
+// logprobs.hip -- log probabilities of given tokens, the entropy and the most likely
+// alternatives of rows of logits: myl_logprobs_dev.
+//
+// A row z has the weights of the integer log-softmax (fixed.h): e_j =
+// exp_lut[(m - z_j) << 2] with m = max z, 0 past the table; S = sum e_j.  In Q16
+//   ln p_j = (z_j - m) 2^10 - ln_q16(S)
+//   -sum p_j ln p_j = ln_q16(S) + RNE(2^10 sum e_j (m - z_j) / S)
+// so both need, of a row, how many of its values lie k below the maximum, for
+// the k that the table covers.  A block counts a chunk of a row below the chunk's own
+// maximum (logp_count_kernel), and one per row adds the chunks' counts up, each shifted by how
+// far its maximum is below the row's (logp_row_kernel).  The row is read once.
+// The n most likely tokens lie in the n tiles of 256 values whose maxima are the
+// largest (of equal ones the first): n others each hold a value before any in
+// another tile.  So the count keeps every tile's maximum, and n tiles are read again.
+#include "abi_internal.h"
+#include "ops.h"
+#include "paged_plan.h"
+#include "wave.h"
+
+#include <string>
+
+namespace myl {
+namespace {
+
+struct Logp {
+    const int32_t* z;
+    const int64_t* tokens;
+    const int16_t* lut;
+    int64_t *logprobs, *entropy, *top_tokens, *top_logprobs;  // entropy may be null
+    size_t ldz;
+    int V, T, n, chunks, tiles;
+    uint32_t bins, words;
+    // the workspace
+    int32_t* cmax;     // [rows][chunks]
+    int32_t* tmax;     // [rows][tiles]
+    uint32_t* counts;  // [rows][chunks][words]
+};
+
+constexpr int kBlk = 256, kRowThreads = 1024;
+constexpr int kQuads = kLogpChunk / (4 * kBlk);
+
+typedef int32_t RowQuad __attribute__((ext_vector_type(4), aligned(4)));
+
+constexpr uint32_t kPerLogit = 1u << (MYL_TV_EXP_INPUT_FRAC - MYL_TV_LOGIT_FRAC_BITS);  // table entries per logit step
+__device__ inline uint32_t weight_below(const Logp& a, uint32_t below) {
+    return below < a.bins ? (uint32_t)max(0, (int32_t)a.lut[below * kPerLogit]) : 0u;
+}
+// By value, then by the smaller index; neither 0 nor ~0.
+__device__ inline uint64_t max_key(int32_t v, uint32_t idx) {
+    return ((uint64_t)((uint32_t)v ^ 0x80000000u) << 32) | (uint64_t)(0x7FFFFFFFu - idx);
+}
+__device__ inline int32_t key_value(uint64_t k) { return (int32_t)((uint32_t)(k >> 32) ^ 0x80000000u); }
+__device__ inline uint32_t key_index(uint64_t k) { return 0x7FFFFFFFu - (uint32_t)k; }
+
+__global__ __launch_bounds__(kBlk) void logp_count_kernel(Logp a) {
+    extern __shared__ uint32_t cnt[];
+    __shared__ int32_t red[kBlk / 64];
+    const int c = blockIdx.x, r = blockIdx.y, tid = threadIdx.x;
+    const int32_t* z = a.z + (size_t)r * a.ldz;
+    RowQuad v[kQuads];
+    int n[kQuads];
+#pragma unroll
+    for (int q = 0; q < kQuads; ++q) {
+        const int i = c * kLogpChunk + q * 4 * kBlk + 4 * tid;
+        n[q] = min(max(a.V - i, 0), 4);
+        if (n[q] == 4) v[q] = *reinterpret_cast<const RowQuad*>(z + i);
+        else
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[q][e] = e < n[q] ? z[i + e] : INT32_MIN;
+    }
+    for (uint32_t i = tid; i < a.words * 2; i += kBlk) cnt[i] = 0;
+    int32_t mx = INT32_MIN;
+#pragma unroll
+    for (int q = 0; q < kQuads; ++q) {
+        const int32_t own = max(max(v[q][0], v[q][1]), max(v[q][2], v[q][3]));
+        mx = max(mx, own);
+        if (a.n) {
+            const int32_t top = wave_max_i32(own);
+            const int tile = (c * kLogpChunk + q * 4 * kBlk) / kLogpTile + (tid >> 6);
+            if ((tid & 63) == 0 && tile < a.tiles) a.tmax[(size_t)r * a.tiles + tile] = top;
+        }
+    }
+    mx = block_max_i32_dpp(mx, red);  // its barrier also publishes the cleared counters
+#pragma unroll
+    for (int q = 0; q < kQuads; ++q) {
+        // a value that fills the wave's quads is counted once: the lanes' adds to one counter follow one another
+        const int32_t first = __builtin_amdgcn_readfirstlane(v[q][0]);
+        if (__all(n[q] == 4 && v[q][0] == first && v[q][1] == first && v[q][2] == first && v[q][3] == first)) {
+            const uint32_t below = (uint32_t)mx - (uint32_t)first;
+            if (below < a.bins && (tid & 63) == 0) atomicAdd(&cnt[below], 256u);
+            continue;
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const uint32_t below = (uint32_t)mx - (uint32_t)v[q][e];
+            if (below < a.bins && e < n[q]) atomicAdd(&cnt[below], 1u);
+        }
+    }
+    __syncthreads();
+    // counts are at most kLogpChunk: 16 bits each
+    uint32_t* out = a.counts + ((size_t)r * a.chunks + c) * a.words;
+    for (uint32_t i = tid; i < a.words; i += kBlk) out[i] = cnt[2 * i] | (cnt[2 * i + 1] << 16);
+    if (tid == 0) a.cmax[(size_t)r * a.chunks + c] = mx;
+}
+
+// RNE(num / den) for num < 2^59, den >= 1 and num / den < 2^24, bit by bit.
+__device__ inline int64_t div_round(uint64_t num, uint64_t den) {
+    uint64_t q = 0;
+    for (int b = 23; b >= 0; --b)
+        if (num >> b >= den) {
+            num -= den << b;
+            q |= 1ull << b;
+        }
+    const uint64_t twice = 2 * num;
+    return (int64_t)(q + (twice > den || (twice == den && (q & 1)) ? 1 : 0));
+}
+
+__global__ __launch_bounds__(kRowThreads) void logp_row_kernel(Logp a) {
+    constexpr int kWaves = kRowThreads / 64;
+    __shared__ uint64_t red[2][kWaves];
+    __shared__ int64_t s_ln;
+    __shared__ uint64_t s_key[kWaves];
+    __shared__ uint64_t s_last;
+    const int r = blockIdx.x, tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
+    const int32_t* z = a.z + (size_t)r * a.ldz;
+    const int32_t* cm = a.cmax + (size_t)r * a.chunks;
+    int32_t m = INT32_MIN;
+    for (int c = lane; c < a.chunks; c += 64) m = max(m, cm[c]);
+    m = wave_max_i32(m);
+    uint64_t s = 0, moment = 0;  // below 2^35 and 2^48
+    for (int c = w; c < a.chunks; c += kWaves) {
+        const uint32_t d = (uint32_t)m - (uint32_t)cm[c];
+        if (d >= a.bins) continue;
+        const uint32_t* n = a.counts + ((size_t)r * a.chunks + c) * a.words;
+        for (uint32_t i = lane; i < a.words; i += 64) {
+            const uint32_t two = n[i], at = d + 2 * i;
+            const uint64_t e0 = (uint64_t)(two & 0xFFFFu) * weight_below(a, at), e1 = (uint64_t)(two >> 16) * weight_below(a, at + 1);
+            s += e0 + e1;
+            moment += e0 * at + e1 * (at + 1);
+        }
+    }
+    s = wave_sum_u64(s);
+    moment = wave_sum_u64(moment);
+    if (lane == 0) {
+        red[0][w] = s;
+        red[1][w] = moment;
+    }
+    __syncthreads();
+    if (w == 0) {
+        s = wave_sum_u64(lane < kWaves ? red[0][lane] : 0);
+        moment = wave_sum_u64(lane < kWaves ? red[1][lane] : 0);
+        const int64_t ln = ln_q16_of_sum(s < 1 ? 1u : s);
+        if (lane == 0) {
+            s_ln = ln;
+            if (a.entropy) a.entropy[r] = s ? ln + div_round(moment << 10, s) : 0;
+        }
+    }
+    __syncthreads();
+    const int64_t ln = s_ln;
+    for (int i = tid; i < a.T; i += kRowThreads) {
+        const int64_t t = a.tokens[(size_t)r * a.T + i];
+        a.logprobs[(size_t)r * a.T + i] = t < 0 || t >= a.V ? 0 : ((int64_t)z[t] - (int64_t)m) * 1024 - ln;
+    }
+    // the largest values one after another
+    uint64_t last = ~0ull;
+    for (int k = 0; k < a.n; ++k) {
+        uint64_t key = 0;
+        for (int i = tid; i < a.V; i += kRowThreads) {
+            const uint64_t o = max_key(z[i], (uint32_t)i);
+            if (o < last && o > key) key = o;
+        }
+        key = wave_max_u64(key);
+        if (lane == 0) s_key[w] = key;
+        __syncthreads();
+        if (w == 0) {
+            key = wave_max_u64(lane < kWaves ? s_key[lane] : 0);
+            if (lane == 0) {
+                s_last = key;
+                a.top_tokens[(size_t)r * a.n + k] = key_index(key);
+                a.top_logprobs[(size_t)r * a.n + k] = ((int64_t)key_value(key) - (int64_t)m) * 1024 - ln;
+            }
+        }
+        __syncthreads();
+        last = s_last;
+    }
+}
+
+}  // namespace
+}  // namespace myl
+
+using namespace myl;
+
+extern "C" {
+
+size_t myl_logprobs_workspace(const myl_ctx* ctx, size_t rows, size_t vocab, size_t top_n, size_t lut_len) {
+    const LogpShape s{rows, vocab, 0, top_n, lut_len};
+    return !ctx || logp_refuse(s) ? 0 : logp_plan(s).bytes;
+}
+
+int myl_logprobs_dev(myl_ctx* ctx, const int32_t* logits, size_t rows, size_t vocab, size_t ldz, const int16_t* exp_lut,
+                     size_t lut_len, const int64_t* tokens, size_t n_tokens, size_t top_n, int64_t* logprobs, int64_t* entropy,
+                     int64_t* top_tokens, int64_t* top_logprobs, void* workspace, size_t workspace_bytes) {
+    if (!ctx) return MYL_E_INVALID;
+    const char* what = "logprobs_dev";
+    auto bad = [&](const char* why) { return ctx->fail(MYL_E_INVALID, std::string(what) + ": " + why); };
+    const LogpShape s{rows, vocab, n_tokens, top_n, lut_len};
+    if (const char* why = logp_refuse(s)) return bad(why);
+    if (ldz < vocab) return bad("leading dimension too small");
+    if (rows == 0) return MYL_OK;
+    if (!logits || !exp_lut || (n_tokens && (!tokens || !logprobs)) || (top_n && (!top_tokens || !top_logprobs))) return bad("null operand");
+    const LogpPlan pl = logp_plan(s);
+    if (!workspace || workspace_bytes < pl.bytes) return bad("workspace too small (myl_logprobs_workspace)");
+    if ((uintptr_t)workspace & 15) return bad("workspace must be 16-byte aligned");
+    const DeviceGuard guard(ctx->device);
+    char* ws = static_cast<char*>(workspace);
+    Logp a{};
+    a.z = logits; a.tokens = tokens; a.lut = exp_lut;
+    a.logprobs = logprobs; a.entropy = entropy; a.top_tokens = top_tokens; a.top_logprobs = top_logprobs;
+    a.ldz = ldz; a.V = (int)vocab; a.T = (int)n_tokens; a.n = (int)top_n;
+    a.chunks = pl.chunks; a.tiles = pl.tiles; a.bins = pl.bins; a.words = pl.words;
+    a.cmax = reinterpret_cast<int32_t*>(ws + pl.off_max);
+    a.tmax = reinterpret_cast<int32_t*>(ws + pl.off_tiles);
+    a.counts = reinterpret_cast<uint32_t*>(ws + pl.off_counts);
+    logp_count_kernel<<<dim3((unsigned)pl.chunks, (unsigned)rows), kBlk, (size_t)pl.words * 8, ctx->stream>>>(a);
+    logp_row_kernel<<<(unsigned)rows, kRowThreads, 0, ctx->stream>>>(a);
+    return ctx->hip(hipGetLastError(), what);
+}
+
+}  // extern "C"

@@ -1,0 +1,126 @@
+// paged_plan.h -- what the host decides for the operators over a paged cache and
+// for log probabilities: which calls are refused, how the work is cut, how the
+// workspace is laid out (Layout, serve_plan.h).  Plain C++ with no HIP dependency:
+// a host build of it runs under AddressSanitizer and UndefinedBehaviorSanitizer
+// in the CPU tests.
+#pragma once
+
+#include "serve_plan.h"
+
+namespace myl {
+
+// ---- the pages of a cache -------------------------------------------------------
+
+// Elements of strides and addresses: pages x page stride is formed in 64 bits.
+constexpr size_t kPagedMaxStride = (size_t)1 << 40, kPagedMaxPage = 65536;
+// int32 ids; a table's places are counted in 32 bits
+constexpr size_t kPagedMaxIds = kInt;
+
+struct PagesShape {
+    size_t n_pages, page_size, page_stride, head_stride, pos_stride, n_seqs, table_len, table_stride, kv_heads, head_dim;
+};
+
+// Strides below a head vector's length are refused where they could be told from
+// others: positions, heads and pages of one would lie in one another.
+inline const char* pages_refuse(const PagesShape& s) {
+    if (s.page_size == 0 || s.page_size > kPagedMaxPage) return "pages hold 1 to 65536 positions";
+    if (s.n_pages == 0 || s.n_pages > kPagedMaxIds || s.table_len > kPagedMaxIds || s.n_seqs > kPagedMaxIds)
+        return "1 to 2^31 - 1 pages, at most 2^31 - 1 sequences and table entries";
+    if ((s.page_size > 1 && s.pos_stride < s.head_dim) || (s.kv_heads > 1 && s.head_stride < s.head_dim) ||
+        (s.n_pages > 1 && s.page_stride < s.head_dim))
+        return "page strides too small";
+    if (s.page_stride > kPagedMaxStride || s.head_stride > kPagedMaxStride || s.pos_stride > kPagedMaxStride)
+        return "page strides too large (2^40)";
+    if (s.n_seqs > 1 && s.table_stride < s.table_len) return "table stride too small";
+    if (s.table_stride > kPagedMaxStride) return "table stride too large (2^40)";
+    return nullptr;
+}
+
+// ---- appending ------------------------------------------------------------------
+
+// A thread takes 8 dimensions and the 8 they rotate with: threads of a call stay below 2^31.
+inline const char* append_refuse(size_t rows, size_t heads, size_t kv_heads, size_t head_dim) {
+    if (heads > kInt || kv_heads > kInt || kv_heads == 0) return "kv_heads must be > 0, heads and kv_heads below 2^31";
+    const size_t per_row = (heads + 2 * kv_heads) * (head_dim / 16);
+    if (per_row > kInt || rows > (kInt - 255) / per_row) return "too many rows or heads (2^31 pieces of 16 dimensions)";
+    return nullptr;
+}
+
+// ---- attention ------------------------------------------------------------------
+
+// At most 131072 keys per row: with non-negative table entries below 2^15 the exp sums
+// stay below 2^32.
+constexpr size_t kPagedMaxKeys = 131072;
+constexpr size_t kPagedMaxRows = 65535;
+constexpr size_t kPagedMaxPairs = (size_t)1 << 22;  // rows x heads
+constexpr size_t kPagedMaxLut = 32768;
+
+struct PagedShape {
+    size_t n_seqs, rows_per_seq, heads, kv_heads, head_dim, max_len;
+};
+
+inline const char* paged_refuse(const PagedShape& s) {
+    if (s.kv_heads == 0 || s.heads == 0 || s.heads % s.kv_heads) return "heads must be a multiple of kv_heads";
+    if (s.heads > kPagedMaxRows || s.n_seqs > kPagedMaxRows || s.rows_per_seq > kPagedMaxRows ||
+        s.n_seqs * s.rows_per_seq > kPagedMaxRows || s.n_seqs * s.rows_per_seq * s.heads > kPagedMaxPairs)
+        return "too many rows or heads (65535 each, 2^22 together)";
+    if (s.max_len > kPagedMaxKeys) return "more than 131072 keys per row";
+    return nullptr;
+}
+
+struct PagedPlan {
+    int keys;      // max_len rounded up to 64
+    size_t pairs;  // rows x heads
+    size_t off_z, bytes;
+};
+
+inline PagedPlan paged_plan(const PagedShape& s, int cus) {
+    PagedPlan p{};
+    Layout l;
+    p.keys = (int)((s.max_len + 63) / 64 * 64);
+    p.pairs = s.n_seqs * s.rows_per_seq * s.heads;
+    p.off_z = l.take(p.pairs * (size_t)p.keys, 4);
+    p.bytes = std::max<size_t>(l.used, 256);  // 0 stands for sizes that a call refuses
+    return p;
+}
+
+// ---- log probabilities ------------------------------------------------------------
+
+constexpr size_t kLogpMaxVocab = (size_t)1 << 20, kLogpMaxRows = 65535, kLogpMaxTokens = 65536, kLogpMaxTop = 32, kLogpMaxLut = 32768;
+constexpr int kLogpChunk = 8192, kLogpTile = 256;  // values of a row per block; per maximum that is kept
+
+struct LogpShape {
+    size_t rows, vocab, n_tokens, top_n, lut_len;
+};
+
+inline const char* logp_refuse(const LogpShape& s) {
+    if (s.vocab == 0 || s.vocab > kLogpMaxVocab) return "the vocabulary must hold 1 to 2^20 tokens";
+    if (s.rows > kLogpMaxRows || s.n_tokens > kLogpMaxTokens) return "too many rows (65535) or tokens of a row (65536)";
+    if (s.top_n > kLogpMaxTop || s.top_n > s.vocab) return "at most 32 alternatives, and as many as the vocabulary holds";
+    if (s.lut_len == 0 || s.lut_len > kLogpMaxLut) return "the exp table must hold 1 to 32768 entries";
+    return nullptr;
+}
+
+// bins: how far below its maximum a logit can lie and have a weight, at four table entries a
+// step; words: pairs of 16-bit counters for them.
+struct LogpPlan {
+    int chunks, tiles;
+    uint32_t bins, words;
+    size_t off_max, off_tiles, off_counts, bytes;
+};
+
+inline LogpPlan logp_plan(const LogpShape& s) {
+    LogpPlan p{};
+    Layout l;
+    p.chunks = (int)((s.vocab + kLogpChunk - 1) / kLogpChunk);
+    p.tiles = (int)((s.vocab + kLogpTile - 1) / kLogpTile);
+    p.bins = (uint32_t)((s.lut_len + 3) / 4);
+    p.words = (p.bins + 1) / 2;
+    p.off_max = l.take(s.rows * (size_t)p.chunks, 4);
+    p.off_tiles = l.take(s.top_n ? s.rows * (size_t)p.tiles : 0, 4);
+    p.off_counts = l.take(s.rows * (size_t)p.chunks * p.words, 4);
+    p.bytes = std::max<size_t>(l.used, 256);
+    return p;
+}
+
+}  // namespace myl
