@@ -1,7 +1,19 @@
 // paged_attn.hip -- integer attention (attention.rs:42-90 with softmax.rs:12-64) of each
-// sequence's newest rows over a paged cache: myl_attention_paged_dev.
+// sequence's newest rows over a paged cache, split over the length and joined:
+// myl_attention_paged_dev.
+//
+// A probability p_j = RNE(e_j 2^f / S) needs the exact maximum and exp sum of its whole
+// row before it is rounded, so a row is not joined from finished pieces; four launches
+// follow one another, each with a block per tile of vectors (query heads of a
+// sequence's rows that read one KV head) and range of keys:
+//   paged_qk_kernel    the scores z_j, kept, and each range's maximum
+//   paged_sum_kernel   e_j = exp_lut[(max - z_j) >> lut_shift] as 16 bits, the ranges' sums
+//   paged_pv_kernel    p_j from e_j and S, sum p_j v_j over each range
+//   paged_out_kernel   the sums over the ranges, rounded and clamped
+// Keys and values are read once each.
 #include "abi_internal.h"
 #include "attn_fixed.h"
+#include "gemm_mfma.h"
 #include "ops.h"
 #include "paged_plan.h"
 #include "wave.h"
@@ -17,76 +29,506 @@ struct PagedAttn {
     const int32_t *tables, *lens;
     const int16_t* lut;
     int16_t* out;
-    int32_t* z;  // [pair][keys]; pair = row * heads + head
+    // the workspace, for each tile: scores [keys / 4][width][4], exp values the same, maxima and
+    // sums [ranges][width], whether a range holds keys on no page [ranges], sums of p v
+    // [ranges][width][hd]
+    int32_t* z;
+    uint16_t* e;
+    int32_t *pmax, *pout, *holes;
+    uint32_t* psum;
     size_t ldq, ldo, ldt, page_stride, head_stride, pos_stride;
     int64_t mult;
-    SmallDiv n, G, page;
-    int heads, max_len, n_pages, keys;
+    ScoreScale scale;
+    SmallDiv n, G, page, kvh, tiles, ranges_d, width_d, heads_d;
+    int heads, max_len, n_pages, keys, range, ranges, width, vectors, places;
     uint32_t lut_len;
     uint8_t shift, lut_shift, prob_frac;
 };
 
-// The keys of row r, counted from position 0: at most max_len and what the table names.
-__device__ inline int keys_of(const PagedAttn& a, int r) { return min(max(a.lens[r], 0), a.max_len); }
+// A block's part of the work.
+struct Part {
+    int seq, g, v0, nv;  // KV head; first vector, vectors of the tile
+    int tile;            // among all
+    int range, j0, j1;   // keys [j0, j1) of the sequence, j1 up to the longest row's end
+    int lmin;            // the shortest row's end
+    int row0;
+};
 
-// The element offset of a position's vector in the pages, or -1: no such page.
-__device__ inline int64_t place_of(const PagedAttn& a, int seq, int pos) {
-    int off;
-    const int at = divmod(a.page, pos, off), id = a.tables[(size_t)seq * a.ldt + at];
-    return id < 0 || id >= a.n_pages ? -1 : (int64_t)((size_t)id * a.page_stride + (size_t)off * a.pos_stride);
+// The row and head of a tile's vector v (places past the last repeat it).
+__device__ inline int vector_of(const PagedAttn& a, const Part& p, int v, int& head) {
+    int h;
+    const int row = p.row0 + divmod(a.G, p.v0 + min(v, p.nv - 1), h);
+    head = p.g * (int)a.G.d + h;
+    return row;
+}
+// The keys of a row, counted from position 0.
+__device__ inline int keys_of(const PagedAttn& a, int row) { return min(max(a.lens[row], 0), a.max_len); }
+
+// False: no keys (p.tile < 0: no tile either).  lim: the keys of the lane's vector, lane % 16.
+// Blocks of the tiles that read one range follow one another on one XCD (block b runs on
+// XCD b % 8).
+__device__ inline bool part_of(const PagedAttn& a, Part& p, int& lim) {
+    int tile, rest;
+    const int q = divmod(a.tiles, (int)(blockIdx.x >> 3), tile), i = 8 * q + (int)(blockIdx.x & 7);
+    p.tile = -1;
+    if (i >= a.places) return false;
+    rest = divmod(a.ranges_d, i, p.range);
+    p.seq = divmod(a.kvh, rest, p.g);
+    p.tile = rest * (int)a.tiles.d + tile;
+    p.v0 = tile * a.width;
+    p.nv = min(a.width, a.vectors - p.v0);
+    p.row0 = p.seq * (int)a.n.d;
+    int head;
+    lim = keys_of(a, vector_of(a, p, threadIdx.x & 15, head));
+    p.j0 = p.range * a.range;
+    p.j1 = min(p.j0 + a.range, wave_max_i32(lim));
+    p.lmin = ~wave_max_i32(~lim);
+    return p.j0 < p.j1;
 }
 
-// A block per (row, head).
-template <int HD>
-__global__ __launch_bounds__(256) void paged_simple_kernel(PagedAttn a) {
-    __shared__ int32_t red[4];
-    __shared__ uint32_t s_extra[2];
-    __shared__ int16_t qs[HD];
+// The element offsets of a range's pages in LDS, kNoPage where a table names none.
+constexpr uint64_t kNoPage = ~0ull;
+__device__ inline int pages_of_range(const PagedAttn& a, const Part& p, uint64_t* tab, int* bad) {
     int rem;
-    const int row = blockIdx.y, head = blockIdx.x, tid = threadIdx.x;
-    const int seq = divmod(a.n, row, rem), g = divmod(a.G, head, rem);
-    const int L = keys_of(a, row);
-    int32_t* z = a.z + ((size_t)row * a.heads + head) * a.keys;
-    if (tid < HD) qs[tid] = a.q[(size_t)row * a.ldq + (size_t)head * HD + tid];
-    __syncthreads();
-    int32_t mx = INT32_MIN, count = 0;
-    for (int j = tid; j < L; j += 256) {
-        const int64_t at = place_of(a, seq, j);
-        if (at < 0) continue;
-        const int16_t* k = a.kp + at + (size_t)g * a.head_stride;
-        uint64_t acc = 0;
-        for (int d = 0; d < HD; ++d) acc += (uint64_t)((int64_t)qs[d] * (int64_t)k[d]);
-        z[j] = (int32_t)rshift_round64(wmul64((int64_t)acc, a.mult), a.shift);
-        mx = max(mx, z[j]);
-        ++count;
+    const int p0 = divmod(a.page, p.j0, rem), n = divmod(a.page, p.j1 - 1, rem) - p0 + 1;
+    const int32_t* t = a.tables + (size_t)p.seq * a.ldt + p0;
+    bool none = false;
+    for (int i = threadIdx.x; i < n; i += blockDim.x) {
+        const int id = t[i];
+        const bool ok = id >= 0 && id < a.n_pages;
+        none |= !ok;
+        tab[i] = ok ? (uint64_t)id * a.page_stride + (uint64_t)p.g * a.head_stride : kNoPage;
     }
-    mx = block_max_i32(mx, red);
-    const uint32_t n = block_sum_u32((uint32_t)count, (uint32_t*)red);
-    uint32_t s = 0;
-    for (int j = tid; j < L; j += 256) {
-        uint32_t e = 0;
-        if (place_of(a, seq, j) >= 0) {
-            const uint32_t i = min((uint32_t)mx - (uint32_t)z[j], 0x7FFFFFFFu) >> (a.lut_shift & 31u);
-            e = i < a.lut_len ? (uint32_t)max((int32_t)a.lut[i], 0) : 0u;
+    const bool any = __any(none);
+    if ((threadIdx.x & 63) == 0) bad[threadIdx.x >> 6] = any ? 1 : 0;
+    return p0;
+}
+// Where position j lies (one on no page: some place of the pages).
+__device__ inline size_t place_of(const PagedAttn& a, const uint64_t* tab, int p0, int j) {
+    int off;
+    const int at = divmod(a.page, j, off) - p0;
+    const uint64_t base = tab[at];
+    return (base == kNoPage ? 0 : base) + (size_t)off * a.pos_stride;
+}
+__device__ inline bool on_page(const PagedAttn& a, const uint64_t* tab, int p0, int j) {
+    int off;
+    return tab[divmod(a.page, j, off) - p0] != kNoPage;
+}
+
+__device__ inline int32_t dot_pairs(uint32_t w, uint32_t x, int32_t acc) {
+    typedef short __attribute__((ext_vector_type(2))) s2;
+    return __builtin_amdgcn_sdot2(__builtin_bit_cast(s2, w), __builtin_bit_cast(s2, x), acc, false);
+}
+__device__ inline void planes8(const uint4& x, uint32_t* h, uint32_t* l) {
+    h[0] = __builtin_amdgcn_perm(x.y, x.x, 0x07050301u);
+    h[1] = __builtin_amdgcn_perm(x.w, x.z, 0x07050301u);
+    l[0] = __builtin_amdgcn_perm(x.y, x.x, 0x06040200u) ^ 0x80808080u;
+    l[1] = __builtin_amdgcn_perm(x.w, x.z, 0x06040200u) ^ 0x80808080u;
+}
+// 16 dimensions (two 16-byte loads) as matrix operands: byte planes x = 256 hi + lo' + 128.
+__device__ inline void planes16(const uint4 (&x)[2], v4i32_t& h, v4i32_t& l) {
+    uint32_t hw[4], lw[4];
+    planes8(x[0], hw, lw);
+    planes8(x[1], hw + 2, lw + 2);
+    h = v4i32_t{(int)hw[0], (int)hw[1], (int)hw[2], (int)hw[3]};
+    l = v4i32_t{(int)lw[0], (int)lw[1], (int)lw[2], (int)lw[3]};
+}
+
+// Scores on v_mfma_i32_16x16x64_i8: K positions are rows, vectors columns, so lane l holds
+// vector l % 16 and positions 4 (l / 16) .. + 3 of a 16-position group.  With byte
+// planes x = 256 hi + lo' + 128 of both operands
+//   q.k = 65536 hh + 256 (hl + lh + 128 sum k_hi) + ll + 128 sum k_lo' + 128 sum q
+// where the sums over k come from the matrix cores too (a B operand of 64s, doubled)
+// and start the accumulators.  As 256 u + r the score takes 32-bit steps (ScoreScale);
+// other scales take the 64-bit form (FAST false).  K rows come in whole lines and reach the
+// operands' lanes through the wave's own LDS, chunk x of row r at x ^ (r % CH): in order
+// within a wave, so without a barrier.
+constexpr int kQkGroups = 2;  // 16-position groups of a wave and step
+template <int HD, bool FAST>
+__global__ __launch_bounds__(256) void paged_qk_kernel(PagedAttn a) {
+    constexpr int NS = HD / 64, GU = kQkGroups, CH = HD / 8, NI = CH / 4, ROWS = 64 / CH;
+    extern __shared__ __align__(16) uint64_t tab[];
+    __shared__ __align__(16) int8_t klds[4 * GU * 32 * HD];
+    __shared__ int32_t red[4][16];
+    __shared__ int bad[4];
+    Part p;
+    int lim;
+    if (!part_of(a, p, lim)) return;
+    const int tid = threadIdx.x, lane = tid & 63, c = lane & 15, kb = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int p0 = pages_of_range(a, p, tab, bad);
+    if (tid / CH < 16) {  // the vectors in whole lines, into the K rows' place
+        const int v = tid / CH;
+        int head;
+        const int row = vector_of(a, p, v, head);
+        const uint4 x = *reinterpret_cast<const uint4*>(a.q + (size_t)row * a.ldq + (size_t)head * HD + 8 * (tid % CH));
+        *reinterpret_cast<uint4*>(klds + v * 2 * HD + (((tid % CH) ^ (v & (CH - 1))) << 4)) = x;
+    }
+    __syncthreads();
+    const bool holes = (bad[0] | bad[1] | bad[2] | bad[3]) != 0;
+    const int krow = lane / CH, kch = lane % CH;
+    int8_t* const kl_w = klds + wave * GU * 32 * HD;
+    uint4 kx[GU][NI];
+    auto load = [&](int j) {
+#pragma unroll
+        for (int g = 0; g < GU; ++g)
+#pragma unroll
+            for (int i = 0; i < NI; ++i) {
+                const int at = min(j + 64 * g + i * ROWS + krow, p.j1 - 1);
+                kx[g][i] = *reinterpret_cast<const uint4*>(a.kp + place_of(a, tab, p0, at) + 8 * kch);
+            }
+    };
+    int j = p.j0 + 16 * wave;
+    load(j);
+    v4i32_t qh[NS], ql[NS];
+    int32_t qsum = 0;
+#pragma unroll
+    for (int s = 0; s < NS; ++s) {
+        uint4 x[2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+            x[i] = *reinterpret_cast<const uint4*>(klds + c * 2 * HD + (((8 * s + 2 * kb + i) ^ (c & (CH - 1))) << 4));
+        planes16(x, qh[s], ql[s]);
+        const uint32_t w[8] = {x[0].x, x[0].y, x[0].z, x[0].w, x[1].x, x[1].y, x[1].z, x[1].w};
+#pragma unroll
+        for (int i = 0; i < 8; ++i) qsum = dot_pairs(w[i], 0x00010001u, qsum);
+    }
+    qsum += __shfl_xor(qsum, 16, 64);
+    qsum = 128 * (qsum + __shfl_xor(qsum, 32, 64));
+    __syncthreads();  // the vectors are read
+    const v4i32_t sixty4 = {0x40404040, 0x40404040, 0x40404040, 0x40404040}, zero = {0, 0, 0, 0};
+    int32_t* const zt = a.z + (size_t)p.tile * a.width * a.keys + 4 * (kb * a.width + c);
+    int32_t best = INT32_MIN;
+    for (; j < p.j1; j += 64 * GU) {
+#pragma unroll
+        for (int g = 0; g < GU; ++g)
+#pragma unroll
+            for (int i = 0; i < NI; ++i) {
+                const int row = i * ROWS + krow;
+                *reinterpret_cast<uint4*>(kl_w + g * 32 * HD + row * 2 * HD + ((kch ^ (row & (CH - 1))) << 4)) = kx[g][i];
+            }
+        load(j + 64 * GU);
+#pragma unroll
+        for (int g = 0; g < GU; ++g) {
+            const int jg = j + 64 * g;
+            v4i32_t kh[NS], kl[NS];
+#pragma unroll
+            for (int s = 0; s < NS; ++s) {
+                uint4 x[2];
+#pragma unroll
+                for (int i = 0; i < 2; ++i)
+                    x[i] = *reinterpret_cast<const uint4*>(kl_w + g * 32 * HD + c * 2 * HD + (((8 * s + 2 * kb + i) ^ (c & (CH - 1))) << 4));
+                planes16(x, kh[s], kl[s]);
+            }
+            v4i32_t hh = zero, mid = zero, ll = zero;
+#pragma unroll
+            for (int s = 0; s < NS; ++s) {
+                mid = __builtin_amdgcn_mfma_i32_16x16x64_i8(kh[s], sixty4, mid, 0, 0, 0);
+                ll = __builtin_amdgcn_mfma_i32_16x16x64_i8(kl[s], sixty4, ll, 0, 0, 0);
+            }
+            mid += mid;
+            ll += ll;
+#pragma unroll
+            for (int s = 0; s < NS; ++s) {
+                hh = __builtin_amdgcn_mfma_i32_16x16x64_i8(kh[s], qh[s], hh, 0, 0, 0);
+                mid = __builtin_amdgcn_mfma_i32_16x16x64_i8(kh[s], ql[s], mid, 0, 0, 0);
+                mid = __builtin_amdgcn_mfma_i32_16x16x64_i8(kl[s], qh[s], mid, 0, 0, 0);
+                ll = __builtin_amdgcn_mfma_i32_16x16x64_i8(kl[s], ql[s], ll, 0, 0, 0);
+            }
+            int32_t z[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const int32_t lo = ll[i] + qsum;
+                const int32_t u = 256 * hh[i] + mid[i] + (lo >> 8);
+                const uint32_t r = (uint32_t)lo & 255u;
+                z[i] = FAST ? a.scale(u, r) : (int32_t)rshift_round64(wmul64(256 * (int64_t)u + (int64_t)r, a.mult), a.shift);
+                bool ok = jg + 4 * kb + i < lim;
+                if (holes) ok = ok && jg + 4 * kb + i < p.j1 && on_page(a, tab, p0, min(jg + 4 * kb + i, p.j1 - 1));
+                best = ok ? max(best, z[i]) : best;
+            }
+            if (jg < p.j1 && c < a.width) *reinterpret_cast<int4*>(zt + (size_t)jg * a.width) = make_int4(z[0], z[1], z[2], z[3]);
         }
-        z[j] = (int32_t)e;
-        s += e;
     }
-    s = block_sum_u32(s, (uint32_t*)red);
-    if (tid == 0 && n) udivmod32(1u << a.prob_frac, n, recip32(n), &s_extra[0], &s_extra[1]);
+    best = max(best, __shfl_xor(best, 16, 64));
+    best = max(best, __shfl_xor(best, 32, 64));
+    if (kb == 0) red[wave][c] = best;
     __syncthreads();
-    if (tid >= HD) return;
-    const ProbDiv div = ProbDiv::of(s ? s : 1u, a.prob_frac);
-    int64_t acc = 0;
-    uint32_t seen = 0;
-    for (int j = 0; j < L; ++j) {
-        const int64_t at = place_of(a, seq, j);
-        if (at < 0) continue;
-        const uint32_t p = s ? div((uint32_t)z[j]) : s_extra[0] + (seen < s_extra[1] ? 1u : 0u);
-        ++seen;
-        acc += (int64_t)p * a.vp[at + (size_t)g * a.head_stride + tid];
+    const size_t at = (size_t)p.tile * a.ranges + p.range;
+    if (tid < a.width) a.pmax[at * a.width + tid] = max(max(red[0][tid], red[1][tid]), max(red[2][tid], red[3][tid]));
+    if (tid == 0) a.holes[at] = holes ? 1 : 0;
+}
+
+// The lane's vector and groups of four keys: c = tid % width, the groups tid / width and on.
+struct Lanes {
+    int c, k, step;  // step 0: the thread has none
+    __device__ static inline Lanes of(const PagedAttn& a) {
+        Lanes l;
+        int rem;
+        l.step = divmod(a.width_d, 256, rem);
+        l.k = divmod(a.width_d, (int)threadIdx.x, l.c);
+        if (l.k >= l.step) l.step = 0;
+        return l;
     }
-    a.out[(size_t)row * a.ldo + (size_t)head * HD + tid] = clamp_i16_i64(rshift_round64(acc, a.prob_frac));
+};
+
+__device__ inline int lim_of(const PagedAttn& a, const Part& p, int v) {
+    int head;
+    return keys_of(a, vector_of(a, p, v, head));
+}
+
+// e_j and their sums.  A few LDS lookups per four keys: bound by the latency of a launch and of
+// reading the scores.
+constexpr uint32_t kSumLut = 8192;  // entries in LDS
+__global__ __launch_bounds__(256) void paged_sum_kernel(PagedAttn a) {
+    extern __shared__ __align__(16) uint64_t tab[];
+    __shared__ uint16_t lut[kSumLut + 1];
+    __shared__ int32_t s_max[16];
+    __shared__ uint32_t s_sum[16];
+    __shared__ int bad[4];
+    Part p;
+    int lane_lim;
+    if (!part_of(a, p, lane_lim)) return;
+    const int tid = threadIdx.x;
+    const Lanes l = Lanes::of(a);
+    const int lim = lim_of(a, p, l.c);
+    const size_t at = (size_t)p.tile * a.ranges;
+    const bool holes = __builtin_amdgcn_readfirstlane(a.holes[at + p.range]) != 0;
+    int p0 = 0;
+    if (holes) p0 = pages_of_range(a, p, tab, bad);
+    if (tid < 16) {
+        s_max[tid] = INT32_MIN;
+        s_sum[tid] = 0;
+    }
+    const uint32_t have = min(a.lut_len, kSumLut);
+    for (uint32_t i = tid; i <= have; i += 256) lut[i] = i < have ? (uint16_t)max((int32_t)a.lut[i], 0) : (uint16_t)0;
+    __syncthreads();
+    int32_t m = INT32_MIN;
+    if (l.step)
+        for (int r = l.k; r < a.ranges && r * a.range < lim; r += l.step) m = max(m, a.pmax[(at + r) * a.width + l.c]);
+    if (l.step) atomicMax(&s_max[l.c], m);
+    __syncthreads();
+    m = s_max[l.c];
+    uint32_t s = 0;
+    const size_t base = (size_t)p.tile * a.width * a.keys;
+    if (l.step)
+        for (int k = (p.j0 >> 2) + l.k; 4 * k < p.j1; k += l.step) {
+            const size_t o = base + ((size_t)k * a.width + l.c) * 4;
+            const int4 z4 = *reinterpret_cast<const int4*>(a.z + o);
+            const int32_t z[4] = {z4.x, z4.y, z4.z, z4.w};
+            uint32_t e[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                // sat_sub and the lookup of softmax.rs:12-38
+                const uint32_t below = min((uint32_t)m - (uint32_t)z[i], 0x7FFFFFFFu) >> (a.lut_shift & 31u);
+                uint32_t v = lut[min(below, have)];
+                if (below >= have && below < a.lut_len) v = (uint32_t)max((int32_t)a.lut[below], 0);
+                bool ok = 4 * k + i < lim;
+                if (holes) ok = ok && on_page(a, tab, p0, min(4 * k + i, p.j1 - 1));
+                e[i] = ok ? v : 0u;
+                s += e[i];
+            }
+            *reinterpret_cast<uint2*>(a.e + o) = make_uint2(e[0] | (e[1] << 16), e[2] | (e[3] << 16));
+        }
+    if (l.step) atomicAdd(&s_sum[l.c], s);
+    __syncthreads();
+    if (tid < a.width) a.psum[(at + p.range) * a.width + tid] = s_sum[tid];
+}
+
+// S = 0: every key that is there has the same share (softmax.rs:42-48), the first ones a unit
+// more.  base and extra of a row of lim keys; before: its keys in front of the range.
+struct Uniform {
+    uint32_t base, extra, before;
+};
+__device__ inline Uniform uniform_of(const PagedAttn& a, const Part& p, int lim) {
+    const int32_t* t = a.tables + (size_t)p.seq * a.ldt;
+    uint32_t n = 0, before = 0;
+    for (int i = 0; i * (int)a.page.d < lim; ++i) {
+        if (t[i] < 0 || t[i] >= a.n_pages) continue;
+        const int first = i * (int)a.page.d;
+        n += (uint32_t)min((int)a.page.d, lim - first);
+        before += (uint32_t)min(max(p.j0 - first, 0), (int)a.page.d);
+    }
+    Uniform u{0, 0, before};
+    if (n) udivmod32(1u << a.prob_frac, n, recip32(n), &u.base, &u.extra);
+    return u;
+}
+
+// sum p_j v_j of a tile's vectors over a range.  A lane holds 8 dimensions of two neighbouring
+// keys, paired for v_dot2 (p <= 2^14 fits a signed 16-bit half), and the pair's p of every
+// vector comes from LDS.  W: 8 or 16 vectors at most.
+constexpr int kPvStep = 128;  // keys of a block's step
+template <int HD, int W>
+__global__ __launch_bounds__(256) void paged_pv_kernel(PagedAttn a) {
+    constexpr int CH = HD / 8, ROWS = 64 / CH, NI = kPvStep / 4 / 2 / ROWS;  // pairs of a wave's step per lane
+    extern __shared__ __align__(16) uint64_t tab[];
+    __shared__ __align__(16) uint32_t ps[kPvStep / 2][W];
+    __shared__ int32_t sums[W][HD];
+    __shared__ uint32_t s_sum[16];
+    __shared__ int bad[4];
+    Part p;
+    int lane_lim;
+    const bool some = part_of(a, p, lane_lim);
+    if (!some && (p.tile < 0 || a.ranges > 1)) return;
+    if (!some) {  // the only range has no key
+        for (int i = threadIdx.x; i < p.nv * HD; i += 256) {
+            int head;
+            const int row = vector_of(a, p, i / HD, head);
+            a.out[(size_t)row * a.ldo + (size_t)head * HD + i % HD] = 0;
+        }
+        return;
+    }
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const Lanes l = Lanes::of(a);
+    const int lim = lim_of(a, p, l.c);
+    const size_t at = (size_t)p.tile * a.ranges;
+    const int p0 = pages_of_range(a, p, tab, bad);
+    if (tid < 16) s_sum[tid] = 0;
+    for (int i = tid; i < W * HD; i += 256) sums[i / HD][i % HD] = 0;
+    for (int i = tid; i < kPvStep / 2 * W; i += 256) ps[i / W][i % W] = 0;  // vectors past the width stay 0
+    __syncthreads();
+    const bool holes = (bad[0] | bad[1] | bad[2] | bad[3]) != 0;
+    uint32_t s = 0;
+    if (l.step)
+        for (int r = l.k; r < a.ranges && r * a.range < lim; r += l.step) s += a.psum[(at + r) * a.width + l.c];
+    if (l.step && s) atomicAdd(&s_sum[l.c], s);
+    const int krow = lane / CH, kch = lane % CH;
+    uint4 vx[NI][2];
+    auto load = [&](int j) {
+#pragma unroll
+        for (int i = 0; i < NI; ++i)
+#pragma unroll
+            for (int b = 0; b < 2; ++b) {
+                const int key = min(j + 2 * ((wave * NI + i) * ROWS + krow) + b, p.j1 - 1);
+                vx[i][b] = *reinterpret_cast<const uint4*>(a.vp + place_of(a, tab, p0, key) + 8 * kch);
+            }
+    };
+    load(p.j0);
+    __syncthreads();
+    s = s_sum[l.c];
+    const ProbDiv div = ProbDiv::of(s ? s : 1u, a.prob_frac);
+    Uniform uni{0, 0, 0};
+    if (s == 0 && l.step) uni = uniform_of(a, p, lim);
+    int32_t acc[W][8];
+#pragma unroll
+    for (int v = 0; v < W; ++v)
+#pragma unroll
+        for (int d = 0; d < 8; ++d) acc[v][d] = 0;
+    const uint16_t* et = a.e + (size_t)p.tile * a.width * a.keys;
+    for (int j = p.j0; j < p.j1; j += kPvStep) {
+        if (l.step)
+            for (int k = l.k; k < kPvStep / 4; k += l.step) {
+                uint2 two = make_uint2(0, 0);
+                const int key = j + 4 * k;
+                if (key < p.j1) {
+                    const uint2 x = *reinterpret_cast<const uint2*>(et + ((size_t)(key >> 2) * a.width + l.c) * 4);
+                    two.x = div(x.x & 0xFFFFu) | (div(x.x >> 16) << 16);
+                    two.y = div(x.y & 0xFFFFu) | (div(x.y >> 16) << 16);
+                    if (s == 0) {
+                        uint32_t u[4];
+                        for (int i = 0; i < 4; ++i) {
+                            uint32_t rank = uni.before;
+                            bool ok = key + i < lim;
+                            if (holes) {
+                                ok = ok && on_page(a, tab, p0, min(key + i, p.j1 - 1));
+                                for (int b = p.j0; ok && b < key + i; ++b) rank += on_page(a, tab, p0, b) ? 1u : 0u;
+                            } else {
+                                rank += (uint32_t)(key + i - p.j0);
+                            }
+                            u[i] = ok ? uni.base + (rank < uni.extra ? 1u : 0u) : 0u;
+                        }
+                        two = make_uint2(u[0] | (u[1] << 16), u[2] | (u[3] << 16));
+                    }
+                }
+                ps[2 * k][l.c] = two.x;
+                ps[2 * k + 1][l.c] = two.y;
+            }
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < NI; ++i) {
+            const uint32_t x0[4] = {vx[i][0].x, vx[i][0].y, vx[i][0].z, vx[i][0].w}, x1[4] = {vx[i][1].x, vx[i][1].y, vx[i][1].z, vx[i][1].w};
+            uint32_t w[8];
+#pragma unroll
+            for (int d = 0; d < 4; ++d) {
+                w[2 * d] = __builtin_amdgcn_perm(x1[d], x0[d], 0x05040100u);
+                w[2 * d + 1] = __builtin_amdgcn_perm(x1[d], x0[d], 0x07060302u);
+            }
+            const uint4* pr = reinterpret_cast<const uint4*>(ps[(wave * NI + i) * ROWS + krow]);
+#pragma unroll
+            for (int v4 = 0; v4 < W / 4; ++v4) {
+                const uint4 q = pr[v4];
+                const uint32_t pv[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+                for (int v = 0; v < 4; ++v)
+#pragma unroll
+                    for (int d = 0; d < 8; ++d) acc[4 * v4 + v][d] = dot_pairs(w[d], pv[v], acc[4 * v4 + v][d]);
+            }
+        }
+        if (j + kPvStep < p.j1) load(j + kPvStep);
+        __syncthreads();
+    }
+#pragma unroll
+    for (int v = 0; v < W; ++v)
+#pragma unroll
+        for (int d = 0; d < 8; ++d) {
+            int32_t x = acc[v][d];
+#pragma unroll
+            for (int o = CH; o < 64; o <<= 1) x += __shfl_xor(x, o, 64);
+            if (krow == 0) atomicAdd(&sums[v][8 * kch + d], x);
+        }
+    __syncthreads();
+    if (a.ranges == 1) {
+        for (int i = tid; i < p.nv * HD; i += 256) {
+            int head;
+            const int row = vector_of(a, p, i / HD, head);
+            a.out[(size_t)row * a.ldo + (size_t)head * HD + i % HD] = clamp_i16(rshift_round32(sums[i / HD][i % HD], a.prob_frac));
+        }
+        return;
+    }
+    int32_t* o = a.pout + (at + p.range) * a.width * HD;
+    for (int i = tid; i < a.width * HD; i += 256) o[i] = sums[i / HD][i % HD];
+}
+
+// The ranges' sums, one rounding (attention.rs:84-86); four dimensions per thread.
+template <int HD>
+__global__ __launch_bounds__(256) void paged_out_kernel(PagedAttn a, int rows) {
+    const int i = (int)(blockIdx.x * 256u + threadIdx.x);  // row, head, four dimensions
+    constexpr int Q = HD / 4;
+    const int pair = i / Q, d = 4 * (i % Q);
+    int head, h, seq_row, g, v;
+    const int row = divmod(a.heads_d, pair, head);
+    if (row >= rows) return;
+    const int seq = divmod(a.n, row, seq_row);
+    g = divmod(a.G, head, h);
+    const int tile = divmod(a.width_d, seq_row * (int)a.G.d + h, v);
+    const int lim = keys_of(a, row);
+    const size_t at = (((size_t)seq * a.kvh.d + g) * a.tiles.d + tile) * a.ranges;
+    int64_t s[4] = {0, 0, 0, 0};
+    for (int r = 0; r < a.ranges && r * a.range < lim; ++r) {
+        const int4 x = *reinterpret_cast<const int4*>(a.pout + ((at + r) * a.width + v) * HD + d);
+        s[0] += x.x;
+        s[1] += x.y;
+        s[2] += x.z;
+        s[3] += x.w;
+    }
+    uint32_t y[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) y[k] = (uint32_t)(uint16_t)clamp_i16_i64(rshift_round64(s[k], a.prob_frac));
+    *reinterpret_cast<uint2*>(a.out + (size_t)row * a.ldo + (size_t)head * HD + d) = make_uint2(y[0] | (y[1] << 16), y[2] | (y[3] << 16));
+}
+
+template <int HD>
+hipError_t paged_launch(const PagedAttn& a, const PagedPlan& pl, int rows, hipStream_t st) {
+    if (pl.ranges) {
+        const unsigned grid = (unsigned)pl.blocks;
+        const size_t tab = ((size_t)a.range / a.page.d + 2) * 8;
+        if (a.scale.fast) paged_qk_kernel<HD, true><<<grid, 256, tab, st>>>(a);
+        else paged_qk_kernel<HD, false><<<grid, 256, tab, st>>>(a);
+        paged_sum_kernel<<<grid, 256, tab, st>>>(a);
+        if (a.width <= 8) paged_pv_kernel<HD, 8><<<grid, 256, tab, st>>>(a);
+        else paged_pv_kernel<HD, 16><<<grid, 256, tab, st>>>(a);
+    }
+    if (pl.ranges != 1) paged_out_kernel<HD><<<(unsigned)(((size_t)rows * a.heads * (HD / 4) + 255) / 256), 256, 0, st>>>(a, rows);
+    return hipGetLastError();
 }
 
 }  // namespace
@@ -133,15 +575,23 @@ int myl_attention_paged_dev(myl_ctx* ctx, const int16_t* q, size_t n_seqs, size_
     PagedAttn a{};
     a.q = q; a.kp = k_pages; a.vp = v_pages; a.tables = tables; a.lens = lens; a.lut = exp_lut; a.out = out;
     a.z = reinterpret_cast<int32_t*>(ws + pl.off_z);
+    a.e = reinterpret_cast<uint16_t*>(ws + pl.off_e);
+    a.pmax = reinterpret_cast<int32_t*>(ws + pl.off_max);
+    a.psum = reinterpret_cast<uint32_t*>(ws + pl.off_sum);
+    a.holes = reinterpret_cast<int32_t*>(ws + pl.off_holes);
+    a.pout = reinterpret_cast<int32_t*>(ws + pl.off_out);
     a.ldq = ldq; a.ldo = ldo; a.ldt = table_stride; a.page_stride = page_stride; a.head_stride = head_stride; a.pos_stride = pos_stride;
     a.mult = score_mult;
-    a.n = SmallDiv::of(rows_per_seq); a.G = SmallDiv::of(heads / kv_heads); a.page = SmallDiv::of(page_size);
+    a.scale = ScoreScale::of(score_mult, score_shift, (int)head_dim);
+    auto div = [](size_t d) { return SmallDiv::of(std::max<size_t>(d, 1)); };
+    a.n = div(rows_per_seq); a.G = div(heads / kv_heads); a.page = div(page_size); a.kvh = div(kv_heads);
+    a.tiles = div((size_t)pl.tiles); a.ranges_d = div((size_t)pl.ranges); a.width_d = div((size_t)pl.width); a.heads_d = div(heads);
     a.heads = (int)heads; a.max_len = (int)max_len; a.n_pages = (int)n_pages; a.keys = pl.keys;
+    a.range = pl.range; a.ranges = pl.ranges; a.width = pl.width; a.vectors = (int)(rows_per_seq * (heads / kv_heads));
+    a.places = (int)(n_seqs * kv_heads * (size_t)pl.ranges);
     a.lut_len = (uint32_t)lut_len; a.shift = score_shift; a.lut_shift = lut_shift; a.prob_frac = prob_frac;
-    const dim3 grid((unsigned)heads, (unsigned)(n_seqs * rows_per_seq));
-    if (head_dim == 128) paged_simple_kernel<128><<<grid, 256, 0, ctx->stream>>>(a);
-    else paged_simple_kernel<64><<<grid, 256, 0, ctx->stream>>>(a);
-    return ctx->hip(hipGetLastError(), what);
+    const int rows = (int)(n_seqs * rows_per_seq);
+    return ctx->hip(head_dim == 128 ? paged_launch<128>(a, pl, rows, ctx->stream) : paged_launch<64>(a, pl, rows, ctx->stream), what);
 }
 
 }  // extern "C"

@@ -68,18 +68,49 @@ inline const char* paged_refuse(const PagedShape& s) {
     return nullptr;
 }
 
+// The query vectors (heads of rows) that read one sequence's KV head are cut into tiles of at
+// most 16, the keys into ranges of a multiple of 64; a block takes one tile and one range.
+// Within a range of at most 2048 keys sum p |v| <= (2^14 + 2^10) 2^15 < 2^30.
+constexpr int kPagedTile = 16, kPagedMaxRange = 2048, kPagedLeastRange = 128;
+
 struct PagedPlan {
-    int keys;      // max_len rounded up to 64
-    size_t pairs;  // rows x heads
-    size_t off_z, bytes;
+    int width, tiles;   // vectors of a tile; tiles of a sequence's KV head
+    int keys;           // max_len rounded up to 64
+    int ranges, range;  // ranges of keys, keys of a range
+    size_t parts;       // sequences x KV heads x tiles
+    int64_t blocks;     // parts x ranges, the last eight filled up
+    size_t off_z, off_e, off_max, off_sum, off_holes, off_out, bytes;
 };
+
+// Blocks of a call as far as the keys allow.
+inline size_t paged_blocks(int cus) { return 4 * (size_t)cus; }
 
 inline PagedPlan paged_plan(const PagedShape& s, int cus) {
     PagedPlan p{};
-    Layout l;
+    const size_t vectors = s.rows_per_seq * (s.heads / s.kv_heads);
+    p.tiles = (int)((vectors + kPagedTile - 1) / kPagedTile);
+    p.width = p.tiles ? (int)((vectors + p.tiles - 1) / p.tiles) : 0;
+    p.parts = s.n_seqs * s.kv_heads * (size_t)p.tiles;
     p.keys = (int)((s.max_len + 63) / 64 * 64);
-    p.pairs = s.n_seqs * s.rows_per_seq * s.heads;
-    p.off_z = l.take(p.pairs * (size_t)p.keys, 4);
+    const size_t most = paged_blocks(cus);
+    if (p.parts && p.keys) {
+        const size_t want = (most + p.parts - 1) / p.parts, each = ((size_t)p.keys + want - 1) / want;
+        p.range = (int)std::min<size_t>(std::max<size_t>((each + 63) / 64 * 64, kPagedLeastRange), kPagedMaxRange);
+        p.ranges = (p.keys + p.range - 1) / p.range;
+    }
+    p.blocks = ((int64_t)s.n_seqs * (int64_t)s.kv_heads * p.ranges + 7) / 8 * 8 * p.tiles;
+    // The ranges of any smaller call: at most as many as the least range makes, and at most
+    // want = ceil(most / parts) or as many as the largest range makes.
+    const size_t vecs = p.parts * (size_t)p.width, keys = (size_t)p.keys;
+    const size_t pieces = std::min(vecs * ((keys + kPagedLeastRange - 1) / kPagedLeastRange),
+                                   vecs * (1 + (keys + kPagedMaxRange - 1) / kPagedMaxRange) + kPagedTile * most);
+    Layout l;
+    p.off_z = l.take(vecs * keys, 4);
+    p.off_e = l.take(vecs * keys, 2);
+    p.off_max = l.take(pieces, 4);
+    p.off_sum = l.take(pieces, 4);
+    p.off_holes = l.take(pieces, 4);
+    p.off_out = l.take(pieces * s.head_dim, 4);
     p.bytes = std::max<size_t>(l.used, 256);  // 0 stands for sizes that a call refuses
     return p;
 }
