@@ -115,6 +115,9 @@ __device__ inline bool on_page(const PagedAttn& a, const uint64_t* tab, int p0, 
     return tab[divmod(a.page, j, off) - p0] != kNoPage;
 }
 
+// A barrier that leaves loads in flight.
+__device__ inline void block_barrier() { asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory"); }
+
 __device__ inline int32_t dot_pairs(uint32_t w, uint32_t x, int32_t acc) {
     typedef short __attribute__((ext_vector_type(2))) s2;
     return __builtin_amdgcn_sdot2(__builtin_bit_cast(s2, w), __builtin_bit_cast(s2, x), acc, false);
@@ -134,52 +137,86 @@ __device__ inline void planes16(const uint4 (&x)[2], v4i32_t& h, v4i32_t& l) {
     l = v4i32_t{(int)lw[0], (int)lw[1], (int)lw[2], (int)lw[3]};
 }
 
+// A wave's 16-key tiles of keys or values, tile after tile straight into a ring of NB places in
+// its own LDS: key r of a tile is row r, its 16-byte chunk x at place x ^ swizzle(r).
+// Loads retire in order, so a tile has landed when only younger ones' are outstanding.
+// Pages of a multiple of 16 positions hold whole tiles: one address for the wave (ALIGNED).
+typedef __attribute__((address_space(1))) const void global_void;
+typedef __attribute__((address_space(3))) void lds_void;
+template <int HD, int NB, bool ALIGNED, bool SWIZZLE>
+struct Tiles {
+    static constexpr int CH = HD / 8, ROWS = 64 / CH, NI = 16 / ROWS, kBytes = 32 * HD;
+    const int16_t* pages;
+    int8_t* ring;
+    uint64_t lane[NI];  // ALIGNED: the lane's elements from the tile's first
+    int row, chunk;
+    __device__ inline void begin(const PagedAttn& a, const int16_t* p, int8_t* lds) {
+        pages = p;
+        ring = lds;
+        const int l = threadIdx.x & 63;
+        row = l / CH;
+        chunk = l % CH;
+#pragma unroll
+        for (int i = 0; i < NI; ++i) lane[i] = (uint64_t)(i * ROWS + row) * a.pos_stride + (uint64_t)(8 * at(i * ROWS + row, chunk));
+    }
+    __device__ static inline int at(int r, int x) { return SWIZZLE ? x ^ (r & (CH - 1)) : x; }
+    // Keys j .. j + 15 into place `slot`; those from j1 on hold anything.
+    __device__ inline void issue(const PagedAttn& a, const uint64_t* tab, int p0, int j, int j1, int slot) const {
+        int8_t* to = ring + slot * kBytes;
+        uint64_t first = 0;
+        if (ALIGNED) {
+            first = place_of(a, tab, p0, j);
+            first = ((uint64_t)__builtin_amdgcn_readfirstlane((uint32_t)(first >> 32)) << 32) | __builtin_amdgcn_readfirstlane((uint32_t)first);
+        }
+#pragma unroll
+        for (int i = 0; i < NI; ++i) {
+            const uint64_t from = ALIGNED ? first + lane[i] : place_of(a, tab, p0, min(j + i * ROWS + row, j1 - 1)) + (uint64_t)(8 * at(i * ROWS + row, chunk));
+            __builtin_amdgcn_global_load_lds((global_void*)(uintptr_t)(pages + from), (lds_void*)(to + i * 1024), 16, 0, 0);
+        }
+    }
+    // The oldest tile has landed when `left` younger ones and `other` accesses behind them remain.
+    template <int OTHER>
+    __device__ static inline void wait(int left) {
+        if (left >= NB - 1) asm volatile("s_waitcnt vmcnt(%0)" ::"n"((NB - 1) * NI + OTHER) : "memory");
+        else if (NB > 2 && left == NB - 2) asm volatile("s_waitcnt vmcnt(%0)" ::"n"((NB > 2 ? NB - 2 : 0) * NI + OTHER) : "memory");
+        else if (NB > 3 && left == NB - 3) asm volatile("s_waitcnt vmcnt(%0)" ::"n"((NB > 3 ? NB - 3 : 0) * NI + OTHER) : "memory");
+        else asm volatile("s_waitcnt vmcnt(%0)" ::"n"(OTHER) : "memory");
+    }
+};
+
 // Scores on v_mfma_i32_16x16x64_i8: K positions are rows, vectors columns, so lane l holds
-// vector l % 16 and positions 4 (l / 16) .. + 3 of a 16-position group.  With byte
+// vector l % 16 and positions 4 (l / 16) .. + 3 of a 16-position tile.  With byte
 // planes x = 256 hi + lo' + 128 of both operands
 //   q.k = 65536 hh + 256 (hl + lh + 128 sum k_hi) + ll + 128 sum k_lo' + 128 sum q
 // where the sums over k come from the matrix cores too (a B operand of 64s, doubled)
 // and start the accumulators.  As 256 u + r the score takes 32-bit steps (ScoreScale);
-// other scales take the 64-bit form (FAST false).  K rows come in whole lines and reach the
-// operands' lanes through the wave's own LDS, chunk x of row r at x ^ (r % CH): in order
-// within a wave, so without a barrier.
-constexpr int kQkGroups = 2;  // 16-position groups of a wave and step
-template <int HD, bool FAST>
+// other scales take the 64-bit form (FAST false).
+constexpr int kQkRing = 3;
+template <int HD, bool FAST, bool ALIGNED>
 __global__ __launch_bounds__(256) void paged_qk_kernel(PagedAttn a) {
-    constexpr int NS = HD / 64, GU = kQkGroups, CH = HD / 8, NI = CH / 4, ROWS = 64 / CH;
-    extern __shared__ __align__(16) uint64_t tab[];
-    __shared__ __align__(16) int8_t klds[4 * GU * 32 * HD];
+    using T = Tiles<HD, kQkRing, ALIGNED, true>;
+    constexpr int NS = HD / 64, CH = HD / 8, NB = kQkRing;
+    extern __shared__ __align__(16) int8_t lds[];  // the waves' rings, the range's pages
     __shared__ int32_t red[4][16];
     __shared__ int bad[4];
+    uint64_t* const tab = reinterpret_cast<uint64_t*>(lds + 4 * NB * T::kBytes);
     Part p;
     int lim;
     if (!part_of(a, p, lim)) return;
     const int tid = threadIdx.x, lane = tid & 63, c = lane & 15, kb = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int p0 = pages_of_range(a, p, tab, bad);
-    if (tid / CH < 16) {  // the vectors in whole lines, into the K rows' place
+    // the vectors in whole lines, into the last wave's ring until they are in registers
+    int8_t* const qlds = lds + 3 * NB * T::kBytes;
+    if (tid / CH < 16) {
         const int v = tid / CH;
         int head;
         const int row = vector_of(a, p, v, head);
         const uint4 x = *reinterpret_cast<const uint4*>(a.q + (size_t)row * a.ldq + (size_t)head * HD + 8 * (tid % CH));
-        *reinterpret_cast<uint4*>(klds + v * 2 * HD + (((tid % CH) ^ (v & (CH - 1))) << 4)) = x;
+        *reinterpret_cast<uint4*>(qlds + v * 2 * HD + (((tid % CH) ^ (v & (CH - 1))) << 4)) = x;
     }
     __syncthreads();
     const bool holes = (bad[0] | bad[1] | bad[2] | bad[3]) != 0;
-    const int krow = lane / CH, kch = lane % CH;
-    int8_t* const kl_w = klds + wave * GU * 32 * HD;
-    uint4 kx[GU][NI];
-    auto load = [&](int j) {
-#pragma unroll
-        for (int g = 0; g < GU; ++g)
-#pragma unroll
-            for (int i = 0; i < NI; ++i) {
-                const int at = min(j + 64 * g + i * ROWS + krow, p.j1 - 1);
-                kx[g][i] = *reinterpret_cast<const uint4*>(a.kp + place_of(a, tab, p0, at) + 8 * kch);
-            }
-    };
-    int j = p.j0 + 16 * wave;
-    load(j);
     v4i32_t qh[NS], ql[NS];
     int32_t qsum = 0;
 #pragma unroll
@@ -187,7 +224,7 @@ __global__ __launch_bounds__(256) void paged_qk_kernel(PagedAttn a) {
         uint4 x[2];
 #pragma unroll
         for (int i = 0; i < 2; ++i)
-            x[i] = *reinterpret_cast<const uint4*>(klds + c * 2 * HD + (((8 * s + 2 * kb + i) ^ (c & (CH - 1))) << 4));
+            x[i] = *reinterpret_cast<const uint4*>(qlds + c * 2 * HD + (((8 * s + 2 * kb + i) ^ (c & (CH - 1))) << 4));
         planes16(x, qh[s], ql[s]);
         const uint32_t w[8] = {x[0].x, x[0].y, x[0].z, x[0].w, x[1].x, x[1].y, x[1].z, x[1].w};
 #pragma unroll
@@ -196,57 +233,74 @@ __global__ __launch_bounds__(256) void paged_qk_kernel(PagedAttn a) {
     qsum += __shfl_xor(qsum, 16, 64);
     qsum = 128 * (qsum + __shfl_xor(qsum, 32, 64));
     __syncthreads();  // the vectors are read
+    T tiles;
+    tiles.begin(a, a.kp, lds + wave * NB * T::kBytes);
+    const int n = max(((p.j1 - p.j0 + 15) >> 4) - wave + 3, 0) >> 2;  // the wave's tiles, every fourth
+    const int jw = p.j0 + 16 * wave;
+#pragma unroll
+    for (int t = 0; t < NB; ++t)
+        if (t < n) tiles.issue(a, tab, p0, jw + 64 * t, p.j1, t);
     const v4i32_t sixty4 = {0x40404040, 0x40404040, 0x40404040, 0x40404040}, zero = {0, 0, 0, 0};
     int32_t* const zt = a.z + (size_t)p.tile * a.width * a.keys + 4 * (kb * a.width + c);
     int32_t best = INT32_MIN;
-    for (; j < p.j1; j += 64 * GU) {
+    int slot = 0;
+    for (int t = 0; t < n; ++t) {
+        const int j = jw + 64 * t;
+        // one score store at least for each of the last NB - 1 tiles lies between
+        if (t >= NB) T::template wait<NB - 1>(n - 1 - t);
+        else T::template wait<0>(n - 1 - t);
+        const int8_t* k8 = tiles.ring + slot * T::kBytes + c * 2 * HD;
+        v4i32_t raw[NS][2];
 #pragma unroll
-        for (int g = 0; g < GU; ++g)
+        for (int s = 0; s < NS; ++s)
 #pragma unroll
-            for (int i = 0; i < NI; ++i) {
-                const int row = i * ROWS + krow;
-                *reinterpret_cast<uint4*>(kl_w + g * 32 * HD + row * 2 * HD + ((kch ^ (row & (CH - 1))) << 4)) = kx[g][i];
-            }
-        load(j + 64 * GU);
+            for (int i = 0; i < 2; ++i) raw[s][i] = *reinterpret_cast<const v4i32_t*>(k8 + (T::at(c, 8 * s + 2 * kb + i) << 4));
+        // in registers before the tile's place is loaded again
+        if (NS == 2) asm volatile("s_waitcnt lgkmcnt(0)" : "+v"(raw[0][0]), "+v"(raw[0][1]), "+v"(raw[NS - 1][0]), "+v"(raw[NS - 1][1])::"memory");
+        else asm volatile("s_waitcnt lgkmcnt(0)" : "+v"(raw[0][0]), "+v"(raw[0][1])::"memory");
+        if (t + NB < n) tiles.issue(a, tab, p0, j + 64 * NB, p.j1, slot);
+        slot = slot + 1 == NB ? 0 : slot + 1;
+        v4i32_t kh[NS], kl[NS];
 #pragma unroll
-        for (int g = 0; g < GU; ++g) {
-            const int jg = j + 64 * g;
-            v4i32_t kh[NS], kl[NS];
+        for (int s = 0; s < NS; ++s) {
+            uint4 x[2];
 #pragma unroll
-            for (int s = 0; s < NS; ++s) {
-                uint4 x[2];
+            for (int i = 0; i < 2; ++i) x[i] = make_uint4((uint32_t)raw[s][i][0], (uint32_t)raw[s][i][1], (uint32_t)raw[s][i][2], (uint32_t)raw[s][i][3]);
+            planes16(x, kh[s], kl[s]);
+        }
+        v4i32_t hh = zero, mid = zero, ll = zero;
 #pragma unroll
-                for (int i = 0; i < 2; ++i)
-                    x[i] = *reinterpret_cast<const uint4*>(kl_w + g * 32 * HD + c * 2 * HD + (((8 * s + 2 * kb + i) ^ (c & (CH - 1))) << 4));
-                planes16(x, kh[s], kl[s]);
-            }
-            v4i32_t hh = zero, mid = zero, ll = zero;
+        for (int s = 0; s < NS; ++s) {
+            mid = __builtin_amdgcn_mfma_i32_16x16x64_i8(kh[s], sixty4, mid, 0, 0, 0);
+            ll = __builtin_amdgcn_mfma_i32_16x16x64_i8(kl[s], sixty4, ll, 0, 0, 0);
+        }
+        mid += mid;
+        ll += ll;
 #pragma unroll
-            for (int s = 0; s < NS; ++s) {
-                mid = __builtin_amdgcn_mfma_i32_16x16x64_i8(kh[s], sixty4, mid, 0, 0, 0);
-                ll = __builtin_amdgcn_mfma_i32_16x16x64_i8(kl[s], sixty4, ll, 0, 0, 0);
-            }
-            mid += mid;
-            ll += ll;
+        for (int s = 0; s < NS; ++s) {
+            hh = __builtin_amdgcn_mfma_i32_16x16x64_i8(kh[s], qh[s], hh, 0, 0, 0);
+            mid = __builtin_amdgcn_mfma_i32_16x16x64_i8(kh[s], ql[s], mid, 0, 0, 0);
+            mid = __builtin_amdgcn_mfma_i32_16x16x64_i8(kl[s], qh[s], mid, 0, 0, 0);
+            ll = __builtin_amdgcn_mfma_i32_16x16x64_i8(kl[s], ql[s], ll, 0, 0, 0);
+        }
+        int32_t z[4];
 #pragma unroll
-            for (int s = 0; s < NS; ++s) {
-                hh = __builtin_amdgcn_mfma_i32_16x16x64_i8(kh[s], qh[s], hh, 0, 0, 0);
-                mid = __builtin_amdgcn_mfma_i32_16x16x64_i8(kh[s], ql[s], mid, 0, 0, 0);
-                mid = __builtin_amdgcn_mfma_i32_16x16x64_i8(kl[s], qh[s], mid, 0, 0, 0);
-                ll = __builtin_amdgcn_mfma_i32_16x16x64_i8(kl[s], ql[s], ll, 0, 0, 0);
-            }
-            int32_t z[4];
+        for (int i = 0; i < 4; ++i) {
+            const int32_t lo = ll[i] + qsum;
+            const int32_t u = 256 * hh[i] + mid[i] + (lo >> 8);
+            const uint32_t r = (uint32_t)lo & 255u;
+            z[i] = FAST ? a.scale(u, r) : (int32_t)rshift_round64(wmul64(256 * (int64_t)u + (int64_t)r, a.mult), a.shift);
+        }
+        if (c < a.width) *reinterpret_cast<int4*>(zt + (size_t)j * a.width) = make_int4(z[0], z[1], z[2], z[3]);
+        if (!holes) {
 #pragma unroll
+            for (int i = 0; i < 4; ++i) best = j + 4 * kb + i < lim ? max(best, z[i]) : best;
+        } else {
             for (int i = 0; i < 4; ++i) {
-                const int32_t lo = ll[i] + qsum;
-                const int32_t u = 256 * hh[i] + mid[i] + (lo >> 8);
-                const uint32_t r = (uint32_t)lo & 255u;
-                z[i] = FAST ? a.scale(u, r) : (int32_t)rshift_round64(wmul64(256 * (int64_t)u + (int64_t)r, a.mult), a.shift);
-                bool ok = jg + 4 * kb + i < lim;
-                if (holes) ok = ok && jg + 4 * kb + i < p.j1 && on_page(a, tab, p0, min(jg + 4 * kb + i, p.j1 - 1));
+                const int key = j + 4 * kb + i;
+                const bool ok = key < min(lim, p.j1) && on_page(a, tab, p0, min(key, p.j1 - 1));
                 best = ok ? max(best, z[i]) : best;
             }
-            if (jg < p.j1 && c < a.width) *reinterpret_cast<int4*>(zt + (size_t)jg * a.width) = make_int4(z[0], z[1], z[2], z[3]);
         }
     }
     best = max(best, __shfl_xor(best, 16, 64));
@@ -353,18 +407,39 @@ __device__ inline Uniform uniform_of(const PagedAttn& a, const Part& p, int lim)
     return u;
 }
 
-// sum p_j v_j of a tile's vectors over a range.  A lane holds 8 dimensions of two neighbouring
-// keys, paired for v_dot2 (p <= 2^14 fits a signed 16-bit half), and the pair's p of every
-// vector comes from LDS.  W: 8 or 16 vectors at most.
-constexpr int kPvStep = 128;  // keys of a block's step
-template <int HD, int W>
+// Sums over the lanes of a wave that hold the same chunk (lane % (HD / 8)) of R registers: after
+// it a lane of row rho = lane / 16 holds register 4 k + {0, 2, 1, 3}[rho] in x[k].
+template <int HD, int R>
+__device__ inline void fold_rows(int32_t (&x)[R]) {
+    if (HD == 64)
+#pragma unroll
+        for (int i = 0; i < R; ++i) x[i] += __builtin_amdgcn_mov_dpp(x[i], 0x128, 0xF, 0xF, true);  // row_ror 8
+#pragma unroll
+    for (int i = 0; i < R / 2; ++i) {
+        const auto s = __builtin_amdgcn_permlane32_swap((uint32_t)x[2 * i], (uint32_t)x[2 * i + 1], false, false);
+        x[i] = (int32_t)(s[0] + s[1]);
+    }
+#pragma unroll
+    for (int i = 0; i < R / 4; ++i) {
+        const auto s = __builtin_amdgcn_permlane16_swap((uint32_t)x[2 * i], (uint32_t)x[2 * i + 1], false, false);
+        x[i] = (int32_t)(s[0] + s[1]);
+    }
+}
+
+// sum p_j v_j of a tile's vectors over a range.  The range's p go to LDS first, pairs of keys of
+// every vector (p <= 2^14 fits a signed 16-bit half), while the first values are on
+// their way; then the values stream through the waves' rings.  A lane holds 8 dimensions
+// of two neighbouring keys, paired for v_dot2.  W: 8 or 16 vectors at most.
+constexpr int kPvRing = 3;
+template <int HD, int W, bool ALIGNED>
 __global__ __launch_bounds__(256) void paged_pv_kernel(PagedAttn a) {
-    constexpr int CH = HD / 8, ROWS = 64 / CH, NI = kPvStep / 4 / 2 / ROWS;  // pairs of a wave's step per lane
-    extern __shared__ __align__(16) uint64_t tab[];
-    __shared__ __align__(16) uint32_t ps[kPvStep / 2][W];
-    __shared__ int32_t sums[W][HD];
+    using T = Tiles<HD, kPvRing, ALIGNED, false>;
+    constexpr int CH = HD / 8, NB = kPvRing, NP = 8 * CH / 64;  // pairs of a tile per lane
+    extern __shared__ __align__(16) int8_t lds[];  // the waves' rings, the range's p, its pages
     __shared__ uint32_t s_sum[16];
     __shared__ int bad[4];
+    uint32_t* const ps = reinterpret_cast<uint32_t*>(lds + 4 * NB * T::kBytes);  // [range / 2][W]
+    uint64_t* const tab = reinterpret_cast<uint64_t*>(ps + (size_t)a.range / 2 * W);
     Part p;
     int lane_lim;
     const bool some = part_of(a, p, lane_lim);
@@ -383,151 +458,187 @@ __global__ __launch_bounds__(256) void paged_pv_kernel(PagedAttn a) {
     const size_t at = (size_t)p.tile * a.ranges;
     const int p0 = pages_of_range(a, p, tab, bad);
     if (tid < 16) s_sum[tid] = 0;
-    for (int i = tid; i < W * HD; i += 256) sums[i / HD][i % HD] = 0;
-    for (int i = tid; i < kPvStep / 2 * W; i += 256) ps[i / W][i % W] = 0;  // vectors past the width stay 0
     __syncthreads();
+    T tiles;
+    tiles.begin(a, a.vp, lds + wave * NB * T::kBytes);
+    const int n = max(((p.j1 - p.j0 + 15) >> 4) - wave + 3, 0) >> 2;
+    const int jw = p.j0 + 16 * wave;
+#pragma unroll
+    for (int t = 0; t < NB; ++t)
+        if (t < n) tiles.issue(a, tab, p0, jw + 64 * t, p.j1, t);
     const bool holes = (bad[0] | bad[1] | bad[2] | bad[3]) != 0;
     uint32_t s = 0;
     if (l.step)
         for (int r = l.k; r < a.ranges && r * a.range < lim; r += l.step) s += a.psum[(at + r) * a.width + l.c];
     if (l.step && s) atomicAdd(&s_sum[l.c], s);
-    const int krow = lane / CH, kch = lane % CH;
-    uint4 vx[NI][2];
-    auto load = [&](int j) {
-#pragma unroll
-        for (int i = 0; i < NI; ++i)
-#pragma unroll
-            for (int b = 0; b < 2; ++b) {
-                const int key = min(j + 2 * ((wave * NI + i) * ROWS + krow) + b, p.j1 - 1);
-                vx[i][b] = *reinterpret_cast<const uint4*>(a.vp + place_of(a, tab, p0, key) + 8 * kch);
-            }
-    };
-    load(p.j0);
-    __syncthreads();
+    block_barrier();
     s = s_sum[l.c];
-    const ProbDiv div = ProbDiv::of(s ? s : 1u, a.prob_frac);
-    Uniform uni{0, 0, 0};
-    if (s == 0 && l.step) uni = uniform_of(a, p, lim);
-    int32_t acc[W][8];
-#pragma unroll
-    for (int v = 0; v < W; ++v)
-#pragma unroll
-        for (int d = 0; d < 8; ++d) acc[v][d] = 0;
-    const uint16_t* et = a.e + (size_t)p.tile * a.width * a.keys;
-    for (int j = p.j0; j < p.j1; j += kPvStep) {
-        if (l.step)
-            for (int k = l.k; k < kPvStep / 4; k += l.step) {
-                uint2 two = make_uint2(0, 0);
-                const int key = j + 4 * k;
-                if (key < p.j1) {
-                    const uint2 x = *reinterpret_cast<const uint2*>(et + ((size_t)(key >> 2) * a.width + l.c) * 4);
-                    two.x = div(x.x & 0xFFFFu) | (div(x.x >> 16) << 16);
-                    two.y = div(x.y & 0xFFFFu) | (div(x.y >> 16) << 16);
-                    if (s == 0) {
-                        uint32_t u[4];
-                        for (int i = 0; i < 4; ++i) {
-                            uint32_t rank = uni.before;
-                            bool ok = key + i < lim;
-                            if (holes) {
-                                ok = ok && on_page(a, tab, p0, min(key + i, p.j1 - 1));
-                                for (int b = p.j0; ok && b < key + i; ++b) rank += on_page(a, tab, p0, b) ? 1u : 0u;
-                            } else {
-                                rank += (uint32_t)(key + i - p.j0);
-                            }
-                            u[i] = ok ? uni.base + (rank < uni.extra ? 1u : 0u) : 0u;
+    if (l.step) {
+        const ProbDiv div = ProbDiv::of(s ? s : 1u, a.prob_frac);
+        Uniform uni{0, 0, 0};
+        if (s == 0) uni = uniform_of(a, p, lim);
+        const uint16_t* et = a.e + ((size_t)p.tile * a.keys + p.j0) * a.width + 4 * l.c;
+        const int groups = (p.j1 - p.j0 + 15) / 16 * 4;
+        for (int k = l.k; k < groups; k += l.step) {
+            uint2 two = make_uint2(0, 0);
+            const int key = p.j0 + 4 * k;
+            if (key < p.j1) {
+                const uint2 x = *reinterpret_cast<const uint2*>(et + (size_t)k * 4 * a.width);
+                two.x = div(x.x & 0xFFFFu) | (div(x.x >> 16) << 16);
+                two.y = div(x.y & 0xFFFFu) | (div(x.y >> 16) << 16);
+                if (s == 0) {
+                    uint32_t u[4];
+                    for (int i = 0; i < 4; ++i) {
+                        uint32_t rank = uni.before;
+                        bool ok = key + i < lim;
+                        if (holes) {
+                            ok = ok && on_page(a, tab, p0, min(key + i, p.j1 - 1));
+                            for (int b = p.j0; ok && b < key + i; ++b) rank += on_page(a, tab, p0, b) ? 1u : 0u;
+                        } else {
+                            rank += (uint32_t)(key + i - p.j0);
                         }
-                        two = make_uint2(u[0] | (u[1] << 16), u[2] | (u[3] << 16));
+                        u[i] = ok ? uni.base + (rank < uni.extra ? 1u : 0u) : 0u;
                     }
+                    two = make_uint2(u[0] | (u[1] << 16), u[2] | (u[3] << 16));
                 }
-                ps[2 * k][l.c] = two.x;
-                ps[2 * k + 1][l.c] = two.y;
             }
-        __syncthreads();
+            ps[2 * k * W + l.c] = two.x;
+            ps[(2 * k + 1) * W + l.c] = two.y;
+        }
+    }
+    block_barrier();
+    int32_t acc[8 * W];
 #pragma unroll
-        for (int i = 0; i < NI; ++i) {
-            const uint32_t x0[4] = {vx[i][0].x, vx[i][0].y, vx[i][0].z, vx[i][0].w}, x1[4] = {vx[i][1].x, vx[i][1].y, vx[i][1].z, vx[i][1].w};
+    for (int i = 0; i < 8 * W; ++i) acc[i] = 0;
+    int slot = 0;
+    for (int t = 0; t < n; ++t) {
+        const int j = 16 * wave + 64 * t;  // from the range's first key
+        T::template wait<0>(n - 1 - t);
+        const int8_t* v8 = tiles.ring + slot * T::kBytes + 16 * tiles.chunk;
+        v4i32_t x[NP][2];
+#pragma unroll
+        for (int i = 0; i < NP; ++i)
+#pragma unroll
+            for (int b = 0; b < 2; ++b) x[i][b] = *reinterpret_cast<const v4i32_t*>(v8 + (2 * (i * T::ROWS + tiles.row) + b) * 2 * HD);
+        v4i32_t pr[NP][W / 4];
+#pragma unroll
+        for (int i = 0; i < NP; ++i)
+#pragma unroll
+            for (int v = 0; v < W / 4; ++v)
+                pr[i][v] = *reinterpret_cast<const v4i32_t*>(ps + (size_t)(j / 2 + i * T::ROWS + tiles.row) * W + 4 * v);
+        // in registers before the tile's place is loaded again
+        if (NP == 2) asm volatile("s_waitcnt lgkmcnt(0)" : "+v"(x[0][0]), "+v"(x[0][1]), "+v"(x[NP - 1][0]), "+v"(x[NP - 1][1])::"memory");
+        else asm volatile("s_waitcnt lgkmcnt(0)" : "+v"(x[0][0]), "+v"(x[0][1])::"memory");
+        if (t + NB < n) tiles.issue(a, tab, p0, jw + 64 * (t + NB), p.j1, slot);
+        slot = slot + 1 == NB ? 0 : slot + 1;
+#pragma unroll
+        for (int i = 0; i < NP; ++i) {
             uint32_t w[8];
 #pragma unroll
             for (int d = 0; d < 4; ++d) {
-                w[2 * d] = __builtin_amdgcn_perm(x1[d], x0[d], 0x05040100u);
-                w[2 * d + 1] = __builtin_amdgcn_perm(x1[d], x0[d], 0x07060302u);
+                w[2 * d] = __builtin_amdgcn_perm((uint32_t)x[i][1][d], (uint32_t)x[i][0][d], 0x05040100u);
+                w[2 * d + 1] = __builtin_amdgcn_perm((uint32_t)x[i][1][d], (uint32_t)x[i][0][d], 0x07060302u);
             }
-            const uint4* pr = reinterpret_cast<const uint4*>(ps[(wave * NI + i) * ROWS + krow]);
 #pragma unroll
-            for (int v4 = 0; v4 < W / 4; ++v4) {
-                const uint4 q = pr[v4];
-                const uint32_t pv[4] = {q.x, q.y, q.z, q.w};
+            for (int v = 0; v < W; ++v)
 #pragma unroll
-                for (int v = 0; v < 4; ++v)
-#pragma unroll
-                    for (int d = 0; d < 8; ++d) acc[4 * v4 + v][d] = dot_pairs(w[d], pv[v], acc[4 * v4 + v][d]);
-            }
+                for (int d = 0; d < 8; ++d) acc[v * 8 + d] = dot_pairs(w[d], (uint32_t)pr[i][v / 4][v % 4], acc[v * 8 + d]);
         }
-        if (j + kPvStep < p.j1) load(j + kPvStep);
-        __syncthreads();
     }
+    // the waves' sums meet in LDS, in place of the rings
+    fold_rows<HD>(acc);
+    block_barrier();
+    int32_t* const sums = reinterpret_cast<int32_t*>(lds);  // [wave][W][HD]
+    static_assert(W * HD * 4 <= NB * 32 * HD, "a wave's sums fit its ring");
+    const int rho = lane >> 4, first = rho == 1 ? 2 : rho == 2 ? 1 : rho;
+    if (HD == 128 || !(lane & 8))
 #pragma unroll
-    for (int v = 0; v < W; ++v)
-#pragma unroll
-        for (int d = 0; d < 8; ++d) {
-            int32_t x = acc[v][d];
-#pragma unroll
-            for (int o = CH; o < 64; o <<= 1) x += __shfl_xor(x, o, 64);
-            if (krow == 0) atomicAdd(&sums[v][8 * kch + d], x);
+        for (int k = 0; k < 2 * W; ++k) {
+            const int reg = 4 * k + first;
+            sums[(wave * W + (reg >> 3)) * HD + 8 * tiles.chunk + (reg & 7)] = acc[k];
         }
-    __syncthreads();
-    if (a.ranges == 1) {
-        for (int i = tid; i < p.nv * HD; i += 256) {
+    block_barrier();
+    int32_t* o = a.pout + (at + p.range) * a.width * HD;
+    for (int i = tid; i < a.width * HD; i += 256) {
+        const int32_t x = sums[i] + sums[W * HD + i] + sums[2 * W * HD + i] + sums[3 * W * HD + i];
+        if (a.ranges > 1) {
+            o[i] = x;
+        } else if (i < p.nv * HD) {
             int head;
             const int row = vector_of(a, p, i / HD, head);
-            a.out[(size_t)row * a.ldo + (size_t)head * HD + i % HD] = clamp_i16(rshift_round32(sums[i / HD][i % HD], a.prob_frac));
+            a.out[(size_t)row * a.ldo + (size_t)head * HD + i % HD] = clamp_i16(rshift_round32(x, a.prob_frac));
         }
-        return;
     }
-    int32_t* o = a.pout + (at + p.range) * a.width * HD;
-    for (int i = tid; i < a.width * HD; i += 256) o[i] = sums[i / HD][i % HD];
 }
 
-// The ranges' sums, one rounding (attention.rs:84-86); four dimensions per thread.
+// The ranges' sums, one rounding (attention.rs:84-86).  A block per row and head: four
+// dimensions and every so-many-th range per thread.
 template <int HD>
-__global__ __launch_bounds__(256) void paged_out_kernel(PagedAttn a, int rows) {
-    const int i = (int)(blockIdx.x * 256u + threadIdx.x);  // row, head, four dimensions
-    constexpr int Q = HD / 4;
-    const int pair = i / Q, d = 4 * (i % Q);
-    int head, h, seq_row, g, v;
-    const int row = divmod(a.heads_d, pair, head);
-    if (row >= rows) return;
-    const int seq = divmod(a.n, row, seq_row);
-    g = divmod(a.G, head, h);
-    const int tile = divmod(a.width_d, seq_row * (int)a.G.d + h, v);
-    const int lim = keys_of(a, row);
+__global__ __launch_bounds__(256) void paged_out_kernel(PagedAttn a) {
+    constexpr int Q = HD / 4, SHARES = 256 / Q;
+    __shared__ int64_t part[SHARES][HD];
+    int head, h, in_seq, v;
+    const int row = divmod(a.heads_d, (int)blockIdx.x, head), q = threadIdx.x % Q, share = threadIdx.x / Q;
+    const int seq = divmod(a.n, row, in_seq), g = divmod(a.G, head, h);
+    const int tile = divmod(a.width_d, in_seq * (int)a.G.d + h, v), lim = keys_of(a, row);
     const size_t at = (((size_t)seq * a.kvh.d + g) * a.tiles.d + tile) * a.ranges;
     int64_t s[4] = {0, 0, 0, 0};
-    for (int r = 0; r < a.ranges && r * a.range < lim; ++r) {
-        const int4 x = *reinterpret_cast<const int4*>(a.pout + ((at + r) * a.width + v) * HD + d);
-        s[0] += x.x;
-        s[1] += x.y;
-        s[2] += x.z;
-        s[3] += x.w;
-    }
-    uint32_t y[4];
+    const int last = min(a.ranges, (lim + a.range - 1) / max(a.range, 1));
+    for (int r0 = share; r0 < last; r0 += 4 * SHARES) {
+        int4 x[4];
 #pragma unroll
-    for (int k = 0; k < 4; ++k) y[k] = (uint32_t)(uint16_t)clamp_i16_i64(rshift_round64(s[k], a.prob_frac));
-    *reinterpret_cast<uint2*>(a.out + (size_t)row * a.ldo + (size_t)head * HD + d) = make_uint2(y[0] | (y[1] << 16), y[2] | (y[3] << 16));
+        for (int k = 0; k < 4; ++k)
+            x[k] = r0 + k * SHARES < last ? *reinterpret_cast<const int4*>(a.pout + ((at + r0 + k * SHARES) * a.width + v) * HD + 4 * q) : make_int4(0, 0, 0, 0);
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            s[0] += x[k].x;
+            s[1] += x[k].y;
+            s[2] += x[k].z;
+            s[3] += x[k].w;
+        }
+    }
+#pragma unroll
+    for (int k = 0; k < 4; ++k) part[share][4 * q + k] = s[k];
+    __syncthreads();
+    if (threadIdx.x < HD) {
+        int64_t y = 0;
+#pragma unroll
+        for (int k = 0; k < SHARES; ++k) y += part[k][threadIdx.x];
+        a.out[(size_t)row * a.ldo + (size_t)head * HD + threadIdx.x] = clamp_i16_i64(rshift_round64(y, a.prob_frac));
+    }
+}
+
+// A launch with more LDS than the 64 KiB it has by default.
+template <class K>
+hipError_t allow_lds(K kernel, size_t bytes) {
+    return bytes <= 65536 ? hipSuccess : hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+}
+
+template <int HD, bool ALIGNED>
+hipError_t paged_ranges(const PagedAttn& a, unsigned grid, hipStream_t st) {
+    const size_t tab = ((size_t)a.range / a.page.d + 2) * 8;
+    const size_t qk = 4 * kQkRing * 32 * HD + tab;
+    auto scores = a.scale.fast ? paged_qk_kernel<HD, true, ALIGNED> : paged_qk_kernel<HD, false, ALIGNED>;
+    hipError_t e = allow_lds(scores, qk);
+    if (e != hipSuccess) return e;
+    scores<<<grid, 256, qk, st>>>(a);
+    paged_sum_kernel<<<grid, 256, tab, st>>>(a);
+    const int W = a.width <= 8 ? 8 : 16;
+    const size_t pv = 4 * kPvRing * 32 * HD + (size_t)a.range * W * 2 + tab;
+    auto values = W == 8 ? paged_pv_kernel<HD, 8, ALIGNED> : paged_pv_kernel<HD, 16, ALIGNED>;
+    e = allow_lds(values, pv);
+    if (e != hipSuccess) return e;
+    values<<<grid, 256, pv, st>>>(a);
+    return hipGetLastError();
 }
 
 template <int HD>
 hipError_t paged_launch(const PagedAttn& a, const PagedPlan& pl, int rows, hipStream_t st) {
     if (pl.ranges) {
-        const unsigned grid = (unsigned)pl.blocks;
-        const size_t tab = ((size_t)a.range / a.page.d + 2) * 8;
-        if (a.scale.fast) paged_qk_kernel<HD, true><<<grid, 256, tab, st>>>(a);
-        else paged_qk_kernel<HD, false><<<grid, 256, tab, st>>>(a);
-        paged_sum_kernel<<<grid, 256, tab, st>>>(a);
-        if (a.width <= 8) paged_pv_kernel<HD, 8><<<grid, 256, tab, st>>>(a);
-        else paged_pv_kernel<HD, 16><<<grid, 256, tab, st>>>(a);
+        const hipError_t e = a.page.d % 16 == 0 ? paged_ranges<HD, true>(a, (unsigned)pl.blocks, st) : paged_ranges<HD, false>(a, (unsigned)pl.blocks, st);
+        if (e != hipSuccess) return e;
     }
-    if (pl.ranges != 1) paged_out_kernel<HD><<<(unsigned)(((size_t)rows * a.heads * (HD / 4) + 255) / 256), 256, 0, st>>>(a, rows);
+    if (pl.ranges != 1) paged_out_kernel<HD><<<(unsigned)(rows * a.heads), 256, 0, st>>>(a);
     return hipGetLastError();
 }
 

@@ -70,8 +70,8 @@ inline const char* paged_refuse(const PagedShape& s) {
 
 // The query vectors (heads of rows) that read one sequence's KV head are cut into tiles of at
 // most 16, the keys into ranges of a multiple of 64; a block takes one tile and one range.
-// Within a range of at most 2048 keys sum p |v| <= (2^14 + 2^10) 2^15 < 2^30.
-constexpr int kPagedTile = 16, kPagedMaxRange = 2048, kPagedLeastRange = 128;
+// Within a range of at most 1024 keys sum p |v| <= (2^14 + 2^9) 2^15 < 2^30.
+constexpr int kPagedTile = 16, kPagedMaxRange = 1024, kPagedLeastRange = 128;
 
 struct PagedPlan {
     int width, tiles;   // vectors of a tile; tiles of a sequence's KV head
