@@ -86,17 +86,19 @@ __device__ inline bool part_of(const PagedAttn& a, Part& p, int& lim) {
     return p.j0 < p.j1;
 }
 
-// The element offsets of a range's pages in LDS, kNoPage where a table names none.
+// The element offsets of a range's pages in LDS, kNoPage where a table names none.  The table
+// names pages up to max_len at least, so its loads need not wait for the rows' lengths.
 constexpr uint64_t kNoPage = ~0ull;
 __device__ inline int pages_of_range(const PagedAttn& a, const Part& p, uint64_t* tab, int* bad) {
     int rem;
-    const int p0 = divmod(a.page, p.j0, rem), n = divmod(a.page, p.j1 - 1, rem) - p0 + 1;
+    const int p0 = divmod(a.page, p.j0, rem);
+    const int most = divmod(a.page, min(p.j0 + a.range, a.max_len) - 1, rem) - p0 + 1, n = divmod(a.page, p.j1 - 1, rem) - p0 + 1;
     const int32_t* t = a.tables + (size_t)p.seq * a.ldt + p0;
     bool none = false;
-    for (int i = threadIdx.x; i < n; i += blockDim.x) {
+    for (int i = threadIdx.x; i < most; i += blockDim.x) {
         const int id = t[i];
         const bool ok = id >= 0 && id < a.n_pages;
-        none |= !ok;
+        none |= !ok && i < n;
         tab[i] = ok ? (uint64_t)id * a.page_stride + (uint64_t)p.g * a.head_stride : kNoPage;
     }
     const bool any = __any(none);
@@ -140,38 +142,43 @@ __device__ inline void planes16(const uint4 (&x)[2], v4i32_t& h, v4i32_t& l) {
 // A wave's 16-key tiles of keys or values, tile after tile straight into a ring of NB places in
 // its own LDS: key r of a tile is row r, its 16-byte chunk x at place x ^ swizzle(r).
 // Loads retire in order, so a tile has landed when only younger ones' are outstanding.
-// Pages of a multiple of 16 positions hold whole tiles: one address for the wave (ALIGNED).
+// Where pages hold whole tiles (ALIGNED: a multiple of 16 positions), a tile is one address for
+// the wave and 32-bit offsets of the lanes.
 typedef __attribute__((address_space(1))) const void global_void;
 typedef __attribute__((address_space(3))) void lds_void;
 template <int HD, int NB, bool ALIGNED, bool SWIZZLE>
 struct Tiles {
     static constexpr int CH = HD / 8, ROWS = 64 / CH, NI = 16 / ROWS, kBytes = 32 * HD;
-    const int16_t* pages;
+    const char* pages;
     int8_t* ring;
-    uint64_t lane[NI];  // ALIGNED: the lane's elements from the tile's first
+    uint32_t lane[NI];  // ALIGNED: the lane's bytes from the tile's first
     int row, chunk;
     __device__ inline void begin(const PagedAttn& a, const int16_t* p, int8_t* lds) {
-        pages = p;
+        pages = reinterpret_cast<const char*>(p);
         ring = lds;
         const int l = threadIdx.x & 63;
         row = l / CH;
         chunk = l % CH;
 #pragma unroll
-        for (int i = 0; i < NI; ++i) lane[i] = (uint64_t)(i * ROWS + row) * a.pos_stride + (uint64_t)(8 * at(i * ROWS + row, chunk));
+        for (int i = 0; i < NI; ++i) lane[i] = 2u * ((uint32_t)(i * ROWS + row) * (uint32_t)a.pos_stride + 8u * (uint32_t)at(i * ROWS + row, chunk));
     }
     __device__ static inline int at(int r, int x) { return SWIZZLE ? x ^ (r & (CH - 1)) : x; }
     // Keys j .. j + 15 into place `slot`; those from j1 on hold anything.
     __device__ inline void issue(const PagedAttn& a, const uint64_t* tab, int p0, int j, int j1, int slot) const {
         int8_t* to = ring + slot * kBytes;
-        uint64_t first = 0;
         if (ALIGNED) {
-            first = place_of(a, tab, p0, j);
-            first = ((uint64_t)__builtin_amdgcn_readfirstlane((uint32_t)(first >> 32)) << 32) | __builtin_amdgcn_readfirstlane((uint32_t)first);
-        }
+            const uint64_t first = place_of(a, tab, p0, j);
+            const uint64_t u = ((uint64_t)__builtin_amdgcn_readfirstlane((uint32_t)(first >> 32)) << 32) | __builtin_amdgcn_readfirstlane((uint32_t)first);
+            const char* base = pages + 2 * u;
 #pragma unroll
-        for (int i = 0; i < NI; ++i) {
-            const uint64_t from = ALIGNED ? first + lane[i] : place_of(a, tab, p0, min(j + i * ROWS + row, j1 - 1)) + (uint64_t)(8 * at(i * ROWS + row, chunk));
-            __builtin_amdgcn_global_load_lds((global_void*)(uintptr_t)(pages + from), (lds_void*)(to + i * 1024), 16, 0, 0);
+            for (int i = 0; i < NI; ++i)
+                __builtin_amdgcn_global_load_lds((global_void*)(uintptr_t)(base + lane[i]), (lds_void*)(to + i * 1024), 16, 0, 0);
+        } else {
+#pragma unroll
+            for (int i = 0; i < NI; ++i) {
+                const uint64_t from = place_of(a, tab, p0, min(j + i * ROWS + row, j1 - 1)) + (uint64_t)(8 * at(i * ROWS + row, chunk));
+                __builtin_amdgcn_global_load_lds((global_void*)(uintptr_t)(pages + 2 * from), (lds_void*)(to + i * 1024), 16, 0, 0);
+            }
         }
     }
     // The oldest tile has landed when `left` younger ones and `other` accesses behind them remain.
@@ -185,62 +192,52 @@ struct Tiles {
 };
 
 // Scores on v_mfma_i32_16x16x64_i8: K positions are rows, vectors columns, so lane l holds
-// vector l % 16 and positions 4 (l / 16) .. + 3 of a 16-position tile.  With byte
-// planes x = 256 hi + lo' + 128 of both operands
-//   q.k = 65536 hh + 256 (hl + lh + 128 sum k_hi) + ll + 128 sum k_lo' + 128 sum q
-// where the sums over k come from the matrix cores too (a B operand of 64s, doubled)
-// and start the accumulators.  As 256 u + r the score takes 32-bit steps (ScoreScale);
+// vector l % 16 and positions 4 (l / 16) .. + 3 of a 16-position tile.  The byte planes of the
+// keys are k = 256 kh + kl + 128 with kl = (k & 255) - 128; those of the queries q = 256 qh +
+// ql with ql the low byte as a signed one, which exist for q < 32640:
+//   q.k = 65536 qh kh + 256 (qh kl + ql kh) + ql kl + 128 sum q
+// with no sum over k.  A tile with a larger q takes q = 256 qh + ql + 128 too (BALANCED
+// false), for which 256 128 sum kh + 128 sum kl come from the matrix cores as well (a B operand
+// of 64s, added twice).  As 256 u + r the score takes 32-bit steps (ScoreScale);
 // other scales take the 64-bit form (FAST false).
-constexpr int kQkRing = 3;
-template <int HD, bool FAST, bool ALIGNED>
-__global__ __launch_bounds__(256) void paged_qk_kernel(PagedAttn a) {
+// Bound by issue and by the loads' latency: about 120 vector and 8 matrix instructions a tile.
+constexpr int kQkRing = 2;
+template <int HD, bool FAST, bool ALIGNED, bool BALANCED>
+__device__ inline void paged_scores(const PagedAttn& a, const Part& p, int lim, const uint64_t* tab, int p0, bool holes, int8_t* ring,
+                                    const uint4 (&qx)[HD / 64][2], int32_t* red) {
     using T = Tiles<HD, kQkRing, ALIGNED, true>;
-    constexpr int NS = HD / 64, CH = HD / 8, NB = kQkRing;
-    extern __shared__ __align__(16) int8_t lds[];  // the waves' rings, the range's pages
-    __shared__ int32_t red[4][16];
-    __shared__ int bad[4];
-    uint64_t* const tab = reinterpret_cast<uint64_t*>(lds + 4 * NB * T::kBytes);
-    Part p;
-    int lim;
-    if (!part_of(a, p, lim)) return;
-    const int tid = threadIdx.x, lane = tid & 63, c = lane & 15, kb = lane >> 4;
-    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int p0 = pages_of_range(a, p, tab, bad);
-    // the vectors in whole lines, into the last wave's ring until they are in registers
-    int8_t* const qlds = lds + 3 * NB * T::kBytes;
-    if (tid / CH < 16) {
-        const int v = tid / CH;
-        int head;
-        const int row = vector_of(a, p, v, head);
-        const uint4 x = *reinterpret_cast<const uint4*>(a.q + (size_t)row * a.ldq + (size_t)head * HD + 8 * (tid % CH));
-        *reinterpret_cast<uint4*>(qlds + v * 2 * HD + (((tid % CH) ^ (v & (CH - 1))) << 4)) = x;
-    }
-    __syncthreads();
-    const bool holes = (bad[0] | bad[1] | bad[2] | bad[3]) != 0;
-    v4i32_t qh[NS], ql[NS];
-    int32_t qsum = 0;
-#pragma unroll
-    for (int s = 0; s < NS; ++s) {
-        uint4 x[2];
-#pragma unroll
-        for (int i = 0; i < 2; ++i)
-            x[i] = *reinterpret_cast<const uint4*>(qlds + c * 2 * HD + (((8 * s + 2 * kb + i) ^ (c & (CH - 1))) << 4));
-        planes16(x, qh[s], ql[s]);
-        const uint32_t w[8] = {x[0].x, x[0].y, x[0].z, x[0].w, x[1].x, x[1].y, x[1].z, x[1].w};
-#pragma unroll
-        for (int i = 0; i < 8; ++i) qsum = dot_pairs(w[i], 0x00010001u, qsum);
-    }
-    qsum += __shfl_xor(qsum, 16, 64);
-    qsum = 128 * (qsum + __shfl_xor(qsum, 32, 64));
-    __syncthreads();  // the vectors are read
+    constexpr int NS = HD / 64, NB = kQkRing;
+    const int lane = threadIdx.x & 63, c = lane & 15, kb = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     T tiles;
-    tiles.begin(a, a.kp, lds + wave * NB * T::kBytes);
+    tiles.begin(a, a.kp, ring);
     const int n = max(((p.j1 - p.j0 + 15) >> 4) - wave + 3, 0) >> 2;  // the wave's tiles, every fourth
     const int jw = p.j0 + 16 * wave;
 #pragma unroll
     for (int t = 0; t < NB; ++t)
         if (t < n) tiles.issue(a, tab, p0, jw + 64 * t, p.j1, t);
-    const v4i32_t sixty4 = {0x40404040, 0x40404040, 0x40404040, 0x40404040}, zero = {0, 0, 0, 0};
+    v4i32_t qh[NS], ql[NS];
+    int32_t qsum = 0;
+#pragma unroll
+    for (int s = 0; s < NS; ++s) {
+        const uint32_t w[8] = {qx[s][0].x, qx[s][0].y, qx[s][0].z, qx[s][0].w, qx[s][1].x, qx[s][1].y, qx[s][1].z, qx[s][1].w};
+#pragma unroll
+        for (int i = 0; i < 8; ++i) qsum = dot_pairs(w[i], 0x00010001u, qsum);
+        if (BALANCED) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                // 128 carries into the high byte; into the upper half's too, where it is taken back
+                auto carried = [](uint32_t x) { return ((x & 0xFFFFu) + 0x80u) | (((x >> 16) + 0x80u) << 16); };
+                qh[s][i] = (int)__builtin_amdgcn_perm(carried(w[2 * i + 1]), carried(w[2 * i]), 0x07050301u);
+                ql[s][i] = (int)__builtin_amdgcn_perm(w[2 * i + 1], w[2 * i], 0x06040200u);
+            }
+        } else {
+            planes16(qx[s], qh[s], ql[s]);
+        }
+    }
+    qsum += __shfl_xor(qsum, 16, 64);
+    qsum = 128 * (qsum + __shfl_xor(qsum, 32, 64));
+    const v4i32_t sixty4 = {0x40404040, 0x40404040, 0x40404040, 0x40404040}, zero = {0, 0, 0, 0}, qs4 = {qsum, qsum, qsum, qsum};
     int32_t* const zt = a.z + (size_t)p.tile * a.width * a.keys + 4 * (kb * a.width + c);
     int32_t best = INT32_MIN;
     int slot = 0;
@@ -249,7 +246,7 @@ __global__ __launch_bounds__(256) void paged_qk_kernel(PagedAttn a) {
         // one score store at least for each of the last NB - 1 tiles lies between
         if (t >= NB) T::template wait<NB - 1>(n - 1 - t);
         else T::template wait<0>(n - 1 - t);
-        const int8_t* k8 = tiles.ring + slot * T::kBytes + c * 2 * HD;
+        const int8_t* k8 = ring + slot * T::kBytes + c * 2 * HD;
         v4i32_t raw[NS][2];
 #pragma unroll
         for (int s = 0; s < NS; ++s)
@@ -268,47 +265,86 @@ __global__ __launch_bounds__(256) void paged_qk_kernel(PagedAttn a) {
             for (int i = 0; i < 2; ++i) x[i] = make_uint4((uint32_t)raw[s][i][0], (uint32_t)raw[s][i][1], (uint32_t)raw[s][i][2], (uint32_t)raw[s][i][3]);
             planes16(x, kh[s], kl[s]);
         }
-        v4i32_t hh = zero, mid = zero, ll = zero;
+        v4i32_t hh = zero, mid = zero, ll = qs4;
+        if (!BALANCED)
+#pragma unroll
+            for (int s = 0; s < 2 * NS; ++s) {
+                mid = __builtin_amdgcn_mfma_i32_16x16x64_i8(kh[s / 2], sixty4, mid, 0, 0, 0);
+                ll = __builtin_amdgcn_mfma_i32_16x16x64_i8(kl[s / 2], sixty4, ll, 0, 0, 0);
+            }
 #pragma unroll
         for (int s = 0; s < NS; ++s) {
-            mid = __builtin_amdgcn_mfma_i32_16x16x64_i8(kh[s], sixty4, mid, 0, 0, 0);
-            ll = __builtin_amdgcn_mfma_i32_16x16x64_i8(kl[s], sixty4, ll, 0, 0, 0);
-        }
-        mid += mid;
-        ll += ll;
-#pragma unroll
-        for (int s = 0; s < NS; ++s) {
-            hh = __builtin_amdgcn_mfma_i32_16x16x64_i8(kh[s], qh[s], hh, 0, 0, 0);
             mid = __builtin_amdgcn_mfma_i32_16x16x64_i8(kh[s], ql[s], mid, 0, 0, 0);
-            mid = __builtin_amdgcn_mfma_i32_16x16x64_i8(kl[s], qh[s], mid, 0, 0, 0);
             ll = __builtin_amdgcn_mfma_i32_16x16x64_i8(kl[s], ql[s], ll, 0, 0, 0);
+            hh = __builtin_amdgcn_mfma_i32_16x16x64_i8(kh[s], qh[s], hh, 0, 0, 0);
+            mid = __builtin_amdgcn_mfma_i32_16x16x64_i8(kl[s], qh[s], mid, 0, 0, 0);
         }
         int32_t z[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            const int32_t lo = ll[i] + qsum;
-            const int32_t u = 256 * hh[i] + mid[i] + (lo >> 8);
-            const uint32_t r = (uint32_t)lo & 255u;
+            const int32_t u = 256 * hh[i] + mid[i] + (ll[i] >> 8);
+            const uint32_t r = (uint32_t)ll[i] & 255u;
             z[i] = FAST ? a.scale(u, r) : (int32_t)rshift_round64(wmul64(256 * (int64_t)u + (int64_t)r, a.mult), a.shift);
         }
         if (c < a.width) *reinterpret_cast<int4*>(zt + (size_t)j * a.width) = make_int4(z[0], z[1], z[2], z[3]);
-        if (!holes) {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) best = j + 4 * kb + i < lim ? max(best, z[i]) : best;
+        if (!holes && j + 16 <= p.lmin) {
+            best = max(best, max(max(z[0], z[1]), max(z[2], z[3])));
         } else {
             for (int i = 0; i < 4; ++i) {
                 const int key = j + 4 * kb + i;
-                const bool ok = key < min(lim, p.j1) && on_page(a, tab, p0, min(key, p.j1 - 1));
+                const bool ok = key < min(lim, p.j1) && (!holes || on_page(a, tab, p0, min(key, p.j1 - 1)));
                 best = ok ? max(best, z[i]) : best;
             }
         }
     }
     best = max(best, __shfl_xor(best, 16, 64));
     best = max(best, __shfl_xor(best, 32, 64));
-    if (kb == 0) red[wave][c] = best;
+    if (kb == 0) red[16 * wave + c] = best;
+}
+
+template <int HD, bool FAST, bool ALIGNED>
+__global__ __launch_bounds__(256, 4) void paged_qk_kernel(PagedAttn a) {
+    using T = Tiles<HD, kQkRing, ALIGNED, true>;
+    constexpr int NS = HD / 64, CH = HD / 8, NB = kQkRing;
+    extern __shared__ __align__(16) int8_t lds[];  // the waves' rings, the range's pages
+    __shared__ __align__(16) int8_t qlds[16 * 2 * HD];
+    __shared__ int32_t red[64];
+    __shared__ int bad[4], large[4];
+    uint64_t* const tab = reinterpret_cast<uint64_t*>(lds + 4 * NB * T::kBytes);
+    Part p;
+    int lim;
+    if (!part_of(a, p, lim)) return;
+    const int tid = threadIdx.x, lane = tid & 63, c = lane & 15, kb = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    // the vectors in whole lines
+    bool over = false;
+    if (tid / CH < 16) {
+        const int v = tid / CH;
+        int head;
+        const int row = vector_of(a, p, v, head);
+        const uint4 x = *reinterpret_cast<const uint4*>(a.q + (size_t)row * a.ldq + (size_t)head * HD + 8 * (tid % CH));
+        *reinterpret_cast<uint4*>(qlds + v * 2 * HD + (((tid % CH) ^ (v & (CH - 1))) << 4)) = x;
+        const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) over |= (int16_t)(w[i] & 0xFFFFu) >= 32640 || (int32_t)w[i] >> 16 >= 32640;
+    }
+    over = __any(over);
+    if (lane == 0) large[wave] = over ? 1 : 0;
+    const int p0 = pages_of_range(a, p, tab, bad);
+    __syncthreads();
+    const bool holes = (bad[0] | bad[1] | bad[2] | bad[3]) != 0;
+    uint4 qx[NS][2];
+#pragma unroll
+    for (int s = 0; s < NS; ++s)
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+            qx[s][i] = *reinterpret_cast<const uint4*>(qlds + c * 2 * HD + (((8 * s + 2 * kb + i) ^ (c & (CH - 1))) << 4));
+    int8_t* const ring = lds + wave * NB * T::kBytes;
+    if (__builtin_amdgcn_readfirstlane(large[0] | large[1] | large[2] | large[3])) paged_scores<HD, FAST, ALIGNED, false>(a, p, lim, tab, p0, holes, ring, qx, red);
+    else paged_scores<HD, FAST, ALIGNED, true>(a, p, lim, tab, p0, holes, ring, qx, red);
     __syncthreads();
     const size_t at = (size_t)p.tile * a.ranges + p.range;
-    if (tid < a.width) a.pmax[at * a.width + tid] = max(max(red[0][tid], red[1][tid]), max(red[2][tid], red[3][tid]));
+    if (tid < a.width) a.pmax[at * a.width + tid] = max(max(red[tid], red[16 + tid]), max(red[32 + tid], red[48 + tid]));
     if (tid == 0) a.holes[at] = holes ? 1 : 0;
 }
 
@@ -430,9 +466,9 @@ __device__ inline void fold_rows(int32_t (&x)[R]) {
 // every vector (p <= 2^14 fits a signed 16-bit half), while the first values are on
 // their way; then the values stream through the waves' rings.  A lane holds 8 dimensions
 // of two neighbouring keys, paired for v_dot2.  W: 8 or 16 vectors at most.
-constexpr int kPvRing = 3;
+constexpr int kPvRing = 2;
 template <int HD, int W, bool ALIGNED>
-__global__ __launch_bounds__(256) void paged_pv_kernel(PagedAttn a) {
+__global__ __launch_bounds__(256, W == 8 ? 4 : 2) void paged_pv_kernel(PagedAttn a) {
     using T = Tiles<HD, kPvRing, ALIGNED, false>;
     constexpr int CH = HD / 8, NB = kPvRing, NP = 8 * CH / 64;  // pairs of a tile per lane
     extern __shared__ __align__(16) int8_t lds[];  // the waves' rings, the range's p, its pages
@@ -608,6 +644,8 @@ __global__ __launch_bounds__(256) void paged_out_kernel(PagedAttn a) {
     }
 }
 
+constexpr size_t kAlignedStride = (size_t)1 << 26;  // 15 of them and a vector are 32 bits of bytes
+
 // A launch with more LDS than the 64 KiB it has by default.
 template <class K>
 hipError_t allow_lds(K kernel, size_t bytes) {
@@ -635,7 +673,7 @@ hipError_t paged_ranges(const PagedAttn& a, unsigned grid, hipStream_t st) {
 template <int HD>
 hipError_t paged_launch(const PagedAttn& a, const PagedPlan& pl, int rows, hipStream_t st) {
     if (pl.ranges) {
-        const hipError_t e = a.page.d % 16 == 0 ? paged_ranges<HD, true>(a, (unsigned)pl.blocks, st) : paged_ranges<HD, false>(a, (unsigned)pl.blocks, st);
+        const hipError_t e = a.page.d % 16 == 0 && a.pos_stride <= kAlignedStride ? paged_ranges<HD, true>(a, (unsigned)pl.blocks, st) : paged_ranges<HD, false>(a, (unsigned)pl.blocks, st);
         if (e != hipSuccess) return e;
     }
     if (pl.ranges != 1) paged_out_kernel<HD><<<(unsigned)(rows * a.heads), 256, 0, st>>>(a);

@@ -290,6 +290,20 @@ def test_attention_scales(backend, exp_lut, length, mult, shift, lut_shift):
     check_attention(backend, s, exp_lut)
 
 
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("top", [32639, 32640, 32767])
+def test_attention_large_queries(backend, exp_lut, hd, top):
+    """Queries about the largest whose low byte is taken as a signed one, in one vector of a tile."""
+    case(f"attention queries up to {top} hd={hd}")
+    s = attention_inputs(16, 3, 1, 6, 2, hd, 700, 16)
+    s["q"] = rng(17).integers(-32768, top + 1, s["q"].shape).astype(np.int16)
+    s["q"][:2] = np.minimum(s["q"][:2], 32000)
+    s["q"][2, 4, hd - 1] = top
+    s["kp"] = rng(18).integers(-32768, 32768, s["kp"].shape).astype(np.int16)
+    s["shift"] = 33
+    check_attention(backend, s, exp_lut)
+
+
 @pytest.mark.parametrize("length", [90, 900])
 def test_attention_tables(backend, length):
     """Exp tables: one entry, negative entries, the largest ones, all of 32768; every prob_frac."""
