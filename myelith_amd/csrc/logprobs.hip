@@ -115,28 +115,87 @@ __device__ inline int64_t div_round(uint64_t num, uint64_t den) {
     return (int64_t)(q + (twice > den || (twice == den && (q & 1)) ? 1 : 0));
 }
 
+// The counts' table in LDS.  Its first entries are on their way while the block loads the maxima.
+struct BinWeights {
+    uint32_t first;
+    __device__ inline void load(const Logp& a) { first = weight_below(a, threadIdx.x); }
+    __device__ inline void store(const Logp& a, uint16_t* wt) const {
+        if (threadIdx.x < a.bins) wt[threadIdx.x] = (uint16_t)first;
+        for (uint32_t i = threadIdx.x + kRowThreads; i < a.bins; i += kRowThreads) wt[i] = (uint16_t)weight_below(a, i);
+    }
+};
+
+// A block per row.  Wave 0 finds the tiles of the alternatives, one after another: a lane holds
+// the largest maximum left among every 64th tile, and the one that is taken looks again.
+// The other waves add the chunks' counts up, a wave per chunk.  Then every wave reads its
+// share of those tiles; values from the last tile's maximum on are candidates, few
+// unless many are equal, and a candidate's place is how many are before it.  More than
+// kLogpCandidates are taken one after another by the whole block.
+constexpr int kLogpCandidates = 512;
 __global__ __launch_bounds__(kRowThreads) void logp_row_kernel(Logp a) {
     constexpr int kWaves = kRowThreads / 64;
-    __shared__ uint64_t red[2][kWaves];
+    extern __shared__ uint16_t wt[];
+    __shared__ uint64_t red[2][kWaves], s_cand[kLogpCandidates], s_last;
     __shared__ int64_t s_ln;
-    __shared__ uint64_t s_key[kWaves];
-    __shared__ uint64_t s_last;
-    const int r = blockIdx.x, tid = threadIdx.x, lane = tid & 63, w = tid >> 6;
+    __shared__ int s_tile[kLogpMaxTop], s_count;
+    __shared__ int32_t s_edge;
+    const int r = blockIdx.x, tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int32_t* z = a.z + (size_t)r * a.ldz;
     const int32_t* cm = a.cmax + (size_t)r * a.chunks;
+    const int32_t* tm = a.tmax + (size_t)r * a.tiles;
+    BinWeights bw;
+    bw.load(a);
     int32_t m = INT32_MIN;
     for (int c = lane; c < a.chunks; c += 64) m = max(m, cm[c]);
+    bw.store(a, wt);
+    if (tid == 0) s_count = 0;
     m = wave_max_i32(m);
+    __syncthreads();
     uint64_t s = 0, moment = 0;  // below 2^35 and 2^48
+    if (w == 0 && a.n) {
+        auto best_below = [&](uint64_t last) {
+            uint64_t key = 0;
+            for (int i0 = lane; i0 < a.tiles; i0 += 64 * 4) {
+                int32_t x[4];
+#pragma unroll
+                for (int k = 0; k < 4; ++k) x[k] = i0 + 64 * k < a.tiles ? tm[i0 + 64 * k] : 0;
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    const uint64_t o = max_key(x[k], (uint32_t)(i0 + 64 * k));
+                    if (i0 + 64 * k < a.tiles && o < last && o > key) key = o;
+                }
+            }
+            return key;
+        };
+        uint64_t own = best_below(~0ull);
+        const int n = min(a.n, a.tiles);
+        for (int k = 0; k < n; ++k) {
+            const uint64_t top = wave_max_u64(own);
+            if (lane == 0) {
+                s_tile[k] = (int)key_index(top);
+                s_edge = key_value(top);
+            }
+            if (own == top) own = best_below(top);
+        }
+        // fewer tiles than alternatives: every value is a candidate
+        if (lane == 0 && a.n > a.tiles) s_edge = INT32_MIN;
+    }
     for (int c = w; c < a.chunks; c += kWaves) {
         const uint32_t d = (uint32_t)m - (uint32_t)cm[c];
         if (d >= a.bins) continue;
         const uint32_t* n = a.counts + ((size_t)r * a.chunks + c) * a.words;
-        for (uint32_t i = lane; i < a.words; i += 64) {
-            const uint32_t two = n[i], at = d + 2 * i;
-            const uint64_t e0 = (uint64_t)(two & 0xFFFFu) * weight_below(a, at), e1 = (uint64_t)(two >> 16) * weight_below(a, at + 1);
-            s += e0 + e1;
-            moment += e0 * at + e1 * (at + 1);
+        for (uint32_t i0 = lane; i0 < a.words; i0 += 4 * 64) {
+            uint32_t two[4];
+#pragma unroll
+            for (int k = 0; k < 4; ++k) two[k] = i0 + 64 * k < a.words ? n[i0 + 64 * k] : 0;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const uint32_t at = d + 2 * (i0 + 64 * k);
+                const uint64_t e0 = (uint64_t)(two[k] & 0xFFFFu) * (at < a.bins ? wt[at] : 0u);
+                const uint64_t e1 = (uint64_t)(two[k] >> 16) * (at + 1 < a.bins ? wt[at + 1] : 0u);
+                s += e0 + e1;
+                moment += e0 * at + e1 * (at + 1);
+            }
         }
     }
     s = wave_sum_u64(s);
@@ -155,29 +214,64 @@ __global__ __launch_bounds__(kRowThreads) void logp_row_kernel(Logp a) {
             if (a.entropy) a.entropy[r] = s ? ln + div_round(moment << 10, s) : 0;
         }
     }
+    // the tiles' values, at most two tiles of a wave
+    constexpr int kEach = ((int)kLogpMaxTop + kWaves - 1) / kWaves;
+    uint64_t key[kEach][4];
+#pragma unroll
+    for (int k = 0; k < kEach; ++k)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) key[k][e] = 0;
+    const int n_tiles = min(a.n, a.tiles);
+#pragma unroll
+    for (int k = 0; k < kEach; ++k) {
+        if (w + k * kWaves >= n_tiles) break;
+        const int i = s_tile[w + k * kWaves] * kLogpTile + 4 * lane;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            if (i + e >= a.V) continue;
+            const int32_t x = z[i + e];
+            if (x < s_edge) continue;
+            key[k][e] = max_key(x, (uint32_t)(i + e));
+            const int at = atomicAdd(&s_count, 1);
+            if (at < kLogpCandidates) s_cand[at] = key[k][e];
+        }
+    }
     __syncthreads();
     const int64_t ln = s_ln;
     for (int i = tid; i < a.T; i += kRowThreads) {
         const int64_t t = a.tokens[(size_t)r * a.T + i];
         a.logprobs[(size_t)r * a.T + i] = t < 0 || t >= a.V ? 0 : ((int64_t)z[t] - (int64_t)m) * 1024 - ln;
     }
-    // the largest values one after another
+    auto answer = [&](int k, uint64_t o) {
+        a.top_tokens[(size_t)r * a.n + k] = key_index(o);
+        a.top_logprobs[(size_t)r * a.n + k] = ((int64_t)key_value(o) - (int64_t)m) * 1024 - ln;
+    };
+    const int count = s_count;  // at least n
+    if (count <= kLogpCandidates) {
+        if (tid < count) {
+            const uint64_t own = s_cand[tid];
+            int before = 0;
+            for (int i = 0; i < count; ++i) before += s_cand[i] > own ? 1 : 0;
+            if (before < a.n) answer(before, own);
+        }
+        return;
+    }
     uint64_t last = ~0ull;
     for (int k = 0; k < a.n; ++k) {
-        uint64_t key = 0;
-        for (int i = tid; i < a.V; i += kRowThreads) {
-            const uint64_t o = max_key(z[i], (uint32_t)i);
-            if (o < last && o > key) key = o;
-        }
-        key = wave_max_u64(key);
-        if (lane == 0) s_key[w] = key;
+        uint64_t best = 0;
+#pragma unroll
+        for (int i = 0; i < kEach; ++i)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                if (key[i][e] < last && key[i][e] > best) best = key[i][e];
+        best = wave_max_u64(best);
+        if (lane == 0) red[0][w] = best;
         __syncthreads();
         if (w == 0) {
-            key = wave_max_u64(lane < kWaves ? s_key[lane] : 0);
+            best = wave_max_u64(lane < kWaves ? red[0][lane] : 0);
             if (lane == 0) {
-                s_last = key;
-                a.top_tokens[(size_t)r * a.n + k] = key_index(key);
-                a.top_logprobs[(size_t)r * a.n + k] = ((int64_t)key_value(key) - (int64_t)m) * 1024 - ln;
+                s_last = best;
+                answer(k, best);
             }
         }
         __syncthreads();
@@ -222,7 +316,7 @@ int myl_logprobs_dev(myl_ctx* ctx, const int32_t* logits, size_t rows, size_t vo
     a.tmax = reinterpret_cast<int32_t*>(ws + pl.off_tiles);
     a.counts = reinterpret_cast<uint32_t*>(ws + pl.off_counts);
     logp_count_kernel<<<dim3((unsigned)pl.chunks, (unsigned)rows), kBlk, (size_t)pl.words * 8, ctx->stream>>>(a);
-    logp_row_kernel<<<(unsigned)rows, kRowThreads, 0, ctx->stream>>>(a);
+    logp_row_kernel<<<(unsigned)rows, kRowThreads, (size_t)pl.bins * 2, ctx->stream>>>(a);
     return ctx->hip(hipGetLastError(), what);
 }
 
