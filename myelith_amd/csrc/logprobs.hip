@@ -36,7 +36,7 @@ struct Logp {
     uint32_t* counts;  // [rows][chunks][words]
 };
 
-constexpr int kBlk = 256, kRowThreads = 1024;
+constexpr int kBlk = 256;
 constexpr int kQuads = kLogpChunk / (4 * kBlk);
 
 typedef int32_t RowQuad __attribute__((ext_vector_type(4), aligned(4)));
@@ -63,7 +63,7 @@ __global__ __launch_bounds__(kBlk) void logp_count_kernel(Logp a) {
     for (int q = 0; q < kQuads; ++q) {
         const int i = c * kLogpChunk + q * 4 * kBlk + 4 * tid;
         n[q] = min(max(a.V - i, 0), 4);
-        if (n[q] == 4) v[q] = *reinterpret_cast<const RowQuad*>(z + i);
+        if (n[q] == 4) v[q] = __builtin_nontemporal_load(reinterpret_cast<const RowQuad*>(z + i));
         else
 #pragma unroll
             for (int e = 0; e < 4; ++e) v[q][e] = e < n[q] ? z[i + e] : INT32_MIN;
@@ -116,43 +116,62 @@ __device__ inline int64_t div_round(uint64_t num, uint64_t den) {
 }
 
 // The counts' table in LDS.  Its first entries are on their way while the block loads the maxima.
+template <int THREADS>
 struct BinWeights {
-    uint32_t first;
-    __device__ inline void load(const Logp& a) { first = weight_below(a, threadIdx.x); }
+    static constexpr int kEach = 1024 / THREADS;
+    uint32_t w[kEach];
+    __device__ inline void load(const Logp& a) {
+#pragma unroll
+        for (int i = 0; i < kEach; ++i) w[i] = weight_below(a, threadIdx.x + i * THREADS);
+    }
     __device__ inline void store(const Logp& a, uint16_t* wt) const {
-        if (threadIdx.x < a.bins) wt[threadIdx.x] = (uint16_t)first;
-        for (uint32_t i = threadIdx.x + kRowThreads; i < a.bins; i += kRowThreads) wt[i] = (uint16_t)weight_below(a, i);
+#pragma unroll
+        for (int i = 0; i < kEach; ++i)
+            if (threadIdx.x + i * THREADS < a.bins) wt[threadIdx.x + i * THREADS] = (uint16_t)w[i];
+        for (uint32_t i = threadIdx.x + 1024; i < a.bins; i += THREADS) wt[i] = (uint16_t)weight_below(a, i);
     }
 };
 
-// A block per row.  Wave 0 finds the tiles of the alternatives, one after another: a lane holds
-// the largest maximum left among every 64th tile, and the one that is taken looks again.
-// The other waves add the chunks' counts up, a wave per chunk.  Then every wave reads its
-// share of those tiles; values from the last tile's maximum on are candidates, few
-// unless many are equal, and a candidate's place is how many are before it.  More than
-// kLogpCandidates are taken one after another by the whole block.
-constexpr int kLogpCandidates = 512;
-__global__ __launch_bounds__(kRowThreads) void logp_row_kernel(Logp a) {
-    constexpr int kWaves = kRowThreads / 64;
-    extern __shared__ uint16_t wt[];
-    __shared__ uint64_t red[2][kWaves], s_cand[kLogpCandidates], s_last;
-    __shared__ int64_t s_ln;
-    __shared__ int s_tile[kLogpMaxTop], s_count;
-    __shared__ int32_t s_edge;
-    const int r = blockIdx.x, tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const int32_t* z = a.z + (size_t)r * a.ldz;
-    const int32_t* cm = a.cmax + (size_t)r * a.chunks;
-    const int32_t* tm = a.tmax + (size_t)r * a.tiles;
-    BinWeights bw;
-    bw.load(a);
-    int32_t m = INT32_MIN;
-    for (int c = lane; c < a.chunks; c += 64) m = max(m, cm[c]);
-    bw.store(a, wt);
-    if (tid == 0) s_count = 0;
-    m = wave_max_i32(m);
-    __syncthreads();
-    uint64_t s = 0, moment = 0;  // below 2^35 and 2^48
-    if (w == 0 && a.n) {
+constexpr size_t kLogpFewRows = 512;  // two blocks of 16 waves per CU
+
+// Where the alternatives are looked for.
+constexpr int kLogpCandidates = 512, kLogpTiles = 128;
+struct TopLds {
+    uint64_t cand[kLogpCandidates], red[16], last;
+    int tile[kLogpTiles];
+    int tiles, count;
+    int32_t edge;
+};
+
+// A value that n tiles at least reach, by one wave: the n-th largest of the maxima over every 64th
+// tile, or the least value where there are fewer tiles.
+__device__ inline int32_t logp_edge(const Logp& a, const int32_t* tm) {
+    const int lane = threadIdx.x & 63;
+    int32_t own = INT32_MIN;
+    for (int i0 = lane; i0 < a.tiles; i0 += 64 * 8) {
+        int32_t x[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) x[k] = i0 + 64 * k < a.tiles ? tm[i0 + 64 * k] : INT32_MIN;
+#pragma unroll
+        for (int k = 0; k < 8; ++k) own = max(own, x[k]);
+    }
+    if (a.n > a.tiles) return INT32_MIN;
+    int before = 0;  // lanes without a tile come last, whatever the others hold
+#pragma unroll
+    for (int j = 0; j < 64; ++j) {
+        const int32_t x = readlane_i32(own, j);
+        before += x > own || (x == own && j < lane) ? 1 : 0;
+    }
+    return readlane_i32(own, (int)__builtin_ctzll(__ballot(before == a.n - 1)));
+}
+
+// The n largest values one after another, by the whole block: of the n tiles with the largest
+// maxima (of equal ones the first), found by the first wave.  For rows with many equal values.
+template <int THREADS, class Answer>
+__device__ inline void logp_top_in_turn(const Logp& a, const int32_t* z, const int32_t* tm, TopLds& t, const Answer& answer) {
+    constexpr int kWaves = THREADS / 64, kEach = (int)kLogpMaxTop / kWaves;
+    const int tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6), n = min(a.n, a.tiles);
+    if (w == 0) {
         auto best_below = [&](uint64_t last) {
             uint64_t key = 0;
             for (int i0 = lane; i0 < a.tiles; i0 += 64 * 4) {
@@ -168,28 +187,83 @@ __global__ __launch_bounds__(kRowThreads) void logp_row_kernel(Logp a) {
             return key;
         };
         uint64_t own = best_below(~0ull);
-        const int n = min(a.n, a.tiles);
         for (int k = 0; k < n; ++k) {
             const uint64_t top = wave_max_u64(own);
-            if (lane == 0) {
-                s_tile[k] = (int)key_index(top);
-                s_edge = key_value(top);
-            }
+            if (lane == 0) t.tile[k] = (int)key_index(top);
             if (own == top) own = best_below(top);
         }
-        // fewer tiles than alternatives: every value is a candidate
-        if (lane == 0 && a.n > a.tiles) s_edge = INT32_MIN;
     }
+    __syncthreads();
+    uint64_t key[kEach][4];
+#pragma unroll
+    for (int k = 0; k < kEach; ++k)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            const int i = w + k * kWaves < n ? t.tile[w + k * kWaves] * kLogpTile + 4 * lane + e : a.V;
+            key[k][e] = i < a.V ? max_key(z[i], (uint32_t)i) : 0;
+        }
+    uint64_t last = ~0ull;
+    for (int k = 0; k < a.n; ++k) {
+        uint64_t best = 0;
+#pragma unroll
+        for (int i = 0; i < kEach; ++i)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                if (key[i][e] < last && key[i][e] > best) best = key[i][e];
+        best = wave_max_u64(best);
+        if (lane == 0) t.red[w] = best;
+        __syncthreads();
+        if (w == 0) {
+            best = wave_max_u64(lane < kWaves ? t.red[lane] : 0);
+            if (lane == 0) {
+                t.last = best;
+                answer(k, best);
+            }
+        }
+        __syncthreads();
+        last = t.last;
+    }
+}
+
+// A block per row adds the chunks' counts up, a wave per chunk, and finds the alternatives: every
+// tile that reaches the edge is read, every value of it that does is a candidate, and a
+// candidate's place is how many are before it.  Few are, unless many values are
+// equal; past the room for them, logp_top_in_turn.  16 waves where few rows wait for it, four
+// where rows fill the chip.
+template <int THREADS>
+__global__ __launch_bounds__(THREADS) void logp_row_kernel(Logp a) {
+    constexpr int kWaves = THREADS / 64;
+    extern __shared__ uint16_t wt[];
+    __shared__ TopLds top;
+    __shared__ uint64_t red[2][kWaves];
+    __shared__ int64_t s_ln;
+    const int r = blockIdx.x, tid = threadIdx.x, lane = tid & 63, w = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int32_t* z = a.z + (size_t)r * a.ldz;
+    const int32_t* cm = a.cmax + (size_t)r * a.chunks;
+    const int32_t* tm = a.tmax + (size_t)r * a.tiles;
+    BinWeights<THREADS> bw;
+    bw.load(a);
+    int32_t m = INT32_MIN;
+    for (int c = lane; c < a.chunks; c += 64) m = max(m, cm[c]);
+    bw.store(a, wt);
+    if (tid == 0) top.count = top.tiles = 0;
+    m = wave_max_i32(m);
+    __syncthreads();
+    if (w == kWaves - 1 && a.n) {
+        const int32_t edge = logp_edge(a, tm);
+        if (lane == 0) top.edge = edge;
+    }
+    uint64_t s = 0, moment = 0;  // below 2^35 and 2^48
     for (int c = w; c < a.chunks; c += kWaves) {
         const uint32_t d = (uint32_t)m - (uint32_t)cm[c];
         if (d >= a.bins) continue;
         const uint32_t* n = a.counts + ((size_t)r * a.chunks + c) * a.words;
-        for (uint32_t i0 = lane; i0 < a.words; i0 += 4 * 64) {
-            uint32_t two[4];
+        for (uint32_t i0 = lane; i0 < a.words; i0 += 8 * 64) {
+            uint32_t two[8];
 #pragma unroll
-            for (int k = 0; k < 4; ++k) two[k] = i0 + 64 * k < a.words ? n[i0 + 64 * k] : 0;
+            for (int k = 0; k < 8; ++k) two[k] = i0 + 64 * k < a.words ? n[i0 + 64 * k] : 0;
 #pragma unroll
-            for (int k = 0; k < 4; ++k) {
+            for (int k = 0; k < 8; ++k) {
                 const uint32_t at = d + 2 * (i0 + 64 * k);
                 const uint64_t e0 = (uint64_t)(two[k] & 0xFFFFu) * (at < a.bins ? wt[at] : 0u);
                 const uint64_t e1 = (uint64_t)(two[k] >> 16) * (at + 1 < a.bins ? wt[at + 1] : 0u);
@@ -214,68 +288,47 @@ __global__ __launch_bounds__(kRowThreads) void logp_row_kernel(Logp a) {
             if (a.entropy) a.entropy[r] = s ? ln + div_round(moment << 10, s) : 0;
         }
     }
-    // the tiles' values, at most two tiles of a wave
-    constexpr int kEach = ((int)kLogpMaxTop + kWaves - 1) / kWaves;
-    uint64_t key[kEach][4];
+    if (a.n) {
+        const int32_t edge = top.edge;
+        for (int i = tid; i < a.tiles; i += THREADS)
+            if (tm[i] >= edge) {
+                const int at = atomicAdd(&top.tiles, 1);
+                if (at < kLogpTiles) top.tile[at] = i;
+            }
+        __syncthreads();
+        const int n = min(top.tiles, kLogpTiles);
+        for (int k = w; k < n; k += kWaves) {
+            const int i = top.tile[k] * kLogpTile + 4 * lane;
 #pragma unroll
-    for (int k = 0; k < kEach; ++k)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) key[k][e] = 0;
-    const int n_tiles = min(a.n, a.tiles);
-#pragma unroll
-    for (int k = 0; k < kEach; ++k) {
-        if (w + k * kWaves >= n_tiles) break;
-        const int i = s_tile[w + k * kWaves] * kLogpTile + 4 * lane;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            if (i + e >= a.V) continue;
-            const int32_t x = z[i + e];
-            if (x < s_edge) continue;
-            key[k][e] = max_key(x, (uint32_t)(i + e));
-            const int at = atomicAdd(&s_count, 1);
-            if (at < kLogpCandidates) s_cand[at] = key[k][e];
+            for (int e = 0; e < 4; ++e) {
+                const int32_t x = i + e < a.V ? z[i + e] : INT32_MIN;
+                if (i + e >= a.V || x < edge) continue;
+                const int at = atomicAdd(&top.count, 1);
+                if (at < kLogpCandidates) top.cand[at] = max_key(x, (uint32_t)(i + e));
+            }
         }
     }
     __syncthreads();
     const int64_t ln = s_ln;
-    for (int i = tid; i < a.T; i += kRowThreads) {
+    for (int i = tid; i < a.T; i += THREADS) {
         const int64_t t = a.tokens[(size_t)r * a.T + i];
         a.logprobs[(size_t)r * a.T + i] = t < 0 || t >= a.V ? 0 : ((int64_t)z[t] - (int64_t)m) * 1024 - ln;
     }
+    if (!a.n) return;
     auto answer = [&](int k, uint64_t o) {
         a.top_tokens[(size_t)r * a.n + k] = key_index(o);
         a.top_logprobs[(size_t)r * a.n + k] = ((int64_t)key_value(o) - (int64_t)m) * 1024 - ln;
     };
-    const int count = s_count;  // at least n
-    if (count <= kLogpCandidates) {
-        if (tid < count) {
-            const uint64_t own = s_cand[tid];
-            int before = 0;
-            for (int i = 0; i < count; ++i) before += s_cand[i] > own ? 1 : 0;
-            if (before < a.n) answer(before, own);
-        }
+    const int count = top.count;  // at least n
+    if (top.tiles > kLogpTiles || count > kLogpCandidates) {
+        logp_top_in_turn<THREADS>(a, z, tm, top, answer);
         return;
     }
-    uint64_t last = ~0ull;
-    for (int k = 0; k < a.n; ++k) {
-        uint64_t best = 0;
-#pragma unroll
-        for (int i = 0; i < kEach; ++i)
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-                if (key[i][e] < last && key[i][e] > best) best = key[i][e];
-        best = wave_max_u64(best);
-        if (lane == 0) red[0][w] = best;
-        __syncthreads();
-        if (w == 0) {
-            best = wave_max_u64(lane < kWaves ? red[0][lane] : 0);
-            if (lane == 0) {
-                s_last = best;
-                answer(k, best);
-            }
-        }
-        __syncthreads();
-        last = s_last;
+    for (int i = tid; i < count; i += THREADS) {
+        const uint64_t own = top.cand[i];
+        int before = 0;
+        for (int j = 0; j < count; ++j) before += top.cand[j] > own ? 1 : 0;
+        if (before < a.n) answer(before, own);
     }
 }
 
@@ -316,7 +369,8 @@ int myl_logprobs_dev(myl_ctx* ctx, const int32_t* logits, size_t rows, size_t vo
     a.tmax = reinterpret_cast<int32_t*>(ws + pl.off_tiles);
     a.counts = reinterpret_cast<uint32_t*>(ws + pl.off_counts);
     logp_count_kernel<<<dim3((unsigned)pl.chunks, (unsigned)rows), kBlk, (size_t)pl.words * 8, ctx->stream>>>(a);
-    logp_row_kernel<<<(unsigned)rows, kRowThreads, (size_t)pl.bins * 2, ctx->stream>>>(a);
+    if (rows <= kLogpFewRows) logp_row_kernel<1024><<<(unsigned)rows, 1024, (size_t)pl.bins * 2, ctx->stream>>>(a);
+    else logp_row_kernel<256><<<(unsigned)rows, 256, (size_t)pl.bins * 2, ctx->stream>>>(a);
     return ctx->hip(hipGetLastError(), what);
 }
 
