@@ -3,8 +3,12 @@
 // keys and values into their pages: myl_kv_append_paged_dev.
 //
 // A thread takes dimensions 8 c .. + 7 of a head and the 8 they rotate with, half a head
-// further on: two 16-byte loads and two 16-byte stores.  A norm's sum of squares goes over
-// the head's hd / 16 neighbouring threads.
+// further on: two 16-byte loads and two 16-byte stores a row.  A norm's sum of squares goes over
+// the head's hd / 16 neighbouring threads.  Bound by the bytes for many rows, so long as
+// few instructions go on each value (with the general shifts and a bias worked out for every row
+// 16384 rows took 89 us): a thread keeps its dimensions over several rows, four of them in flight,
+// and the biases are brought to their scale once for all of them; the rounding shifts take
+// 32-bit steps where their shifts allow it.
 #include "abi_internal.h"
 #include "ops.h"
 #include "paged_plan.h"
@@ -27,7 +31,8 @@ struct Append {
     RmsParams rms;
     size_t ldq, ldk, ldv, ldo, page_stride, head_stride, pos_stride, ldt;
     SmallDiv per_row, n_pos, page;
-    int items, heads, kv_heads, n_seqs, table_len, n_pages;
+    int items, rows, group;  // threads; rows of a thread
+    int heads, kv_heads, n_seqs, table_len, n_pages;
     uint8_t q_frac, k_frac, v_frac, q_norm_frac, k_norm_frac, rope_frac;
 };
 
@@ -46,92 +51,188 @@ __device__ inline uint4 pack8(const int32_t (&v)[8]) {
     return make_uint4(w[0], w[1], w[2], w[3]);
 }
 __device__ inline uint4 load8(const int16_t* p) { return *reinterpret_cast<const uint4*>(p); }
+__device__ inline int32_t sat16(int32_t x) { return min(max(x, -32768), 32767); }
 
-__device__ inline void add_bias8(const Append& a, size_t at, uint8_t frac, int32_t (&x)[8]) {
-    int32_t b[8];
+// The biases of 8 dimensions at the rows' scale (linear.rs:132-145).
+__device__ inline void bias8(const Append& a, size_t at, uint8_t frac, int32_t (&b)[8]) {
     unpack8(load8(a.bias + at), b);
     const uint2 s = *reinterpret_cast<const uint2*>(a.bias_shifts + at);
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-        const uint8_t sh = (uint8_t)((i < 4 ? s.x : s.y) >> (8 * (i & 3)));
-        x[i] = clamp_i16_i64((int64_t)x[i] + (int64_t)rescale32(b[i], sh, frac));
+        const int32_t r = rescale32(b[i], (uint8_t)((i < 4 ? s.x : s.y) >> (8 * (i & 3))), frac);
+        b[i] = min(max(r, -65536), 65536);  // added to 16 bits and clamped to them: the same
     }
 }
 
-template <int HD, bool BIAS, bool NORM>
+// clamp_i16(rshift_round32(v, s)) for shifts of 1 .. 16: half a unit less a bit, and the bit that
+// makes a tie even, carry into the result; where that passes 2^31 the result is past 16 bits.
+struct TurnRound {
+    uint32_t s;
+    int32_t half;
+    bool fast;
+    __device__ inline static TurnRound of(uint8_t frac) {
+        const bool ok = frac >= 1 && frac <= 16;
+        return TurnRound{ok ? frac : 1u, ok ? (1 << (frac - 1)) - 1 : 0, ok};
+    }
+    __device__ inline int32_t operator()(int32_t v) const {
+        return sat16(__builtin_elementwise_add_sat(v, half + (int32_t)(((uint32_t)v >> s) & 1u)) >> s);
+    }
+};
+
+// A thread's 8 channels of a norm.
+struct Gamma8 {
+    int32_t g[8];
+    uint32_t s[8], least, most;
+    __device__ inline void load(const int8_t* gamma, const uint8_t* shifts) {
+        const uint2 gw = *reinterpret_cast<const uint2*>(gamma), sw = *reinterpret_cast<const uint2*>(shifts);
+        least = 255;
+        most = 0;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            g[i] = (int32_t)(int8_t)((i < 4 ? gw.x : gw.y) >> (8 * (i & 3)));
+            s[i] = ((i < 4 ? sw.x : sw.y) >> (8 * (i & 3))) & 255u;
+            least = min(least, s[i]);
+            most = max(most, s[i]);
+        }
+    }
+    // rms_out of 8 values.  |x gamma lut| < 2^37, so right shifts by 6 .. 31 leave 32 bits.
+    __device__ inline void apply(const RmsFactor& f, uint8_t frac, int32_t (&x)[8]) const {
+        const int32_t base = (int32_t)f.norm_frac - (int32_t)frac;
+        if (!f.zero && base + (int32_t)least >= 6 && base + (int32_t)most <= 31) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const uint32_t sh = (uint32_t)base + s[i];
+                const int64_t p = (int64_t)(x[i] * g[i]) * (int64_t)(int32_t)f.lut_val;
+                const uint32_t lo = (uint32_t)p, hi = (uint32_t)((uint64_t)p >> 32);
+                const uint32_t q = __builtin_amdgcn_alignbit(hi, lo, sh);
+                const uint32_t rest = lo & ((1u << sh) - 1u);
+                x[i] = sat16((int32_t)(q + ((rest + ((1u << (sh - 1)) - 1u) + (q & 1u)) >> sh)));
+            }
+            return;
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[i] = rms_out((int16_t)x[i], 0, (int8_t)g[i], (uint8_t)s[i], f, frac);
+    }
+};
+
+// R rows at a time, `group` of them to a thread.
+template <int HD, bool BIAS, bool NORM, int R>
 __global__ __launch_bounds__(256) void append_kernel(Append a) {
     constexpr int CH = HD / 16, HALF = HD / 2;
     const int t = (int)(blockIdx.x * 256u + threadIdx.x);
     if (t >= a.items) return;
     int rem;
-    const int row = divmod(a.per_row, t, rem), hh = rem / CH, d = 8 * (rem % CH);
-    const int pos = a.pos[row], seq = a.seqs ? a.seqs[row] : row;
-    if (pos < 0 || seq < 0 || seq >= a.n_seqs) return;
+    const int first = divmod(a.per_row, t, rem) * a.group, hh = rem / CH, d = 8 * (rem % CH);
     const int kind = hh < a.heads ? 0 : hh < a.heads + a.kv_heads ? 1 : 2;  // q, k, v
     const int h = hh - (kind == 0 ? 0 : kind == 1 ? a.heads : a.heads + a.kv_heads);
-    const int16_t* src = (kind == 0 ? a.q + (size_t)row * a.ldq : kind == 1 ? a.k + (size_t)row * a.ldk : a.v + (size_t)row * a.ldv) +
-                         (size_t)h * HD + d;
-    int32_t x0[8], x1[8];
-    unpack8(load8(src), x0);
-    unpack8(load8(src + HALF), x1);
+    const size_t ld = kind == 0 ? a.ldq : kind == 1 ? a.ldk : a.ldv;
+    const int16_t* src = (kind == 0 ? a.q : kind == 1 ? a.k : a.v) + (size_t)h * HD + d;
+    const TurnRound turn_round = TurnRound::of(a.rope_frac);
+    int32_t b0[8], b1[8];
     if (BIAS) {
         const uint8_t frac = kind == 0 ? a.q_frac : kind == 1 ? a.k_frac : a.v_frac;
-        add_bias8(a, (size_t)hh * HD + d, frac, x0);
-        add_bias8(a, (size_t)hh * HD + d + HALF, frac, x1);
+        bias8(a, (size_t)hh * HD + d, frac, b0);
+        bias8(a, (size_t)hh * HD + d + HALF, frac, b1);
     }
-    if (NORM) {
-        const int8_t* gamma = kind == 0 ? a.q_gamma : kind == 1 ? a.k_gamma : nullptr;
+    Gamma8 g0, g1;
+    const int8_t* gamma = kind == 0 ? a.q_gamma : kind == 1 ? a.k_gamma : nullptr;
+    const uint8_t norm_frac = kind == 0 ? a.q_norm_frac : a.k_norm_frac;
+    if (NORM && gamma) {
         const uint8_t* shifts = kind == 0 ? a.q_gamma_shifts : a.k_gamma_shifts;
-        uint64_t s = 0;  // at most 128 2^30
+        g0.load(gamma + d, shifts + d);
+        g1.load(gamma + d + HALF, shifts + d + HALF);
+    }
+    for (int row0 = first; row0 < min(first + a.group, a.rows); row0 += R) {
+        int pos[R], seq[R], id[R], off[R];
+        uint4 raw[R][2], cs[R][2];
+        bool in[R];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) s += (uint64_t)((int64_t)x0[i] * x0[i]) + (uint64_t)((int64_t)x1[i] * x1[i]);
-        s = dpp_add64<dpp::kXor1>(s);
-        s = dpp_add64<dpp::kXor2>(s);
-        if (CH == 8) s = dpp_add64<dpp::kHalfMirror>(s);
-        if (gamma) {
-            const RmsFactor f = rms_factor_of((myl_i128)s, 0, a.rms);
-            const uint8_t frac = kind == 0 ? a.q_norm_frac : a.k_norm_frac;
+        for (int r = 0; r < R; ++r) {
+            const int row = min(row0 + r, a.rows - 1);
+            raw[r][0] = load8(src + (size_t)row * ld);
+            raw[r][1] = load8(src + (size_t)row * ld + HALF);
+            pos[r] = a.pos[row];
+            seq[r] = a.seqs ? a.seqs[row] : row;
+            in[r] = row0 + r < a.rows;
+        }
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                x0[i] = rms_out((int16_t)x0[i], 0, gamma[d + i], shifts[d + i], f, frac);
-                x1[i] = rms_out((int16_t)x1[i], 0, gamma[d + HALF + i], shifts[d + HALF + i], f, frac);
+        for (int r = 0; r < R; ++r) {
+            in[r] = in[r] && pos[r] >= 0 && seq[r] >= 0 && seq[r] < a.n_seqs;
+            if (!in[r]) pos[r] = 0;
+            if (kind < 2) {
+                int turn;
+                divmod(a.n_pos, pos[r], turn);
+                cs[r][0] = load8(a.cos + (size_t)turn * HALF + d);
+                cs[r][1] = load8(a.sin + (size_t)turn * HALF + d);
+            }
+            id[r] = -1;
+            if (kind > 0) {
+                const int at = divmod(a.page, pos[r], off[r]);
+                if (in[r] && at < a.table_len) id[r] = a.tables[(size_t)seq[r] * a.ldt + at];
             }
         }
-    }
-    if (kind < 2) {
-        int turn;
-        divmod(a.n_pos, pos, turn);
-        int32_t c[8], s[8];
-        unpack8(load8(a.cos + (size_t)turn * HALF + d), c);
-        unpack8(load8(a.sin + (size_t)turn * HALF + d), s);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const int32_t u = x0[i], w = x1[i];
-            x0[i] = clamp_i16(rshift_round32(wsub32(wmul32(u, c[i]), wmul32(w, s[i])), a.rope_frac));
-            x1[i] = clamp_i16(rshift_round32(wadd32(wmul32(w, c[i]), wmul32(u, s[i])), a.rope_frac));
+        for (int r = 0; r < R; ++r) {
+            int32_t x0[8], x1[8];
+            unpack8(raw[r][0], x0);
+            unpack8(raw[r][1], x1);
+            if (BIAS)
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    x0[i] = sat16(x0[i] + b0[i]);
+                    x1[i] = sat16(x1[i] + b1[i]);
+                }
+            if (NORM) {
+                uint64_t s = 0;  // at most 128 2^30
+#pragma unroll
+                for (int i = 0; i < 8; ++i) s += (uint64_t)((int64_t)x0[i] * x0[i]) + (uint64_t)((int64_t)x1[i] * x1[i]);
+                s = dpp_add64<dpp::kXor1>(s);
+                s = dpp_add64<dpp::kXor2>(s);
+                if (CH == 8) s = dpp_add64<dpp::kHalfMirror>(s);
+                if (gamma) {
+                    const RmsFactor f = rms_factor_of((myl_i128)s, 0, a.rms);
+                    g0.apply(f, norm_frac, x0);
+                    g1.apply(f, norm_frac, x1);
+                }
+            }
+            if (kind < 2) {
+                int32_t c[8], s[8];
+                unpack8(cs[r][0], c);
+                unpack8(cs[r][1], s);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const int32_t u = x0[i], w = x1[i];
+                    const int32_t y0 = wsub32(wmul32(u, c[i]), wmul32(w, s[i])), y1 = wadd32(wmul32(w, c[i]), wmul32(u, s[i]));
+                    x0[i] = turn_round.fast ? turn_round(y0) : clamp_i16(rshift_round32(y0, a.rope_frac));
+                    x1[i] = turn_round.fast ? turn_round(y1) : clamp_i16(rshift_round32(y1, a.rope_frac));
+                }
+            }
+            if (!in[r]) continue;
+            int16_t* dst;
+            if (kind == 0) {
+                dst = a.qo + (size_t)(row0 + r) * a.ldo + (size_t)h * HD + d;
+            } else {
+                if (id[r] < 0 || id[r] >= a.n_pages) continue;
+                dst = (kind == 1 ? a.kp : a.vp) + (size_t)id[r] * a.page_stride + (size_t)h * a.head_stride + (size_t)off[r] * a.pos_stride + d;
+            }
+            *reinterpret_cast<uint4*>(dst) = pack8(x0);
+            *reinterpret_cast<uint4*>(dst + HALF) = pack8(x1);
         }
     }
-    int16_t* dst;
-    if (kind == 0) {
-        dst = a.qo + (size_t)row * a.ldo + (size_t)h * HD + d;
-    } else {
-        int off;
-        const int at = divmod(a.page, pos, off);
-        const int id = at < a.table_len ? a.tables[(size_t)seq * a.ldt + at] : -1;
-        if (id < 0 || id >= a.n_pages) return;
-        dst = (kind == 1 ? a.kp : a.vp) + (size_t)id * a.page_stride + (size_t)h * a.head_stride + (size_t)off * a.pos_stride + d;
-    }
-    *reinterpret_cast<uint4*>(dst) = pack8(x0);
-    *reinterpret_cast<uint4*>(dst + HALF) = pack8(x1);
 }
 
+template <int HD, bool BIAS, bool NORM>
+void append_rows(const Append& a, hipStream_t st) {
+    const unsigned grid = (unsigned)((a.items + 255) / 256);
+    if (a.group == 1) append_kernel<HD, BIAS, NORM, 1><<<grid, 256, 0, st>>>(a);
+    else append_kernel<HD, BIAS, NORM, 4><<<grid, 256, 0, st>>>(a);
+}
 template <int HD>
 void append_launch(const Append& a, bool norm, hipStream_t st) {
-    const unsigned grid = (unsigned)((a.items + 255) / 256);
-    if (a.bias && norm) append_kernel<HD, true, true><<<grid, 256, 0, st>>>(a);
-    else if (a.bias) append_kernel<HD, true, false><<<grid, 256, 0, st>>>(a);
-    else if (norm) append_kernel<HD, false, true><<<grid, 256, 0, st>>>(a);
-    else append_kernel<HD, false, false><<<grid, 256, 0, st>>>(a);
+    if (a.bias && norm) append_rows<HD, true, true>(a, st);
+    else if (a.bias) append_rows<HD, true, false>(a, st);
+    else if (norm) append_rows<HD, false, true>(a, st);
+    else append_rows<HD, false, false>(a, st);
 }
 
 }  // namespace
@@ -184,7 +285,8 @@ int myl_kv_append_paged_dev(myl_ctx* ctx, const int16_t* q, size_t ldq, const in
     a.page_stride = page_stride; a.head_stride = head_stride; a.pos_stride = pos_stride; a.ldt = table_stride;
     const size_t per_row = (heads + 2 * kv_heads) * (head_dim / 16);
     a.per_row = SmallDiv::of(per_row); a.n_pos = SmallDiv::of(lut_len / half); a.page = SmallDiv::of(page_size);
-    a.items = (int)(rows * per_row); a.heads = (int)heads; a.kv_heads = (int)kv_heads;
+    a.rows = (int)rows; a.group = append_group(rows, per_row, ctx->prop.multiProcessorCount);
+    a.items = (int)((rows + (size_t)a.group - 1) / (size_t)a.group * per_row); a.heads = (int)heads; a.kv_heads = (int)kv_heads;
     a.n_seqs = (int)n_seqs; a.table_len = (int)table_len; a.n_pages = (int)n_pages;
     a.q_frac = q_frac; a.k_frac = k_frac; a.v_frac = v_frac; a.rope_frac = rope_frac;
     const bool normed = norm && (norm->q_gamma || norm->k_gamma);

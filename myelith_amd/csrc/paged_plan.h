@@ -46,6 +46,12 @@ inline const char* append_refuse(size_t rows, size_t heads, size_t kv_heads, siz
     return nullptr;
 }
 
+// Rows of a thread: as many as leave a CU eight blocks of 256 threads, in fours (or one).
+inline int append_group(size_t rows, size_t per_row, int cus) {
+    const size_t each = rows * per_row / ((size_t)cus * 8 * 256);
+    return each < 4 ? 1 : (int)std::min<size_t>(each / 4 * 4, 16);
+}
+
 // ---- attention ------------------------------------------------------------------
 
 // At most 131072 keys per row: with non-negative table entries below 2^15 the exp sums
