@@ -659,9 +659,14 @@ class RocmBackend:
         return accepted, out
 
     # ---- a serving step over a paged cache --------------------------------------
+    # Small calls are bound by these checks: the ordinary case is one condition, and what
+    # fails it is looked at piece by piece.
     @staticmethod
     def _rows_of(what: str, name: str, t, inner: int) -> int:
         """The row stride of [rows x heads x hd] whose heads follow one another."""
+        row, head, one = t.stride()
+        if one == 1 and head == t.shape[2] and row >= inner and t.shape[0] > 1:
+            return row
         row, head, one = _strides(t)
         if head not in (None, t.shape[2]) or one not in (None, 1):
             raise ValueError(f"{what}: the heads of a row of {name} follow one another")
@@ -671,17 +676,18 @@ class RocmBackend:
     def _pages_of(what: str, k_pages, v_pages, tables):
         """(page, head, position) strides of [pages x kv_heads x page_size x hd] tensors, and
         the table rows' stride."""
-        n, KH, page, hd = k_pages.shape
+        _, KH, page, hd = k_pages.shape
         if v_pages.shape != k_pages.shape:
             raise ValueError(f"{what}: k_pages and v_pages [pages x kv_heads x page_size x hd]")
-        _need_dev(what, k_pages.device, k_pages=(k_pages, "int16", None), v_pages=(v_pages, "int16", None), tables=(tables, "int32", None))
+        if tables.dim() != 2:
+            raise ValueError(f"{what}: tables must be [sequences x pages of each]")
+        if k_pages.is_contiguous() and v_pages.is_contiguous() and tables.is_contiguous():
+            return KH * page * hd, page * hd, hd, tables.shape[1]
         st = _strides(k_pages)
         if k_pages.stride() != v_pages.stride() and st != _strides(v_pages):
             raise ValueError(f"{what}: keys and values have the same strides")
         if st[3] not in (None, 1):
             raise ValueError(f"{what}: the elements of a position follow one another")
-        if tables.dim() != 2:
-            raise ValueError(f"{what}: tables must be [sequences x pages of each]")
         row, one = _strides(tables)
         if one not in (None, 1):
             raise ValueError(f"{what}: the entries of a sequence's table follow one another")
@@ -698,31 +704,42 @@ class RocmBackend:
         [positions x hd / 2], bias int16 and bias_shifts uint8 [(heads + 2 kv_heads) hd] or
         None, norm a HeadNorm or None.  Returns q_out, the rotated queries; it may be q
         itself.  include/myl_hip.h states the arithmetic."""
+        import torch
         what = "kv_append_paged_dev"
         if (rope_frac | q_frac | k_frac | v_frac) >> 8:
             _need_bytes(what, rope_frac=rope_frac, q_frac=q_frac, k_frac=k_frac, v_frac=v_frac)
         R, H, hd = q.shape
-        KH, page = k_pages.shape[1:3]
+        n_pages, KH, page, page_hd = k_pages.shape
         dev = q.device
-        if not (k.shape == v.shape == (R, KH, hd) and k_pages.shape[3] == hd):
+        if not (k.shape == v.shape == (R, KH, hd) and page_hd == hd):
             raise ValueError(f"{what}: q [rows x heads x hd], k and v [rows x kv_heads x hd], pages of those heads")
         strides = self._pages_of(what, k_pages, v_pages, tables)
-        _need_dev(what, dev, q=(q, "int16", None), k=(k, "int16", None), v=(v, "int16", None), k_pages=(k_pages, "int16", None),
-                  positions=(positions, "int32", (R,)), cos_lut=(cos_lut, "int16", (cos_lut.shape[0], hd // 2)),
-                  sin_lut=(sin_lut, "int16", cos_lut.shape))
-        if seqs is not None:
-            _need_dev(what, dev, seqs=(seqs, "int32", (R,)))
         if (bias is None) != (bias_shifts is None):
             raise ValueError(f"{what}: bias and bias_shifts go together")
-        if bias is not None:
-            n = ((H + 2 * KH) * hd,)
-            _need_dev(what, dev, bias=(bias, "int16", n), bias_shifts=(bias_shifts, "uint8", n))
+        i16, i32, d = torch.int16, torch.int32, q.get_device()
+        n_lut, n_bias = cos_lut.numel(), (H + 2 * KH) * hd
+        if not (q.dtype is i16 and k.dtype is i16 and v.dtype is i16 and k_pages.dtype is i16 and v_pages.dtype is i16 and
+                cos_lut.dtype is i16 and sin_lut.dtype is i16 and tables.dtype is i32 and positions.dtype is i32 and
+                k.get_device() == d and v.get_device() == d and k_pages.get_device() == d and v_pages.get_device() == d and
+                cos_lut.get_device() == d and sin_lut.get_device() == d and tables.get_device() == d and positions.get_device() == d and
+                positions.shape == (R,) and positions.is_contiguous() and cos_lut.shape == sin_lut.shape == (n_lut // max(hd // 2, 1), hd // 2) and
+                cos_lut.is_contiguous() and sin_lut.is_contiguous()):
+            _need_dev(what, dev, q=(q, "int16", None), k=(k, "int16", None), v=(v, "int16", None), k_pages=(k_pages, "int16", None),
+                      v_pages=(v_pages, "int16", None), tables=(tables, "int32", None), positions=(positions, "int32", (R,)),
+                      cos_lut=(cos_lut, "int16", (cos_lut.shape[0], hd // 2)), sin_lut=(sin_lut, "int16", cos_lut.shape))
+        if seqs is not None and not (seqs.dtype is i32 and seqs.get_device() == d and seqs.shape == (R,) and seqs.is_contiguous()):
+            _need_dev(what, dev, seqs=(seqs, "int32", (R,)))
+        if bias is not None and not (bias.dtype is i16 and bias_shifts.dtype is torch.uint8 and bias.get_device() == d and
+                                     bias_shifts.get_device() == d and bias.shape == bias_shifts.shape == (n_bias,) and bias.is_contiguous() and
+                                     bias_shifts.is_contiguous()):
+            _need_dev(what, dev, bias=(bias, "int16", (n_bias,)), bias_shifts=(bias_shifts, "uint8", (n_bias,)))
         if norm is not None and (norm.device != dev or norm.head_dim != hd):
             raise ValueError(f"{what}: norm must be of head_dim values on {dev}")
         stream = self._other_stream(dev) if q_out is None else None
         if q_out is None:
             q_out = self._empty((R, H, hd), "int16", dev, stream)
-        _need_dev(what, dev, q_out=(q_out, "int16", None))
+        elif not (q_out.dtype is i16 and q_out.get_device() == d):
+            _need_dev(what, dev, q_out=(q_out, "int16", None))
         if q_out.shape != q.shape:
             raise ValueError(f"{what}: q_out must have q's shape")
         ldq, ldo = self._rows_of(what, "q", q, H * hd), self._rows_of(what, "q_out", q_out, H * hd)
@@ -733,9 +750,9 @@ class RocmBackend:
         rc = lib().myl_kv_append_paged_dev(
             self._h, q.data_ptr(), ldq, k.data_ptr(), ldk, v.data_ptr(), ldv, R, H, KH, hd,
             None if bias is None else bias.data_ptr(), None if bias is None else bias_shifts.data_ptr(), q_frac, k_frac, v_frac,
-            None if norm is None else C.byref(norm.args), cos_lut.data_ptr(), sin_lut.data_ptr(), cos_lut.numel(), rope_frac,
+            None if norm is None else C.byref(norm.args), cos_lut.data_ptr(), sin_lut.data_ptr(), n_lut, rope_frac,
             positions.data_ptr(), None if seqs is None else seqs.data_ptr(), tables.data_ptr(), tables.shape[0], tables.shape[1],
-            strides[3], k_pages.data_ptr(), v_pages.data_ptr(), k_pages.shape[0], page, *strides[:3], q_out.data_ptr(), ldo)
+            strides[3], k_pages.data_ptr(), v_pages.data_ptr(), n_pages, page, strides[0], strides[1], strides[2], q_out.data_ptr(), ldo)
         if rc:
             self.check(rc, what)
         return q_out
@@ -755,15 +772,16 @@ class RocmBackend:
         lens[r] positions of its sequence (at most max_len, by default all that the table
         names) that lie on a page; without any its output is zero.  include/myl_hip.h
         states the arithmetic."""
+        import torch
         what = "attention_paged_dev"
         if (score_shift | lut_shift | prob_frac) >> 8:
             _need_bytes(what, score_shift=score_shift, lut_shift=lut_shift, prob_frac=prob_frac)
         if not -2**63 <= score_mult < 2**63:
             raise ValueError(f"{what}: score_mult must be an int64, not {score_mult}")
         R, H, hd = q.shape
-        n_pages, KH, page = k_pages.shape[:3]
+        n_pages, KH, page, page_hd = k_pages.shape
         dev = q.device
-        if k_pages.shape[3] != hd:
+        if page_hd != hd:
             raise ValueError(f"{what}: pages of q's head_dim")
         strides = self._pages_of(what, k_pages, v_pages, tables)
         n_seqs, table_len = tables.shape
@@ -774,12 +792,19 @@ class RocmBackend:
             max_len = most
         elif not 0 <= max_len <= most:
             raise ValueError(f"{what}: max_len is at most what the tables name")
-        _need_dev(what, dev, q=(q, "int16", None), k_pages=(k_pages, "int16", None), lens=(lens, "int32", (R,)),
-                  exp_lut=(exp_lut, "int16", (exp_lut.numel(),)))
+        i16, i32, d = torch.int16, torch.int32, q.get_device()
+        n_lut = exp_lut.numel()
+        if not (q.dtype is i16 and k_pages.dtype is i16 and v_pages.dtype is i16 and exp_lut.dtype is i16 and tables.dtype is i32 and
+                lens.dtype is i32 and k_pages.get_device() == d and v_pages.get_device() == d and exp_lut.get_device() == d and
+                tables.get_device() == d and lens.get_device() == d and lens.shape == (R,) and lens.is_contiguous() and
+                exp_lut.dim() == 1 and exp_lut.is_contiguous()):
+            _need_dev(what, dev, q=(q, "int16", None), k_pages=(k_pages, "int16", None), v_pages=(v_pages, "int16", None),
+                      tables=(tables, "int32", None), lens=(lens, "int32", (R,)), exp_lut=(exp_lut, "int16", (n_lut,)))
         stream = self._other_stream(dev) if out is None or workspace is None else None
         if out is None:
             out = self._empty((R, H, hd), "int16", dev, stream)
-        _need_dev(what, dev, out=(out, "int16", None))
+        elif not (out.dtype is i16 and out.get_device() == d):
+            _need_dev(what, dev, out=(out, "int16", None))
         if out.shape != q.shape:
             raise ValueError(f"{what}: out must have q's shape")
         ldq, ldo = self._rows_of(what, "q", q, H * hd), self._rows_of(what, "out", out, H * hd)
@@ -789,8 +814,8 @@ class RocmBackend:
             self._after_last_use(what, dev, stream)
         rc = lib().myl_attention_paged_dev(
             self._h, q.data_ptr(), n_seqs, rows_per_seq, ldq, H, KH, hd, k_pages.data_ptr(), v_pages.data_ptr(), n_pages, page,
-            *strides[:3], tables.data_ptr(), table_len, strides[3], lens.data_ptr(), max_len, score_mult, score_shift,
-            exp_lut.data_ptr(), exp_lut.numel(), lut_shift, prob_frac, out.data_ptr(), ldo, ws.data_ptr(),
+            strides[0], strides[1], strides[2], tables.data_ptr(), table_len, strides[3], lens.data_ptr(), max_len, score_mult,
+            score_shift, exp_lut.data_ptr(), n_lut, lut_shift, prob_frac, out.data_ptr(), ldo, ws.data_ptr(),
             ws.numel() * ws.element_size())
         if rc:
             self.check(rc, what)
@@ -808,16 +833,20 @@ class RocmBackend:
         [rows x n] (one outside the vocabulary gives 0), exp_lut int16.  Returns
         (logprobs of tokens' shape, entropy [rows], top_tokens and top_logprobs
         [rows x top_n]); include/myl_hip.h states the arithmetic."""
+        import torch
         what = "logprobs_dev"
         R, V = logits.shape
-        dev = logits.device
-        T = tokens.shape[1] if tokens.dim() == 2 else 1
-        if tokens.dim() not in (1, 2):
+        dev, shape = logits.device, tokens.shape
+        if len(shape) not in (1, 2):
             raise ValueError(f"{what}: tokens must be [rows] or [rows x n]")
+        T = shape[1] if len(shape) == 2 else 1
         if top_n < 0:
             raise ValueError(f"{what}: top_n must not be negative")
-        _need_dev(what, dev, logits=(logits, "int32", None), tokens=(tokens, "int64", (R, *tokens.shape[1:])),
-                  exp_lut=(exp_lut, "int16", (exp_lut.numel(),)))
+        i64, d = torch.int64, logits.get_device()
+        n_lut = exp_lut.numel()
+        if not (logits.dtype is torch.int32 and tokens.dtype is i64 and exp_lut.dtype is torch.int16 and tokens.get_device() == d and
+                exp_lut.get_device() == d and shape[0] == R and tokens.is_contiguous() and exp_lut.dim() == 1 and exp_lut.is_contiguous()):
+            _need_dev(what, dev, logits=(logits, "int32", None), tokens=(tokens, "int64", (R, *shape[1:])), exp_lut=(exp_lut, "int16", (n_lut,)))
         ldz, one = _strides(logits)
         if one not in (None, 1):
             raise ValueError(f"{what}: the logits of a row follow one another")
@@ -825,21 +854,25 @@ class RocmBackend:
         left_out = logprobs is None or entropy is None or top_tokens is None or top_logprobs is None
         stream = self._other_stream(dev) if left_out or workspace is None else None
         if logprobs is None:
-            logprobs = self._empty(tokens.shape, "int64", dev, stream)
+            logprobs = self._empty(shape, "int64", dev, stream)
         if entropy is None:
             entropy = self._empty(R, "int64", dev, stream)
         if top_tokens is None:
             top_tokens = self._empty((R, top_n), "int64", dev, stream)
         if top_logprobs is None:
             top_logprobs = self._empty((R, top_n), "int64", dev, stream)
-        _need_dev(what, dev, logprobs=(logprobs, "int64", tokens.shape), entropy=(entropy, "int64", (R,)),
-                  top_tokens=(top_tokens, "int64", (R, top_n)), top_logprobs=(top_logprobs, "int64", (R, top_n)))
+        if not (logprobs.dtype is i64 and entropy.dtype is i64 and top_tokens.dtype is i64 and top_logprobs.dtype is i64 and
+                logprobs.get_device() == d and entropy.get_device() == d and top_tokens.get_device() == d and top_logprobs.get_device() == d and
+                logprobs.shape == shape and entropy.shape == (R,) and top_tokens.shape == top_logprobs.shape == (R, top_n) and
+                logprobs.is_contiguous() and entropy.is_contiguous() and top_tokens.is_contiguous() and top_logprobs.is_contiguous()):
+            _need_dev(what, dev, logprobs=(logprobs, "int64", shape), entropy=(entropy, "int64", (R,)),
+                      top_tokens=(top_tokens, "int64", (R, top_n)), top_logprobs=(top_logprobs, "int64", (R, top_n)))
         self._need_here(what, dev)
-        ws = self._workspace(dev, workspace, stream, lib().myl_logprobs_workspace, R, V, top_n, exp_lut.numel())
+        ws = self._workspace(dev, workspace, stream, lib().myl_logprobs_workspace, R, V, top_n, n_lut)
         if stream is not None:
             self._after_last_use(what, dev, stream)
         rc = lib().myl_logprobs_dev(
-            self._h, logits.data_ptr(), R, V, ldz, exp_lut.data_ptr(), exp_lut.numel(), tokens.data_ptr(), T, top_n,
+            self._h, logits.data_ptr(), R, V, ldz, exp_lut.data_ptr(), n_lut, tokens.data_ptr(), T, top_n,
             logprobs.data_ptr(), entropy.data_ptr(), top_tokens.data_ptr(), top_logprobs.data_ptr(), ws.data_ptr(),
             ws.numel() * ws.element_size())
         if rc:

@@ -64,10 +64,9 @@ __device__ inline int vector_of(const PagedAttn& a, const Part& p, int v, int& h
 // The keys of a row, counted from position 0.
 __device__ inline int keys_of(const PagedAttn& a, int row) { return min(max(a.lens[row], 0), a.max_len); }
 
-// False: no keys (p.tile < 0: no tile either).  lim: the keys of the lane's vector, lane % 16.
-// Blocks of the tiles that read one range follow one another on one XCD (block b runs on
-// XCD b % 8).
-__device__ inline bool part_of(const PagedAttn& a, Part& p, int& lim) {
+// The block's tile and range; false: none.  Blocks of the tiles that read one range follow one
+// another on one XCD (block b runs on XCD b % 8).
+__device__ inline bool place_of_block(const PagedAttn& a, Part& p) {
     int tile, rest;
     const int q = divmod(a.tiles, (int)(blockIdx.x >> 3), tile), i = 8 * q + (int)(blockIdx.x & 7);
     p.tile = -1;
@@ -78,12 +77,24 @@ __device__ inline bool part_of(const PagedAttn& a, Part& p, int& lim) {
     p.v0 = tile * a.width;
     p.nv = min(a.width, a.vectors - p.v0);
     p.row0 = p.seq * (int)a.n.d;
-    int head;
-    lim = keys_of(a, vector_of(a, p, threadIdx.x & 15, head));
     p.j0 = p.range * a.range;
+    return true;
+}
+// The range's end; false: it has no key.  Returns the keys of the thread's vector, v % 16, in lim.
+__device__ inline bool ends_of(const PagedAttn& a, Part& p, int v, int& lim) {
+    int head;
+    lim = keys_of(a, vector_of(a, p, v & 15, head));
     p.j1 = min(p.j0 + a.range, wave_max_i32(lim));
     p.lmin = ~wave_max_i32(~lim);
     return p.j0 < p.j1;
+}
+__device__ inline bool ends_of(const PagedAttn& a, Part& p, int v) {
+    int lim;
+    return ends_of(a, p, v, lim);
+}
+// Both; lim of vector lane % 16.  p.tile < 0: the block has no tile.
+__device__ inline bool part_of(const PagedAttn& a, Part& p, int& lim) {
+    return place_of_block(a, p) && ends_of(a, p, threadIdx.x, lim);
 }
 
 // The element offsets of a range's pages in LDS, kNoPage where a table names none.  The table
@@ -374,60 +385,98 @@ __device__ inline int lim_of(const PagedAttn& a, const Part& p, int v) {
     return keys_of(a, vector_of(a, p, v, head));
 }
 
-// e_j and their sums.  A few LDS lookups per four keys: bound by the latency of a launch and of
-// reading the scores.
+// e_j and their sums.  Bound by latency (a launch that loads, computes and stores once), so every
+// load that needs no other's result is issued first: the rows' lengths, the ranges' maxima, the
+// table's start and the thread's first scores.
 constexpr uint32_t kSumLut = 8192;  // entries in LDS
+constexpr int kSumAhead = 4, kFoldAhead = 4;
+// Eight table entries, negative ones as 0, and 0 from entry n on.
+__device__ inline uint4 table8(const int16_t* lut, uint32_t i, uint32_t n) {
+    uint32_t w[4] = {0, 0, 0, 0};
+    if (i + 8 <= n) {
+        const uint4 x = *reinterpret_cast<const uint4*>(lut + i);
+        w[0] = x.x; w[1] = x.y; w[2] = x.z; w[3] = x.w;
+    } else {
+#pragma unroll
+        for (uint32_t k = 0; k < 8; ++k)
+            if (i + k < n) w[k / 2] |= (uint32_t)(uint16_t)lut[i + k] << (16 * (k & 1));
+    }
+#pragma unroll
+    for (int k = 0; k < 4; ++k) w[k] &= ((w[k] & 0x8000u) ? 0u : 0xFFFFu) | ((w[k] >> 31) ? 0u : 0xFFFF0000u);
+    return make_uint4(w[0], w[1], w[2], w[3]);
+}
 __global__ __launch_bounds__(256) void paged_sum_kernel(PagedAttn a) {
     extern __shared__ __align__(16) uint64_t tab[];
-    __shared__ uint16_t lut[kSumLut + 1];
+    __shared__ __align__(16) uint16_t lut[kSumLut + 8];
     __shared__ int32_t s_max[16];
     __shared__ uint32_t s_sum[16];
     __shared__ int bad[4];
     Part p;
-    int lane_lim;
-    if (!part_of(a, p, lane_lim)) return;
+    if (!place_of_block(a, p)) return;
     const int tid = threadIdx.x;
     const Lanes l = Lanes::of(a);
+    const size_t at = (size_t)p.tile * a.ranges, base = (size_t)p.tile * a.width * a.keys;
+    const uint32_t have = min(a.lut_len, kSumLut);
+    // within the workspace whatever the lengths: groups of four keys below a.keys
+    auto group = [&](int i) { return (p.j0 >> 2) + l.k + i * l.step; };
+    int4 z4[kSumAhead];
+#pragma unroll
+    for (int i = 0; i < kSumAhead; ++i) z4[i] = *reinterpret_cast<const int4*>(a.z + base + ((size_t)min(group(i), a.keys / 4 - 1) * a.width + l.c) * 4);
+    int32_t m4[kFoldAhead];
+#pragma unroll
+    for (int i = 0; i < kFoldAhead; ++i) m4[i] = a.pmax[(at + min(l.k + i * l.step, a.ranges - 1)) * a.width + l.c];
+    const int any_holes = a.holes[at + p.range];
+    uint4 t8[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) t8[i] = table8(a.lut, 8u * (tid + 256u * i), have);
     const int lim = lim_of(a, p, l.c);
-    const size_t at = (size_t)p.tile * a.ranges;
-    const bool holes = __builtin_amdgcn_readfirstlane(a.holes[at + p.range]) != 0;
+    if (!ends_of(a, p, tid)) return;
+    const bool holes = __builtin_amdgcn_readfirstlane(any_holes) != 0;
     int p0 = 0;
     if (holes) p0 = pages_of_range(a, p, tab, bad);
     if (tid < 16) {
         s_max[tid] = INT32_MIN;
         s_sum[tid] = 0;
     }
-    const uint32_t have = min(a.lut_len, kSumLut);
-    for (uint32_t i = tid; i <= have; i += 256) lut[i] = i < have ? (uint16_t)max((int32_t)a.lut[i], 0) : (uint16_t)0;
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+        if (8u * (tid + 256u * i) <= have) *reinterpret_cast<uint4*>(lut + 8 * (tid + 256 * i)) = t8[i];
+    for (uint32_t i = 8u * (tid + 512u); i <= have; i += 8u * 256u) *reinterpret_cast<uint4*>(lut + i) = table8(a.lut, i, have);
     __syncthreads();
     int32_t m = INT32_MIN;
-    if (l.step)
-        for (int r = l.k; r < a.ranges && r * a.range < lim; r += l.step) m = max(m, a.pmax[(at + r) * a.width + l.c]);
-    if (l.step) atomicMax(&s_max[l.c], m);
+#pragma unroll
+    for (int i = 0; i < kFoldAhead; ++i)
+        if (l.k + i * l.step < a.ranges && (l.k + i * l.step) * a.range < lim) m = max(m, m4[i]);
+    if (l.step) {
+        for (int r = l.k + kFoldAhead * l.step; r < a.ranges && r * a.range < lim; r += l.step) m = max(m, a.pmax[(at + r) * a.width + l.c]);
+        atomicMax(&s_max[l.c], m);
+    }
     __syncthreads();
     m = s_max[l.c];
     uint32_t s = 0;
-    const size_t base = (size_t)p.tile * a.width * a.keys;
-    if (l.step)
-        for (int k = (p.j0 >> 2) + l.k; 4 * k < p.j1; k += l.step) {
-            const size_t o = base + ((size_t)k * a.width + l.c) * 4;
-            const int4 z4 = *reinterpret_cast<const int4*>(a.z + o);
-            const int32_t z[4] = {z4.x, z4.y, z4.z, z4.w};
-            uint32_t e[4];
+    auto one = [&](int k, const int4& v) {
+        const int32_t z[4] = {v.x, v.y, v.z, v.w};
+        uint32_t e[4];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                // sat_sub and the lookup of softmax.rs:12-38
-                const uint32_t below = min((uint32_t)m - (uint32_t)z[i], 0x7FFFFFFFu) >> (a.lut_shift & 31u);
-                uint32_t v = lut[min(below, have)];
-                if (below >= have && below < a.lut_len) v = (uint32_t)max((int32_t)a.lut[below], 0);
-                bool ok = 4 * k + i < lim;
-                if (holes) ok = ok && on_page(a, tab, p0, min(4 * k + i, p.j1 - 1));
-                e[i] = ok ? v : 0u;
-                s += e[i];
-            }
-            *reinterpret_cast<uint2*>(a.e + o) = make_uint2(e[0] | (e[1] << 16), e[2] | (e[3] << 16));
+        for (int i = 0; i < 4; ++i) {
+            // sat_sub and the lookup of softmax.rs:12-38
+            const uint32_t below = min((uint32_t)m - (uint32_t)z[i], 0x7FFFFFFFu) >> (a.lut_shift & 31u);
+            uint32_t x = lut[min(below, have)];
+            if (below >= have && below < a.lut_len) x = (uint32_t)max((int32_t)a.lut[below], 0);
+            bool ok = 4 * k + i < lim;
+            if (holes) ok = ok && on_page(a, tab, p0, min(4 * k + i, p.j1 - 1));
+            e[i] = ok ? x : 0u;
+            s += e[i];
         }
-    if (l.step) atomicAdd(&s_sum[l.c], s);
+        *reinterpret_cast<uint2*>(a.e + base + ((size_t)k * a.width + l.c) * 4) = make_uint2(e[0] | (e[1] << 16), e[2] | (e[3] << 16));
+    };
+    if (l.step) {
+#pragma unroll
+        for (int i = 0; i < kSumAhead; ++i)
+            if (4 * group(i) < p.j1) one(group(i), z4[i]);
+        for (int k = group(kSumAhead); 4 * k < p.j1; k += l.step) one(k, *reinterpret_cast<const int4*>(a.z + base + ((size_t)k * a.width + l.c) * 4));
+        atomicAdd(&s_sum[l.c], s);
+    }
     __syncthreads();
     if (tid < a.width) a.psum[(at + p.range) * a.width + tid] = s_sum[tid];
 }
@@ -474,7 +523,7 @@ __device__ inline void fold_rows(int32_t (&x)[R]) {
 // every vector (p <= 2^14 fits a signed 16-bit half), while the first values are on
 // their way; then the values stream through the waves' rings.  A lane holds 8 dimensions
 // of two neighbouring keys, paired for v_dot2.  W: 8 or 16 vectors at most.
-constexpr int kPvRing = 2;
+constexpr int kPvRing = 2, kPvAhead = 4;
 template <int HD, int W, bool ALIGNED>
 __global__ __launch_bounds__(256, W == 8 ? 4 : 2) void paged_pv_kernel(PagedAttn a) {
     using T = Tiles<HD, kPvRing, ALIGNED, false>;
@@ -485,9 +534,21 @@ __global__ __launch_bounds__(256, W == 8 ? 4 : 2) void paged_pv_kernel(PagedAttn
     uint32_t* const ps = reinterpret_cast<uint32_t*>(lds + 4 * NB * T::kBytes);  // [range / 2][W]
     uint64_t* const tab = reinterpret_cast<uint64_t*>(ps + (size_t)a.range / 2 * W);
     Part p;
-    int lane_lim;
-    const bool some = part_of(a, p, lane_lim);
-    if (!some && (p.tile < 0 || a.ranges > 1)) return;
+    if (!place_of_block(a, p)) return;
+    // what needs no other load's result first: sums of ranges, exp values (within the workspace
+    // whatever the lengths)
+    const Lanes l = Lanes::of(a);
+    const size_t at = (size_t)p.tile * a.ranges;
+    const uint16_t* et = a.e + (size_t)p.tile * a.keys * a.width + 4 * l.c;
+    auto exps = [&](int k) { return reinterpret_cast<const uint2*>(et + (size_t)min(p.j0 + 4 * k, a.keys - 4) * a.width); };
+    uint2 e4[kPvAhead];
+    uint32_t s4[kFoldAhead];
+#pragma unroll
+    for (int i = 0; i < kFoldAhead; ++i) s4[i] = a.psum[(at + min(l.k + i * l.step, a.ranges - 1)) * a.width + l.c];
+#pragma unroll
+    for (int i = 0; i < kPvAhead; ++i) e4[i] = *exps(l.k + i * l.step);
+    const bool some = ends_of(a, p, threadIdx.x);
+    if (!some && a.ranges > 1) return;
     if (!some) {  // the only range has no key
         for (int i = threadIdx.x; i < p.nv * HD; i += 256) {
             int head;
@@ -497,11 +558,9 @@ __global__ __launch_bounds__(256, W == 8 ? 4 : 2) void paged_pv_kernel(PagedAttn
         return;
     }
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    const Lanes l = Lanes::of(a);
     const int lim = lim_of(a, p, l.c);
-    const size_t at = (size_t)p.tile * a.ranges;
-    const int p0 = pages_of_range(a, p, tab, bad);
     if (tid < 16) s_sum[tid] = 0;
+    const int p0 = pages_of_range(a, p, tab, bad);
     __syncthreads();
     T tiles;
     tiles.begin(a, a.vp, lds + wave * NB * T::kBytes);
@@ -512,22 +571,24 @@ __global__ __launch_bounds__(256, W == 8 ? 4 : 2) void paged_pv_kernel(PagedAttn
         if (t < n) tiles.issue(a, tab, p0, jw + 64 * t, p.j1, t);
     const bool holes = (bad[0] | bad[1] | bad[2] | bad[3]) != 0;
     uint32_t s = 0;
-    if (l.step)
-        for (int r = l.k; r < a.ranges && r * a.range < lim; r += l.step) s += a.psum[(at + r) * a.width + l.c];
-    if (l.step && s) atomicAdd(&s_sum[l.c], s);
+#pragma unroll
+    for (int i = 0; i < kFoldAhead; ++i)
+        if (l.k + i * l.step < a.ranges && (l.k + i * l.step) * a.range < lim) s += s4[i];
+    if (l.step) {
+        for (int r = l.k + kFoldAhead * l.step; r < a.ranges && r * a.range < lim; r += l.step) s += a.psum[(at + r) * a.width + l.c];
+        if (s) atomicAdd(&s_sum[l.c], s);
+    }
     block_barrier();
     s = s_sum[l.c];
     if (l.step) {
         const ProbDiv div = ProbDiv::of(s ? s : 1u, a.prob_frac);
         Uniform uni{0, 0, 0};
         if (s == 0) uni = uniform_of(a, p, lim);
-        const uint16_t* et = a.e + ((size_t)p.tile * a.keys + p.j0) * a.width + 4 * l.c;
         const int groups = (p.j1 - p.j0 + 15) / 16 * 4;
-        for (int k = l.k; k < groups; k += l.step) {
+        auto one = [&](int k, const uint2& x) {
             uint2 two = make_uint2(0, 0);
             const int key = p.j0 + 4 * k;
             if (key < p.j1) {
-                const uint2 x = *reinterpret_cast<const uint2*>(et + (size_t)k * 4 * a.width);
                 two.x = div(x.x & 0xFFFFu) | (div(x.x >> 16) << 16);
                 two.y = div(x.y & 0xFFFFu) | (div(x.y >> 16) << 16);
                 if (s == 0) {
@@ -548,7 +609,11 @@ __global__ __launch_bounds__(256, W == 8 ? 4 : 2) void paged_pv_kernel(PagedAttn
             }
             ps[2 * k * W + l.c] = two.x;
             ps[(2 * k + 1) * W + l.c] = two.y;
-        }
+        };
+#pragma unroll
+        for (int i = 0; i < kPvAhead; ++i)
+            if (l.k + i * l.step < groups) one(l.k + i * l.step, e4[i]);
+        for (int k = l.k + kPvAhead * l.step; k < groups; k += l.step) one(k, *exps(k));
     }
     block_barrier();
     int32_t acc[8 * W];
@@ -628,13 +693,13 @@ __global__ __launch_bounds__(256) void paged_out_kernel(PagedAttn a) {
     const size_t at = (((size_t)seq * a.kvh.d + g) * a.tiles.d + tile) * a.ranges;
     int64_t s[4] = {0, 0, 0, 0};
     const int last = min(a.ranges, (lim + a.range - 1) / max(a.range, 1));
-    for (int r0 = share; r0 < last; r0 += 4 * SHARES) {
-        int4 x[4];
+    for (int r0 = share; r0 < last; r0 += 8 * SHARES) {
+        int4 x[8];
 #pragma unroll
-        for (int k = 0; k < 4; ++k)
+        for (int k = 0; k < 8; ++k)
             x[k] = r0 + k * SHARES < last ? *reinterpret_cast<const int4*>(a.pout + ((at + r0 + k * SHARES) * a.width + v) * HD + 4 * q) : make_int4(0, 0, 0, 0);
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
+        for (int k = 0; k < 8; ++k) {
             s[0] += x[k].x;
             s[1] += x[k].y;
             s[2] += x[k].z;
