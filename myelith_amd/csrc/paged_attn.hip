@@ -210,6 +210,13 @@ struct Tiles {
     }
 };
 
+// How many of a range's tiles fall to a wave, every NW-th.
+template <int NW>
+__device__ inline int tiles_of_wave(const Part& p, int wave) {
+    static_assert((NW & (NW - 1)) == 0, "a shift");
+    return max(((p.j1 - p.j0 + 15) >> 4) - wave + NW - 1, 0) / NW;
+}
+
 // Scores on v_mfma_i32_16x16x64_i8: K positions are rows, vectors columns, so lane l holds
 // vector l % 16 and positions 4 (l / 16) .. + 3 of a 16-position tile.  The byte planes of the
 // keys are k = 256 kh + kl + 128 with kl = (k & 255) - 128; those of the queries q = 256 qh +
@@ -221,20 +228,20 @@ struct Tiles {
 // other scales take the 64-bit form (FAST false).
 // Bound by issue and by the loads' latency: about 120 vector and 8 matrix instructions a tile.
 constexpr int kQkRing = 2;
-template <int HD, bool FAST, bool ALIGNED, bool BALANCED>
+// NW: waves of the block, a tile in turn each.  STORED: the scores go to memory, not LDS.
+template <int HD, bool FAST, bool ALIGNED, bool BALANCED, int NW, bool STORED>
 __device__ inline void paged_scores(const PagedAttn& a, const Part& p, int lim, const uint64_t* tab, int p0, bool holes, int8_t* ring,
-                                    const uint4 (&qx)[HD / 64][2], int32_t* red) {
+                                    const uint4 (&qx)[HD / 64][2], int32_t* z0, int32_t* red) {
     using T = Tiles<HD, kQkRing, ALIGNED, true>;
     constexpr int NS = HD / 64, NB = kQkRing;
     const int lane = threadIdx.x & 63, c = lane & 15, kb = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     T tiles;
     tiles.begin(a, a.kp, ring);
-    const int n = max(((p.j1 - p.j0 + 15) >> 4) - wave + 3, 0) >> 2;  // the wave's tiles, every fourth
-    const int jw = p.j0 + 16 * wave;
+    const int n = tiles_of_wave<NW>(p, wave), jw = p.j0 + 16 * wave;
 #pragma unroll
     for (int t = 0; t < NB; ++t)
-        if (t < n) tiles.issue(a, tab, p0, jw + 64 * t, p.j1, t);
+        if (t < n) tiles.issue(a, tab, p0, jw + 16 * NW * t, p.j1, t);
     v4i32_t qh[NS], ql[NS];
     int32_t qsum = 0;
 #pragma unroll
@@ -257,13 +264,13 @@ __device__ inline void paged_scores(const PagedAttn& a, const Part& p, int lim, 
     qsum += __shfl_xor(qsum, 16, 64);
     qsum = 128 * (qsum + __shfl_xor(qsum, 32, 64));
     const v4i32_t sixty4 = {0x40404040, 0x40404040, 0x40404040, 0x40404040}, zero = {0, 0, 0, 0}, qs4 = {qsum, qsum, qsum, qsum};
-    int32_t* const zt = a.z + (size_t)p.tile * a.width * a.keys + 4 * (kb * a.width + c);
+    int32_t* const zt = z0 + 4 * (kb * a.width + c);
     int32_t best = INT32_MIN;
     int slot = 0;
     for (int t = 0; t < n; ++t) {
-        const int j = jw + 64 * t;
+        const int j = jw + 16 * NW * t;
         // one score store at least for each of the last NB - 1 tiles lies between
-        if (t >= NB) T::template wait<NB - 1>(n - 1 - t);
+        if (STORED && t >= NB) T::template wait<NB - 1>(n - 1 - t);
         else T::template wait<0>(n - 1 - t);
         const int8_t* k8 = ring + slot * T::kBytes + c * 2 * HD;
         v4i32_t raw[NS][2];
@@ -274,7 +281,7 @@ __device__ inline void paged_scores(const PagedAttn& a, const Part& p, int lim, 
         // in registers before the tile's place is loaded again
         if (NS == 2) asm volatile("s_waitcnt lgkmcnt(0)" : "+v"(raw[0][0]), "+v"(raw[0][1]), "+v"(raw[NS - 1][0]), "+v"(raw[NS - 1][1])::"memory");
         else asm volatile("s_waitcnt lgkmcnt(0)" : "+v"(raw[0][0]), "+v"(raw[0][1])::"memory");
-        if (t + NB < n) tiles.issue(a, tab, p0, j + 64 * NB, p.j1, slot);
+        if (t + NB < n) tiles.issue(a, tab, p0, j + 16 * NW * NB, p.j1, slot);
         slot = slot + 1 == NB ? 0 : slot + 1;
         v4i32_t kh[NS], kl[NS];
 #pragma unroll
@@ -321,24 +328,13 @@ __device__ inline void paged_scores(const PagedAttn& a, const Part& p, int lim, 
     if (kb == 0) red[16 * wave + c] = best;
 }
 
-template <int HD, bool FAST, bool ALIGNED>
-__global__ __launch_bounds__(256, 4) void paged_qk_kernel(PagedAttn a) {
-    using T = Tiles<HD, kQkRing, ALIGNED, true>;
-    constexpr int NS = HD / 64, CH = HD / 8, NB = kQkRing;
-    extern __shared__ __align__(16) int8_t lds[];  // the waves' rings, the range's pages
-    __shared__ __align__(16) int8_t qlds[16 * 2 * HD];
-    __shared__ int32_t red[64];
-    __shared__ int bad[4], large[4];
-    uint64_t* const tab = reinterpret_cast<uint64_t*>(lds + 4 * NB * T::kBytes);
-    Part p;
-    int lim;
-    if (!part_of(a, p, lim)) return;
-    const int tid = threadIdx.x, lane = tid & 63, c = lane & 15, kb = lane >> 4;
-    const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    // the vectors in whole lines
+// A tile's vectors in whole lines to LDS; whether one is too large for the signed low byte, by wave.
+template <int HD>
+__device__ inline void stage_queries(const PagedAttn& a, const Part& p, int8_t* qlds, int* large) {
+    constexpr int CH = HD / 8;
+    const int tid = threadIdx.x, v = tid / CH;
     bool over = false;
-    if (tid / CH < 16) {
-        const int v = tid / CH;
+    if (v < 16) {
         int head;
         const int row = vector_of(a, p, v, head);
         const uint4 x = *reinterpret_cast<const uint4*>(a.q + (size_t)row * a.ldq + (size_t)head * HD + 8 * (tid % CH));
@@ -348,19 +344,49 @@ __global__ __launch_bounds__(256, 4) void paged_qk_kernel(PagedAttn a) {
         for (int i = 0; i < 4; ++i) over |= (int16_t)(w[i] & 0xFFFFu) >= 32640 || (int32_t)w[i] >> 16 >= 32640;
     }
     over = __any(over);
-    if (lane == 0) large[wave] = over ? 1 : 0;
-    const int p0 = pages_of_range(a, p, tab, bad);
-    __syncthreads();
-    const bool holes = (bad[0] | bad[1] | bad[2] | bad[3]) != 0;
+    if ((tid & 63) == 0) large[tid >> 6] = over ? 1 : 0;
+}
+template <int N>
+__device__ inline bool any_of(const int (&x)[N]) {
+    int s = 0;
+#pragma unroll
+    for (int i = 0; i < N; ++i) s |= x[i];
+    return __builtin_amdgcn_readfirstlane(s) != 0;
+}
+
+template <int HD, bool FAST, bool ALIGNED, int NW, bool STORED>
+__device__ inline void scores_of_range(const PagedAttn& a, const Part& p, int lim, const uint64_t* tab, int p0, bool holes, int8_t* rings,
+                                       const int8_t* qlds, bool large, int32_t* z0, int32_t* red) {
+    constexpr int NS = HD / 64, CH = HD / 8;
+    const int lane = threadIdx.x & 63, c = lane & 15, kb = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     uint4 qx[NS][2];
 #pragma unroll
     for (int s = 0; s < NS; ++s)
 #pragma unroll
         for (int i = 0; i < 2; ++i)
             qx[s][i] = *reinterpret_cast<const uint4*>(qlds + c * 2 * HD + (((8 * s + 2 * kb + i) ^ (c & (CH - 1))) << 4));
-    int8_t* const ring = lds + wave * NB * T::kBytes;
-    if (__builtin_amdgcn_readfirstlane(large[0] | large[1] | large[2] | large[3])) paged_scores<HD, FAST, ALIGNED, false>(a, p, lim, tab, p0, holes, ring, qx, red);
-    else paged_scores<HD, FAST, ALIGNED, true>(a, p, lim, tab, p0, holes, ring, qx, red);
+    int8_t* const ring = rings + wave * kQkRing * 32 * HD;
+    if (large) paged_scores<HD, FAST, ALIGNED, false, NW, STORED>(a, p, lim, tab, p0, holes, ring, qx, z0, red);
+    else paged_scores<HD, FAST, ALIGNED, true, NW, STORED>(a, p, lim, tab, p0, holes, ring, qx, z0, red);
+}
+
+template <int HD, bool FAST, bool ALIGNED>
+__global__ __launch_bounds__(256, 4) void paged_qk_kernel(PagedAttn a) {
+    extern __shared__ __align__(16) int8_t lds[];  // the waves' rings, the range's pages
+    __shared__ __align__(16) int8_t qlds[16 * 2 * HD];
+    __shared__ int32_t red[64];
+    __shared__ int bad[4], large[4];
+    uint64_t* const tab = reinterpret_cast<uint64_t*>(lds + 4 * kQkRing * 32 * HD);
+    Part p;
+    int lim;
+    if (!part_of(a, p, lim)) return;
+    const int tid = threadIdx.x;
+    stage_queries<HD>(a, p, qlds, large);
+    const int p0 = pages_of_range(a, p, tab, bad);
+    __syncthreads();
+    const bool holes = any_of(bad);
+    scores_of_range<HD, FAST, ALIGNED, 4, true>(a, p, lim, tab, p0, holes, lds, qlds, any_of(large), a.z + (size_t)p.tile * a.width * a.keys, red);
     __syncthreads();
     const size_t at = (size_t)p.tile * a.ranges + p.range;
     if (tid < a.width) a.pmax[at * a.width + tid] = max(max(red[tid], red[16 + tid]), max(red[32 + tid], red[48 + tid]));
@@ -373,7 +399,7 @@ struct Lanes {
     __device__ static inline Lanes of(const PagedAttn& a) {
         Lanes l;
         int rem;
-        l.step = divmod(a.width_d, 256, rem);
+        l.step = divmod(a.width_d, (int)blockDim.x, rem);
         l.k = divmod(a.width_d, (int)threadIdx.x, l.c);
         if (l.k >= l.step) l.step = 0;
         return l;
@@ -388,7 +414,7 @@ __device__ inline int lim_of(const PagedAttn& a, const Part& p, int v) {
 // e_j and their sums.  Bound by latency (a launch that loads, computes and stores once), so every
 // load that needs no other's result is issued first: the rows' lengths, the ranges' maxima, the
 // table's start and the thread's first scores.
-constexpr uint32_t kSumLut = 8192;  // entries in LDS
+constexpr uint32_t kSumLut = kPagedLdsLut;  // entries in LDS
 constexpr int kSumAhead = 4, kFoldAhead = 4;
 // Eight table entries, negative ones as 0, and 0 from entry n on.
 __device__ inline uint4 table8(const int16_t* lut, uint32_t i, uint32_t n) {
@@ -405,6 +431,43 @@ __device__ inline uint4 table8(const int16_t* lut, uint32_t i, uint32_t n) {
     for (int k = 0; k < 4; ++k) w[k] &= ((w[k] & 0x8000u) ? 0u : 0xFFFFu) | ((w[k] >> 31) ? 0u : 0xFFFF0000u);
     return make_uint4(w[0], w[1], w[2], w[3]);
 }
+// The copy's first entries, before what they wait behind; the rest, and the copy's `have` entries and a 0.
+template <int THREADS>
+struct TableCopy {
+    static constexpr int kEach = 512 / THREADS;
+    uint4 x[kEach];
+    __device__ inline void load(const PagedAttn& a, uint32_t have) {
+#pragma unroll
+        for (int i = 0; i < kEach; ++i) x[i] = table8(a.lut, 8u * (threadIdx.x + (uint32_t)THREADS * i), have);
+    }
+    __device__ inline void store(const PagedAttn& a, uint32_t have, uint16_t* lut) const {
+#pragma unroll
+        for (int i = 0; i < kEach; ++i) {
+            const uint32_t at = 8u * (threadIdx.x + (uint32_t)THREADS * i);
+            if (at <= have) *reinterpret_cast<uint4*>(lut + at) = x[i];
+        }
+        for (uint32_t i = 8u * (threadIdx.x + 512u); i <= have; i += 8u * THREADS) *reinterpret_cast<uint4*>(lut + i) = table8(a.lut, i, have);
+    }
+};
+// e of four keys of a vector with the maximum m, and their sum.
+__device__ inline uint32_t exps_of(const PagedAttn& a, const Part& p, const uint16_t* lut, uint32_t have, int32_t m, const int4& v, int key, int lim,
+                                   bool holes, const uint64_t* tab, int p0, uint32_t (&e)[4]) {
+    const int32_t z[4] = {v.x, v.y, v.z, v.w};
+    uint32_t s = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        // sat_sub and the lookup of softmax.rs:12-38
+        const uint32_t below = min((uint32_t)m - (uint32_t)z[i], 0x7FFFFFFFu) >> (a.lut_shift & 31u);
+        uint32_t x = lut[min(below, have)];
+        if (below >= have && below < a.lut_len) x = (uint32_t)max((int32_t)a.lut[below], 0);
+        bool ok = key + i < lim;
+        if (holes) ok = ok && on_page(a, tab, p0, min(key + i, p.j1 - 1));
+        e[i] = ok ? x : 0u;
+        s += e[i];
+    }
+    return s;
+}
+
 __global__ __launch_bounds__(256) void paged_sum_kernel(PagedAttn a) {
     extern __shared__ __align__(16) uint64_t tab[];
     __shared__ __align__(16) uint16_t lut[kSumLut + 8];
@@ -426,9 +489,8 @@ __global__ __launch_bounds__(256) void paged_sum_kernel(PagedAttn a) {
 #pragma unroll
     for (int i = 0; i < kFoldAhead; ++i) m4[i] = a.pmax[(at + min(l.k + i * l.step, a.ranges - 1)) * a.width + l.c];
     const int any_holes = a.holes[at + p.range];
-    uint4 t8[2];
-#pragma unroll
-    for (int i = 0; i < 2; ++i) t8[i] = table8(a.lut, 8u * (tid + 256u * i), have);
+    TableCopy<256> table;
+    table.load(a, have);
     const int lim = lim_of(a, p, l.c);
     if (!ends_of(a, p, tid)) return;
     const bool holes = __builtin_amdgcn_readfirstlane(any_holes) != 0;
@@ -438,10 +500,7 @@ __global__ __launch_bounds__(256) void paged_sum_kernel(PagedAttn a) {
         s_max[tid] = INT32_MIN;
         s_sum[tid] = 0;
     }
-#pragma unroll
-    for (int i = 0; i < 2; ++i)
-        if (8u * (tid + 256u * i) <= have) *reinterpret_cast<uint4*>(lut + 8 * (tid + 256 * i)) = t8[i];
-    for (uint32_t i = 8u * (tid + 512u); i <= have; i += 8u * 256u) *reinterpret_cast<uint4*>(lut + i) = table8(a.lut, i, have);
+    table.store(a, have, lut);
     __syncthreads();
     int32_t m = INT32_MIN;
 #pragma unroll
@@ -455,19 +514,8 @@ __global__ __launch_bounds__(256) void paged_sum_kernel(PagedAttn a) {
     m = s_max[l.c];
     uint32_t s = 0;
     auto one = [&](int k, const int4& v) {
-        const int32_t z[4] = {v.x, v.y, v.z, v.w};
         uint32_t e[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            // sat_sub and the lookup of softmax.rs:12-38
-            const uint32_t below = min((uint32_t)m - (uint32_t)z[i], 0x7FFFFFFFu) >> (a.lut_shift & 31u);
-            uint32_t x = lut[min(below, have)];
-            if (below >= have && below < a.lut_len) x = (uint32_t)max((int32_t)a.lut[below], 0);
-            bool ok = 4 * k + i < lim;
-            if (holes) ok = ok && on_page(a, tab, p0, min(4 * k + i, p.j1 - 1));
-            e[i] = ok ? x : 0u;
-            s += e[i];
-        }
+        s += exps_of(a, p, lut, have, m, v, 4 * k, lim, holes, tab, p0, e);
         *reinterpret_cast<uint2*>(a.e + base + ((size_t)k * a.width + l.c) * 4) = make_uint2(e[0] | (e[1] << 16), e[2] | (e[3] << 16));
     };
     if (l.step) {
@@ -524,10 +572,119 @@ __device__ inline void fold_rows(int32_t (&x)[R]) {
 // their way; then the values stream through the waves' rings.  A lane holds 8 dimensions
 // of two neighbouring keys, paired for v_dot2.  W: 8 or 16 vectors at most.
 constexpr int kPvRing = 2, kPvAhead = 4;
+
+// p of the four keys from `key` on, from their e, as two pairs.
+struct Probs {
+    ProbDiv div;
+    Uniform uni;
+    uint32_t s;
+    int lim;
+    __device__ inline static Probs of(const PagedAttn& a, const Part& p, uint32_t s, int lim) {
+        Probs r{ProbDiv::of(s ? s : 1u, a.prob_frac), Uniform{0, 0, 0}, s, lim};
+        if (s == 0) r.uni = uniform_of(a, p, lim);
+        return r;
+    }
+    __device__ inline uint2 operator()(const PagedAttn& a, const Part& p, int key, const uint2& e, bool holes, const uint64_t* tab, int p0) const {
+        if (key >= p.j1) return make_uint2(0, 0);
+        if (s) return make_uint2(div(e.x & 0xFFFFu) | (div(e.x >> 16) << 16), div(e.y & 0xFFFFu) | (div(e.y >> 16) << 16));
+        uint32_t u[4];
+        for (int i = 0; i < 4; ++i) {
+            uint32_t rank = uni.before;
+            bool ok = key + i < lim;
+            if (holes) {
+                ok = ok && on_page(a, tab, p0, min(key + i, p.j1 - 1));
+                for (int b = p.j0; ok && b < key + i; ++b) rank += on_page(a, tab, p0, b) ? 1u : 0u;
+            } else {
+                rank += (uint32_t)(key + i - p.j0);
+            }
+            u[i] = ok ? uni.base + (rank < uni.extra ? 1u : 0u) : 0u;
+        }
+        return make_uint2(u[0] | (u[1] << 16), u[2] | (u[3] << 16));
+    }
+};
+
+// The wave's tiles of values, whose first NB are on their way, against the pairs in ps.
+template <int HD, int W, bool ALIGNED, int NW>
+__device__ inline void paged_values(const PagedAttn& a, const Part& p, const uint64_t* tab, int p0, const Tiles<HD, kPvRing, ALIGNED, false>& tiles, int n,
+                                    const uint32_t* ps, int32_t (&acc)[8 * W]) {
+    using T = Tiles<HD, kPvRing, ALIGNED, false>;
+    constexpr int NB = kPvRing, NP = 8 * T::CH / 64;  // pairs of a tile per lane
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+#pragma unroll
+    for (int i = 0; i < 8 * W; ++i) acc[i] = 0;
+    int slot = 0;
+    for (int t = 0; t < n; ++t) {
+        const int j = 16 * wave + 16 * NW * t;  // from the range's first key
+        T::template wait<0>(n - 1 - t);
+        const int8_t* v8 = tiles.ring + slot * T::kBytes + 16 * tiles.chunk;
+        v4i32_t x[NP][2];
+#pragma unroll
+        for (int i = 0; i < NP; ++i)
+#pragma unroll
+            for (int b = 0; b < 2; ++b) x[i][b] = *reinterpret_cast<const v4i32_t*>(v8 + (2 * (i * T::ROWS + tiles.row) + b) * 2 * HD);
+        v4i32_t pr[NP][W / 4];
+#pragma unroll
+        for (int i = 0; i < NP; ++i)
+#pragma unroll
+            for (int v = 0; v < W / 4; ++v)
+                pr[i][v] = *reinterpret_cast<const v4i32_t*>(ps + (size_t)(j / 2 + i * T::ROWS + tiles.row) * W + 4 * v);
+        // in registers before the tile's place is loaded again
+        if (NP == 2) asm volatile("s_waitcnt lgkmcnt(0)" : "+v"(x[0][0]), "+v"(x[0][1]), "+v"(x[NP - 1][0]), "+v"(x[NP - 1][1])::"memory");
+        else asm volatile("s_waitcnt lgkmcnt(0)" : "+v"(x[0][0]), "+v"(x[0][1])::"memory");
+        if (t + NB < n) tiles.issue(a, tab, p0, p.j0 + j + 16 * NW * NB, p.j1, slot);
+        slot = slot + 1 == NB ? 0 : slot + 1;
+#pragma unroll
+        for (int i = 0; i < NP; ++i) {
+            uint32_t w[8];
+#pragma unroll
+            for (int d = 0; d < 4; ++d) {
+                w[2 * d] = __builtin_amdgcn_perm((uint32_t)x[i][1][d], (uint32_t)x[i][0][d], 0x05040100u);
+                w[2 * d + 1] = __builtin_amdgcn_perm((uint32_t)x[i][1][d], (uint32_t)x[i][0][d], 0x07060302u);
+            }
+#pragma unroll
+            for (int v = 0; v < W; ++v)
+#pragma unroll
+                for (int d = 0; d < 8; ++d) acc[v * 8 + d] = dot_pairs(w[d], (uint32_t)pr[i][v / 4][v % 4], acc[v * 8 + d]);
+        }
+    }
+}
+
+// The waves' sums meet in LDS, in place of the rings; emit(i, sum) of vector i / HD, dimension i % HD.
+template <int HD, int W, int NW, class Emit>
+__device__ inline void paged_meet(const PagedAttn& a, int8_t* rings, int chunk, int32_t (&acc)[8 * W], const Emit& emit) {
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    fold_rows<HD>(acc);
+    block_barrier();
+    int32_t* const sums = reinterpret_cast<int32_t*>(rings);  // [wave][W][HD]
+    static_assert(W * HD * 4 <= kPvRing * 32 * HD, "a wave's sums fit its ring");
+    const int rho = lane >> 4, first = rho == 1 ? 2 : rho == 2 ? 1 : rho;
+    if (HD == 128 || !(lane & 8))
+#pragma unroll
+        for (int k = 0; k < 2 * W; ++k) {
+            const int reg = 4 * k + first;
+            sums[(wave * W + (reg >> 3)) * HD + 8 * chunk + (reg & 7)] = acc[k];
+        }
+    block_barrier();
+    for (int i = tid; i < a.width * HD; i += 64 * NW) {
+        int32_t x = 0;
+#pragma unroll
+        for (int w = 0; w < NW; ++w) x += sums[w * W * HD + i];
+        emit(i, x);
+    }
+}
+
+template <int HD>
+__device__ inline void write_out(const PagedAttn& a, const Part& p, int i, int32_t sum) {
+    if (i >= p.nv * HD) return;
+    int head;
+    const int row = vector_of(a, p, i / HD, head);
+    a.out[(size_t)row * a.ldo + (size_t)head * HD + i % HD] = clamp_i16(rshift_round32(sum, a.prob_frac));
+}
+
 template <int HD, int W, bool ALIGNED>
 __global__ __launch_bounds__(256, W == 8 ? 4 : 2) void paged_pv_kernel(PagedAttn a) {
     using T = Tiles<HD, kPvRing, ALIGNED, false>;
-    constexpr int CH = HD / 8, NB = kPvRing, NP = 8 * CH / 64;  // pairs of a tile per lane
+    constexpr int NB = kPvRing;
     extern __shared__ __align__(16) int8_t lds[];  // the waves' rings, the range's p, its pages
     __shared__ uint32_t s_sum[16];
     __shared__ int bad[4];
@@ -548,28 +705,23 @@ __global__ __launch_bounds__(256, W == 8 ? 4 : 2) void paged_pv_kernel(PagedAttn
 #pragma unroll
     for (int i = 0; i < kPvAhead; ++i) e4[i] = *exps(l.k + i * l.step);
     const bool some = ends_of(a, p, threadIdx.x);
-    if (!some && a.ranges > 1) return;
-    if (!some) {  // the only range has no key
-        for (int i = threadIdx.x; i < p.nv * HD; i += 256) {
-            int head;
-            const int row = vector_of(a, p, i / HD, head);
-            a.out[(size_t)row * a.ldo + (size_t)head * HD + i % HD] = 0;
-        }
+    if (!some) {
+        if (a.ranges == 1)  // no key at all
+            for (int i = threadIdx.x; i < p.nv * HD; i += 256) write_out<HD>(a, p, i, 0);
         return;
     }
-    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int lim = lim_of(a, p, l.c);
     if (tid < 16) s_sum[tid] = 0;
     const int p0 = pages_of_range(a, p, tab, bad);
     __syncthreads();
     T tiles;
     tiles.begin(a, a.vp, lds + wave * NB * T::kBytes);
-    const int n = max(((p.j1 - p.j0 + 15) >> 4) - wave + 3, 0) >> 2;
-    const int jw = p.j0 + 16 * wave;
+    const int n = tiles_of_wave<4>(p, wave);
 #pragma unroll
     for (int t = 0; t < NB; ++t)
-        if (t < n) tiles.issue(a, tab, p0, jw + 64 * t, p.j1, t);
-    const bool holes = (bad[0] | bad[1] | bad[2] | bad[3]) != 0;
+        if (t < n) tiles.issue(a, tab, p0, p.j0 + 16 * wave + 64 * t, p.j1, t);
+    const bool holes = any_of(bad);
     uint32_t s = 0;
 #pragma unroll
     for (int i = 0; i < kFoldAhead; ++i)
@@ -579,34 +731,11 @@ __global__ __launch_bounds__(256, W == 8 ? 4 : 2) void paged_pv_kernel(PagedAttn
         if (s) atomicAdd(&s_sum[l.c], s);
     }
     block_barrier();
-    s = s_sum[l.c];
     if (l.step) {
-        const ProbDiv div = ProbDiv::of(s ? s : 1u, a.prob_frac);
-        Uniform uni{0, 0, 0};
-        if (s == 0) uni = uniform_of(a, p, lim);
+        const Probs probs = Probs::of(a, p, s_sum[l.c], lim);
         const int groups = (p.j1 - p.j0 + 15) / 16 * 4;
         auto one = [&](int k, const uint2& x) {
-            uint2 two = make_uint2(0, 0);
-            const int key = p.j0 + 4 * k;
-            if (key < p.j1) {
-                two.x = div(x.x & 0xFFFFu) | (div(x.x >> 16) << 16);
-                two.y = div(x.y & 0xFFFFu) | (div(x.y >> 16) << 16);
-                if (s == 0) {
-                    uint32_t u[4];
-                    for (int i = 0; i < 4; ++i) {
-                        uint32_t rank = uni.before;
-                        bool ok = key + i < lim;
-                        if (holes) {
-                            ok = ok && on_page(a, tab, p0, min(key + i, p.j1 - 1));
-                            for (int b = p.j0; ok && b < key + i; ++b) rank += on_page(a, tab, p0, b) ? 1u : 0u;
-                        } else {
-                            rank += (uint32_t)(key + i - p.j0);
-                        }
-                        u[i] = ok ? uni.base + (rank < uni.extra ? 1u : 0u) : 0u;
-                    }
-                    two = make_uint2(u[0] | (u[1] << 16), u[2] | (u[3] << 16));
-                }
-            }
+            const uint2 two = probs(a, p, p.j0 + 4 * k, x, holes, tab, p0);
             ps[2 * k * W + l.c] = two.x;
             ps[(2 * k + 1) * W + l.c] = two.y;
         };
@@ -617,74 +746,92 @@ __global__ __launch_bounds__(256, W == 8 ? 4 : 2) void paged_pv_kernel(PagedAttn
     }
     block_barrier();
     int32_t acc[8 * W];
-#pragma unroll
-    for (int i = 0; i < 8 * W; ++i) acc[i] = 0;
-    int slot = 0;
-    for (int t = 0; t < n; ++t) {
-        const int j = 16 * wave + 64 * t;  // from the range's first key
-        T::template wait<0>(n - 1 - t);
-        const int8_t* v8 = tiles.ring + slot * T::kBytes + 16 * tiles.chunk;
-        v4i32_t x[NP][2];
-#pragma unroll
-        for (int i = 0; i < NP; ++i)
-#pragma unroll
-            for (int b = 0; b < 2; ++b) x[i][b] = *reinterpret_cast<const v4i32_t*>(v8 + (2 * (i * T::ROWS + tiles.row) + b) * 2 * HD);
-        v4i32_t pr[NP][W / 4];
-#pragma unroll
-        for (int i = 0; i < NP; ++i)
-#pragma unroll
-            for (int v = 0; v < W / 4; ++v)
-                pr[i][v] = *reinterpret_cast<const v4i32_t*>(ps + (size_t)(j / 2 + i * T::ROWS + tiles.row) * W + 4 * v);
-        // in registers before the tile's place is loaded again
-        if (NP == 2) asm volatile("s_waitcnt lgkmcnt(0)" : "+v"(x[0][0]), "+v"(x[0][1]), "+v"(x[NP - 1][0]), "+v"(x[NP - 1][1])::"memory");
-        else asm volatile("s_waitcnt lgkmcnt(0)" : "+v"(x[0][0]), "+v"(x[0][1])::"memory");
-        if (t + NB < n) tiles.issue(a, tab, p0, jw + 64 * (t + NB), p.j1, slot);
-        slot = slot + 1 == NB ? 0 : slot + 1;
-#pragma unroll
-        for (int i = 0; i < NP; ++i) {
-            uint32_t w[8];
-#pragma unroll
-            for (int d = 0; d < 4; ++d) {
-                w[2 * d] = __builtin_amdgcn_perm((uint32_t)x[i][1][d], (uint32_t)x[i][0][d], 0x05040100u);
-                w[2 * d + 1] = __builtin_amdgcn_perm((uint32_t)x[i][1][d], (uint32_t)x[i][0][d], 0x07060302u);
-            }
-#pragma unroll
-            for (int v = 0; v < W; ++v)
-#pragma unroll
-                for (int d = 0; d < 8; ++d) acc[v * 8 + d] = dot_pairs(w[d], (uint32_t)pr[i][v / 4][v % 4], acc[v * 8 + d]);
-        }
-    }
-    // the waves' sums meet in LDS, in place of the rings
-    fold_rows<HD>(acc);
-    block_barrier();
-    int32_t* const sums = reinterpret_cast<int32_t*>(lds);  // [wave][W][HD]
-    static_assert(W * HD * 4 <= NB * 32 * HD, "a wave's sums fit its ring");
-    const int rho = lane >> 4, first = rho == 1 ? 2 : rho == 2 ? 1 : rho;
-    if (HD == 128 || !(lane & 8))
-#pragma unroll
-        for (int k = 0; k < 2 * W; ++k) {
-            const int reg = 4 * k + first;
-            sums[(wave * W + (reg >> 3)) * HD + 8 * tiles.chunk + (reg & 7)] = acc[k];
-        }
-    block_barrier();
+    paged_values<HD, W, ALIGNED, 4>(a, p, tab, p0, tiles, n, ps, acc);
     int32_t* o = a.pout + (at + p.range) * a.width * HD;
-    for (int i = tid; i < a.width * HD; i += 256) {
-        const int32_t x = sums[i] + sums[W * HD + i] + sums[2 * W * HD + i] + sums[3 * W * HD + i];
-        if (a.ranges > 1) {
-            o[i] = x;
-        } else if (i < p.nv * HD) {
-            int head;
-            const int row = vector_of(a, p, i / HD, head);
-            a.out[(size_t)row * a.ldo + (size_t)head * HD + i % HD] = clamp_i16(rshift_round32(x, a.prob_frac));
+    paged_meet<HD, W, 4>(a, lds, tiles.chunk, acc, [&](int i, int32_t x) {
+        if (a.ranges > 1) o[i] = x;
+        else write_out<HD>(a, p, i, x);
+    });
+}
+
+// Few keys: a block per tile does all of it in one launch, the scores in LDS.
+constexpr int kShortWaves = 8;
+template <int HD, int W, bool FAST, bool ALIGNED>
+__global__ __launch_bounds__(64 * kShortWaves, W == 8 ? 4 : 2) void paged_short_kernel(PagedAttn a) {
+    using T = Tiles<HD, kPvRing, ALIGNED, false>;
+    constexpr int NB = kPvRing, NW = kShortWaves, kThreads = 64 * NW;
+    static_assert(kPvRing == kQkRing, "the rings lie in the same place");
+    extern __shared__ __align__(16) int8_t lds[];  // the waves' rings, scores, p, pages, the exp table
+    __shared__ __align__(16) int8_t qlds[16 * 2 * HD];
+    __shared__ int32_t red[16 * NW];
+    __shared__ uint32_t s_sum[16];
+    __shared__ int bad[NW], large[NW];
+    int32_t* const z = reinterpret_cast<int32_t*>(lds + NW * NB * T::kBytes);  // [keys / 4][width][4]
+    uint32_t* const ps = reinterpret_cast<uint32_t*>(z + (size_t)a.keys * a.width);  // [keys / 2][W]
+    uint64_t* const tab = reinterpret_cast<uint64_t*>(ps + (size_t)a.keys / 2 * W);
+    uint16_t* const lut = reinterpret_cast<uint16_t*>(tab + paged_table_entries(a.range, (int)a.page.d));
+    Part p;
+    int lane_lim;
+    if (!place_of_block(a, p)) return;
+    const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const uint32_t have = min(a.lut_len, kSumLut);
+    TableCopy<kThreads> table;
+    table.load(a, have);
+    if (!ends_of(a, p, tid, lane_lim)) {
+        for (int i = tid; i < p.nv * HD; i += kThreads) write_out<HD>(a, p, i, 0);
+        return;
+    }
+    const Lanes l = Lanes::of(a);
+    const int lim = lim_of(a, p, l.c);
+    stage_queries<HD>(a, p, qlds, large);
+    const int p0 = pages_of_range(a, p, tab, bad);
+    if (tid < 16) s_sum[tid] = 0;
+    table.store(a, have, lut);
+    __syncthreads();
+    const bool holes = any_of(bad);
+    scores_of_range<HD, FAST, ALIGNED, NW, false>(a, p, lane_lim, tab, p0, holes, lds, qlds, any_of(large), z, red);
+    // the wave's ring is free: values while the softmax runs
+    T tiles;
+    tiles.begin(a, a.vp, lds + wave * NB * T::kBytes);
+    const int n = tiles_of_wave<NW>(p, wave);
+#pragma unroll
+    for (int t = 0; t < NB; ++t)
+        if (t < n) tiles.issue(a, tab, p0, p.j0 + 16 * wave + 16 * NW * t, p.j1, t);
+    block_barrier();
+    int32_t m = red[l.c];
+#pragma unroll
+    for (int w = 1; w < NW; ++w) m = max(m, red[16 * w + l.c]);
+    const int groups = (p.j1 + 15) / 16 * 4;
+    if (l.step) {
+        uint32_t s = 0;
+        for (int k = l.k; k < groups; k += l.step) {
+            int4* const at = reinterpret_cast<int4*>(z + (size_t)(k * a.width + l.c) * 4);
+            uint32_t e[4];
+            s += exps_of(a, p, lut, have, m, *at, 4 * k, lim, holes, tab, p0, e);
+            *reinterpret_cast<uint2*>(at) = make_uint2(e[0] | (e[1] << 16), e[2] | (e[3] << 16));
+        }
+        atomicAdd(&s_sum[l.c], s);
+    }
+    block_barrier();
+    if (l.step) {
+        const Probs probs = Probs::of(a, p, s_sum[l.c], lim);
+        for (int k = l.k; k < groups; k += l.step) {
+            const uint2 two = probs(a, p, 4 * k, *reinterpret_cast<const uint2*>(z + (size_t)(k * a.width + l.c) * 4), holes, tab, p0);
+            ps[2 * k * W + l.c] = two.x;
+            ps[(2 * k + 1) * W + l.c] = two.y;
         }
     }
+    block_barrier();
+    int32_t acc[8 * W];
+    paged_values<HD, W, ALIGNED, NW>(a, p, tab, p0, tiles, n, ps, acc);
+    paged_meet<HD, W, NW>(a, lds, tiles.chunk, acc, [&](int i, int32_t x) { write_out<HD>(a, p, i, x); });
 }
 
 // The ranges' sums, one rounding (attention.rs:84-86).  A block per row and head: four
 // dimensions and every so-many-th range per thread.
-template <int HD>
-__global__ __launch_bounds__(256) void paged_out_kernel(PagedAttn a) {
-    constexpr int Q = HD / 4, SHARES = 256 / Q;
+template <int HD, int THREADS>
+__global__ __launch_bounds__(THREADS) void paged_out_kernel(PagedAttn a) {
+    constexpr int Q = HD / 4, SHARES = THREADS / Q;
     __shared__ int64_t part[SHARES][HD];
     int head, h, in_seq, v;
     const int row = divmod(a.heads_d, (int)blockIdx.x, head), q = threadIdx.x % Q, share = threadIdx.x / Q;
@@ -725,16 +872,28 @@ hipError_t allow_lds(K kernel, size_t bytes) {
     return bytes <= 65536 ? hipSuccess : hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
 }
 
+template <int HD, bool ALIGNED, int W>
+hipError_t paged_in_one(const PagedAttn& a, const PagedPlan& pl, hipStream_t st) {
+    const size_t bytes = paged_short_lds(pl, HD, (int)a.page.d, a.lut_len);
+    auto kernel = a.scale.fast ? paged_short_kernel<HD, W, true, ALIGNED> : paged_short_kernel<HD, W, false, ALIGNED>;
+    const hipError_t e = allow_lds(kernel, bytes);
+    if (e != hipSuccess) return e;
+    kernel<<<(unsigned)pl.blocks, 64 * kShortWaves, bytes, st>>>(a);
+    return hipGetLastError();
+}
+
 template <int HD, bool ALIGNED>
-hipError_t paged_ranges(const PagedAttn& a, unsigned grid, hipStream_t st) {
-    const size_t tab = ((size_t)a.range / a.page.d + 2) * 8;
+hipError_t paged_ranges(const PagedAttn& a, const PagedPlan& pl, hipStream_t st) {
+    const int W = a.width <= 8 ? 8 : 16;
+    if (pl.in_one) return W == 8 ? paged_in_one<HD, ALIGNED, 8>(a, pl, st) : paged_in_one<HD, ALIGNED, 16>(a, pl, st);
+    const unsigned grid = (unsigned)pl.blocks;
+    const size_t tab = (size_t)paged_table_entries(a.range, (int)a.page.d) * 8;
     const size_t qk = 4 * kQkRing * 32 * HD + tab;
     auto scores = a.scale.fast ? paged_qk_kernel<HD, true, ALIGNED> : paged_qk_kernel<HD, false, ALIGNED>;
     hipError_t e = allow_lds(scores, qk);
     if (e != hipSuccess) return e;
     scores<<<grid, 256, qk, st>>>(a);
     paged_sum_kernel<<<grid, 256, tab, st>>>(a);
-    const int W = a.width <= 8 ? 8 : 16;
     const size_t pv = 4 * kPvRing * 32 * HD + (size_t)a.range * W * 2 + tab;
     auto values = W == 8 ? paged_pv_kernel<HD, 8, ALIGNED> : paged_pv_kernel<HD, 16, ALIGNED>;
     e = allow_lds(values, pv);
@@ -746,10 +905,11 @@ hipError_t paged_ranges(const PagedAttn& a, unsigned grid, hipStream_t st) {
 template <int HD>
 hipError_t paged_launch(const PagedAttn& a, const PagedPlan& pl, int rows, hipStream_t st) {
     if (pl.ranges) {
-        const hipError_t e = a.page.d % 16 == 0 && a.pos_stride <= kAlignedStride ? paged_ranges<HD, true>(a, (unsigned)pl.blocks, st) : paged_ranges<HD, false>(a, (unsigned)pl.blocks, st);
+        const hipError_t e = a.page.d % 16 == 0 && a.pos_stride <= kAlignedStride ? paged_ranges<HD, true>(a, pl, st) : paged_ranges<HD, false>(a, pl, st);
         if (e != hipSuccess) return e;
     }
-    if (pl.ranges != 1) paged_out_kernel<HD><<<(unsigned)(rows * a.heads), 256, 0, st>>>(a);
+    if (pl.ranges > 32) paged_out_kernel<HD, 1024><<<(unsigned)(rows * a.heads), 1024, 0, st>>>(a);
+    else if (pl.ranges != 1) paged_out_kernel<HD, 256><<<(unsigned)(rows * a.heads), 256, 0, st>>>(a);
     return hipGetLastError();
 }
 

@@ -77,19 +77,39 @@ inline const char* paged_refuse(const PagedShape& s) {
 // The query vectors (heads of rows) that read one sequence's KV head are cut into tiles of at
 // most 16, the keys into ranges of a multiple of 64; a block takes one tile and one range.
 // Within a range of at most 1024 keys sum p |v| <= (2^14 + 2^9) 2^15 < 2^30.
-constexpr int kPagedTile = 16, kPagedMaxRange = 1024, kPagedLeastRange = 128;
+constexpr int kPagedTile = 16, kPagedMaxRange = 1024, kPagedMidRange = 512, kPagedLeastRange = 128;
+constexpr int kPagedLdsLut = 8192;  // exp table entries that a block copies
+
+// The pages that a range of keys can touch.
+constexpr int paged_table_entries(int range, int page) { return (range / page + 3) / 2 * 2; }  // an even number: what follows is 16-byte aligned
 
 struct PagedPlan {
     int width, tiles;   // vectors of a tile; tiles of a sequence's KV head
     int keys;           // max_len rounded up to 64
     int ranges, range;  // ranges of keys, keys of a range
+    bool in_one;        // one launch, a block per tile
     size_t parts;       // sequences x KV heads x tiles
     int64_t blocks;     // parts x ranges, the last eight filled up
     size_t off_z, off_e, off_max, off_sum, off_holes, off_out, bytes;
 };
 
-// Blocks of a call as far as the keys allow.
-inline size_t paged_blocks(int cus) { return 4 * (size_t)cus; }
+// LDS of a block that does all of a tile by itself: rings of eight waves, scores, p, pages, table.
+constexpr size_t kPagedShortKeys = 1024, kPagedShortScores = 8192;
+inline size_t paged_short_lds(const PagedPlan& p, size_t hd, int page, uint32_t lut_len) {
+    const size_t w = p.width <= 8 ? 8 : 16, keys = (size_t)p.keys;
+    const size_t lut = (std::min<size_t>(lut_len, kPagedLdsLut) + 8) / 8 * 16;
+    return 8 * 2 * 32 * hd + keys * ((size_t)p.width * 4 + w * 2) + (size_t)paged_table_entries(p.range, page) * 8 + lut;
+}
+
+// One launch with a block per tile, or four that split the keys: up to 640 keys of 128, or 1024 keys
+// (as far as their scores fit) where an eighth of the CUs has a block.  us of a call's launches, in
+// one / split, heads of 128, seven to a KV head of four: one row of 130 keys 9.8 / 17.0, 600 16.2 / 17.6,
+// 1000 21.9 / 17.9; eight rows of 1000 20.4 / 20.2; 64 of 300 13.6 / 22.1, of 1000 26.3 / 41.8; 256 of
+// 1000 93 / 106.
+inline bool paged_in_one(const PagedShape& s, const PagedPlan& p, int cus) {
+    return s.max_len <= kPagedShortKeys && s.max_len * (size_t)p.width <= kPagedShortScores &&
+           (s.max_len * s.head_dim <= 640 * 128 || p.parts * 8 >= (size_t)cus);
+}
 
 inline PagedPlan paged_plan(const PagedShape& s, int cus) {
     PagedPlan p{};
@@ -98,18 +118,27 @@ inline PagedPlan paged_plan(const PagedShape& s, int cus) {
     p.width = p.tiles ? (int)((vectors + p.tiles - 1) / p.tiles) : 0;
     p.parts = s.n_seqs * s.kv_heads * (size_t)p.tiles;
     p.keys = (int)((s.max_len + 63) / 64 * 64);
-    const size_t most = paged_blocks(cus);
     if (p.parts && p.keys) {
-        const size_t want = (most + p.parts - 1) / p.parts, each = ((size_t)p.keys + want - 1) / want;
-        p.range = (int)std::min<size_t>(std::max<size_t>((each + 63) / 64 * 64, kPagedLeastRange), kPagedMaxRange);
+        if (paged_in_one(s, p, cus)) {
+            p.in_one = true;
+            p.range = p.keys;
+        } else {
+            // A block per CU where ranges of 128 to 512 keys make it, 1024 keys where that leaves four
+            // per CU.  us of a call's launches at 128 / 256 / 512 keys, heads of 128: one row of 5000
+            // keys 20.4 / 21.6 / 25.8, 10000 25.8 / 23.9 / 26.9, 30000 38.8 / 32.9 / 30.7; eight of 2000
+            // 25.1 / 23.7 / 27.2; 64 of 300 28.8 / 29.3 / 22.3 (one range); 24 of 2500 40.6 / 40.7 / 38.2.
+            const size_t work = p.parts * (size_t)p.keys, each = (work + (size_t)cus - 1) / (size_t)cus;
+            p.range = (int)std::min<size_t>(std::max<size_t>((each + 63) / 64 * 64, kPagedLeastRange), kPagedMidRange);
+            if (work / kPagedMaxRange >= 4 * (size_t)cus) p.range = kPagedMaxRange;
+        }
         p.ranges = (p.keys + p.range - 1) / p.range;
     }
     p.blocks = ((int64_t)s.n_seqs * (int64_t)s.kv_heads * p.ranges + 7) / 8 * 8 * p.tiles;
-    // The ranges of any smaller call: at most as many as the least range makes, and at most
-    // want = ceil(most / parts) or as many as the largest range makes.
+    // The ranges of any smaller call, ceil(keys / range): at most as many as the least range makes,
+    // as many as the middle one makes, or those of which a CU has about one.
     const size_t vecs = p.parts * (size_t)p.width, keys = (size_t)p.keys;
     const size_t pieces = std::min(vecs * ((keys + kPagedLeastRange - 1) / kPagedLeastRange),
-                                   vecs * (1 + (keys + kPagedMaxRange - 1) / kPagedMaxRange) + kPagedTile * most);
+                                   vecs * (1 + (keys + kPagedMidRange - 1) / kPagedMidRange) + (size_t)kPagedTile * (size_t)cus);
     Layout l;
     p.off_z = l.take(vecs * keys, 4);
     p.off_e = l.take(vecs * keys, 2);
