@@ -84,8 +84,8 @@ __device__ inline bool place_of_block(const PagedAttn& a, Part& p) {
 __device__ inline bool ends_of(const PagedAttn& a, Part& p, int v, int& lim) {
     int head;
     lim = keys_of(a, vector_of(a, p, v & 15, head));
-    p.j1 = min(p.j0 + a.range, wave_max_i32(lim));
-    p.lmin = ~wave_max_i32(~lim);
+    p.j1 = min(p.j0 + a.range, __builtin_amdgcn_readfirstlane(wave_max_i32(lim)));
+    p.lmin = __builtin_amdgcn_readfirstlane(~wave_max_i32(~lim));
     return p.j0 < p.j1;
 }
 __device__ inline bool ends_of(const PagedAttn& a, Part& p, int v) {
@@ -548,30 +548,7 @@ __device__ inline Uniform uniform_of(const PagedAttn& a, const Part& p, int lim)
     return u;
 }
 
-// Sums over the lanes of a wave that hold the same chunk (lane % (HD / 8)) of R registers: after
-// it a lane of row rho = lane / 16 holds register 4 k + {0, 2, 1, 3}[rho] in x[k].
-template <int HD, int R>
-__device__ inline void fold_rows(int32_t (&x)[R]) {
-    if (HD == 64)
-#pragma unroll
-        for (int i = 0; i < R; ++i) x[i] += __builtin_amdgcn_mov_dpp(x[i], 0x128, 0xF, 0xF, true);  // row_ror 8
-#pragma unroll
-    for (int i = 0; i < R / 2; ++i) {
-        const auto s = __builtin_amdgcn_permlane32_swap((uint32_t)x[2 * i], (uint32_t)x[2 * i + 1], false, false);
-        x[i] = (int32_t)(s[0] + s[1]);
-    }
-#pragma unroll
-    for (int i = 0; i < R / 4; ++i) {
-        const auto s = __builtin_amdgcn_permlane16_swap((uint32_t)x[2 * i], (uint32_t)x[2 * i + 1], false, false);
-        x[i] = (int32_t)(s[0] + s[1]);
-    }
-}
-
-// sum p_j v_j of a tile's vectors over a range.  The range's p go to LDS first, pairs of keys of
-// every vector (p <= 2^14 fits a signed 16-bit half), while the first values are on
-// their way; then the values stream through the waves' rings.  A lane holds 8 dimensions
-// of two neighbouring keys, paired for v_dot2.  W: 8 or 16 vectors at most.
-constexpr int kPvRing = 2, kPvAhead = 4;
+constexpr int kPvAhead = 4;
 
 // p of the four keys from `key` on, from their e, as two pairs.
 struct Probs {
@@ -603,93 +580,186 @@ struct Probs {
     }
 };
 
-// The wave's tiles of values, whose first NB are on their way, against the pairs in ps.
-template <int HD, int W, bool ALIGNED, int NW>
-__device__ inline void paged_values(const PagedAttn& a, const Part& p, const uint64_t* tab, int p0, const Tiles<HD, kPvRing, ALIGNED, false>& tiles, int n,
-                                    const uint32_t* ps, int32_t (&acc)[8 * W]) {
-    using T = Tiles<HD, kPvRing, ALIGNED, false>;
-    constexpr int NB = kPvRing, NP = 8 * T::CH / 64;  // pairs of a tile per lane
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+// The byte planes of a range's p, p = 256 ph + pl with pl the low byte as a signed one (p <= 2^14),
+// in LDS: [16 keys][W vectors][16], first ph of the whole range, then pl.
+template <int W>
+__device__ inline void store_planes(int8_t* ph, int8_t* pl, int k, int c, const uint2& two) {
+    const int at = (k >> 2) * 16 * W + 16 * c + 4 * (k & 3);
+    *reinterpret_cast<uint32_t*>(pl + at) = __builtin_amdgcn_perm(two.y, two.x, 0x06040200u);
+    // 128 carries into the high byte
+    *reinterpret_cast<uint32_t*>(ph + at) = __builtin_amdgcn_perm(two.y + 0x00800080u, two.x + 0x00800080u, 0x07050301u);
+}
+
+// Units of 64 values in a ring of NB places in the block's LDS, each wave loading 64 / NW of them:
+// key r of a unit is row r, its 16-byte chunk x at place x ^ turn(r), so that the transposing reads
+// of 8 keys and the 16 bytes of one chunk meet different banks.
+template <int HD, int NB, bool ALIGNED, int NW>
+struct Units {
+    static constexpr int CH = HD / 8, ROWS = 64 / CH, RW = 64 / NW, NI = RW / ROWS, kBytes = 64 * 2 * HD;
+    const char* pages;
+    int8_t* ring;
+    uint32_t lane[NI];  // ALIGNED: the lane's bytes from the wave's first key
+    int first, row, chunk;
+    __device__ static inline int turn(int r) { return HD == 128 ? (r & 7) | (((r >> 4) & 1) << 3) : (r & 7) ^ ((r >> 4) & 1); }
+    __device__ inline void begin(const PagedAttn& a, int8_t* lds) {
+        pages = reinterpret_cast<const char*>(a.vp);
+        ring = lds;
+        const int l = threadIdx.x & 63;
+        first = RW * __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+        row = l / CH;
+        chunk = l % CH;
 #pragma unroll
-    for (int i = 0; i < 8 * W; ++i) acc[i] = 0;
-    int slot = 0;
-    for (int t = 0; t < n; ++t) {
-        const int j = 16 * wave + 16 * NW * t;  // from the range's first key
-        T::template wait<0>(n - 1 - t);
-        const int8_t* v8 = tiles.ring + slot * T::kBytes + 16 * tiles.chunk;
-        v4i32_t x[NP][2];
+        for (int i = 0; i < NI; ++i) {
+            const int r = i * ROWS + row;
+            lane[i] = 2u * ((uint32_t)r * (uint32_t)a.pos_stride + 8u * (uint32_t)(chunk ^ turn(first + r)));
+        }
+    }
+    // How many units of the keys [j0, j1) the wave has a part of.
+    __device__ inline int count(const Part& p) const { return max(p.j1 - p.j0 - first + 63, 0) >> 6; }
+    // The wave's part of unit u to place `slot`; keys from j1 on hold anything.
+    __device__ inline void issue(const PagedAttn& a, const Part& p, const uint64_t* tab, int p0, int u, int slot) const {
+        const int j = p.j0 + 64 * u + first;
+        int8_t* to = ring + slot * kBytes + first * 2 * HD;
+        if (ALIGNED) {
+            const uint64_t at = place_of(a, tab, p0, j);
+            const uint64_t s = ((uint64_t)__builtin_amdgcn_readfirstlane((uint32_t)(at >> 32)) << 32) | __builtin_amdgcn_readfirstlane((uint32_t)at);
+            const char* base = pages + 2 * s;
+            if (a.tiles.d == 1)
 #pragma unroll
-        for (int i = 0; i < NP; ++i)
+                for (int i = 0; i < NI; ++i)
+                    __builtin_amdgcn_global_load_lds((global_void*)(uintptr_t)(base + lane[i]), (lds_void*)(to + i * 1024), 16, 0, kOnce);
+            else
 #pragma unroll
-            for (int b = 0; b < 2; ++b) x[i][b] = *reinterpret_cast<const v4i32_t*>(v8 + (2 * (i * T::ROWS + tiles.row) + b) * 2 * HD);
-        v4i32_t pr[NP][W / 4];
+                for (int i = 0; i < NI; ++i)
+                    __builtin_amdgcn_global_load_lds((global_void*)(uintptr_t)(base + lane[i]), (lds_void*)(to + i * 1024), 16, 0, 0);
+        } else {
 #pragma unroll
-        for (int i = 0; i < NP; ++i)
-#pragma unroll
-            for (int v = 0; v < W / 4; ++v)
-                pr[i][v] = *reinterpret_cast<const v4i32_t*>(ps + (size_t)(j / 2 + i * T::ROWS + tiles.row) * W + 4 * v);
-        // in registers before the tile's place is loaded again
-        if (NP == 2) asm volatile("s_waitcnt lgkmcnt(0)" : "+v"(x[0][0]), "+v"(x[0][1]), "+v"(x[NP - 1][0]), "+v"(x[NP - 1][1])::"memory");
-        else asm volatile("s_waitcnt lgkmcnt(0)" : "+v"(x[0][0]), "+v"(x[0][1])::"memory");
-        if (t + NB < n) tiles.issue(a, tab, p0, p.j0 + j + 16 * NW * NB, p.j1, slot);
-        slot = slot + 1 == NB ? 0 : slot + 1;
-#pragma unroll
-        for (int i = 0; i < NP; ++i) {
-            uint32_t w[8];
-#pragma unroll
-            for (int d = 0; d < 4; ++d) {
-                w[2 * d] = __builtin_amdgcn_perm((uint32_t)x[i][1][d], (uint32_t)x[i][0][d], 0x05040100u);
-                w[2 * d + 1] = __builtin_amdgcn_perm((uint32_t)x[i][1][d], (uint32_t)x[i][0][d], 0x07060302u);
+            for (int i = 0; i < NI; ++i) {
+                const int r = i * ROWS + row;
+                const uint64_t from = place_of(a, tab, p0, min(j + r, p.j1 - 1)) + (uint64_t)(8 * (chunk ^ turn(first + r)));
+                __builtin_amdgcn_global_load_lds((global_void*)(uintptr_t)(pages + 2 * from), (lds_void*)(to + i * 1024), 16, 0, 0);
             }
-#pragma unroll
-            for (int v = 0; v < W; ++v)
-#pragma unroll
-                for (int d = 0; d < 8; ++d) acc[v * 8 + d] = dot_pairs(w[d], (uint32_t)pr[i][v / 4][v % 4], acc[v * 8 + d]);
         }
+    }
+    // The oldest unit's part has landed when `left` (at most NB - 2) younger ones remain.
+    __device__ static inline void wait(int left) {
+        static_assert(NB >= 2 && NB <= 4, "the cases below");
+        if (NB > 3 && left >= 2) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(2 * NI) : "memory");
+        else if (NB > 2 && left >= 1) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(NI) : "memory");
+        else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    }
+};
+
+typedef int v2i32_t __attribute__((ext_vector_type(2)));
+__device__ inline uint32_t lds_addr(const void* p) { return (uint32_t)(uintptr_t)(lds_void*)p; }
+
+// A unit's operands from LDS, there when it returns: the p planes (16 bytes each) and, for each of
+// G chunks, 8 keys of a byte by two transposing reads, the second 8 rows further on.  In one
+// statement with its wait: for reads of its own the compiler waits for every load to LDS in flight.
+template <int HD, int G>
+__device__ inline void read_unit(uint32_t ph, uint32_t pl, const uint32_t (&at)[G], v4i32_t& bh, v4i32_t& bl, v2i32_t (&v)[G][2]) {
+    constexpr int kNext = 8 * 2 * HD;
+    if constexpr (G == 1)
+        asm volatile("ds_read_b128 %0, %4\n\tds_read_b128 %1, %5\n\tds_read_b64_tr_b8 %2, %6\n\tds_read_b64_tr_b8 %3, %6 offset:%7\n\ts_waitcnt lgkmcnt(0)"
+                     : "=&v"(bh), "=&v"(bl), "=&v"(v[0][0]), "=&v"(v[0][1])
+                     : "v"(ph), "v"(pl), "v"(at[0]), "n"(kNext)
+                     : "memory");
+    else if constexpr (G == 2)
+        asm volatile("ds_read_b128 %0, %6\n\tds_read_b128 %1, %7\n\tds_read_b64_tr_b8 %2, %8\n\tds_read_b64_tr_b8 %3, %8 offset:%10\n\t"
+                     "ds_read_b64_tr_b8 %4, %9\n\tds_read_b64_tr_b8 %5, %9 offset:%10\n\ts_waitcnt lgkmcnt(0)"
+                     : "=&v"(bh), "=&v"(bl), "=&v"(v[0][0]), "=&v"(v[0][1]), "=&v"(v[1][0]), "=&v"(v[1][1])
+                     : "v"(ph), "v"(pl), "v"(at[0]), "v"(at[1]), "n"(kNext)
+                     : "memory");
+    else {
+        static_assert(G == 4, "chunks of a wave");
+        asm volatile("ds_read_b128 %0, %10\n\tds_read_b128 %1, %11\n\tds_read_b64_tr_b8 %2, %12\n\tds_read_b64_tr_b8 %3, %12 offset:%16\n\t"
+                     "ds_read_b64_tr_b8 %4, %13\n\tds_read_b64_tr_b8 %5, %13 offset:%16\n\tds_read_b64_tr_b8 %6, %14\n\t"
+                     "ds_read_b64_tr_b8 %7, %14 offset:%16\n\tds_read_b64_tr_b8 %8, %15\n\tds_read_b64_tr_b8 %9, %15 offset:%16\n\ts_waitcnt lgkmcnt(0)"
+                     : "=&v"(bh), "=&v"(bl), "=&v"(v[0][0]), "=&v"(v[0][1]), "=&v"(v[1][0]), "=&v"(v[1][1]), "=&v"(v[2][0]), "=&v"(v[2][1]), "=&v"(v[3][0]),
+                       "=&v"(v[3][1])
+                     : "v"(ph), "v"(pl), "v"(at[0]), "v"(at[1]), "v"(at[2]), "v"(at[3]), "n"(kNext)
+                     : "memory");
     }
 }
 
-// The waves' sums meet in LDS, in place of the rings; emit(i, sum) of vector i / HD, dimension i % HD.
-template <int HD, int W, int NW, class Emit>
-__device__ inline void paged_meet(const PagedAttn& a, int8_t* rings, int chunk, int32_t (&acc)[8 * W], const Emit& emit) {
-    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    fold_rows<HD>(acc);
-    block_barrier();
-    int32_t* const sums = reinterpret_cast<int32_t*>(rings);  // [wave][W][HD]
-    static_assert(W * HD * 4 <= kPvRing * 32 * HD, "a wave's sums fit its ring");
-    const int rho = lane >> 4, first = rho == 1 ? 2 : rho == 2 ? 1 : rho;
-    if (HD == 128 || !(lane & 8))
+// sum p_j v_j over a range, whose first NB - 1 units are on their way.  A wave takes 2 HD / NW bytes
+// of every vector (whole chunks of 8 dimensions: its low and high bytes in turn) as rows of
+// v_mfma_i32_16x16x64_i8, the p planes as columns, so with v = 256 vh + vl + 128
+//   sum p v = 65536 (ph vh) + 256 (ph vl + pl vh) + pl vl + 128 sum p
+// modulo 2^32, which holds the whole sum, from rows 2 d and 2 d + 1 that one lane has.  The transposing
+// read gives a lane 8 keys of one byte of a chunk: no vector instruction goes on the layout but the
+// low bytes' sign.  emit(vector, dimension, two sums), dimension even.
+template <int HD, int W, int NB, bool ALIGNED, int NW, class Emit>
+__device__ inline void paged_values(const PagedAttn& a, const Part& p, const uint64_t* tab, int p0, const Units<HD, NB, ALIGNED, NW>& units,
+                                    const int8_t* ph, const int8_t* pl, const uint32_t* p_sum, const Emit& emit) {
+    using U = Units<HD, NB, ALIGNED, NW>;
+    constexpr int GROUPS = HD / 8 / NW;  // chunks of a wave
+    const int lane = threadIdx.x & 63, c = lane & 15, kb = lane >> 4;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    v4i32_t ah[GROUPS], al[GROUPS];
+    uint32_t at[GROUPS];
 #pragma unroll
-        for (int k = 0; k < 2 * W; ++k) {
-            const int reg = 4 * k + first;
-            sums[(wave * W + (reg >> 3)) * HD + 8 * chunk + (reg & 7)] = acc[k];
+    for (int g = 0; g < GROUPS; ++g) {
+        ah[g] = al[g] = v4i32_t{0, 0, 0, 0};
+        // in a group of 16 lanes lane 2 k + h gives bytes 8 h .. + 7 of key k (U::turn is key + 8's too)
+        const int key = 16 * kb + (c >> 1), x = wave * GROUPS + g;
+        at[g] = lds_addr(units.ring) + (uint32_t)(key * 2 * HD + ((x ^ U::turn(key)) << 4) + 8 * (c & 1));
+    }
+    const uint32_t p_at = (uint32_t)((kb * W + (c & (W - 1))) * 16), ph0 = lds_addr(ph) + p_at, pl0 = lds_addr(pl) + p_at;
+    const int sign = c & 1 ? 0 : (int)0x80808080;  // low bytes are the even rows
+    const int own = units.count(p), n = (p.j1 - p.j0 + 63) >> 6;
+    int slot = 0;
+    for (int u = 0; u < n; ++u) {
+        if (u < own) U::wait(min(own - 1 - u, NB - 2));
+        block_barrier();  // the unit is there; the one before it is done with
+        if (u + NB - 1 < own) units.issue(a, p, tab, p0, u + NB - 1, slot == 0 ? NB - 1 : slot - 1);
+        v4i32_t bh, bl;
+        v2i32_t v[GROUPS][2];
+        uint32_t now[GROUPS];
+#pragma unroll
+        for (int g = 0; g < GROUPS; ++g) now[g] = at[g] + (uint32_t)(slot * U::kBytes);
+        slot = slot + 1 == NB ? 0 : slot + 1;
+        read_unit<HD, GROUPS>(ph0 + (uint32_t)(u * 64 * W), pl0 + (uint32_t)(u * 64 * W), now, bh, bl, v);
+#pragma unroll
+        for (int g = 0; g < GROUPS; ++g) {
+            const v4i32_t x = {v[g][0][0] ^ sign, v[g][0][1] ^ sign, v[g][1][0] ^ sign, v[g][1][1] ^ sign};
+            ah[g] = __builtin_amdgcn_mfma_i32_16x16x64_i8(x, bh, ah[g], 0, 0, 0);
+            al[g] = __builtin_amdgcn_mfma_i32_16x16x64_i8(x, bl, al[g], 0, 0, 0);
         }
-    block_barrier();
-    for (int i = tid; i < a.width * HD; i += 64 * NW) {
-        int32_t x = 0;
+    }
+    if (c >= a.width) return;
+    const uint32_t add = 128u * p_sum[c];
 #pragma unroll
-        for (int w = 0; w < NW; ++w) x += sums[w * W * HD + i];
-        emit(i, x);
+    for (int g = 0; g < GROUPS; ++g) {
+        uint32_t y[2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+            y[i] = ((uint32_t)ah[g][2 * i + 1] << 16) + (((uint32_t)ah[g][2 * i] + (uint32_t)al[g][2 * i + 1]) << 8) + (uint32_t)al[g][2 * i] + add;
+        emit(c, 8 * (wave * GROUPS + g) + 2 * kb, (int32_t)y[0], (int32_t)y[1]);
     }
 }
 
+// Two dimensions of a tile's vector v, rounded and clamped.
 template <int HD>
-__device__ inline void write_out(const PagedAttn& a, const Part& p, int i, int32_t sum) {
-    if (i >= p.nv * HD) return;
+__device__ inline void write_two(const PagedAttn& a, const Part& p, int v, int d, int32_t x, int32_t y) {
+    if (v >= p.nv) return;
     int head;
-    const int row = vector_of(a, p, i / HD, head);
-    a.out[(size_t)row * a.ldo + (size_t)head * HD + i % HD] = clamp_i16(rshift_round32(sum, a.prob_frac));
+    const int row = vector_of(a, p, v, head);
+    const uint32_t lo = (uint32_t)(uint16_t)clamp_i16(rshift_round32(x, a.prob_frac)), hi = (uint32_t)(uint16_t)clamp_i16(rshift_round32(y, a.prob_frac));
+    *reinterpret_cast<uint32_t*>(a.out + (size_t)row * a.ldo + (size_t)head * HD + d) = lo | (hi << 16);
 }
 
+constexpr int kPvRing = 3;
 template <int HD, int W, bool ALIGNED>
-__global__ __launch_bounds__(256, W == 8 ? 4 : 2) void paged_pv_kernel(PagedAttn a) {
-    using T = Tiles<HD, kPvRing, ALIGNED, false>;
+__global__ __launch_bounds__(256, 4) void paged_pv_kernel(PagedAttn a) {
+    using U = Units<HD, kPvRing, ALIGNED, 4>;
     constexpr int NB = kPvRing;
-    extern __shared__ __align__(16) int8_t lds[];  // the waves' rings, the range's p, its pages
-    __shared__ uint32_t s_sum[16];
+    extern __shared__ __align__(16) int8_t lds[];  // the ring, the range's p planes, its pages
+    __shared__ uint32_t s_sum[16], p_sum[16];
     __shared__ int bad[4];
-    uint32_t* const ps = reinterpret_cast<uint32_t*>(lds + 4 * NB * T::kBytes);  // [range / 2][W]
-    uint64_t* const tab = reinterpret_cast<uint64_t*>(ps + (size_t)a.range / 2 * W);
+    int8_t* const ph = lds + NB * U::kBytes;
+    int8_t* const pl = ph + a.range * W;
+    uint64_t* const tab = reinterpret_cast<uint64_t*>(pl + a.range * W);
     Part p;
     if (!place_of_block(a, p)) return;
     // what needs no other load's result first: sums of ranges, exp values (within the workspace
@@ -707,20 +777,19 @@ __global__ __launch_bounds__(256, W == 8 ? 4 : 2) void paged_pv_kernel(PagedAttn
     const bool some = ends_of(a, p, threadIdx.x);
     if (!some) {
         if (a.ranges == 1)  // no key at all
-            for (int i = threadIdx.x; i < p.nv * HD; i += 256) write_out<HD>(a, p, i, 0);
+            for (int i = threadIdx.x; i < p.nv * (HD / 2); i += 256) write_two<HD>(a, p, i / (HD / 2), 2 * (i % (HD / 2)), 0, 0);
         return;
     }
-    const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int tid = threadIdx.x;
     const int lim = lim_of(a, p, l.c);
-    if (tid < 16) s_sum[tid] = 0;
+    if (tid < 16) s_sum[tid] = p_sum[tid] = 0;
     const int p0 = pages_of_range(a, p, tab, bad);
     __syncthreads();
-    T tiles;
-    tiles.begin(a, a.vp, lds + wave * NB * T::kBytes);
-    const int n = tiles_of_wave<4>(p, wave);
+    U units;
+    units.begin(a, lds);
 #pragma unroll
-    for (int t = 0; t < NB; ++t)
-        if (t < n) tiles.issue(a, tab, p0, p.j0 + 16 * wave + 64 * t, p.j1, t);
+    for (int u = 0; u < NB - 1; ++u)
+        if (u < units.count(p)) units.issue(a, p, tab, p0, u, u);
     const bool holes = any_of(bad);
     uint32_t s = 0;
 #pragma unroll
@@ -733,78 +802,77 @@ __global__ __launch_bounds__(256, W == 8 ? 4 : 2) void paged_pv_kernel(PagedAttn
     block_barrier();
     if (l.step) {
         const Probs probs = Probs::of(a, p, s_sum[l.c], lim);
-        const int groups = (p.j1 - p.j0 + 15) / 16 * 4;
+        const int groups = (p.j1 - p.j0 + 63) / 64 * 16;
+        uint32_t sum = 0;
         auto one = [&](int k, const uint2& x) {
             const uint2 two = probs(a, p, p.j0 + 4 * k, x, holes, tab, p0);
-            ps[2 * k * W + l.c] = two.x;
-            ps[(2 * k + 1) * W + l.c] = two.y;
+            sum = (uint32_t)dot_pairs(two.x, 0x00010001u, dot_pairs(two.y, 0x00010001u, (int32_t)sum));
+            store_planes<W>(ph, pl, k, l.c, two);
         };
 #pragma unroll
         for (int i = 0; i < kPvAhead; ++i)
             if (l.k + i * l.step < groups) one(l.k + i * l.step, e4[i]);
         for (int k = l.k + kPvAhead * l.step; k < groups; k += l.step) one(k, *exps(k));
+        atomicAdd(&p_sum[l.c], sum);
     }
-    block_barrier();
-    int32_t acc[8 * W];
-    paged_values<HD, W, ALIGNED, 4>(a, p, tab, p0, tiles, n, ps, acc);
+    // the loop's first barrier stands between the planes and their use, p_sum's too
     int32_t* o = a.pout + (at + p.range) * a.width * HD;
-    paged_meet<HD, W, 4>(a, lds, tiles.chunk, acc, [&](int i, int32_t x) {
-        if (a.ranges > 1) o[i] = x;
-        else write_out<HD>(a, p, i, x);
+    paged_values<HD, W, NB, ALIGNED, 4>(a, p, tab, p0, units, ph, pl, p_sum, [&](int v, int d, int32_t x, int32_t y) {
+        if (a.ranges > 1) *reinterpret_cast<int2*>(o + v * HD + d) = make_int2(x, y);
+        else write_two<HD>(a, p, v, d, x, y);
     });
 }
 
 // Few keys: a block per tile does all of it in one launch, the scores in LDS.
-constexpr int kShortWaves = 8;
+constexpr int kShortWaves = 8, kShortRing = 4;
 template <int HD, int W, bool FAST, bool ALIGNED>
-__global__ __launch_bounds__(64 * kShortWaves, W == 8 ? 4 : 2) void paged_short_kernel(PagedAttn a) {
-    using T = Tiles<HD, kPvRing, ALIGNED, false>;
-    constexpr int NB = kPvRing, NW = kShortWaves, kThreads = 64 * NW;
-    static_assert(kPvRing == kQkRing, "the rings lie in the same place");
-    extern __shared__ __align__(16) int8_t lds[];  // the waves' rings, scores, p, pages, the exp table
+__global__ __launch_bounds__(64 * kShortWaves, 4) void paged_short_kernel(PagedAttn a) {
+    constexpr int NB = kShortRing, NW = kShortWaves, kThreads = 64 * NW;
+    using U = Units<HD, NB, ALIGNED, NW>;
+    static_assert(NB * U::kBytes == NW * kQkRing * 32 * HD, "the values' ring lies where the keys' rings were");
+    extern __shared__ __align__(16) int8_t lds[];  // the rings, scores, p planes, pages, the exp table
     __shared__ __align__(16) int8_t qlds[16 * 2 * HD];
     __shared__ int32_t red[16 * NW];
-    __shared__ uint32_t s_sum[16];
+    __shared__ uint32_t s_sum[16], p_sum[16];
     __shared__ int bad[NW], large[NW];
-    int32_t* const z = reinterpret_cast<int32_t*>(lds + NW * NB * T::kBytes);  // [keys / 4][width][4]
-    uint32_t* const ps = reinterpret_cast<uint32_t*>(z + (size_t)a.keys * a.width);  // [keys / 2][W]
-    uint64_t* const tab = reinterpret_cast<uint64_t*>(ps + (size_t)a.keys / 2 * W);
+    int32_t* const z = reinterpret_cast<int32_t*>(lds + NB * U::kBytes);  // [keys / 4][width][4]
+    int8_t* const ph = reinterpret_cast<int8_t*>(z + (size_t)a.keys * a.width);
+    int8_t* const pl = ph + a.keys * W;
+    uint64_t* const tab = reinterpret_cast<uint64_t*>(pl + a.keys * W);
     uint16_t* const lut = reinterpret_cast<uint16_t*>(tab + paged_table_entries(a.range, (int)a.page.d));
     Part p;
     int lane_lim;
     if (!place_of_block(a, p)) return;
-    const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int tid = threadIdx.x;
     const uint32_t have = min(a.lut_len, kSumLut);
     TableCopy<kThreads> table;
     table.load(a, have);
     if (!ends_of(a, p, tid, lane_lim)) {
-        for (int i = tid; i < p.nv * HD; i += kThreads) write_out<HD>(a, p, i, 0);
+        for (int i = tid; i < p.nv * (HD / 2); i += kThreads) write_two<HD>(a, p, i / (HD / 2), 2 * (i % (HD / 2)), 0, 0);
         return;
     }
     const Lanes l = Lanes::of(a);
     const int lim = lim_of(a, p, l.c);
     stage_queries<HD>(a, p, qlds, large);
     const int p0 = pages_of_range(a, p, tab, bad);
-    if (tid < 16) s_sum[tid] = 0;
+    if (tid < 16) s_sum[tid] = p_sum[tid] = 0;
     table.store(a, have, lut);
     __syncthreads();
     const bool holes = any_of(bad);
     scores_of_range<HD, FAST, ALIGNED, NW, false>(a, p, lane_lim, tab, p0, holes, lds, qlds, any_of(large), z, red);
-    // the wave's ring is free: values while the softmax runs
-    T tiles;
-    tiles.begin(a, a.vp, lds + wave * NB * T::kBytes);
-    const int n = tiles_of_wave<NW>(p, wave);
+    block_barrier();  // the scores are there, the keys' rings free
+    U units;
+    units.begin(a, lds);
 #pragma unroll
-    for (int t = 0; t < NB; ++t)
-        if (t < n) tiles.issue(a, tab, p0, p.j0 + 16 * wave + 16 * NW * t, p.j1, t);
-    block_barrier();
+    for (int u = 0; u < NB - 1; ++u)  // on their way while the softmax runs
+        if (u < units.count(p)) units.issue(a, p, tab, p0, u, u);
     int32_t m = red[l.c];
 #pragma unroll
     for (int w = 1; w < NW; ++w) m = max(m, red[16 * w + l.c]);
-    const int groups = (p.j1 + 15) / 16 * 4;
+    const int groups = (p.j1 + 63) / 64 * 16;
     if (l.step) {
         uint32_t s = 0;
-        for (int k = l.k; k < groups; k += l.step) {
+        for (int k = l.k; 4 * k < p.j1; k += l.step) {
             int4* const at = reinterpret_cast<int4*>(z + (size_t)(k * a.width + l.c) * 4);
             uint32_t e[4];
             s += exps_of(a, p, lut, have, m, *at, 4 * k, lim, holes, tab, p0, e);
@@ -815,16 +883,16 @@ __global__ __launch_bounds__(64 * kShortWaves, W == 8 ? 4 : 2) void paged_short_
     block_barrier();
     if (l.step) {
         const Probs probs = Probs::of(a, p, s_sum[l.c], lim);
+        uint32_t sum = 0;
         for (int k = l.k; k < groups; k += l.step) {
             const uint2 two = probs(a, p, 4 * k, *reinterpret_cast<const uint2*>(z + (size_t)(k * a.width + l.c) * 4), holes, tab, p0);
-            ps[2 * k * W + l.c] = two.x;
-            ps[(2 * k + 1) * W + l.c] = two.y;
+            sum = (uint32_t)dot_pairs(two.x, 0x00010001u, dot_pairs(two.y, 0x00010001u, (int32_t)sum));
+            store_planes<W>(ph, pl, k, l.c, two);
         }
+        atomicAdd(&p_sum[l.c], sum);
     }
-    block_barrier();
-    int32_t acc[8 * W];
-    paged_values<HD, W, ALIGNED, NW>(a, p, tab, p0, tiles, n, ps, acc);
-    paged_meet<HD, W, NW>(a, lds, tiles.chunk, acc, [&](int i, int32_t x) { write_out<HD>(a, p, i, x); });
+    // the loop's first barrier stands between the planes and their use, p_sum's too
+    paged_values<HD, W, NB, ALIGNED, NW>(a, p, tab, p0, units, ph, pl, p_sum, [&](int v, int d, int32_t x, int32_t y) { write_two<HD>(a, p, v, d, x, y); });
 }
 
 // The ranges' sums, one rounding (attention.rs:84-86).  A block per row and head: four
@@ -894,7 +962,7 @@ hipError_t paged_ranges(const PagedAttn& a, const PagedPlan& pl, hipStream_t st)
     if (e != hipSuccess) return e;
     scores<<<grid, 256, qk, st>>>(a);
     paged_sum_kernel<<<grid, 256, tab, st>>>(a);
-    const size_t pv = 4 * kPvRing * 32 * HD + (size_t)a.range * W * 2 + tab;
+    const size_t pv = kPvRing * 64 * 2 * HD + (size_t)a.range * W * 2 + tab;
     auto values = W == 8 ? paged_pv_kernel<HD, 8, ALIGNED> : paged_pv_kernel<HD, 16, ALIGNED>;
     e = allow_lds(values, pv);
     if (e != hipSuccess) return e;
