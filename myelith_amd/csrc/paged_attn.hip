@@ -459,7 +459,7 @@ __device__ inline uint32_t exps_of(const PagedAttn& a, const Part& p, const uint
         // sat_sub and the lookup of softmax.rs:12-38
         const uint32_t below = min((uint32_t)m - (uint32_t)z[i], 0x7FFFFFFFu) >> (a.lut_shift & 31u);
         uint32_t x = lut[min(below, have)];
-        if (below >= have && below < a.lut_len) x = (uint32_t)max((int32_t)a.lut[below], 0);
+        if (a.lut_len > kSumLut && below >= have && below < a.lut_len) x = (uint32_t)max((int32_t)a.lut[below], 0);
         bool ok = key + i < lim;
         if (holes) ok = ok && on_page(a, tab, p0, min(key + i, p.j1 - 1));
         e[i] = ok ? x : 0u;
