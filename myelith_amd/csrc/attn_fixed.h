@@ -39,7 +39,7 @@ struct ScoreScale {
     }
 };
 
-// RNE(e 2^f / S) for 0 <= e < 2^15, f <= 14 and 1 <= S < 2^31.  With l =
+// RNE(e 2^f / S) for 0 <= e < 2^15, f <= 14 and 1 <= S < 2^32.  With l =
 // ceil(log2 S), K = 16 + l and m = ceil(2^(K+f) / S),
 //   e m / 2^K = e 2^f / S + d,  0 <= d < e / 2^K < 2^-(1+l) <= 1 / (2 S),
 // and e 2^f / S + 1/2 is a whole number or at least 1 / (2 S) below the next, so

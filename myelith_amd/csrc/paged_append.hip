@@ -274,6 +274,8 @@ int myl_kv_append_paged_dev(myl_ctx* ctx, const int16_t* q, size_t ldq, const in
         return bad("null operand");
     uintptr_t ptrs = (uintptr_t)q | (uintptr_t)k | (uintptr_t)v | (uintptr_t)q_out | (uintptr_t)bias | (uintptr_t)bias_shifts |
                      (uintptr_t)cos_lut | (uintptr_t)sin_lut | (uintptr_t)k_pages | (uintptr_t)v_pages;
+    if (norm)
+        ptrs |= (uintptr_t)norm->q_gamma | (uintptr_t)norm->q_gamma_shifts | (uintptr_t)norm->k_gamma | (uintptr_t)norm->k_gamma_shifts;
     if ((ptrs & 15) || ((ldq | ldk | ldv | ldo | page_stride | head_stride | pos_stride) & 7))
         return bad("operands must be 16-byte aligned, strides multiples of 8");
     const DeviceGuard guard(ctx->device);

@@ -181,9 +181,7 @@ struct Tiles {
     __device__ inline void issue(const PagedAttn& a, const uint64_t* tab, int p0, int j, int j1, int slot) const {
         int8_t* to = ring + slot * kBytes;
         if (ALIGNED) {
-            const uint64_t first = place_of(a, tab, p0, j);
-            const uint64_t u = ((uint64_t)__builtin_amdgcn_readfirstlane((uint32_t)(first >> 32)) << 32) | __builtin_amdgcn_readfirstlane((uint32_t)first);
-            const char* base = pages + 2 * u;
+            const char* base = pages + 2 * uniform_u64(place_of(a, tab, p0, j));
             if (a.tiles.d == 1)
 #pragma unroll
                 for (int i = 0; i < NI; ++i)
@@ -621,9 +619,7 @@ struct Units {
         const int j = p.j0 + 64 * u + first;
         int8_t* to = ring + slot * kBytes + first * 2 * HD;
         if (ALIGNED) {
-            const uint64_t at = place_of(a, tab, p0, j);
-            const uint64_t s = ((uint64_t)__builtin_amdgcn_readfirstlane((uint32_t)(at >> 32)) << 32) | __builtin_amdgcn_readfirstlane((uint32_t)at);
-            const char* base = pages + 2 * s;
+            const char* base = pages + 2 * uniform_u64(place_of(a, tab, p0, j));
             if (a.tiles.d == 1)
 #pragma unroll
                 for (int i = 0; i < NI; ++i)

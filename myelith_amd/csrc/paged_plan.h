@@ -60,6 +60,8 @@ constexpr size_t kPagedMaxKeys = 131072;
 constexpr size_t kPagedMaxRows = 65535;
 constexpr size_t kPagedMaxPairs = (size_t)1 << 22;  // rows x heads
 constexpr size_t kPagedMaxLut = 32768;
+constexpr size_t kPagedMaxWork = (size_t)1 << 33;  // keys of all tiles: blocks of 256 threads below 2^32 of them
+constexpr int kPagedTile = 16;                     // query vectors of a tile
 
 struct PagedShape {
     size_t n_seqs, rows_per_seq, heads, kv_heads, head_dim, max_len;
@@ -71,13 +73,15 @@ inline const char* paged_refuse(const PagedShape& s) {
         s.n_seqs * s.rows_per_seq > kPagedMaxRows || s.n_seqs * s.rows_per_seq * s.heads > kPagedMaxPairs)
         return "too many rows or heads (65535 each, 2^22 together)";
     if (s.max_len > kPagedMaxKeys) return "more than 131072 keys per row";
+    const size_t tiles = (s.rows_per_seq * (s.heads / s.kv_heads) + kPagedTile - 1) / kPagedTile;
+    if (s.n_seqs * s.kv_heads * tiles * s.max_len > kPagedMaxWork) return "too many keys in all (2^33 for each 16 query heads that share a KV head)";
     return nullptr;
 }
 
 // The query vectors (heads of rows) that read one sequence's KV head are cut into tiles of at
 // most 16, the keys into ranges of a multiple of 64; a block takes one tile and one range.
 // Within a range of at most 1024 keys sum p |v| <= (2^14 + 2^9) 2^15 < 2^30.
-constexpr int kPagedTile = 16, kPagedMaxRange = 1024, kPagedMidRange = 512, kPagedLeastRange = 128;
+constexpr int kPagedMaxRange = 1024, kPagedMidRange = 512, kPagedLeastRange = 128;
 constexpr int kPagedLdsLut = 8192;  // exp table entries that a block copies
 
 // The pages that a range of keys can touch.

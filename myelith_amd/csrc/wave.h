@@ -56,6 +56,12 @@ __device__ inline uint64_t row_sum16_u64(uint64_t v) {
     return v;
 }
 
+// A value that a wave's lanes share, in scalar registers.  The builtin returns a signed int: the
+// halves are joined as unsigned ones.
+__device__ inline uint64_t uniform_u64(uint64_t v) {
+    const uint32_t lo = __builtin_amdgcn_readfirstlane((uint32_t)v), hi = __builtin_amdgcn_readfirstlane((uint32_t)(v >> 32));
+    return ((uint64_t)hi << 32) | lo;
+}
 __device__ inline int32_t readlane_i32(int32_t v, int lane) { return __builtin_amdgcn_readlane(v, lane); }
 
 __device__ inline uint64_t readlane_u64(uint64_t v, int lane) {
