@@ -39,8 +39,8 @@ struct PagedAttn {
     size_t ldq, ldo, ldt, page_stride, head_stride, pos_stride;
     int64_t mult;
     ScoreScale scale;
-    SmallDiv n, G, page, kvh, tiles, ranges_d, width_d, heads_d;
-    int heads, max_len, n_pages, keys, range, ranges, width, vectors, places;
+    SmallDiv n, G, page, kvh, tiles, ranges_d, width_d, heads_d, range_d;
+    int heads, max_len, n_pages, keys, range, ranges, width, vectors, places, entries;  // entries: of a block's page table
     uint32_t lut_len;
     uint8_t shift, lut_shift, prob_frac;
 };
@@ -835,7 +835,7 @@ __global__ __launch_bounds__(64 * kShortWaves, 4) void paged_short_kernel(PagedA
     int8_t* const ph = reinterpret_cast<int8_t*>(z + (size_t)a.keys * a.width);
     int8_t* const pl = ph + a.keys * W;
     uint64_t* const tab = reinterpret_cast<uint64_t*>(pl + a.keys * W);
-    uint16_t* const lut = reinterpret_cast<uint16_t*>(tab + paged_table_entries(a.range, (int)a.page.d));
+    uint16_t* const lut = reinterpret_cast<uint16_t*>(tab + a.entries);
     Part p;
     int lane_lim;
     if (!place_of_block(a, p)) return;
@@ -903,7 +903,8 @@ __global__ __launch_bounds__(THREADS) void paged_out_kernel(PagedAttn a) {
     const int tile = divmod(a.width_d, in_seq * (int)a.G.d + h, v), lim = keys_of(a, row);
     const size_t at = (((size_t)seq * a.kvh.d + g) * a.tiles.d + tile) * a.ranges;
     int64_t s[4] = {0, 0, 0, 0};
-    const int last = min(a.ranges, (lim + a.range - 1) / max(a.range, 1));
+    int rem;
+    const int last = min(a.ranges, divmod(a.range_d, lim + a.range - 1, rem));
     for (int r0 = share; r0 < last; r0 += 8 * SHARES) {
         int4 x[8];
 #pragma unroll
@@ -951,7 +952,7 @@ hipError_t paged_ranges(const PagedAttn& a, const PagedPlan& pl, hipStream_t st)
     const int W = a.width <= 8 ? 8 : 16;
     if (pl.in_one) return W == 8 ? paged_in_one<HD, ALIGNED, 8>(a, pl, st) : paged_in_one<HD, ALIGNED, 16>(a, pl, st);
     const unsigned grid = (unsigned)pl.blocks;
-    const size_t tab = (size_t)paged_table_entries(a.range, (int)a.page.d) * 8;
+    const size_t tab = (size_t)a.entries * 8;
     const size_t qk = 4 * kQkRing * 32 * HD + tab;
     auto scores = a.scale.fast ? paged_qk_kernel<HD, true, ALIGNED> : paged_qk_kernel<HD, false, ALIGNED>;
     hipError_t e = allow_lds(scores, qk);
@@ -1032,6 +1033,7 @@ int myl_attention_paged_dev(myl_ctx* ctx, const int16_t* q, size_t n_seqs, size_
     auto div = [](size_t d) { return SmallDiv::of(std::max<size_t>(d, 1)); };
     a.n = div(rows_per_seq); a.G = div(heads / kv_heads); a.page = div(page_size); a.kvh = div(kv_heads);
     a.tiles = div((size_t)pl.tiles); a.ranges_d = div((size_t)pl.ranges); a.width_d = div((size_t)pl.width); a.heads_d = div(heads);
+    a.range_d = div((size_t)pl.range); a.entries = pl.ranges ? paged_table_entries(pl.range, (int)page_size) : 0;
     a.heads = (int)heads; a.max_len = (int)max_len; a.n_pages = (int)n_pages; a.keys = pl.keys;
     a.range = pl.range; a.ranges = pl.ranges; a.width = pl.width; a.vectors = (int)(rows_per_seq * (heads / kv_heads));
     a.places = (int)(n_seqs * kv_heads * (size_t)pl.ranges);
