@@ -665,8 +665,12 @@ class RocmBackend:
     def _rows_of(what: str, name: str, t, inner: int) -> int:
         """The row stride of [rows x heads x hd] whose heads follow one another."""
         row, head, one = t.stride()
-        if one == 1 and head == t.shape[2] and row >= inner and t.shape[0] > 1:
-            return row
+        if one == 1 and head == t.shape[2]:
+            n = t.shape[0]
+            if n > 1 and row >= inner:
+                return row
+            if n == 1:
+                return inner
         row, head, one = _strides(t)
         if head not in (None, t.shape[2]) or one not in (None, 1):
             raise ValueError(f"{what}: the heads of a row of {name} follow one another")

@@ -79,20 +79,20 @@ struct TurnRound {
     }
 };
 
-// A thread's 8 channels of a norm.
+// A thread's 8 channels of a norm, as they are in memory: unpacked where they are used.
 struct Gamma8 {
-    int32_t g[8];
-    uint32_t s[8], least, most;
+    uint2 g, s;
+    uint32_t least, most;
+    __device__ static inline uint32_t byte(const uint2& w, int i) { return ((i < 4 ? w.x : w.y) >> (8 * (i & 3))) & 255u; }
     __device__ inline void load(const int8_t* gamma, const uint8_t* shifts) {
-        const uint2 gw = *reinterpret_cast<const uint2*>(gamma), sw = *reinterpret_cast<const uint2*>(shifts);
+        g = *reinterpret_cast<const uint2*>(gamma);
+        s = *reinterpret_cast<const uint2*>(shifts);
         least = 255;
         most = 0;
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-            g[i] = (int32_t)(int8_t)((i < 4 ? gw.x : gw.y) >> (8 * (i & 3)));
-            s[i] = ((i < 4 ? sw.x : sw.y) >> (8 * (i & 3))) & 255u;
-            least = min(least, s[i]);
-            most = max(most, s[i]);
+            least = min(least, byte(s, i));
+            most = max(most, byte(s, i));
         }
     }
     // rms_out of 8 values.  |x gamma lut| < 2^37, so right shifts by 6 .. 31 leave 32 bits.
@@ -101,8 +101,8 @@ struct Gamma8 {
         if (!f.zero && base + (int32_t)least >= 6 && base + (int32_t)most <= 31) {
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-                const uint32_t sh = (uint32_t)base + s[i];
-                const int64_t p = (int64_t)(x[i] * g[i]) * (int64_t)(int32_t)f.lut_val;
+                const uint32_t sh = (uint32_t)base + byte(s, i);
+                const int64_t p = (int64_t)(x[i] * (int32_t)(int8_t)byte(g, i)) * (int64_t)(int32_t)f.lut_val;
                 const uint32_t lo = (uint32_t)p, hi = (uint32_t)((uint64_t)p >> 32);
                 const uint32_t q = __builtin_amdgcn_alignbit(hi, lo, sh);
                 const uint32_t rest = lo & ((1u << sh) - 1u);
@@ -111,9 +111,33 @@ struct Gamma8 {
             return;
         }
 #pragma unroll
-        for (int i = 0; i < 8; ++i) x[i] = rms_out((int16_t)x[i], 0, (int8_t)g[i], (uint8_t)s[i], f, frac);
+        for (int i = 0; i < 8; ++i) x[i] = rms_out((int16_t)x[i], 0, (int8_t)byte(g, i), (uint8_t)byte(s, i), f, frac);
     }
 };
+
+// The sum of 8 squares in pairs: 2^31 at most each, unsigned.
+__device__ inline uint64_t squares8(const uint4 x) {
+    typedef short __attribute__((ext_vector_type(2))) s2;
+    const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+    uint64_t s = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) s += (uint32_t)__builtin_amdgcn_sdot2(__builtin_bit_cast(s2, w[i]), __builtin_bit_cast(s2, w[i]), 0, false);
+    return s;
+}
+
+// rms_factor_of a head's sum of squares, at most 2^37: (sum inv_n) >> 20 with inv_n <= 2^20 in 64 bits.
+__device__ inline RmsFactor head_factor(uint64_t sum, const RmsParams& p) {
+    RmsIdx r{sum == 0, 0, 0};
+    if (!r.zero) {
+        const uint64_t m = (sum * (uint64_t)(uint32_t)p.inv_n_q20) >> 20;
+        const uint32_t most = (uint32_t)p.lut_len - 1u;
+        const uint32_t bm = 64u - (uint32_t)__builtin_clzll(m | 1u), bi = 32u - (uint32_t)__builtin_clz(most);
+        r.q = bm > bi ? (bm - bi) & ~1u : 0u;
+        if (m >> r.q > most) r.q += 2;
+        r.idx = (int)min((uint32_t)rne_shift64_small((int64_t)m, r.q), most);
+    }
+    return rms_factor_at(r, 0, p, r.zero ? 0 : (int64_t)p.lut[r.idx]);
+}
 
 // R rows at a time, `group` of them to a thread.
 template <int HD, bool BIAS, bool NORM, int R>
@@ -183,14 +207,12 @@ __global__ __launch_bounds__(256) void append_kernel(Append a) {
                     x1[i] = sat16(x1[i] + b1[i]);
                 }
             if (NORM) {
-                uint64_t s = 0;  // at most 128 2^30
-#pragma unroll
-                for (int i = 0; i < 8; ++i) s += (uint64_t)((int64_t)x0[i] * x0[i]) + (uint64_t)((int64_t)x1[i] * x1[i]);
+                uint64_t s = BIAS ? squares8(pack8(x0)) + squares8(pack8(x1)) : squares8(raw[r][0]) + squares8(raw[r][1]);  // at most 128 2^30
                 s = dpp_add64<dpp::kXor1>(s);
                 s = dpp_add64<dpp::kXor2>(s);
                 if (CH == 8) s = dpp_add64<dpp::kHalfMirror>(s);
                 if (gamma) {
-                    const RmsFactor f = rms_factor_of((myl_i128)s, 0, a.rms);
+                    const RmsFactor f = head_factor(s, a.rms);
                     g0.apply(f, norm_frac, x0);
                     g1.apply(f, norm_frac, x1);
                 }

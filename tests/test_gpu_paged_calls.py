@@ -100,13 +100,13 @@ def test_steps_together(backend, exp_lut, seqs, rows, H, KH, hd, page, start):
         s.advance()
 
 
-@pytest.mark.parametrize("start", [30, 2200])
-def test_captured_steps(backend, exp_lut, start):
+@pytest.mark.parametrize("start,hd,seqs", [(30, 64, 4), (2200, 64, 4), (500, 128, 4), (12000, 128, 9)])
+def test_captured_steps(backend, exp_lut, start, hd, seqs):
     """The three calls captured and replayed, each replay a step further, with the program's own eager
     work and synchronizations between."""
     import torch
-    case(f"captured steps from {start}")
-    s = Step(backend, exp_lut, seqs=4, H=14, KH=2, start=start, steps=6, seed=2)
+    case(f"captured steps of {seqs} sequences from {start}, heads of {hd}")
+    s = Step(backend, exp_lut, seqs=seqs, H=14, KH=2, hd=hd, start=start, steps=6, seed=2)
     stream = torch.cuda.Stream()
     try:
         s.product()
