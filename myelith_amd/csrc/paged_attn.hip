@@ -10,7 +10,13 @@
 //   paged_sum_kernel   e_j = exp_lut[(max - z_j) >> lut_shift] as 16 bits, the ranges' sums
 //   paged_pv_kernel    p_j from e_j and S, sum p_j v_j over each range
 //   paged_out_kernel   the sums over the ranges, rounded and clamped
-// Keys and values are read once each.
+// Keys and values are read once each, the scores and exp values (6 bytes a key and head) written
+// and read beside them.  us by kernel in that order, heads of 128, seven to a KV head of four: 64 rows of up to
+// 12000 keys 118 + 24 + 124 + 6 (282 a call; 4.1 TB/s of keys and values), one row of 100000 23 + 8.5 +
+// 23 + 4.5 (59), 24 rows of up to 2500 13 + 6 + 14.5 + 4 (36), of which starting and draining four launches
+// is most.  Joining the ranges in the tile's last block instead of a fourth launch took longer
+// (24 x 2500: 38.7 us with write-through stores and loads, 107 with device fences).  Few keys take one
+// launch (paged_short_kernel).
 #include "abi_internal.h"
 #include "attn_fixed.h"
 #include "gemm_mfma.h"
@@ -224,7 +230,8 @@ __device__ inline int tiles_of_wave(const Part& p, int wave) {
 // false), for which 256 128 sum kh + 128 sum kl come from the matrix cores as well (a B operand
 // of 64s, added twice).  As 256 u + r the score takes 32-bit steps (ScoreScale);
 // other scales take the 64-bit form (FAST false).
-// Bound by issue and by the loads' latency: about 120 vector and 8 matrix instructions a tile.
+// 64 rows of up to 12000 keys: 118 us, bound by bytes; short calls by the loads' latency: two
+// tiles a wave are on their way.
 constexpr int kQkRing = 2;
 // NW: waves of the block, a tile in turn each.  STORED: the scores go to memory, not LDS.
 template <int HD, bool FAST, bool ALIGNED, bool BALANCED, int NW, bool STORED>
