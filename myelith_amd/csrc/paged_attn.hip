@@ -553,7 +553,9 @@ __device__ inline Uniform uniform_of(const PagedAttn& a, const Part& p, int lim)
     return u;
 }
 
-constexpr int kPvAhead = 4;
+// Groups of four keys a thread has on their way from the start.  us of a call with 4 / 6 / 8: 12 x 4 rows of
+// 3001 keys 41.7 / 40.0 / 40.3, one row of 100000 58.9 / 57.9 / 57.9, 24 rows of 2500 36.3 / 36.3 / 36.6.
+constexpr int kPvAhead = 6;
 
 // p of the four keys from `key` on, from their e, as two pairs.
 struct Probs {
