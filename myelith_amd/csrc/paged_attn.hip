@@ -12,8 +12,8 @@
 //   paged_out_kernel   the sums over the ranges, rounded and clamped
 // Keys and values are read once each, the scores and exp values (6 bytes a key and head) written
 // and read beside them.  us by kernel in that order, heads of 128, seven to a KV head of four: 64 rows of up to
-// 12000 keys 118 + 24 + 124 + 6 (282 a call; 4.1 TB/s of keys and values), one row of 100000 23 + 8.5 +
-// 23 + 4.5 (59), 24 rows of up to 2500 13 + 6 + 14.5 + 4 (36), of which starting and draining four launches
+// 12000 keys 119 + 24 + 121 + 6 (282 a call; 4.1 TB/s of keys and values), one row of 100000 23 + 8.5 +
+// 22 + 4.6 (58), 24 rows of up to 2500 13 + 7 + 14 + 4 (36), of which starting and draining four launches
 // is most.  Joining the ranges in the tile's last block instead of a fourth launch took longer
 // (24 x 2500: 38.7 us with write-through stores and loads, 107 with device fences).  Few keys take one
 // launch (paged_short_kernel).
@@ -230,7 +230,7 @@ __device__ inline int tiles_of_wave(const Part& p, int wave) {
 // false), for which 256 128 sum kh + 128 sum kl come from the matrix cores as well (a B operand
 // of 64s, added twice).  As 256 u + r the score takes 32-bit steps (ScoreScale);
 // other scales take the 64-bit form (FAST false).
-// 64 rows of up to 12000 keys: 118 us, bound by bytes; short calls by the loads' latency: two
+// 64 rows of up to 12000 keys: 119 us, bound by bytes; short calls by the loads' latency: two
 // tiles a wave are on their way.
 constexpr int kQkRing = 2;
 // NW: waves of the block, a tile in turn each.  STORED: the scores go to memory, not LDS.

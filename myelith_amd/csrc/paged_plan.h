@@ -127,8 +127,9 @@ inline PagedPlan paged_plan(const PagedShape& s, int cus) {
             p.in_one = true;
             p.range = p.keys;
         } else {
-            // A block per CU where ranges of 128 to 512 keys make it, then two where up to 1024 keys do.  us of a call's launches at 128 / 256 / 512 keys, heads of 128: one row of 5000
-            // keys 20.4 / 21.6 / 25.8, 10000 25.8 / 23.9 / 26.9, 30000 38.8 / 32.9 / 30.7; eight of 2000
+            // A block per CU where ranges of 128 to 512 keys make it, then two where up to 1024 keys
+            // do.  us of a call's launches at 128 / 256 / 512 keys, heads of 128: one row of 5000 keys
+            // 20.4 / 21.6 / 25.8, 10000 25.8 / 23.9 / 26.9, 30000 38.8 / 32.9 / 30.7; eight of 2000
             // 25.1 / 23.7 / 27.2; 64 of 300 28.8 / 29.3 / 22.3 (one range); 24 of 2500 40.6 / 40.7 / 38.2.
             const size_t each = (p.parts * (size_t)p.keys + (size_t)cus - 1) / (size_t)cus;
             const size_t want = each <= kPagedMidRange ? std::max<size_t>(each, kPagedLeastRange) : std::max<size_t>(each / 2, kPagedMidRange);
