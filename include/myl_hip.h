@@ -328,7 +328,7 @@ int myl_verify_drafts_dev(myl_ctx* ctx, const int32_t* target, size_t ldt, const
  * and [page][position][head] both do.  A sequence's positions lie in the pages that its
  * row of `tables` (n_seqs rows of table_len int32, table_stride apart) names in turn:
  * position pos in page tables[seq][pos / page_size], at pos % page_size.  Sequences may
- * share pages.  An id outside [0, n_pages) names no page.  Pointers to int16 and uint8 and
+ * share pages.  An id outside [0, n_pages) names no page.  Pointers to int16, int8, uint8 and
  * the workspace are 16-byte aligned; head_dim is 64 or 128 (MYL_E_UNSUPPORTED
  * otherwise). */
 
