@@ -707,7 +707,9 @@ class RocmBackend:
         pages), tables int32 [sequences x pages of each], cos_lut and sin_lut int16
         [positions x hd / 2], bias int16 and bias_shifts uint8 [(heads + 2 kv_heads) hd] or
         None, norm a HeadNorm or None.  Returns q_out, the rotated queries; it may be q
-        itself.  include/myl_hip.h states the arithmetic."""
+        itself.  Rows that are left out stay as they were in a given q_out and are zero in
+        one that the call allocates (cleared by a launch of its own, so a program keeps
+        one from step to step).  include/myl_hip.h states the arithmetic."""
         import torch
         what = "kv_append_paged_dev"
         if (rope_frac | q_frac | k_frac | v_frac) >> 8:
@@ -741,7 +743,7 @@ class RocmBackend:
             raise ValueError(f"{what}: norm must be of head_dim values on {dev}")
         stream = self._other_stream(dev) if q_out is None else None
         if q_out is None:
-            q_out = self._empty((R, H, hd), "int16", dev, stream)
+            q_out = self._empty((R, H, hd), "int16", dev, stream).zero_()  # the library leaves rows that are left out as they were
         elif not (q_out.dtype is i16 and q_out.get_device() == d):
             _need_dev(what, dev, q_out=(q_out, "int16", None))
         if q_out.shape != q.shape:

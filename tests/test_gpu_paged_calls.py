@@ -338,3 +338,32 @@ def test_logprobs_more_equal_values_than_candidates(backend, exp_lut, R):
         z[r, (r * 37) % V::(r % 700) + 1] = r
     check_logprobs(backend, z, np.arange(R), exp_lut, 32)
     check_logprobs(backend, z, np.arange(R), exp_lut, 1)
+
+
+@pytest.mark.parametrize("rows", [6, 3000])
+def test_append_rows_left_out_of_allocated_queries(backend, rows):
+    """Without q_out, rows that are left out answer with zeros, whatever the memory held before."""
+    import torch
+    case(f"append rows left out of an allocated output, {rows} rows")
+    s = append_inputs(80 + rows, rows, 4, 2, 64, 16, seqs=6, context=600)
+    s["positions"][::3] = -1
+    s["seqs"][1::6] = 6
+    want = ref.append(s["q"], s["k"], s["v"], s["positions"], s["kp"], s["vp"], s["tables"], s["cos"], s["sin"], 8, np.zeros_like(s["q"]), s["seqs"],
+                      s["bias"], s["bias_shifts"], FRACS)
+    try:
+        for stream in (None, torch.cuda.Stream()):  # torch's stream, and the context's own beside it
+            if stream is not None:
+                torch.cuda.synchronize()
+                with torch.cuda.stream(stream):
+                    backend.use_torch_stream()
+            d = dict(on_gpu(s), norm=None)
+            used = [torch.full((rows, 4, 64), 77, dtype=torch.int16, device="cuda") for _ in range(4)]
+            torch.cuda.synchronize()
+            del used
+            got = run_append(backend, d, None)
+            torch.cuda.synchronize()
+            for what, g, w in zip(("queries", "keys", "values"), (got, d["kp"], d["vp"]), want):
+                same(g, w, what)
+    finally:
+        torch.cuda.synchronize()
+        backend.use_torch_stream()

@@ -397,3 +397,15 @@ def test_scalars_outside_their_type_are_refused(recorded):  # noqa: F811
         with pytest.raises(ValueError, match="score_mult"):
             b.attention_paged_dev(**paged_args(score_mult=v))
     assert not log
+
+
+def test_allocated_queries_of_left_out_rows_are_zero(recorded, monkeypatch):  # noqa: F811
+    """The kernel writes nothing for a row that is left out: memory that the call allocates is
+    cleared before it, a caller's q_out is not touched."""
+    b, log = recorded
+    empty = torch.empty
+    monkeypatch.setattr(torch, "empty", lambda *a, **k: empty(*a, **k).fill_(77))
+    got = b.kv_append_paged_dev(**append_args(positions=torch.tensor([0, -1, 5], dtype=torch.int32)))
+    assert log[-1][0] == "myl_kv_append_paged_dev" and log[-1][1][34] == got.data_ptr() and not got.any()
+    given = torch.full((3, 4, 64), -7, dtype=torch.int16)
+    assert b.kv_append_paged_dev(**append_args(q_out=given)) is given and (given == -7).all()
