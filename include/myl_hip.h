@@ -380,8 +380,9 @@ int myl_kv_append_paged_dev(myl_ctx* ctx, const int16_t* q, size_t ldq, const in
  * prob_frac is at most 14, heads and rows at most 65535 each and 2^22 together, the exp
  * table 1 to 32768 entries; negative ones count as 0.  max_len, for each 16 (or fewer) query
  * heads of a sequence that share a KV head, is at most 2^33 in all.  A max_len close to the
- * longest row's keeps the launches small; the workspace holds 6 bytes per row, head and position
- * below max_len, and serves fewer rows and keys of the same heads. */
+ * longest row's keeps the launches small; the workspace holds 6 bytes and a sixteenth of them
+ * per row, head and position below max_len, and serves calls of the same heads with no more rows in
+ * all, however many of them a sequence has, and no more keys. */
 size_t myl_attention_paged_workspace(const myl_ctx* ctx, size_t n_seqs, size_t rows_per_seq, size_t heads,
                                      size_t kv_heads, size_t head_dim, size_t max_len);
 int myl_attention_paged_dev(myl_ctx* ctx, const int16_t* q, size_t n_seqs, size_t rows_per_seq, size_t ldq,

@@ -764,7 +764,8 @@ class RocmBackend:
         return q_out
 
     def attention_paged_workspace(self, q, k_pages, max_len: int, rows_per_seq: int = 1):
-        """A workspace for attention_paged_dev on operands of these shapes, and on fewer rows or keys."""
+        """A workspace for attention_paged_dev on operands of these shapes, and of the same heads on
+        no more rows in all, however many of them a sequence has, and no more keys."""
         n = lib().myl_attention_paged_workspace(self._h, q.shape[0] // max(1, rows_per_seq), rows_per_seq, q.shape[1],
                                                 k_pages.shape[1], q.shape[2], max_len)
         return self._new_workspace(n, q.device, "attention_paged_dev")

@@ -138,9 +138,11 @@ inline PagedPlan paged_plan(const PagedShape& s, int cus) {
         p.ranges = (p.keys + p.range - 1) / p.range;
     }
     p.blocks = ((int64_t)s.n_seqs * (int64_t)s.kv_heads * p.ranges + 7) / 8 * 8 * p.tiles;
-    // The ranges of any smaller call, ceil(keys / range): at most as many as the least range makes,
-    // as many as the middle one makes, or those of which a CU has about one.
-    const size_t vecs = p.parts * (size_t)p.width, keys = (size_t)p.keys;
+    // Room for any call of no more rows in all, however they lie in sequences, and no more keys.  A
+    // sequence's v vectors take tiles x width <= v + tiles - 1 <= v + (v - 1) / 16 places; and its ranges,
+    // ceil(keys / range), are at most as many as the least range makes, as many as the middle one
+    // makes, or those of which a CU has about one.
+    const size_t pairs = s.n_seqs * s.rows_per_seq * s.heads, vecs = pairs + pairs / kPagedTile, keys = (size_t)p.keys;
     const size_t pieces = std::min(vecs * ((keys + kPagedLeastRange - 1) / kPagedLeastRange),
                                    vecs * (1 + (keys + kPagedMidRange - 1) / kPagedMidRange) + (size_t)kPagedTile * (size_t)cus);
     Layout l;

@@ -367,3 +367,14 @@ def test_append_rows_left_out_of_allocated_queries(backend, rows):
     finally:
         torch.cuda.synchronize()
         backend.use_torch_stream()
+
+
+def test_attention_of_drafts_in_the_workspace_of_a_decode_batch(backend, exp_lut):
+    """64 requests of one row each keep a workspace; 21 of them then take three drafted rows."""
+    case("attention of 21 x 3 rows in the workspace of 64 x 1")
+    s = attention_inputs(81, 21, 3, 28, 4, 64, 1300, 16)
+    d = on_gpu(s)
+    one = d["q"].new_empty((64, 28, 64))
+    ws = dirty(backend.attention_paged_workspace(one, d["kp"], 1300))
+    got = backend.attention_paged_dev(d["q"], d["kp"], d["vp"], d["tables"], d["lens"], s["mult"], 21, gpu(exp_lut), 6, 14, rows_per_seq=3, max_len=1300, workspace=ws)
+    same(got, ref.attention(**s, lut=exp_lut), "kept workspace")

@@ -409,3 +409,46 @@ def test_allocated_queries_of_left_out_rows_are_zero(recorded, monkeypatch):  # 
     assert log[-1][0] == "myl_kv_append_paged_dev" and log[-1][1][34] == got.data_ptr() and not got.any()
     given = torch.full((3, 4, 64), -7, dtype=torch.int16)
     assert b.kv_append_paged_dev(**append_args(q_out=given)) is given and (given == -7).all()
+
+
+KEPT = PLANS[:PLANS.index("// pieces of a workspace")].replace('#include "serve_plan.h"', '#include "paged_plan.h"') + r"""
+// A size of the smaller call: often the same, one less, a half, or any.
+static size_t below(size_t n) {
+    const uint64_t r = next() % 6;
+    return r < 2 ? n : r == 2 ? n - 1 : r == 3 ? n / 2 : r == 4 ? n - n / 8 : (size_t)(next() % (n + 1));
+}
+static void hold(PagedShape l, PagedShape s, int cus) {
+    if (paged_refuse(l) || paged_refuse(s)) return;
+    const size_t large = paged_plan(l, cus).bytes, small = paged_plan(s, cus).bytes;
+    CHECK(small <= large, "%zu bytes for %zu x %zu rows of %zu keys, %zu for %zu x %zu of %zu, heads %zu / %zu", small, s.n_seqs, s.rows_per_seq, s.max_len, large,
+          l.n_seqs, l.rows_per_seq, l.max_len, l.heads, l.kv_heads);
+}
+int main() {
+    hold({64, 1, 28, 4, 128, 2500}, {21, 3, 28, 4, 128, 2500}, 256);
+    hold({241, 1, 1, 1, 64, 2500}, {1, 241, 1, 1, 64, 2500}, 256);
+    for (int i = 0; i < 300000; ++i) {
+        const size_t kvh = upto(16), hd = i & 1 ? 64 : 128;
+        const PagedShape l{upto(i & 2 ? 80 : 3000), upto(i & 4 ? 9 : 3000), kvh * upto(20), kvh, hd, upto(131073) - 1};
+        PagedShape s = l;
+        s.rows_per_seq = i & 8 ? upto(40) : upto(l.n_seqs * l.rows_per_seq);
+        s.n_seqs = below(l.n_seqs * l.rows_per_seq / s.rows_per_seq);
+        s.max_len = below(l.max_len);
+        hold(l, s, i % 3 ? 256 : (int)upto(512));
+    }
+    std::printf("checked %ld bad %ld\n", checked, bad);
+    return bad != 0;
+}
+"""
+
+
+@pytest.mark.skipif(shutil.which("g++") is None, reason="g++ absent")
+def test_an_attention_workspace_serves_as_many_rows_of_any_sequences(tmp_path):
+    """Rows may change from one per sequence to several (drafts of fewer requests): no more rows in
+    all, of the same heads, and no more keys, fit where the former did."""
+    src, exe = tmp_path / "kept.cpp", tmp_path / "kept"
+    src.write_text(KEPT)
+    subprocess.run(["g++", "-std=c++17", "-O1", "-g", "-fsanitize=address,undefined", "-fno-sanitize-recover=all", "-I", str(CSRC),
+                    str(src), "-o", str(exe)], check=True, capture_output=True, timeout=300)
+    r = subprocess.run([str(exe)], capture_output=True, text=True, timeout=600)
+    assert r.returncode == 0, (r.stdout[-3000:], r.stderr[-3000:])
+    assert int(re.match(r"checked (\d+) bad 0", r.stdout.strip().splitlines()[-1]).group(1)) > 100000
