@@ -382,6 +382,7 @@ __global__ __launch_bounds__(256, 4) void paged_qk_kernel(PagedAttn a) {
     __shared__ __align__(16) int8_t qlds[16 * 2 * HD];
     __shared__ int32_t red[64];
     __shared__ int bad[4], large[4];
+    static_assert(sizeof qlds + sizeof red + sizeof bad + sizeof large <= kPagedOwnLds, "paged_ranges");
     uint64_t* const tab = reinterpret_cast<uint64_t*>(lds + 4 * kQkRing * 32 * HD);
     Part p;
     int lim;
@@ -762,6 +763,7 @@ __global__ __launch_bounds__(256, 4) void paged_pv_kernel(PagedAttn a) {
     extern __shared__ __align__(16) int8_t lds[];  // the ring, the range's p planes, its pages
     __shared__ uint32_t s_sum[16], p_sum[16];
     __shared__ int bad[4];
+    static_assert(sizeof s_sum + sizeof p_sum + sizeof bad <= kPagedOwnLds, "allow_lds");
     int8_t* const ph = lds + NB * U::kBytes;
     int8_t* const pl = ph + a.range * W;
     uint64_t* const tab = reinterpret_cast<uint64_t*>(pl + a.range * W);
@@ -840,6 +842,7 @@ __global__ __launch_bounds__(64 * kShortWaves, 4) void paged_short_kernel(PagedA
     __shared__ int32_t red[16 * NW];
     __shared__ uint32_t s_sum[16], p_sum[16];
     __shared__ int bad[NW], large[NW];
+    static_assert(sizeof qlds + sizeof red + sizeof s_sum + sizeof p_sum + sizeof bad + sizeof large <= kPagedOwnLds, "allow_lds");
     int32_t* const z = reinterpret_cast<int32_t*>(lds + NB * U::kBytes);  // [keys / 4][width][4]
     int8_t* const ph = reinterpret_cast<int8_t*>(z + (size_t)a.keys * a.width);
     int8_t* const pl = ph + a.keys * W;
@@ -940,10 +943,10 @@ __global__ __launch_bounds__(THREADS) void paged_out_kernel(PagedAttn a) {
 
 constexpr size_t kAlignedStride = (size_t)1 << 26;  // 15 of them and a vector are 32 bits of bytes
 
-// A launch with more LDS than the 64 KiB it has by default.
+// A launch with more LDS than the 64 KiB it has by default, the kernel's own included.
 template <class K>
 hipError_t allow_lds(K kernel, size_t bytes) {
-    return bytes <= 65536 ? hipSuccess : hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+    return bytes + kPagedOwnLds <= 65536 ? hipSuccess : hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
 }
 
 template <int HD, bool ALIGNED, int W>
@@ -963,14 +966,13 @@ hipError_t paged_ranges(const PagedAttn& a, const PagedPlan& pl, hipStream_t st)
     const unsigned grid = (unsigned)pl.blocks;
     const size_t tab = (size_t)a.entries * 8;
     const size_t qk = 4 * kQkRing * 32 * HD + tab;
+    static_assert(4 * kQkRing * 32 * HD + paged_table_entries(kPagedMaxRange, 1) * 8 + kPagedOwnLds <= 65536, "rings, pages and its own");
     auto scores = a.scale.fast ? paged_qk_kernel<HD, true, ALIGNED> : paged_qk_kernel<HD, false, ALIGNED>;
-    hipError_t e = allow_lds(scores, qk);
-    if (e != hipSuccess) return e;
     scores<<<grid, 256, qk, st>>>(a);
     paged_sum_kernel<<<grid, 256, tab, st>>>(a);
     const size_t pv = kPvRing * 64 * 2 * HD + (size_t)a.range * W * 2 + tab;
     auto values = W == 8 ? paged_pv_kernel<HD, 8, ALIGNED> : paged_pv_kernel<HD, 16, ALIGNED>;
-    e = allow_lds(values, pv);
+    const hipError_t e = allow_lds(values, pv);
     if (e != hipSuccess) return e;
     values<<<grid, 256, pv, st>>>(a);
     return hipGetLastError();

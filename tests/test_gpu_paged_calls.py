@@ -378,3 +378,21 @@ def test_attention_of_drafts_in_the_workspace_of_a_decode_batch(backend, exp_lut
     ws = dirty(backend.attention_paged_workspace(one, d["kp"], 1300))
     got = backend.attention_paged_dev(d["q"], d["kp"], d["vp"], d["tables"], d["lens"], s["mult"], 21, gpu(exp_lut), 6, 14, rows_per_seq=3, max_len=1300, workspace=ws)
     same(got, ref.attention(**s, lut=exp_lut), "kept workspace")
+
+
+@pytest.mark.parametrize("keys", [513, 560, 576])
+def test_attention_of_launches_just_past_64_kib(backend, exp_lut, keys):
+    """One launch whose rings, scores, pages and table pass 64 KiB only with what the kernel declares."""
+    case(f"attention of {keys} keys, 14 heads on 2 of 64")
+    check_attention(backend, attention_inputs(82, 3, 1, 14, 2, 64, keys, 16), exp_lut)
+
+
+def test_attention_of_ranges_just_past_64_kib(backend, exp_lut):
+    """Ranges of 960 keys by pages of 8: the same for P.V over ranges."""
+    case("attention of 48 rows of 10000 keys, pages of 8")
+    r = rng(83)
+    s = attention_inputs(83, 1, 1, 1, 1, 128, 2400, 8)
+    s.update(q=gauss16(r, (48, 1, 128), 2048), tables=r.integers(0, s["kp"].shape[0], (48, 1250)).astype(np.int32), max_len=10000,
+             lens=r.integers(1, 10001, 48).astype(np.int32))
+    s["lens"][0] = 10000
+    check_attention(backend, s, exp_lut)

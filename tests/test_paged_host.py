@@ -452,3 +452,67 @@ def test_an_attention_workspace_serves_as_many_rows_of_any_sequences(tmp_path):
     r = subprocess.run([str(exe)], capture_output=True, text=True, timeout=600)
     assert r.returncode == 0, (r.stdout[-3000:], r.stderr[-3000:])
     assert int(re.match(r"checked (\d+) bad 0", r.stdout.strip().splitlines()[-1]).group(1)) > 100000
+
+
+# the launches with what each kernel was allowed before: dynamic LDS by function
+LDS = PROGRAM[:PROGRAM.index("static long calls")].replace("#include <vector>", "#include <vector>\n#include <map>\n#include <set>\n#include \"paged_plan.h\"").replace(
+    "struct Launch { dim3 grid, block; size_t lds; };", "struct Launch { dim3 grid, block; size_t lds, allowed; };\nstatic std::map<const void*, std::vector<int>> attributes;").replace(
+    "hipLaunchKernel(const void*, dim3", "hipLaunchKernel(const void* f, dim3").replace(
+    "launches.push_back({grid, block, lds});", "launches.push_back({grid, block, lds, attributes[f].empty() ? 0 : (size_t)attributes[f].back()});").replace(
+    "hipError_t hipFuncSetAttribute(const void*, hipFuncAttribute, int) { return", "hipError_t hipFuncSetAttribute(const void* f, hipFuncAttribute, int v) { return attributes[f].push_back(v),") + r"""
+template <class T>
+static T* at(size_t n) { return reinterpret_cast<T*>(n); }  // never read on the host
+static myl_ctx* c = nullptr;
+static int attend(size_t seqs, size_t heads, size_t kvh, size_t hd, size_t keys, size_t page, size_t lut) {
+    const size_t bytes = myl_attention_paged_workspace(c, seqs, 1, heads, kvh, hd, keys), ld = heads * hd, len = (keys + page - 1) / page;
+    const int16_t* x = at<int16_t>(1 << 20);
+    return myl_attention_paged_dev(c, x, seqs, 1, ld, heads, kvh, hd, x, x, 1000, page, kvh * page * hd, page * hd, hd, at<int32_t>(64), len, len, at<int32_t>(64), keys, 2896, 21, x,
+                                   lut, 6, 14, at<int16_t>(1 << 22), ld, at<void>(1 << 23), bytes);
+}
+int main() {
+    if (myl_init(0, &c) != MYL_OK) return 2;
+    long n = 0, large = 0, bad = 0;
+    for (size_t hd : {(size_t)64, (size_t)128})
+        for (size_t lut : {(size_t)1, (size_t)2662, (size_t)32768})
+            for (size_t page : {(size_t)1, (size_t)8, (size_t)16, (size_t)64})
+                for (size_t g : {(size_t)1, (size_t)7, (size_t)8, (size_t)9, (size_t)16})
+                    for (size_t seqs : {(size_t)1, (size_t)24, (size_t)64})
+                        for (size_t keys = 64; keys <= 40000; keys += keys < 1024 ? 64 : keys / 3) {
+                            attributes.clear();  // the first call of a process
+                            launches.clear();
+                            if (attend(seqs, 2 * g, 2, hd, keys, page, lut) != MYL_OK) return 3;
+                            for (const Launch& l : launches) {
+                                ++n;
+                                // 64 KiB of both without the attribute; paged_sum_kernel's table is its own
+                                const bool more = l.lds + 4800 > 65536;
+                                large += more;
+                                if ((more && l.allowed < l.lds) || l.lds + 4800 > 160 * 1024) {
+                                    if (bad++ < 10) std::printf("%zu x %zu heads of %zu, %zu keys, pages of %zu: %zu bytes, %zu allowed\n", seqs, 2 * g, hd, keys, page, l.lds, l.allowed);
+                                }
+                            }
+                        }
+    std::printf("launches %ld large %ld bad %ld\n", n, large, bad);
+    return bad != 0;
+}
+"""
+
+
+def run_program(tmp_path, text):
+    """A program that has its own functions in place of HIP's."""
+    from myelith_amd._lib import lib
+    lib()
+    so = ROOT / "myelith_amd" / "libmyl_hip.so"
+    src, exe = tmp_path / "t.cpp", tmp_path / "t"
+    src.write_text(text)
+    subprocess.run([HIPCC, "-O1", "-std=c++17", "-I", str(ROOT / "include"), "-I", str(CSRC), str(src), f"-L{so.parent}", f"-l:{so.name}", f"-Wl,-rpath,{so.parent}",
+                    "-Wl,--export-dynamic", "-o", str(exe)], check=True, capture_output=True, timeout=300)
+    r = subprocess.run([str(exe)], capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0, (r.stdout[-3000:], r.stderr[-1000:])
+    return r.stdout
+
+
+@pytest.mark.skipif(not Path(HIPCC).exists(), reason="hipcc absent")
+def test_launches_past_64_kib_of_both_kinds_of_lds_ask_for_it(tmp_path):
+    """What a kernel declares counts beside what a launch gives it."""
+    n = re.match(r"launches (\d+) large (\d+) bad 0", run_program(tmp_path, LDS).strip().splitlines()[-1])
+    assert int(n.group(1)) > 5000 and int(n.group(2)) > 500
