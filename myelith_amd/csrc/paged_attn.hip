@@ -943,10 +943,12 @@ __global__ __launch_bounds__(THREADS) void paged_out_kernel(PagedAttn a) {
 
 constexpr size_t kAlignedStride = (size_t)1 << 26;  // 15 of them and a vector are 32 bits of bytes
 
-// A launch with more LDS than the 64 KiB it has by default, the kernel's own included.
+// A launch with more LDS than the 64 KiB it has by default, the kernel's own included.  The attribute
+// is the process's, so every call sets the same: another thread's launch may lie behind this one.
 template <class K>
 hipError_t allow_lds(K kernel, size_t bytes) {
-    return bytes + kPagedOwnLds <= 65536 ? hipSuccess : hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+    return bytes + kPagedOwnLds <= 65536 ? hipSuccess
+                                         : hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (int)(kPagedLds - kPagedOwnLds));
 }
 
 template <int HD, bool ALIGNED, int W>

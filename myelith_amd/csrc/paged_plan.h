@@ -83,6 +83,7 @@ inline const char* paged_refuse(const PagedShape& s) {
 // Within a range of at most 1024 keys sum p |v| <= (2^14 + 2^9) 2^15 < 2^30.
 constexpr int kPagedMaxRange = 1024, kPagedMidRange = 512, kPagedLeastRange = 128;
 constexpr int kPagedLdsLut = 8192;  // exp table entries that a block copies
+constexpr size_t kPagedLds = 160 * 1024;  // of a block, all told
 constexpr size_t kPagedOwnLds = 4800;  // the most LDS that a kernel declares beside what a launch may have to ask for
 
 // The pages that a range of keys can touch.

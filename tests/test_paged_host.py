@@ -516,3 +516,32 @@ def test_launches_past_64_kib_of_both_kinds_of_lds_ask_for_it(tmp_path):
     """What a kernel declares counts beside what a launch gives it."""
     n = re.match(r"launches (\d+) large (\d+) bad 0", run_program(tmp_path, LDS).strip().splitlines()[-1])
     assert int(n.group(1)) > 5000 and int(n.group(2)) > 500
+
+
+@pytest.mark.skipif(not Path(HIPCC).exists(), reason="hipcc absent")
+def test_a_kernel_asks_for_the_same_lds_in_every_call(tmp_path):
+    """The attribute belongs to the process: what one call asks for must not lower another's, made at
+    once from another host thread."""
+    text = LDS[:LDS.index("int main() {")] + r"""
+int main() {
+    if (myl_init(0, &c) != MYL_OK) return 2;
+    for (size_t hd : {(size_t)64, (size_t)128})
+        for (size_t page : {(size_t)8, (size_t)16})
+            for (size_t g : {(size_t)7, (size_t)16})
+                for (size_t seqs : {(size_t)24, (size_t)64})
+                    for (size_t keys = 64; keys <= 40000; keys += keys < 1024 ? 64 : keys / 3)
+                        if (attend(seqs, 2 * g, 2, hd, keys, page, 2662) != MYL_OK) return 3;
+    long several = 0, kernels = 0, least = 1 << 30;
+    for (const auto& f : attributes) {
+        if (f.second.empty()) continue;  // looked up by a launch
+        const std::set<int> values(f.second.begin(), f.second.end());
+        ++kernels;
+        several += values.size() > 1;
+        least = std::min(least, (long)*values.begin());
+    }
+    std::printf("kernels %ld several %ld least %ld\n", kernels, several, least);
+    return 0;
+}
+"""
+    n = re.match(r"kernels (\d+) several (\d+) least (\d+)", run_program(tmp_path, text).strip().splitlines()[-1])
+    assert int(n.group(1)) >= 8 and int(n.group(2)) == 0 and int(n.group(3)) <= 160 * 1024 - 4800, n.group(0)
