@@ -156,8 +156,8 @@ __device__ inline void planes16(const uint4 (&x)[2], v4i32_t& h, v4i32_t& l) {
     l = v4i32_t{(int)lw[0], (int)lw[1], (int)lw[2], (int)lw[3]};
 }
 
-// A wave's 16-key tiles of keys or values, tile after tile straight into a ring of NB places in
-// its own LDS: key r of a tile is row r, its 16-byte chunk x at place x ^ swizzle(r).
+// A wave's 16-key tiles of keys or values, tile after tile straight into a ring of NB (two) places in
+// its own LDS: key r of a tile is row r, its 16-byte chunk x at place x ^ (r mod chunks).
 // Loads retire in order, so a tile has landed when only younger ones' are outstanding.
 // Where pages hold whole tiles (ALIGNED: a multiple of 16 positions), a tile is one address for
 // the wave and 32-bit offsets of the lanes.  What one block alone reads is loaded past the caches'
@@ -166,7 +166,7 @@ __device__ inline void planes16(const uint4 (&x)[2], v4i32_t& h, v4i32_t& l) {
 typedef __attribute__((address_space(1))) const void global_void;
 typedef __attribute__((address_space(3))) void lds_void;
 constexpr int kOnce = 2;  // nontemporal
-template <int HD, int NB, bool ALIGNED, bool SWIZZLE>
+template <int HD, int NB, bool ALIGNED>
 struct Tiles {
     static constexpr int CH = HD / 8, ROWS = 64 / CH, NI = 16 / ROWS, kBytes = 32 * HD;
     const char* pages;
@@ -182,7 +182,7 @@ struct Tiles {
 #pragma unroll
         for (int i = 0; i < NI; ++i) lane[i] = 2u * ((uint32_t)(i * ROWS + row) * (uint32_t)a.pos_stride + 8u * (uint32_t)at(i * ROWS + row, chunk));
     }
-    __device__ static inline int at(int r, int x) { return SWIZZLE ? x ^ (r & (CH - 1)) : x; }
+    __device__ static inline int at(int r, int x) { return x ^ (r & (CH - 1)); }
     // Keys j .. j + 15 into place `slot`; those from j1 on hold anything.
     __device__ inline void issue(const PagedAttn& a, const uint64_t* tab, int p0, int j, int j1, int slot) const {
         int8_t* to = ring + slot * kBytes;
@@ -204,12 +204,11 @@ struct Tiles {
             }
         }
     }
-    // The oldest tile has landed when `left` younger ones and `other` accesses behind them remain.
+    // The oldest tile has landed when `left` younger ones and OTHER accesses behind them remain.
     template <int OTHER>
     __device__ static inline void wait(int left) {
-        if (left >= NB - 1) asm volatile("s_waitcnt vmcnt(%0)" ::"n"((NB - 1) * NI + OTHER) : "memory");
-        else if (NB > 2 && left == NB - 2) asm volatile("s_waitcnt vmcnt(%0)" ::"n"((NB > 2 ? NB - 2 : 0) * NI + OTHER) : "memory");
-        else if (NB > 3 && left == NB - 3) asm volatile("s_waitcnt vmcnt(%0)" ::"n"((NB > 3 ? NB - 3 : 0) * NI + OTHER) : "memory");
+        static_assert(NB == 2, "the cases below");
+        if (left >= 1) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(NI + OTHER) : "memory");
         else asm volatile("s_waitcnt vmcnt(%0)" ::"n"(OTHER) : "memory");
     }
 };
@@ -237,7 +236,7 @@ constexpr int kQkRing = 2;
 template <int HD, bool FAST, bool ALIGNED, bool BALANCED, int NW, bool STORED>
 __device__ inline void paged_scores(const PagedAttn& a, const Part& p, int lim, const uint64_t* tab, int p0, bool holes, int8_t* ring,
                                     const uint4 (&qx)[HD / 64][2], int32_t* z0, int32_t* red) {
-    using T = Tiles<HD, kQkRing, ALIGNED, true>;
+    using T = Tiles<HD, kQkRing, ALIGNED>;
     constexpr int NS = HD / 64, NB = kQkRing;
     const int lane = threadIdx.x & 63, c = lane & 15, kb = lane >> 4;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
