@@ -399,16 +399,24 @@ def test_scalars_outside_their_type_are_refused(recorded):  # noqa: F811
     assert not log
 
 
-def test_allocated_queries_of_left_out_rows_are_zero(recorded, monkeypatch):  # noqa: F811
+def test_allocated_queries_of_left_out_rows_are_zero(streams, monkeypatch):  # noqa: F811
     """The kernel writes nothing for a row that is left out: memory that the call allocates is
-    cleared before it, a caller's q_out is not touched."""
-    b, log = recorded
-    empty = torch.empty
+    cleared before it on the context's stream, a caller's q_out is not touched."""
+    b, log = streams
+    empty, zero = torch.empty, OnGpu.zero_
     monkeypatch.setattr(torch, "empty", lambda *a, **k: empty(*a, **k).fill_(77))
-    got = b.kv_append_paged_dev(**append_args(positions=torch.tensor([0, -1, 5], dtype=torch.int32)))
-    assert log[-1][0] == "myl_kv_append_paged_dev" and log[-1][1][34] == got.data_ptr() and not got.any()
-    given = torch.full((3, 4, 64), -7, dtype=torch.int16)
-    assert b.kv_append_paged_dev(**append_args(q_out=given)) is given and (given == -7).all()
+    monkeypatch.setattr(OnGpu, "zero_", lambda t: (log.append(("zero", torch.cuda.current_stream().cuda_stream)), zero(t))[1])
+    args = on_gpu(append_args(positions=torch.tensor([0, -1, 5], dtype=torch.int32)))
+    for torchs, own, kinds in ((7, 3, ["empty", "wait", "zero", "launch"]), (9, 3, ["empty", "zero", "launch"]), (0, 9, ["empty", "zero", "launch"])):
+        monkeypatch.setattr(FakeStream, "torchs", torchs)
+        b._own_stream = own
+        log.clear()
+        got = b.kv_append_paged_dev(**args)
+        assert [e[0] if e[0] in ("empty", "wait", "zero") else "launch" for e in log] == kinds and ("zero", 9) in log
+        assert log[-1][0] == "myl_kv_append_paged_dev" and log[-1][1][34] == got.data_ptr() and not got.any()
+    log.clear()
+    given = torch.full((3, 4, 64), -7, dtype=torch.int16).as_subclass(OnGpu)
+    assert b.kv_append_paged_dev(**dict(args, q_out=given)) is given and (given == -7).all() and len(log) == 1
 
 
 KEPT = PLANS[:PLANS.index("// pieces of a workspace")].replace('#include "serve_plan.h"', '#include "paged_plan.h"') + r"""
