@@ -328,7 +328,8 @@ int myl_verify_drafts_dev(myl_ctx* ctx, const int32_t* target, size_t ldt, const
  * and [page][position][head] both do.  A sequence's positions lie in the pages that its
  * row of `tables` (n_seqs rows of table_len int32, table_stride apart) names in turn:
  * position pos in page tables[seq][pos / page_size], at pos % page_size.  Sequences may
- * share pages.  An id outside [0, n_pages) names no page.  Pointers to int16, int8, uint8 and
+ * share pages.  An id outside [0, n_pages) names no page: no value of it is used, though some place of
+ * page 0 may be read instead.  Pointers to int16, int8, uint8 and
  * the workspace are 16-byte aligned; head_dim is 64 or 128 (MYL_E_UNSUPPORTED
  * otherwise). */
 
@@ -360,8 +361,8 @@ typedef struct myl_head_norm {
  * values to the position's place in the pages.  A row whose position is negative or
  * whose sequence is outside [0, n_seqs) is left out: nothing of it is written.  A
  * position past the table or on no page keeps its query only.  Rows of one call name
- * different places; of two with the same place, either may be what stays.  heads
- * may be 0 (keys and values alone). */
+ * different places; of two with the same place, each 16 bytes that stay may be either's.
+ * heads may be 0 (keys and values alone). */
 int myl_kv_append_paged_dev(myl_ctx* ctx, const int16_t* q, size_t ldq, const int16_t* k, size_t ldk, const int16_t* v,
                             size_t ldv, size_t rows, size_t heads, size_t kv_heads, size_t head_dim, const int16_t* bias,
                             const uint8_t* bias_shifts, uint8_t q_frac, uint8_t k_frac, uint8_t v_frac,
@@ -382,7 +383,9 @@ int myl_kv_append_paged_dev(myl_ctx* ctx, const int16_t* q, size_t ldq, const in
  * heads of a sequence that share a KV head, is at most 2^33 in all.  A max_len close to the
  * longest row's keeps the launches small; the workspace holds 6 bytes and a sixteenth of them
  * per row, head and position below max_len, and serves calls of the same heads with no more rows in
- * all, however many of them a sequence has, and no more keys. */
+ * all, however many of them a sequence has, and no more keys.  Made for a sequence's newest rows
+ * (tokens, drafts): a prompt's hundreds of rows are right too, but the time and the workspace are those
+ * of rows x keys scores that go through memory, so a program bounds its chunks. */
 size_t myl_attention_paged_workspace(const myl_ctx* ctx, size_t n_seqs, size_t rows_per_seq, size_t heads,
                                      size_t kv_heads, size_t head_dim, size_t max_len);
 int myl_attention_paged_dev(myl_ctx* ctx, const int16_t* q, size_t n_seqs, size_t rows_per_seq, size_t ldq,

@@ -791,8 +791,9 @@ class RocmBackend:
         and v_pages [pages x kv_heads x page_size x hd] (any strides between positions,
         heads and pages); tables int32 [sequences x pages of each].  Row r attends the first
         lens[r] positions of its sequence (at most max_len, by default all that the table
-        names) that lie on a page; without any its output is zero.  include/myl_hip.h
-        states the arithmetic."""
+        names) that lie on a page; without any its output is zero.  Made for the newest few
+        rows of each sequence: the workspace grows with rows x heads x max_len.
+        include/myl_hip.h states the arithmetic."""
         import torch
         what = "attention_paged_dev"
         if (score_shift | lut_shift | prob_frac) >> 8:

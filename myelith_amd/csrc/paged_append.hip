@@ -11,7 +11,8 @@
 // 32-bit steps where their shifts allow it.  16384 rows of 36 heads of 128 take 69 us (4.4 TB/s;
 // loads past the caches 68, but 13.6 against 12.8 for 1503 rows with norms, so not taken).  With
 // norms registers bound it too (96 for 16 values and their channels; held to 80 or 64, 1503 rows took 16
-// and 23 us instead of 12.8).  Few rows: the launch and two loads that follow one another, 5 us.
+// and 23 us instead of 12.8; 16384 rows, four of them in flight at 150, 94).  Few rows: the launch and two loads that
+// follow one another, 5 us.
 #include "abi_internal.h"
 #include "ops.h"
 #include "paged_plan.h"

@@ -11,12 +11,14 @@
 //   paged_pv_kernel    p_j from e_j and S, sum p_j v_j over each range
 //   paged_out_kernel   the sums over the ranges, rounded and clamped
 // Keys and values are read once each, the scores and exp values (6 bytes a key and head) written
-// and read beside them.  us by kernel in that order, heads of 128, seven to a KV head of four: 64 rows of up to
-// 12000 keys 119 + 24 + 121 + 6 (282 a call; 4.1 TB/s of keys and values), one row of 100000 23 + 8.5 +
-// 22 + 4.6 (58), 24 rows of up to 2500 13 + 7 + 14 + 4 (36), of which starting and draining four launches
-// is most.  Joining the ranges in the tile's last block instead of a fourth launch took longer
-// (24 x 2500: 38.7 us with write-through stores and loads, 107 with device fences).  Few keys take one
-// launch (paged_short_kernel).
+// and read beside them.  us by traced kernel in that order (apart from the calls, not adding up to them),
+// heads of 128, seven to a KV head of four: 64 rows of up to 12000 keys 120 + 24 + 122 + 6 (284 a call;
+// 4.1 TB/s of keys and values), one row of 100000 23 + 8.5 + 22 + 4.8 (58), 24 rows of up to 2500
+// 13 + 7 + 14 + 4 (36), of which starting and draining four launches is most; 3 x 500 rows of prompts
+// before 2000 keys 111 + 79 + 344 + 49 (581: made for a sequence's newest few rows).  Joining the
+// ranges in the tile's last block instead of a fourth launch took longer (24 x 2500: 38.7 us with
+// write-through stores and loads, 107 with device fences).  Few keys take one launch
+// (paged_short_kernel).
 #include "abi_internal.h"
 #include "attn_fixed.h"
 #include "gemm_mfma.h"
@@ -156,11 +158,12 @@ __device__ inline void planes16(const uint4 (&x)[2], v4i32_t& h, v4i32_t& l) {
     l = v4i32_t{(int)lw[0], (int)lw[1], (int)lw[2], (int)lw[3]};
 }
 
-// A wave's 16-key tiles of keys or values, tile after tile straight into a ring of NB (two) places in
+// A wave's 16-key tiles of keys, tile after tile straight into a ring of NB (two) places in
 // its own LDS: key r of a tile is row r, its 16-byte chunk x at place x ^ (r mod chunks).
 // Loads retire in order, so a tile has landed when only younger ones' are outstanding.
 // Where pages hold whole tiles (ALIGNED: a multiple of 16 positions), a tile is one address for
-// the wave and 32-bit offsets of the lanes.  What one block alone reads is loaded past the caches'
+// the wave and 32-bit offsets of the lanes; elsewhere each lane and load divides (64 rows of 12000 keys by
+// pages of 100 310 us, of 64 281; 12 x 4 of 3001 by 24 46.1, by 16 41.3).  What one block alone reads is loaded past the caches'
 // usual order (64 rows of 12000 keys: 284 us a call, 306 without; two tiles that share their
 // keys: 55.9 against 52.2, so there not).
 typedef __attribute__((address_space(1))) const void global_void;

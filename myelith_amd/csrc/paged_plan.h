@@ -46,7 +46,11 @@ inline const char* append_refuse(size_t rows, size_t heads, size_t kv_heads, siz
     return nullptr;
 }
 
-// Rows of a thread: as many as leave a CU eight blocks of 256 threads, in fours (or one).
+// Rows of a thread: as many as leave a CU eight blocks of 256 threads, in fours (or one).  us with 1 / 4 / 8 / 16
+// rows a thread, 28 + 2 x 4 heads of 128: with biases 1503 rows 13.9 / 13.3 / 16.1 / 25.0, 8000 49.0 / 40.5 /
+// 40.8 / 42.1, 16384 92.4 / 70.6 / 69.9 / 75.3; with norms (three to five blocks fit a CU at once)
+// 1503 14.0 / 16.9 / 21.3 / 36.5, 4000 27.5 / 32.3 / 36.2 / 48.8, 8000 52.6 / 52.5 / 56.9 / 64.6, 16384
+// 96.8 / 92.1 / 94.1 / 107; with both 16384 160 / 114 / 106 / 114.
 inline int append_group(size_t rows, size_t per_row, int cus) {
     const size_t each = rows * per_row / ((size_t)cus * 8 * 256);
     return each < 4 ? 1 : (int)std::min<size_t>(each / 4 * 4, 16);
@@ -109,9 +113,9 @@ inline size_t paged_short_lds(const PagedPlan& p, size_t hd, int page, uint32_t 
 
 // One launch with a block per tile, or four that split the keys: up to 640 keys of 128, or 1024 keys
 // (as far as their scores fit) where an eighth of the CUs has a block.  us of a call's launches, in
-// one / split, heads of 128, seven to a KV head of four: one row of 130 keys 9.8 / 17.0, 600 16.2 / 17.6,
-// 1000 21.9 / 17.9; eight rows of 1000 20.4 / 20.2; 64 of 300 13.6 / 22.1, of 1000 26.3 / 41.8; 256 of
-// 1000 93 / 106.
+// one / split, heads of 128, seven to a KV head of four: one row of 130 keys 8.8 / 16.4, 600 15.1 / 17.0,
+// 1000 21.9 / 17.6; eight rows of 1000 21.4 / 21.0; 64 of 300 13.0 / 22.4, of 1000 25.6 / 39.8; 256 of
+// 1000 88 / 100.
 inline bool paged_in_one(const PagedShape& s, const PagedPlan& p, int cus) {
     return s.max_len <= kPagedShortKeys && s.max_len * (size_t)p.width <= kPagedShortScores &&
            (s.max_len * s.head_dim <= 640 * 128 || p.parts * 8 >= (size_t)cus);
@@ -131,8 +135,8 @@ inline PagedPlan paged_plan(const PagedShape& s, int cus) {
         } else {
             // A block per CU where ranges of 128 to 512 keys make it, then two where up to 1024 keys
             // do.  us of a call's launches at 128 / 256 / 512 keys, heads of 128: one row of 5000 keys
-            // 20.4 / 21.6 / 25.8, 10000 25.8 / 23.9 / 26.9, 30000 38.8 / 32.9 / 30.7; eight of 2000
-            // 25.1 / 23.7 / 27.2; 64 of 300 28.8 / 29.3 / 22.3 (one range); 24 of 2500 40.6 / 40.7 / 38.2.
+            // 21.1 / 21.0 / 24.9, 10000 25.6 / 23.9 / 26.3, 30000 40.5 / 31.1 / 31.2; eight of 2000
+            // 25.1 / 24.0 / 26.3; 64 of 300 27.7 / 28.4 / 22.2 (one range); 24 of 2500 48.7 / 41.9 / 37.1.
             const size_t each = (p.parts * (size_t)p.keys + (size_t)cus - 1) / (size_t)cus;
             const size_t want = each <= kPagedMidRange ? std::max<size_t>(each, kPagedLeastRange) : std::max<size_t>(each / 2, kPagedMidRange);
             p.range = (int)std::min<size_t>((want + 63) / 64 * 64, kPagedMaxRange);
