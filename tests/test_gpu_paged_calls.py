@@ -396,3 +396,32 @@ def test_attention_of_ranges_just_past_64_kib(backend, exp_lut):
              lens=r.integers(1, 10001, 48).astype(np.int32))
     s["lens"][0] = 10000
     check_attention(backend, s, exp_lut)
+
+
+def test_append_captured_with_its_allocated_queries(backend):
+    """A captured call that allocates its queries clears them on every replay."""
+    import torch
+    case("append captured with allocated queries")
+    s = append_inputs(84, 40, 4, 2, 64, 16, seqs=6, context=60)
+    s["positions"][::4] = -5
+    want = ref.append(s["q"], s["k"], s["v"], s["positions"], s["kp"], s["vp"], s["tables"], s["cos"], s["sin"], 8, np.zeros_like(s["q"]), s["seqs"],
+                      s["bias"], s["bias_shifts"], FRACS)
+    d, stream, graph = dict(on_gpu(s), norm=None), torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    try:
+        with torch.cuda.stream(stream):
+            backend.use_torch_stream()
+        with torch.cuda.graph(graph, stream=stream):
+            got = run_append(backend, d, None)
+        for turn in range(4):
+            got.fill_(77)
+            d["kp"].copy_(gpu(s["kp"]))
+            d["vp"].copy_(gpu(s["vp"]))
+            torch.cuda.synchronize()
+            graph.replay()
+            torch.cuda.synchronize()
+            for what, g, w in zip(("queries", "keys", "values"), (got, d["kp"], d["vp"]), want):
+                same(g, w, f"replay {turn}: {what}")
+    finally:
+        torch.cuda.synchronize()
+        backend.use_torch_stream()
